@@ -1,6 +1,7 @@
 /*
- * C ABI of the Kimi Delta Attention (KDA) decode kernels: the recurrent-state
- * step and its launch-fused preparation (short convolutions, gates).
+ * C ABI of the Kimi Delta Attention (KDA) kernels: for decode the recurrent-state
+ * step and its launch-fused preparation (short convolutions, gates), for
+ * prompts the short convolutions and the recurrence over packed sequences.
  *
  * Same conventions as lk_w4a16.h: device pointers, element counts, a
  * hipStream_t passed as void*, LK_OK or an error code (message from
@@ -102,6 +103,47 @@ LK_API int lk_kda_decode_layer_split(const void* q_in, const void* k_in, const v
                                      float* out, int64_t batch, int64_t heads, int64_t head_dim,
                                      float eps, float scale, int value_dtype, int weight_dtype,
                                      int decay_dtype, int beta_dtype, void* stream);
+
+/* ---- prompts: the short convolutions and the recurrence over packed sequences
+ *
+ * Sequences are packed one behind the other over the rows of a call: sequence
+ * s has rows cu_seqlens[s] to cu_seqlens[s + 1] - 1 (int32 [sequences + 1] on
+ * the device, starting with 0; clamped to the rows), or with a null cu_seqlens
+ * tokens / sequences rows each. A sequence may be empty: its state is kept.
+ * Output rows behind the last sequence are set to zero. A state may be
+ * updated in place (state_out = state) or written elsewhere. */
+
+/* the three width-4 convolutions of a prompt: what lk_kda_short_conv_triple
+ * computes token by token. inputs [tokens, C] in value_dtype, row_stride
+ * elements from one row to the next (the same for all three; >= C); states
+ * [sequences, C, 4]; weights [C, 4] in weight_dtype; outputs [tokens, C]
+ * dense, in value_dtype. 16-byte accesses where C and row_stride are
+ * multiples of 16 bytes and every input and output starts on one. */
+LK_API int lk_kda_short_conv_prefill(const void* q_in, const void* k_in, const void* v_in,
+                                     const void* q_state, const void* k_state,
+                                     const void* v_state, void* q_state_out, void* k_state_out,
+                                     void* v_state_out, const void* q_weight,
+                                     const void* k_weight, const void* v_weight, void* q_out,
+                                     void* k_out, void* v_out, const int32_t* cu_seqlens,
+                                     int64_t sequences, int64_t tokens, int64_t channels,
+                                     int64_t row_stride, int value_dtype, int weight_dtype,
+                                     void* stream);
+
+/* the recurrence of a prompt: what lk_kda_decode_step computes token by token.
+ * q, k, decay fp32 [tokens, H, d_k], beta fp32 [tokens, H] (lk_kda_gates
+ * writes them for any number of rows), v [tokens, H, d_v] and out
+ * [tokens, H, d_v] in value_dtype, state fp32 [sequences, H, d_k, d_v].
+ * decay <= 0 (a log decay). d_k <= 256; tensors start on 16 bytes. All sums
+ * and the state are fp32; out is rounded once. workspace:
+ * lk_kda_prefill_workspace() bytes on 16 bytes (may be null where that is 0). */
+LK_API int64_t lk_kda_prefill_workspace(int64_t sequences, int64_t tokens, int64_t heads,
+                                        int64_t d_k, int64_t d_v);
+
+LK_API int lk_kda_prefill(const float* state, float* state_out, const float* q, const float* k,
+                          const void* v, const float* decay, const float* beta, void* out,
+                          const int32_t* cu_seqlens, int64_t sequences, int64_t tokens,
+                          int64_t heads, int64_t d_k, int64_t d_v, float scale, int value_dtype,
+                          void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

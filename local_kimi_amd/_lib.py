@@ -1,6 +1,6 @@
 """ctypes binding of the in-tree HIP library (``liblkamd.so``).
 
-The library exposes the C ABI declared in ``include/lk_w4a16.h``. This module
+The library exposes the C ABI declared in ``include/lk_*.h``. This module
 declares each entry point's argument types once, and :func:`call` turns a
 non-zero status into ``RuntimeError`` with the library's message. There is no
 fallback: if the library is missing, every kernel call raises.
@@ -77,6 +77,12 @@ SIGNATURES: dict[str, list] = {
                             _I64, _I64, _I64, _F, _F, _I, _I, _I, _I, _P],
     "lk_kda_decode_layer_split": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                   _P, _P, _P, _I64, _I64, _I64, _F, _F, _I, _I, _I, _I, _P],
+    "lk_kda_short_conv_prefill": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+                                  _I64, _I64, _I64, _I64, _I, _I, _P],
+    "lk_kda_prefill": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _I,
+                       _P, _I64, _P],
+    "lk_attention_prefill": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                             _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _P, _I64, _P],
     "lk_rms_norm": [_P, _P, _P, _I64, _I64, _F, _I, _I, _P],
     "lk_add_rms_norm": [_P, _P, _P, _P, _P, _I64, _I64, _F, _I, _I, _P],
     "lk_rms_gated_norm": [_P, _P, _P, _P, _I64, _I64, _F, _I, _I, _I, _I, _P],
@@ -91,6 +97,8 @@ QUERIES: dict[str, list] = {
     "lk_w4a16_grouped_gemm_workspace": [_I64, _I64, _I64],
     "lk_w4a16_moe_forward_workspace": [_I64, _I64, _I64, _I64, _I64],
     "lk_mxfp4_moe_forward_workspace": [_I64, _I64, _I64, _I64, _I64],
+    "lk_kda_prefill_workspace": [_I64, _I64, _I64, _I64, _I64],
+    "lk_attention_prefill_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I64],
 }
 
 _lock = threading.Lock()

@@ -1,11 +1,15 @@
-"""Kimi Delta Attention decode ops on HIP: the recurrence step and its fused preparation.
+"""Kimi Delta Attention ops on HIP: the recurrence step and its fused preparation for
+decode, the short convolutions and the recurrence for prompts.
 
 Same names, signatures, validation and in-place semantics as the reference's
 engine/kernels/kda_step.py:273-293 (``kda_decode_step``) and
 engine/kernels/kda_prepare.py:479-538 (``fused_short_conv_triple``), :630-686
 (``fused_kda_gates``); each runs one launch of ``local_kimi_amd/csrc/kda.hip``.
 ``kda_decode_layer`` (no reference counterpart) runs all three for one decode
-token in a single launch.
+token in a single launch. A prompt takes ``short_conv_prefill_triple``,
+``fused_kda_gates`` (any sequence length) and ``kda_prefill``
+(``local_kimi_amd/csrc/kda_prefill.hip``): the same functions of the same states,
+over equal or packed sequences, so a decode loop continues from their states.
 
 Beyond the reference's checks: values and states of the short convolutions
 and the q / k / raw inputs of the gates must be float32, float16 or bfloat16
@@ -355,4 +359,219 @@ def _layer_split(ins, states, outs, weights, raw_decay, dt_bias, a_log, raw_beta
                   _code(raw_beta, "raw_beta"), _w._stream(state.device))
     if work is not state:
         state.copy_(work)
+    return out
+
+
+# ---------------------------------------------------------------------------
+# prompts (the token-by-token loop of the ops above, over whole sequences)
+
+
+def _offsets(cu_seqlens: torch.Tensor | None, batch: int, device: torch.device,
+             what: str = "cu_seqlens") -> tuple[torch.Tensor | None, int]:
+    """int32 offsets of packed sequences (or None) and the number of sequences."""
+    if cu_seqlens is None:
+        return None, batch
+    if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 2:
+        raise ValueError(f"{what} must have shape [sequences + 1]")
+    if cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what} must be int32 or int64, got {cu_seqlens.dtype}")
+    if cu_seqlens.device != device:
+        raise ValueError(f"{what} must be on the inputs' device")
+    if batch != 1:
+        raise ValueError(f"{what} takes inputs of batch one that hold the packed sequences")
+    return _w._c(cu_seqlens.to(torch.int32)), cu_seqlens.shape[0] - 1
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """A dense copy that starts on 16 bytes, or ``t`` if it is one."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _packed_rows(tensors) -> tuple[list[torch.Tensor], int]:
+    """[B, S, C] tensors as rows one stride apart (the same for all of them):
+    views of one projection's rows as they are, other layouts copied."""
+    first = tensors[0]
+    batch, rows, width = first.shape
+    stride = first.stride(1)
+    fits = stride >= width and all(
+        (width == 1 or t.stride(2) == 1) and t.stride(1) == stride and
+        (batch == 1 or t.stride(0) == rows * stride) for t in tensors)
+    if fits and rows > 1:
+        return list(tensors), stride
+    return [_w._c(t) for t in tensors], width
+
+
+def short_conv_prefill_triple(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torch.Tensor,
+                              q_state: torch.Tensor, k_state: torch.Tensor,
+                              v_state: torch.Tensor, q_weight: torch.Tensor,
+                              k_weight: torch.Tensor, v_weight: torch.Tensor, *,
+                              cu_seqlens: torch.Tensor | None = None,
+                              conv_states_out: tuple[torch.Tensor, torch.Tensor, torch.Tensor]
+                              | None = None
+                              ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The three width-4 convolutions of whole prompts in one launch.
+
+    ``q_in``, ``k_in``, ``v_in`` [B, S, C]; states [B, C, 4] and weights
+    [C, 1, 4] (or [C, 4]) as ``fused_short_conv_triple`` takes them, which
+    this equals token by token. With ``cu_seqlens`` [N + 1] (int32 or int64, on
+    the device, from 0) B is one, the S rows hold N packed sequences and the
+    states are [N, C, 4]; offsets are clamped to the rows, and output rows
+    behind the last sequence are zero. A sequence may be empty (its state
+    stays). A fresh prompt's state is zeros.
+
+    Returns the outputs in the input dtype; the states are updated in place,
+    or with ``conv_states_out`` left as they are and the new ones written
+    there. Equal row strides (views of one fused projection) are read in
+    place.
+    """
+    values, states = (q_in, k_in, v_in), (q_state, k_state, v_state)
+    weights = (q_weight, k_weight, v_weight)
+    if any(t.ndim != 3 for t in values):
+        raise ValueError("q_in, k_in, and v_in must have shape [batch, sequence, channels]")
+    if not (q_in.shape == k_in.shape == v_in.shape):
+        raise ValueError("q_in, k_in, and v_in must have identical shapes")
+    batch, rows, channels = q_in.shape
+    if batch == 0 or channels == 0:
+        raise ValueError("short convolutions need a nonempty batch and channels")
+    dev = q_in.device
+    if any(t.device != dev for t in (*values[1:], *states, *weights)):
+        raise ValueError("all short convolution tensors must share one device")
+    offsets, count = _offsets(cu_seqlens, batch, dev)
+    if any(tuple(t.shape) != (count, channels, CONV_WIDTH) for t in states):
+        raise ValueError("each short convolution state must have shape [sequences, channels, 4]")
+    if any(tuple(t.shape) not in {(channels, CONV_WIDTH), (channels, 1, CONV_WIDTH)}
+           for t in weights):
+        raise ValueError("each short convolution weight must have shape [channels, 1, 4]")
+    if any(t.dtype != q_in.dtype for t in (*values[1:], *states)):
+        raise TypeError("short convolution inputs and states must share a dtype")
+    vcode = _code(q_in, "short convolution inputs and states")
+    if any(not t.is_floating_point() for t in weights):
+        raise TypeError("short convolution weights must be floating point")
+    if dev.type != "cuda":
+        raise ValueError("prompt short convolutions require CUDA tensors")
+    if any(_overlaps(states[i], states[j]) for i, j in ((0, 1), (0, 2), (1, 2))):
+        raise ValueError("the three convolution states must not overlap")
+    targets = states
+    if conv_states_out is not None:
+        targets = tuple(conv_states_out)
+        if len(targets) != 3:
+            raise ValueError("conv_states_out must hold the q, k and v states")
+        if any(o.shape != st.shape or o.dtype != st.dtype or o.device != dev
+               for st, o in zip(states, targets)):
+            raise ValueError("each conv_states_out tensor must match its state's shape, dtype "
+                             "and device")
+        for i, o in enumerate(targets):
+            if any(_overlaps(o, t) for t in (*states, *targets[i + 1:])):
+                raise ValueError(f"conv_states_out[{i}] overlaps another state")
+    weights = [_weight_view(w) for w in weights]
+    if weights[0].dtype not in _DTYPE_CODES or any(w.dtype != weights[0].dtype for w in weights):
+        weights = [w.float() for w in weights]
+    wcode = _DTYPE_CODES[weights[0].dtype]
+    weights = [_w._c(w) for w in weights]
+    ins, stride = _packed_rows(values)
+    src = [_aligned(st) for st in states]
+    if conv_states_out is None:
+        work = src
+    else:
+        work = [o if o.is_contiguous() and o.data_ptr() % 16 == 0 else
+                torch.empty(o.shape, dtype=o.dtype, device=dev) for o in targets]
+    outs = [torch.empty((batch, rows, channels), dtype=q_in.dtype, device=dev) for _ in range(3)]
+    with _w._on(dev):
+        _lib.call("lk_kda_short_conv_prefill", *(t.data_ptr() for t in ins),
+                  *(t.data_ptr() for t in src), *(t.data_ptr() for t in work),
+                  *(t.data_ptr() for t in weights), *(t.data_ptr() for t in outs),
+                  None if offsets is None else offsets.data_ptr(), count, batch * rows, channels,
+                  stride, vcode, wcode, _w._stream(dev))
+    for target, w in zip(targets, work):
+        if w is not target:
+            target.copy_(w)
+    return outs[0], outs[1], outs[2]
+
+
+def kda_prefill(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                decay: torch.Tensor, beta: torch.Tensor, *, scale: float,
+                cu_seqlens: torch.Tensor | None = None,
+                state_out: torch.Tensor | None = None) -> torch.Tensor:
+    """The KDA recurrence over whole prompts; what ``kda_decode_step`` computes
+    token by token.
+
+    ``q``, ``k``, ``decay`` [B, S, H, d_k] and ``beta`` [B, S, H] float32 (as
+    ``fused_kda_gates`` returns them, ``decay`` <= 0), ``v`` [B, S, H, d_v] float32,
+    float16 or bfloat16, ``state`` float32 [B, H, d_k, d_v]. With
+    ``cu_seqlens`` [N + 1] (int32 or int64, on the device, from 0) B is one,
+    the S rows hold N packed sequences and ``state`` is [N, H, d_k, d_v];
+    offsets are clamped to the rows, and output rows behind the last sequence
+    are zero. A sequence may be empty (its state stays). A fresh prompt's
+    state is zeros.
+
+    Returns the output [B, S, H, d_v] in v's dtype (sums and state are fp32,
+    one rounding at the end); ``state`` is updated in place, or with
+    ``state_out`` left as it is and the new one written there. d_k up to 256.
+    """
+    if q.ndim != 4:
+        raise ValueError("q must have shape [batch, sequence, heads, d_k]")
+    batch, rows, heads, d_k = q.shape
+    if any(t.dtype != torch.float32 for t in (state, q, k, decay, beta)):
+        raise TypeError("KDA prefill takes torch.float32 state, q, k, decay and beta")
+    vcode = _code(v, "v")
+    if not all(t.device == q.device for t in (state, k, v, decay, beta)):
+        raise ValueError("KDA prefill inputs must share one device")
+    if k.shape != q.shape:
+        raise ValueError("k must have shape [batch, sequence, heads, d_k]")
+    if decay.shape != q.shape:
+        raise ValueError("decay must have shape [batch, sequence, heads, d_k]")
+    if beta.shape != q.shape[:3]:
+        raise ValueError("beta must have shape [batch, sequence, heads]")
+    if v.ndim != 4 or v.shape[:3] != q.shape[:3]:
+        raise ValueError("v must have shape [batch, sequence, heads, d_v]")
+    d_v = v.shape[3]
+    if batch == 0 or heads == 0 or d_k == 0 or d_v == 0:
+        raise ValueError("KDA prefill dimensions must be nonzero")
+    offsets, count = _offsets(cu_seqlens, batch, q.device)
+    if tuple(state.shape) != (count, heads, d_k, d_v):
+        raise ValueError("state must have shape [sequences, heads, d_k, d_v]")
+    if state_out is not None:
+        if state_out.shape != state.shape or state_out.dtype != state.dtype \
+                or state_out.device != state.device:
+            raise ValueError("state_out must match the state's shape, dtype and device")
+        if _overlaps(state_out, state):
+            raise ValueError("state_out overlaps the state it is computed from")
+    if q.device.type != "cuda":
+        raise ValueError("KDA prefill requires CUDA inputs")
+    if d_k > KDA_MAX_KEY_DIM:
+        raise ValueError(f"KDA prefill supports d_k up to {KDA_MAX_KEY_DIM}, got {d_k}")
+    qc, kc, vc, dc, bc = (_aligned(t) for t in (q, k, v, decay, beta))
+    src = _aligned(state)
+    target = state if state_out is None else state_out
+    if state_out is None:
+        work = src
+    elif target.is_contiguous() and target.data_ptr() % 16 == 0:
+        work = target
+    else:
+        work = torch.empty(target.shape, dtype=torch.float32, device=q.device)
+    out = torch.empty(v.shape, dtype=v.dtype, device=q.device)
+    need = _lib.query("lk_kda_prefill_workspace", count, batch * rows, heads, d_k, d_v)
+    ws = _w.workspace(need, q.device) if need else None
+    with _w._on(q.device):
+        _lib.call("lk_kda_prefill", src.data_ptr(), work.data_ptr(), qc.data_ptr(), kc.data_ptr(),
+                  vc.data_ptr(), dc.data_ptr(), bc.data_ptr(), out.data_ptr(),
+                  None if offsets is None else offsets.data_ptr(), count, batch * rows, heads,
+                  d_k, d_v, float(scale), vcode, None if ws is None else ws.data_ptr(), need,
+                  _w._stream(q.device))
+    if work is not target:
+        target.copy_(work)
     return out

@@ -121,3 +121,48 @@ def gates(raw_decay: np.ndarray, dt_bias: np.ndarray, a_log: np.ndarray,
     qn = qn / np.sqrt((qn * qn).sum(axis=-1, keepdims=True) + eps)
     kn = kn / np.sqrt((kn * kn).sum(axis=-1, keepdims=True) + eps)
     return decay, beta, qn, kn
+
+
+# ---------------------------------------------------------------------------
+# whole prompts: the functions above, token by token, over packed sequences
+
+
+def sequence_bounds(cu: np.ndarray | None, rows: int, sequences: int) -> list[tuple[int, int]]:
+    """(begin, end) of each sequence: offsets clamped to the rows (a decreasing
+    pair is empty), or equal sequences."""
+    if cu is None:
+        n = rows // sequences
+        return [(s * n, (s + 1) * n) for s in range(sequences)]
+    at = np.clip(np.asarray(cu, dtype=np.int64), 0, rows)
+    return [(int(a), int(max(a, b))) for a, b in zip(at[:-1], at[1:])]
+
+
+def short_conv_prefill(values: np.ndarray, state: np.ndarray, weight: np.ndarray, dtype: str,
+                       cu: np.ndarray | None = None) -> tuple[np.ndarray, np.ndarray]:
+    """``short_conv`` over the tokens of packed sequences: values [T, C] (rows
+    of the sequences one behind the other), state [N, C, 4]; returns (outputs
+    [T, C] rounded to dtype, new states). Rows of no sequence are zero."""
+    x = np.asarray(values, dtype=np.float64)
+    new = np.array(state, dtype=np.float64)
+    out = np.zeros_like(x)
+    for s, (a, b) in enumerate(sequence_bounds(cu, x.shape[0], new.shape[0])):
+        for t in range(a, b):
+            y, st = short_conv(x[t][None, None], new[s][None], weight, dtype)
+            out[t], new[s] = y[0, 0], st[0]
+    return out, new
+
+
+def prefill(state: np.ndarray, q: np.ndarray, k: np.ndarray, v: np.ndarray, decay: np.ndarray,
+            beta: np.ndarray, scale: float, cu: np.ndarray | None = None
+            ) -> tuple[np.ndarray, np.ndarray]:
+    """``decode_step`` over the tokens of packed sequences: state [N, H, dk,
+    dv], q/k/decay [T, H, dk], v [T, H, dv], beta [T, H]. Returns (new states,
+    outputs [T, H, dv]), float64; rows of no sequence are zero."""
+    new = np.array(state, dtype=np.float64)
+    out = np.zeros(np.asarray(v).shape, dtype=np.float64)
+    for s, (a, b) in enumerate(sequence_bounds(cu, out.shape[0], new.shape[0])):
+        for t in range(a, b):
+            st, y = decode_step(new[s][None], q[t][None], k[t][None], v[t][None], decay[t][None],
+                                beta[t][None], scale)
+            new[s], out[t] = st[0], y[0]
+    return new, out
