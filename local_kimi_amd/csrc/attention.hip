@@ -1,14 +1,12 @@
 // Causal softmax attention over packed prompts, for gfx950.
 
 #include "lk_attention.h"
-#include "lk_common.hpp"
+#include "lk_gemm.hpp"
 #include "lk_sequences.hpp"
 
 namespace lk {
 namespace {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kAttnThreads = 256;
@@ -25,7 +23,8 @@ struct AttnArgs {
   int heads, group, d_qk, d_v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   int64_t tiles;
-  float scale_log2;  // scale * log2(e)
+  float scale_log2;  // |scale| * log2(e), 1 where scale is 0
+  uint32_t q_keep, q_flip;  // bits of q kept (none where scale is 0), flipped (signs, scale < 0)
 };
 
 template <bool BF16>
@@ -60,30 +59,48 @@ __device__ inline bool any_nonfinite(u32x4_t x) {
   return (hit & 0x80008000u) != 0;
 }
 
-// o += V^T P^T for 16 keys of which a query may not see some, where V holds an
-// infinity or a NaN: p = 0 would not silence it, so each key's product is
-// taken alone and dropped where the key is not seen. Rare and slow.
+// The eight values with those set to zero.
 template <bool BF16>
-__device__ __attribute__((noinline)) f32x16_t mfma_seen(u32x4_t v, u32x4_t p, f32x16_t o, int half,
-                                                        int first, int seen) {
-  for (int slot = 0; slot < 16; ++slot) {
-    const int j = slot & 7, owner = slot >> 3;
-    const uint32_t mask = half != owner ? 0u : (j & 1 ? 0xFFFF0000u : 0xFFFFu);
-    u32x4_t v1, p1;
+__device__ inline u32x4_t finite_only(u32x4_t x) {
+  constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      v1[w] = w == j / 2 ? v[w] & mask : 0u;
-      p1[w] = w == j / 2 ? p[w] & mask : 0u;
-    }
-    f32x16_t part;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) part[r] = 0.f;
-    part = mfma32<BF16>(v1, p1, part);
-    const int key = first + 8 * (j / 4) + 4 * owner + j % 4;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[r] = key < seen ? o[r] + part[r] : o[r];
-  }
-  return o;
+  for (int i = 0; i < 4; ++i) x[i] &= ~((((x[i] & kExp) + kOne) >> 15 & 0x00010001u) * 0xFFFFu);
+  return x;
+}
+
+template <bool BF16>
+__device__ inline float value_of(uint32_t x) {
+  if constexpr (BF16) return bf16_to_f32(static_cast<uint16_t>(x));
+  else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(x)));
+}
+
+// Staging. A tile of K (V) in LDS is kAttnKeys rows of C 16-byte chunks, filled
+// by direct loads (a wave-wide load fills 1 KB in slot order), row r's chunk c
+// in slot r C + (c ^ swizzle(r)). A matrix row's chunks are read by 16 or 32 lanes
+// with consecutive rows at once, so the swizzle spreads 16 consecutive rows over
+// all 16-byte columns of the 64 banks; rows shorter than 256 bytes share one
+// pass over the banks with their neighbours, and longer ones than 256 start at
+// either half of them, hence the row's upper bits there.
+template <int C>
+__device__ inline int key_swizzle(int r) {
+  return C % 16 == 0 ? r & 15 : (r >> 1) & 7;
+}
+// V is read down its columns (four rows of 32 bytes by 16 lanes, twice that by a
+// half-wave): four consecutive rows go to four quarters of the banks.
+template <int C>
+__device__ inline int value_swizzle(int r) {
+  return C % 16 == 0 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
+}
+
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+
+// Four rows of 16 columns, by 16 lanes: lane l gives the address of row l / 4,
+// columns 4 (l % 4) to + 3, and gets column l of the four rows.
+__device__ inline uint2 lds_read_transposed(const uint16_t* p) {
+  const i16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lds_i16x4_t*)(const __attribute__((address_space(3))) uint16_t*)(p));
+  return __builtin_bit_cast(uint2, v);
 }
 
 // Block = 128 queries of one head, a wave 32 of them. Scores are computed
@@ -93,38 +110,46 @@ __device__ __attribute__((noinline)) f32x16_t mfma_seen(u32x4_t v, u32x4_t p, f3
 // a scalar per lane, and the score registers, rounded, are the B operand of
 // O^T += V^T P^T as they stand.
 template <bool BF16, int DQ, int DV>
-__global__ void __launch_bounds__(kAttnThreads) attention_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) {
   constexpr int kQSteps = DQ / 16;
   constexpr int kVTiles = DV / 32;
-  constexpr int kKStride = DQ + 8;
-  constexpr int kVStride = kAttnKeys + 8;
-  __shared__ alignas(16) uint16_t lk_[kAttnKeys * kKStride];
-  __shared__ alignas(16) uint16_t lvt[DV * kVStride];
-  const int64_t number = blockIdx.x % a.tiles;
-  const int h = static_cast<int>(blockIdx.x / a.tiles);
+  constexpr int kKChunks = DQ / 8, kVChunks = DV / 8;
+  constexpr int kKLoads = kAttnKeys * kKChunks / kAttnThreads;
+  constexpr int kVLoads = kAttnKeys * kVChunks / kAttnThreads;
+  constexpr int kStage = kAttnKeys * (DQ + DV);  // values of one stage
+  // p is stored as 2^kLift times itself: fp16 keeps 2^-24 at the least
+  constexpr float kLift = BF16 ? 0.f : 6.f;
+  __shared__ alignas(16) uint16_t stage[2 * kStage];
+  const int64_t total = a.tiles * a.heads;
+  const int64_t id = blockIdx.x;
+  const int h = static_cast<int>(id % a.heads);
+  const int64_t number = a.tiles - 1 - id / a.heads;
+  (void)total;
   const SequenceTile at = find_sequence_tile(a.sq, number, kAttnQueries);
   const RowRange rq = sequence_rows(a.sq, at.sequence);
   const int64_t lq = rq.end - rq.begin;
   const int64_t q0 = at.tile * kAttnQueries;
   if (q0 >= lq) return;
-  const int tid = threadIdx.x, wave = tid / kWave, lane = tid & (kWave - 1);
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int n = lane & 31, half = lane >> 5;
-  const int64_t qi = q0 + wave * 32 + n;  // the lane's query
-  uint16_t* const orow = a.out + ((rq.begin + qi) * a.heads + h) * a.d_v;
+  const int64_t qw = q0 + wave * 32;  // the wave's first query
+  const int64_t qi = qw + n;          // the lane's
   f32x16_t o[kVTiles];
 #pragma unroll
   for (int t = 0; t < kVTiles; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
-  float m = -INFINITY, sum = 0.f;
-
+  float top = -INFINITY;  // (scaled) maximum that p is taken against
+  float sum = 0.f;
   if (at.sequence < a.sq.count) {
     const RowRange rk = sequence_rows(a.sk, at.sequence);
     const int64_t lk = rk.end - rk.begin;
     const int64_t ahead = lk - lq;
-    // keys seen by the block's last query
+    // keys seen by the block's last query, and by the wave's
     const int64_t last = q0 + kAttnQueries < lq ? q0 + kAttnQueries : lq;
     const int64_t keys = last + ahead < 0 ? 0 : last + ahead;
+    const int64_t keys_wave = qw + 32 + ahead < keys ? qw + 32 + ahead : keys;
     const int hk = h / a.group;
     const uint16_t* const kb = a.k + rk.begin * a.k_row + hk * a.k_head;
     const uint16_t* const vb = a.v + rk.begin * a.v_row + hk * a.v_head;
@@ -136,102 +161,175 @@ __global__ void __launch_bounds__(kAttnThreads) attention_kernel(AttnArgs a) {
         const int d = 16 * i + 8 * half;
         const u32x4_t z = {0u, 0u, 0u, 0u};
         qf[i] = d < a.d_qk ? *reinterpret_cast<const u32x4_t*>(qp + d) : z;
+        qf[i] = (qf[i] & a.q_keep) ^ a.q_flip;
       }
     }
-    for (int64_t k0 = 0; k0 < keys; k0 += kAttnKeys) {
-      __syncthreads();
-      for (int c = tid; c < kAttnKeys * (DQ / 8); c += kAttnThreads) {
-        const int r = c / (DQ / 8), d = c % (DQ / 8) * 8;
-        const u32x4_t z = {0u, 0u, 0u, 0u};
-        *reinterpret_cast<u32x4_t*>(lk_ + r * kKStride + d) =
-            k0 + r < lk && d < a.d_qk
-                ? *reinterpret_cast<const u32x4_t*>(kb + (k0 + r) * a.k_row + d)
-                : z;
-      }
-      for (int c = tid; c < kAttnKeys * (DV / 8); c += kAttnThreads) {
-        const int r = c / (DV / 8), d = c % (DV / 8) * 8;
-        u32x4_t x = {0u, 0u, 0u, 0u};
-        if (k0 + r < lk && d < a.d_v)
-          x = *reinterpret_cast<const u32x4_t*>(vb + (k0 + r) * a.v_row + d);
+    // byte offsets of this lane's chunks from a tile's first row
+    uint32_t koff[kKLoads], voff[kVLoads];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) lvt[(d + j) * kVStride + r] = static_cast<uint16_t>(x[j / 2] >> (16 * (j & 1)));
-      }
-      __syncthreads();
-      f32x16_t s[2];
+    for (int i = 0; i < kKLoads; ++i) {
+      const int slot = (wave * kKLoads + i) * kWave + lane, r = slot / kKChunks;
+      const int c = slot % kKChunks ^ key_swizzle<kKChunks>(r);
+      koff[i] = 8 * c < a.d_qk ? static_cast<uint32_t>(r * a.k_row + 8 * c) * 2u : 0xFFFFFFF0u;
+    }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+    for (int i = 0; i < kVLoads; ++i) {
+      const int slot = (wave * kVLoads + i) * kWave + lane, r = slot / kVChunks;
+      const int c = slot % kVChunks ^ value_swizzle<kVChunks>(r);
+      voff[i] = 8 * c < a.d_v ? static_cast<uint32_t>(r * a.v_row + 8 * c) * 2u : 0xFFFFFFF0u;
+    }
+    const uint32_t lds = lds_offset(stage);
+    auto fetch = [&](int64_t k0, int buf) {
+      // rows behind the sequence's last read as zeros
+      const int64_t rows = lk - k0 < kAttnKeys ? lk - k0 : kAttnKeys;
+      const u32x4_t rk_ = buffer_rsrc(kb + k0 * a.k_row, ((rows - 1) * a.k_row + a.d_qk) * 2);
+      const u32x4_t rv_ = buffer_rsrc(vb + k0 * a.v_row, ((rows - 1) * a.v_row + a.d_v) * 2);
+      const uint32_t base = lds + buf * kStage * 2;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+      for (int i = 0; i < kKLoads; ++i)
+        lds_direct16(rk_, base + (wave * kKLoads + i) * kWave * 16, koff[i], 0);
+#pragma unroll
+      for (int i = 0; i < kVLoads; ++i)
+        lds_direct16(rv_, base + kAttnKeys * DQ * 2 + (wave * kVLoads + i) * kWave * 16, voff[i], 0);
+    };
+    // LDS reads of this lane, in values from a stage's start: K row n (+ 32 t), V
+    // rows 4 half + lane % 16 / 4 (+ 8 x), columns 16 (lane / 16 % 2) + 4 (lane % 4)
+    const int vrow = 4 * half + (lane & 15) / 4;
+    const int vcol = 16 * (lane / 16 & 1) + 4 * (lane & 3);
+
+    if (keys > 0) fetch(0, 0);
+    wait_vmcnt<0>();
+    __syncthreads();
+    int buf = 0;
+    bool bad = false;  // V has an infinity or a NaN in a tile that not every query sees
+    for (int64_t k0 = 0; k0 < keys; k0 += kAttnKeys, buf ^= 1) {
+      if (k0 + kAttnKeys < keys) fetch(k0 + kAttnKeys, buf ^ 1);
+      if (k0 < keys_wave) {
+        const uint16_t* const lk_ = stage + buf * kStage;
+        const uint16_t* const lv = lk_ + kAttnKeys * DQ;
+        f32x16_t s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
 #pragma unroll
         for (int i = 0; i < kQSteps; ++i)
-          s[t] = mfma32<BF16>(*reinterpret_cast<const u32x4_t*>(lk_ + (32 * t + n) * kKStride +
-                                                               16 * i + 8 * half),
-                              qf[i], s[t]);
-      }
-      // a query of the wave does not see all of these keys
-      const bool edge = k0 + kAttnKeys - 1 > q0 + wave * 32 + ahead;
-      // register r of tile t: key k0 + 32 t + 8 (r / 4) + 4 half + r % 4
-      float top = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < 2; ++t) {
+            const int r = 32 * t + n;
+            const int c = (2 * i + half) ^ key_swizzle<kKChunks>(r);
+            s[t] = mfma32<BF16>(*reinterpret_cast<const u32x4_t*>(lk_ + r * DQ + 8 * c), qf[i], s[t]);
+          }
+        // register r of tile t: key k0 + 32 t + 8 (r / 4) + 4 half + r % 4. What a
+        // query does not see is left out of its maximum and gets p = 0, which
+        // an infinity or a NaN in V would turn into one of its own: such values
+        // are taken out of the product there and added at the end, for the
+        // queries that see them.
+        const bool edge = k0 + kAttnKeys - 1 > qw + ahead;  // a query does not see all of them
+        const int seen = static_cast<int>(qi + ahead - k0 < kAttnKeys ? qi + ahead - k0 + 1 : kAttnKeys);
+        if (edge) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int64_t key = k0 + 32 * t + 8 * (r / 4) + 4 * half + r % 4;
-          s[t][r] = key > qi + ahead ? -INFINITY : s[t][r] * a.scale_log2;
-          top = fmaxf(top, s[t][r]);
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (32 * t + 8 * (r / 4) + 4 * half + r % 4 >= seen) s[t][r] = -INFINITY;
         }
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float mn = fmaxf(m, top);
-      const float base = mn == -INFINITY ? 0.f : mn;
-      const float fade = __builtin_amdgcn_exp2f(m - base);
-      m = mn;
-      float part = 0.f;
+        float most = s[0][0];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[t][r] = __builtin_amdgcn_exp2f(s[t][r] - base);
-          part += s[t][r];
+          for (int r = 0; r < 16; ++r) most = fmaxf(most, s[t][r]);
+        most = fmaxf(most, __shfl_xor(most, 32)) * a.scale_log2;
+        // the maximum only moves when it has grown by more than 2^kSlack: p stays
+        // below that, and most passes leave the accumulators alone
+        constexpr float kSlack = 8.f;
+        if (__any(most > top + kSlack || (top == -INFINITY && most > top))) {
+          const float next = fmaxf(top, most);
+          const float fade = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
+          top = next;
+          sum *= fade;
+#pragma unroll
+          for (int t = 0; t < kVTiles; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[t][r] *= fade;
         }
-      sum = sum * fade + part;
+        const float base = kLift - (top == -INFINITY ? 0.f : top);
+        float part[2] = {0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < kVTiles; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[t][r] *= fade;
-      // k-slots of MFMA step i: keys 16 i + 4 half + {0..3} and + 8
+          for (int r = 0; r < 16; ++r) {
+            s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2, base));
+            part[t] += s[t][r];
+          }
+        sum += part[0] + part[1];
+        // k-slots of MFMA step i: keys 16 i + 4 half + {0..3} and + 8
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = i / 2, r = 8 * (i & 1);
-        const u32x4_t p = {pack2<BF16>(s[t][r], s[t][r + 1]), pack2<BF16>(s[t][r + 2], s[t][r + 3]),
-                           pack2<BF16>(s[t][r + 4], s[t][r + 5]),
-                           pack2<BF16>(s[t][r + 6], s[t][r + 7])};
+        for (int i = 0; i < 4; ++i) {
+          const int t = i / 2, r = 8 * (i & 1);
+          const u32x4_t p = {pack2<BF16>(s[t][r], s[t][r + 1]), pack2<BF16>(s[t][r + 2], s[t][r + 3]),
+                             pack2<BF16>(s[t][r + 4], s[t][r + 5]),
+                             pack2<BF16>(s[t][r + 6], s[t][r + 7])};
 #pragma unroll
-        for (int vt = 0; vt < kVTiles; ++vt) {
-          const uint16_t* const vp = lvt + (32 * vt + n) * kVStride + 16 * i + 4 * half;
-          const uint2 lo = *reinterpret_cast<const uint2*>(vp);
-          const uint2 hi = *reinterpret_cast<const uint2*>(vp + 8);
-          const u32x4_t vf = {lo.x, lo.y, hi.x, hi.y};
-          if (__builtin_expect(edge && __any(any_nonfinite<BF16>(vf)), 0))
-            o[vt] = mfma_seen<BF16>(vf, p, o[vt], half, 16 * i, static_cast<int>(qi + ahead - k0 + 1));
-          else
+          for (int vt = 0; vt < kVTiles; ++vt) {
+            u32x4_t vf;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int row = 16 * i + 8 * x + vrow, col = 32 * vt + vcol;
+              const uint2 v = lds_read_transposed(
+                  lv + row * DV + 8 * ((col / 8) ^ value_swizzle<kVChunks>(row)) + col % 8);
+              vf[2 * x] = v.x;
+              vf[2 * x + 1] = v.y;
+            }
+            if (edge && __builtin_expect(__any(any_nonfinite<BF16>(vf)), 0)) {
+              bad = true;
+              vf = finite_only<BF16>(vf);
+            }
             o[vt] = mfma32<BF16>(vf, p, o[vt]);
+          }
         }
       }
+      wait_vmcnt<0>();  // the next tile has landed
+      __syncthreads();
     }
     sum += __shfl_xor(sum, 32);
+    if (__builtin_expect(bad, 0)) {
+      // the infinities and NaNs left out above, for the queries that see them
+      int64_t key = qw + ahead + 1 < 0 ? 0 : (qw + ahead + 1) / kAttnKeys * kAttnKeys;
+#pragma unroll 1
+      for (; key < keys_wave; ++key) {
+        const uint16_t* const row = vb + key * a.v_row;
+#pragma unroll
+        for (int t = 0; t < kVTiles; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int d = 32 * t + 8 * (r / 4) + 4 * half + r % 4;
+            const float x = d < a.d_v && key <= qi + ahead ? value_of<BF16>(row[d]) : 0.f;
+            if (x - x != 0.f) o[t][r] += x;
+          }
+      }
+    }
   }
-  if (qi >= lq) return;
-  const float inv = sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  // whole rows through the wave's share of LDS (every wave has left the loop)
+  constexpr int kOutStride = DV + 8;
+  static_assert(kAttnWaves * 32 * kOutStride <= 2 * kStage, "output tile in LDS");
+  uint16_t* const rows = stage + wave * 32 * kOutStride;
 #pragma unroll
   for (int t = 0; t < kVTiles; ++t)
 #pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int d = 32 * t + 8 * (r / 4) + 4 * half;
-      if (d < a.d_v)
-        *reinterpret_cast<uint2*>(orow + d) =
-            make_uint2(pack2<BF16>(o[t][r] * inv, o[t][r + 1] * inv),
-                       pack2<BF16>(o[t][r + 2] * inv, o[t][r + 3] * inv));
-    }
+    for (int r = 0; r < 16; r += 4)
+      *reinterpret_cast<uint2*>(rows + n * kOutStride + 32 * t + 8 * (r / 4) + 4 * half) =
+          make_uint2(pack2<BF16>(o[t][r] * inv, o[t][r + 1] * inv),
+                     pack2<BF16>(o[t][r + 2] * inv, o[t][r + 3] * inv));
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 32 * kVChunks / kWave; ++i) {
+    const int slot = i * kWave + lane, r = slot / kVChunks, d = slot % kVChunks * 8;
+    if (qw + r < lq && d < a.d_v)
+      *reinterpret_cast<u32x4_t*>(a.out + ((rq.begin + qw + r) * a.heads + h) * a.d_v + d) =
+          *reinterpret_cast<const u32x4_t*>(rows + r * kOutStride + d);
+  }
 }
 
 template <bool BF16>
@@ -295,6 +393,8 @@ int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
   LK_REQUIRE(q_row_stride >= 0 && q_head_stride >= 0 && k_row_stride >= 0 && k_head_stride >= 0 &&
                  v_row_stride >= 0 && v_head_stride >= 0,
              "attention strides must not be negative");
+  LK_REQUIRE(k_row_stride < (int64_t{1} << 24) && v_row_stride < (int64_t{1} << 24),
+             "attention row strides must be below 2^24 elements");
   LK_REQUIRE(scale == scale && scale - scale == 0.f, "the attention scale must be finite");
   if (rows_q == 0) return LK_OK;
   LK_REQUIRE(q && out && (rows_k == 0 || (k && v)), "null pointer argument");
@@ -320,7 +420,9 @@ int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
                    q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride,
                    v_head_stride,
                    sequence_tiles(rows_q, sequences, kAttnQueries),
-                   scale * 1.4426950408889634f};
+                   scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f,
+                   scale == 0.f ? 0u : 0xFFFFFFFFu,
+                   scale < 0.f ? 0x80008000u : 0u};
   const hipStream_t s = as_stream(stream);
   return dtype == LK_DTYPE_BF16 ? launch_attention<true>(a, s) : launch_attention<false>(a, s);
 }

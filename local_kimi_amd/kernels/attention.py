@@ -30,7 +30,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     16-byte steps."""
     fits = ((t.shape[3] == 1 or t.stride(3) == 1) and
             (t.shape[0] == 1 or t.stride(0) == t.shape[1] * t.stride(1)) and
-            t.stride(1) % 8 == 0 and t.stride(2) % 8 == 0 and t.data_ptr() % 16 == 0)
+            t.stride(1) % 8 == 0 and t.stride(2) % 8 == 0 and t.stride(1) < 1 << 24 and
+            t.data_ptr() % 16 == 0)
     return t if fits else t.clone(memory_format=torch.contiguous_format)
 
 
