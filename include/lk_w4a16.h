@@ -58,6 +58,7 @@ LK_API int lk_abi_version(void);
  *   "moe_fused_schedule" auto | off       (router + schedule in one launch)
  *   "moe_split_swiglu"   auto | off       (split gate/up units, SwiGLU in the
  *                                          down GEMM's staging)
+ *   "kda_prefill"        auto | steps | chunks (KDA recurrence of a prompt)
  * Process-wide; set it between calls, not while another thread launches.
  * lk_get_path returns the current choice's index (0 = auto), -1 for an
  * unknown knob. */

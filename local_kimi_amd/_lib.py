@@ -178,6 +178,7 @@ PATH_KNOBS: dict[str, tuple[str, ...]] = {
     "mxfp4_mfma": ("auto", "fp4", "bf16"),
     "moe_fused_schedule": ("auto", "off"),
     "moe_split_swiglu": ("auto", "off"),
+    "kda_prefill": ("auto", "steps", "chunks"),
 }
 
 

@@ -344,6 +344,384 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(ScanArgs a,
   }
 }
 
+// ---------------------------------------------------------------------------
+// The recurrence in chunks of 16 steps. Within a chunk with the state S before
+// it, D_i the product of e^g over its steps up to i (per key row) and D_(j,i] that
+// of the steps behind j up to i,
+//   A_ij = beta_j sum_d k_i k_j D_(j,i]   (j < i)
+//   P_ij = scale beta_j sum_d q_i k_j D_(j,i]   (j <= i)
+//   (I + A) [W | U0] = [k D | v]
+//   U = U0 - W S,   o = scale (q D) S + P U,   S = D_15 S + (beta k D_(.,15])^T U,
+// which is the step form with its corrections u solved for together. Only the
+// last line follows from chunk to chunk, so one launch computes W, U0, P and the
+// scaled rows of every chunk (chunk_prepare_kernel) and another takes the
+// states through them (chunk_scan_kernel), on fp32 matrix instructions: state and
+// sums keep fp32, as the step form has them.
+//
+// Decays are multiplied up, never divided or taken as differences of sums: every
+// product of e^g <= 1 stays in [0, 1] with a relative error of 2^-24 a factor,
+// whatever the decays (a sum of logs of 100 would carry 2^-17 of error into its
+// exponential, a quotient of products overflows where a channel fades within
+// the chunk). That fixes the chunk at 16 steps: A and P cost 120 + 136
+// products of every channel in VALU work, 41 us of a GPU at 8192 tokens x 32 heads
+// of 128, and a longer chunk would square that.
+//
+// Records. A chunk and head has one record in the workspace, its parts in the
+// order in which the second launch's lanes load them (16 bytes a lane, 1 KB a
+// wave): with m = lane % 16, g = lane / 16, r = 0..3,
+//   W, Q (scale q D):  [tile t][lane][r] = row m, channel 16 t + 4 g + r
+//   K (beta k D_(.,15]): [tile t][lane][r] = channel 16 t + m, step 4 g + r
+//   D (D_15):          [channel]
+//   P:                 [lane][r] = row m, column 4 g + r
+//   U0:                [tile t][lane][r] = value column 16 t + m, step 4 g + r
+// These are the A operands of v_mfma_f32_16x16x4 for B operands that are the
+// accumulators of an earlier one as they stand: lane (m, g) of a 16 x 16 result
+// holds column m, rows 4 g + r, and register r of it serves as the rows 4 g + r of a
+// product over 16.
+constexpr int kChunk = 16;
+constexpr int kChunkThreads = 256;
+
+struct ChunkArgs {
+  float* records;
+  int64_t first, count;  // chunk numbers of this window
+  int64_t record;        // floats of one record
+  int v_tiles;           // 16-column tiles of d_v
+};
+
+template <int RT>
+struct ChunkLayout {  // float offsets of a record's parts; 64 RT channels
+  static constexpr int kChannels = 64 * RT;
+  static constexpr int kW = 0, kQ = kChannels * kChunk, kK = 2 * kChannels * kChunk,
+                       kD = 3 * kChannels * kChunk, kP = kD + kChannels, kU = kP + 256;
+};
+
+// Four values of each lane of a quad, transposed: lane r gets value r of the four.
+__device__ inline void quad_transpose(float (&v)[4], int r) {
+  const bool odd = r & 1, high = r & 2;
+  float t0 = dpp_f32<kQuadXor1>(odd ? v[0] : v[1]), t1 = dpp_f32<kQuadXor1>(odd ? v[2] : v[3]);
+  const float a0 = odd ? t0 : v[0], a1 = odd ? v[1] : t0, a2 = odd ? t1 : v[2],
+              a3 = odd ? v[3] : t1;
+  t0 = dpp_f32<kQuadXor2>(high ? a0 : a2);
+  t1 = dpp_f32<kQuadXor2>(high ? a1 : a3);
+  v[0] = high ? t0 : a0;
+  v[1] = high ? t1 : a1;
+  v[2] = high ? a2 : t0;
+  v[3] = high ? a3 : t1;
+}
+
+// Sums of four values of each lane over the wave's four 16-lane rows: row g is left
+// with that of value (g & 1) + 2 (g >> 1), by two exchanges that each halve what a
+// lane still holds.
+__device__ inline float rows_reduce(const float (&v)[4]) {
+  float h[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]),
+                                                    __float_as_uint(v[i + 2]), false, false);
+    h[i] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(h[0]), __float_as_uint(h[1]),
+                                                  false, false);
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+
+// `at` again, as a value that is known only once x is: keeps the LDS reads at it
+// below x's computation. (The compiler otherwise moves the reads of all unrolled
+// rows to the front: 420 registers, one wave on a SIMD.)
+__device__ inline int after(int at, float x) {
+  asm volatile("" : "+v"(at) : "v"(x));
+  return at;
+}
+
+template <int DT, int RT>
+__global__ void __launch_bounds__(kChunkThreads, 4) chunk_prepare_kernel(ScanArgs a, ChunkArgs c) {
+  using T = typename Storage<DT>::type;
+  using L = ChunkLayout<RT>;
+  constexpr int kStride = L::kChannels + 4;  // rows 16 bytes apart in the banks
+  __shared__ alignas(16) float sq[kChunk][kStride], sk[kChunk][kStride], sg[kChunk][kStride];
+  __shared__ float part[2][4][kChunk * kChunk];
+  __shared__ alignas(16) float sa[kChunk][kChunk];
+  __shared__ float sb[kChunk];
+  const int h = static_cast<int>(blockIdx.x % a.heads);
+  const int64_t local = blockIdx.x / a.heads;
+  const SequenceTile at = find_sequence_tile(a.seq, c.first + local, kChunk);
+  if (at.sequence == a.seq.count) return;
+  const RowRange rows = sequence_rows(a.seq, at.sequence);
+  const int64_t t0 = rows.begin + at.tile * kChunk;
+  if (t0 >= rows.end) return;
+  const int tid = threadIdx.x, i16 = tid >> 4, l = tid & 15;
+  const int wave = tid / kWave, lane = tid & (kWave - 1);
+
+  {  // steps behind the sequence's end: no decay, no key, no query
+    const int64_t t = t0 + i16;
+    const bool ok = t < rows.end;
+    const int64_t base = ((ok ? t : t0) * a.heads + h) * a.d_k;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      float q[4], k[4], g[4];
+      const int d = 4 * (l + 16 * i);
+      load_rows<4>(a.q + base, d, a.d_k, ok, q);
+      load_rows<4>(a.k + base, d, a.d_k, ok, k);
+      load_rows<4>(a.decay + base, d, a.d_k, ok, g);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) g[x] = expf(g[x]);
+      *reinterpret_cast<float4*>(&sq[i16][d]) = make_float4(q[0], q[1], q[2], q[3]);
+      *reinterpret_cast<float4*>(&sk[i16][d]) = make_float4(k[0], k[1], k[2], k[3]);
+      *reinterpret_cast<float4*>(&sg[i16][d]) = make_float4(g[0], g[1], g[2], g[3]);
+    }
+    if (l == 0) sb[i16] = ok ? a.beta[t * a.heads + h] : 0.f;
+  }
+  __syncthreads();
+
+  // A and P: lane (j, g) of wave w has key j against every row i >= j, over a
+  // 16th of the channels; its product of decays runs along with i. Rows i < j
+  // are dropped below.
+  {
+    const float beta = sb[l];
+    const int g = lane >> 4, d0 = wave * 16 * RT + g * 4 * RT;
+    float4 f[RT];
+#pragma unroll 1
+    for (int i0 = 0; i0 < kChunk; i0 += 4) {  // four rows at a time
+      float kk[4] = {0.f, 0.f, 0.f, 0.f}, qk[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < RT; ++x) {
+        const int d = d0 + 4 * x;
+        const float4 own = *reinterpret_cast<const float4*>(&sk[l][d]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 e = *reinterpret_cast<const float4*>(&sg[i0 + i][d]);
+          const float4 k = *reinterpret_cast<const float4*>(&sk[i0 + i][d]);
+          const float4 q = *reinterpret_cast<const float4*>(&sq[i0 + i][d]);
+          const bool first = i0 + i <= l;
+          f[x].x = first ? own.x * beta : f[x].x * e.x;
+          f[x].y = first ? own.y * beta : f[x].y * e.y;
+          f[x].z = first ? own.z * beta : f[x].z * e.z;
+          f[x].w = first ? own.w * beta : f[x].w * e.w;
+          kk[i] = fmaf(k.x, f[x].x, fmaf(k.y, f[x].y, fmaf(k.z, f[x].z, fmaf(k.w, f[x].w, kk[i]))));
+          qk[i] = fmaf(q.x, f[x].x, fmaf(q.y, f[x].y, fmaf(q.z, f[x].z, fmaf(q.w, f[x].w, qk[i]))));
+        }
+      }
+      const int i = i0 + (g & 1) + 2 * (g >> 1);
+      part[0][wave][i * 16 + l] = rows_reduce(kk);
+      part[1][wave][i * 16 + l] = rows_reduce(qk);
+    }
+  }
+  __syncthreads();
+  float* const rec = c.records + (local * a.heads + h) * c.record;
+  {
+    const float kk = (part[0][0][tid] + part[0][1][tid]) + (part[0][2][tid] + part[0][3][tid]);
+    const float qk = (part[1][0][tid] + part[1][1][tid]) + (part[1][2][tid] + part[1][3][tid]);
+    sa[i16][l] = l < i16 ? kk : 0.f;
+    rec[L::kP + (i16 + 16 * (l >> 2)) * 4 + (l & 3)] = l <= i16 ? a.scale * qk : 0.f;
+  }
+  __syncthreads();
+
+  // columns of [W | U0]: one thread solves a column, row by row
+  const int columns = L::kChannels + 16 * c.v_tiles;
+  for (int col = tid; col < columns; col += kChunkThreads) {
+    float x[kChunk];
+    const bool key = col < L::kChannels;  // uniform in each wave: 64 channels apart
+    const int vc = col - L::kChannels;
+    if (key) {
+      float keep = 1.f;
+      float q[kChunk];
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        keep *= sg[i][col];
+        x[i] = sk[i][col] * keep;
+        q[i] = sq[i][col] * (a.scale * keep);
+      }
+      const int t = col >> 4, g = (col >> 2) & 3, r = col & 3;
+#pragma unroll
+      for (int m = 0; m < kChunk; m += 4) {
+        float y[4] = {q[m], q[m + 1], q[m + 2], q[m + 3]};
+        quad_transpose(y, r);
+        *reinterpret_cast<float4*>(rec + L::kQ + (t * 64 + m + r + 16 * g) * 4) =
+            make_float4(y[0], y[1], y[2], y[3]);
+      }
+      float left = 1.f, kept[kChunk];
+#pragma unroll
+      for (int j = kChunk - 1; j >= 0; --j) {
+        kept[j] = sb[j] * sk[j][col] * left;
+        left *= sg[j][col];
+      }
+#pragma unroll
+      for (int m = 0; m < kChunk; m += 4)
+        *reinterpret_cast<float4*>(rec + L::kK + (t * 64 + (col & 15) + 4 * m) * 4) =
+            make_float4(kept[m], kept[m + 1], kept[m + 2], kept[m + 3]);
+      rec[L::kD + col] = keep;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i)
+        x[i] = t0 + i < rows.end && vc < a.d_v
+                   ? to_f32<DT>(static_cast<const T*>(a.v)[((t0 + i) * a.heads + h) * a.d_v + vc])
+                   : 0.f;
+    }
+#pragma unroll
+    for (int i = 1; i < kChunk; ++i) {
+      const int at0 = i < 4 ? 0 : after(0, x[i - 4]);  // three rows of A ahead
+#pragma unroll
+      for (int j = 0; j < i; j += 4) {
+        const float4 r = *reinterpret_cast<const float4*>(&sa[i][4 * at0 + j]);
+        const float rj[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (j + y < i) x[i] = fmaf(-rj[y], x[j + y], x[i]);
+      }
+    }
+    if (key) {
+      const int t = col >> 4, g = (col >> 2) & 3, r = col & 3;
+#pragma unroll
+      for (int m = 0; m < kChunk; m += 4) {
+        float y[4] = {x[m], x[m + 1], x[m + 2], x[m + 3]};
+        quad_transpose(y, r);
+        *reinterpret_cast<float4*>(rec + L::kW + (t * 64 + m + r + 16 * g) * 4) =
+            make_float4(y[0], y[1], y[2], y[3]);
+      }
+    } else {
+#pragma unroll
+      for (int m = 0; m < kChunk; m += 4)
+        *reinterpret_cast<float4*>(rec + L::kU + ((vc >> 4) * 64 + (vc & 15) + 4 * m) * 4) =
+            make_float4(x[m], x[m + 1], x[m + 2], x[m + 3]);
+    }
+  }
+}
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+// Block = one sequence's and head's 16 value columns, through the chunks of the
+// window. Each of the four waves keeps 16 RT key rows of the state as accumulators;
+// the sums over all rows (W S and Q S) meet in LDS once a chunk, in wave order.
+// The next chunk's record is in flight meanwhile.
+template <int DT, int RT>
+__global__ void __launch_bounds__(kChunkThreads) chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
+  using T = typename Storage<DT>::type;
+  using L = ChunkLayout<RT>;
+  __shared__ f32x4_t parts[2][2][4][kWave];
+  const int ct = static_cast<int>(blockIdx.x % c.v_tiles);
+  const int64_t sh = blockIdx.x / c.v_tiles;
+  const int h = static_cast<int>(sh % a.heads);
+  const int s = static_cast<int>(sh / a.heads);
+  const RowRange rows = sequence_rows(a.seq, s);
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int m = lane & 15, g = lane >> 4;
+  const int col = ct * 16 + m;
+  if (s == a.seq.count) {  // rows behind the last sequence
+    if (c.first == 0)
+      for (int64_t t = rows.begin + (tid >> 4); t < rows.end; t += 16)
+        if (ct * 16 + (tid & 15) < a.d_v)
+          static_cast<T*>(a.out)[(t * a.heads + h) * a.d_v + ct * 16 + (tid & 15)] = 0;
+    return;
+  }
+  // the sequence's chunk numbers, at least one, and those of the window
+  const int64_t number = rows.begin / kChunk + s;
+  const int64_t chunks = (rows.end - rows.begin + kChunk - 1) / kChunk;
+  const int64_t end_all = number + (chunks > 0 ? chunks : 1);
+  const int64_t lo = number > c.first ? number : c.first;
+  const int64_t hi = end_all < c.first + c.count ? end_all : c.first + c.count;
+  if (lo >= hi) return;
+  const float* const src = lo == number ? a.state : a.state_out;
+  const int64_t sbase = sh * a.d_k * a.d_v;
+  f32x4_t st[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * (wave * RT + t) + 4 * g + r;
+      st[t][r] = row < a.d_k && col < a.d_v ? src[sbase + static_cast<int64_t>(row) * a.d_v + col] : 0.f;
+    }
+
+  struct Record {
+    f32x4_t w[RT], q[RT], k[RT], d[RT], u, p;
+  };
+  auto fetch = [&](int64_t chunk, Record& f) {
+    const float* const rec = c.records + ((chunk - c.first) * a.heads + h) * c.record;
+    const f32x4_t* const v4 = reinterpret_cast<const f32x4_t*>(rec);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int tile = wave * RT + t;
+      f.w[t] = v4[L::kW / 4 + tile * 64 + lane];
+      f.q[t] = v4[L::kQ / 4 + tile * 64 + lane];
+      f.k[t] = v4[L::kK / 4 + tile * 64 + lane];
+      f.d[t] = v4[L::kD / 4 + tile * 4 + g];
+    }
+    f.u = v4[L::kU / 4 + ct * 64 + lane];
+    f.p = v4[L::kP / 4 + lane];
+  };
+  if (chunks > 0) {
+    Record cur, next;
+    fetch(lo, cur);
+    for (int64_t ch = lo; ch < hi; ++ch) {
+      if (ch + 1 < hi) fetch(ch + 1, next);
+      const int buf = static_cast<int>(ch & 1);
+      f32x4_t x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.w[t][r], st[t][r], x, 0, 0, 0);
+      parts[buf][0][wave][lane] = x;
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          y = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.q[t][r], st[t][r], y, 0, 0, 0);
+      parts[buf][1][wave][lane] = y;
+      __syncthreads();
+      const f32x4_t u = cur.u - ((parts[buf][0][0][lane] + parts[buf][0][1][lane]) +
+                                 (parts[buf][0][2][lane] + parts[buf][0][3][lane]));
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        st[t] *= cur.d[t];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.k[t][r], u[r], st[t], 0, 0, 0);
+      }
+      if (wave == (ch & 3)) {
+        f32x4_t o = (parts[buf][1][0][lane] + parts[buf][1][1][lane]) +
+                    (parts[buf][1][2][lane] + parts[buf][1][3][lane]);
+        f32x4_t past;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) past[r] = u[r] - u[r] == 0.f ? u[r] : 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          o = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.p[r], past[r], o, 0, 0, 0);
+        const bool fine = (u[0] - u[0]) + (u[1] - u[1]) + (u[2] - u[2]) + (u[3] - u[3]) == 0.f;
+        if (__builtin_expect(!__all(fine), 0)) {
+          // infinities and NaNs, which P's zeros would hand to the steps
+          // before their own: the steps from theirs on take them one by one
+          const float* const rec = c.records + ((ch - c.first) * a.heads + h) * c.record;
+#pragma unroll 1
+          for (int j = 0; j < kChunk; ++j) {
+            const float mine = (j & 2) ? ((j & 1) ? u[3] : u[2]) : ((j & 1) ? u[1] : u[0]);
+            const float uj = __shfl(mine, m + 16 * (j >> 2));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float pij = rec[L::kP + ((4 * g + r) + 16 * (j >> 2)) * 4 + (j & 3)];
+              if (j <= 4 * g + r && uj - uj != 0.f) o[r] = fmaf(pij, uj, o[r]);
+            }
+          }
+        }
+        const int64_t t0 = rows.begin + (ch - number) * kChunk + 4 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (t0 + r < rows.end && col < a.d_v)
+            static_cast<T*>(a.out)[((t0 + r) * a.heads + h) * a.d_v + col] = from_f32<DT>(o[r]);
+      }
+      cur = next;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * (wave * RT + t) + 4 * g + r;
+      if (row < a.d_k && col < a.d_v)
+        a.state_out[sbase + static_cast<int64_t>(row) * a.d_v + col] = st[t][r];
+    }
+}
+
 bool known_dtype(int d) { return d == LK_DTYPE_F32 || d == LK_DTYPE_F16 || d == LK_DTYPE_BF16; }
 bool aligned(const void* p, int64_t bytes) {
   return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0;
@@ -389,6 +767,56 @@ int launch_serial(const ScanArgs& a, hipStream_t s) {
   else
     scan_serial_kernel<DT, 16><<<grid, kSerialThreads, 0, s>>>(a, cb);
   return check_launch("lk_kda_prefill");
+}
+
+// Floats of a chunk's and head's record.
+int64_t chunk_record(int64_t d_k, int64_t d_v) {
+  const int64_t channels = d_k <= 64 ? 64 : 128;
+  return channels * (3 * kChunk + 1) + 256 + (d_v + 15) / 16 * 16 * kChunk;
+}
+
+// Chunks of one window: the records of a window are written by one launch and
+// read by the next, so they are kept within the 256 MB cache in front of HBM.
+constexpr int64_t kWindowBytes = int64_t{128} << 20;
+int64_t chunk_window(int64_t chunks, int64_t heads, int64_t record) {
+  const int64_t most = kWindowBytes / (heads * record * 4);
+  const int64_t w = most < 1 ? 1 : most;
+  return w < chunks ? w : chunks;
+}
+
+bool takes_chunks(int64_t sequences, int64_t tokens, int64_t d_k) {
+  const int choice = path_choice(kKnobKdaPrefill);
+  if (d_k > 128 || tokens == 0 || choice == 1) return false;
+  return choice == 2 || tokens >= 32 * sequences;
+}
+
+template <int DT, int RT>
+int launch_chunks(const ScanArgs& a, float* records, hipStream_t s) {
+  ChunkArgs c;
+  c.records = records;
+  c.record = chunk_record(a.d_k, a.d_v);
+  c.v_tiles = (a.d_v + 15) / 16;
+  const int64_t chunks = sequence_tiles(a.seq.rows, a.seq.count, kChunk);
+  const int64_t window = chunk_window(chunks, a.heads, c.record);
+  const int64_t scans = (a.seq.count + 1) * static_cast<int64_t>(a.heads) * c.v_tiles;
+  LK_REQUIRE(window * a.heads < (int64_t{1} << 31) && scans < (int64_t{1} << 31),
+             "too many sequences x heads for one call");
+  for (c.first = 0; c.first < chunks; c.first += window) {
+    c.count = window < chunks - c.first ? window : chunks - c.first;
+    chunk_prepare_kernel<DT, RT>
+        <<<static_cast<unsigned>(c.count * a.heads), kChunkThreads, 0, s>>>(a, c);
+    if (const int st = check_launch("lk_kda_prefill")) return st;
+    chunk_scan_kernel<DT, RT><<<static_cast<unsigned>(scans), kChunkThreads, 0, s>>>(a, c);
+    if (const int st = check_launch("lk_kda_prefill")) return st;
+  }
+  return LK_OK;
+}
+
+template <int DT>
+int launch_scan(const ScanArgs& a, bool chunks, void* workspace, hipStream_t s) {
+  if (!chunks) return launch_serial<DT>(a, s);
+  float* const records = static_cast<float*>(workspace);
+  return a.d_k <= 64 ? launch_chunks<DT, 1>(a, records, s) : launch_chunks<DT, 2>(a, records, s);
 }
 
 }  // namespace
@@ -442,7 +870,9 @@ int lk_kda_short_conv_prefill(const void* q_in, const void* k_in, const void* v_
 int64_t lk_kda_prefill_workspace(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k,
                                  int64_t d_v) {
   if (sequences <= 0 || tokens < 0 || heads <= 0 || d_k <= 0 || d_v <= 0 || d_k > 256) return -1;
-  return 0;
+  if (!takes_chunks(sequences, tokens, d_k)) return 0;
+  const int64_t record = chunk_record(d_k, d_v);
+  return chunk_window(sequence_tiles(tokens, sequences, kChunk), heads, record) * heads * record * 4;
 }
 
 int lk_kda_prefill(const float* state, float* state_out, const float* q, const float* k,
@@ -468,10 +898,12 @@ int lk_kda_prefill(const float* state, float* state_out, const float* q, const f
   const ScanArgs a{state, state_out, q, k, v, decay, beta, out,
                    Sequences{cu_seqlens, tokens, tokens / sequences, static_cast<int>(sequences)},
                    static_cast<int>(heads), static_cast<int>(d_k), static_cast<int>(d_v), scale};
+  LK_REQUIRE(aligned(workspace, 16), "KDA prefill workspace must be 16-byte aligned");
   const hipStream_t s = as_stream(stream);
-  if (value_dtype == LK_DTYPE_F32) return launch_serial<LK_DTYPE_F32>(a, s);
-  if (value_dtype == LK_DTYPE_F16) return launch_serial<LK_DTYPE_F16>(a, s);
-  return launch_serial<LK_DTYPE_BF16>(a, s);
+  const bool chunks = takes_chunks(sequences, tokens, d_k);
+  if (value_dtype == LK_DTYPE_F32) return launch_scan<LK_DTYPE_F32>(a, chunks, workspace, s);
+  if (value_dtype == LK_DTYPE_F16) return launch_scan<LK_DTYPE_F16>(a, chunks, workspace, s);
+  return launch_scan<LK_DTYPE_BF16>(a, chunks, workspace, s);
 }
 
 }  // extern "C"

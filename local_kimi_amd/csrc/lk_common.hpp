@@ -30,6 +30,7 @@ enum Knob : int {
   kKnobMxfp4Mfma,         // 0 auto, 1 fp4, 2 bf16
   kKnobMoeFusedSchedule,  // 0 auto, 1 off
   kKnobMoeSplitSwiglu,    // 0 auto, 1 off
+  kKnobKdaPrefill,        // 0 auto, 1 steps, 2 chunks
   kKnobCount
 };
 int path_choice(Knob knob);

@@ -58,6 +58,7 @@ constexpr KnobSpec kKnobs[kKnobCount] = {
     {"mxfp4_mfma", {"auto", "fp4", "bf16", nullptr}},
     {"moe_fused_schedule", {"auto", "off", nullptr, nullptr}},
     {"moe_split_swiglu", {"auto", "off", nullptr, nullptr}},
+    {"kda_prefill", {"auto", "steps", "chunks", nullptr}},
 };
 
 std::atomic<int> g_knobs[kKnobCount];  // zero-initialised: "auto"

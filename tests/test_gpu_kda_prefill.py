@@ -164,6 +164,15 @@ def test_conv_keeps_infinities_in_their_own_sequence(rng):
 # recurrence
 
 
+@pytest.fixture(params=["steps", "chunks"])
+def form(request):
+    """Both forms of the recurrence (d_k above 128 takes steps either way)."""
+    from local_kimi_amd import _lib
+
+    with _lib.forced_path("kda_prefill", request.param):
+        yield request.param
+
+
 def _scan_inputs(rng, rows, h, dk, dv, n, dtype=torch.float32, rate=0.1):
     def unit(shape):
         a = rng.normal(size=shape)
@@ -207,7 +216,7 @@ def _run_scan(a, cu, dtype, scale, **kw):
     ([16, 15, 1, 0, 33], 2, 32, 40), ([70], 2, 72, 30), ([40], 1, 5, 3), ([21, 50], 1, 200, 24),
     ([90], 1, 100, 1), ([300], 2, 128, 64)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_scan_matches_oracle(rng, lengths, h, dk, dv, dtype):
+def test_scan_matches_oracle(rng, form, lengths, h, dk, dv, dtype):
     cu, n, rows = _cu(lengths), len(lengths), sum(lengths) + 3
     a = _scan_inputs(rng, rows, h, dk, dv, n, dtype)
     want_state, want = K.prefill(*a, dk ** -0.5, cu)
@@ -221,7 +230,7 @@ def test_scan_matches_oracle(rng, lengths, h, dk, dv, dtype):
 
 
 @pytest.mark.parametrize("rate", [0.0, 1e-4, 3.0, 40.0, 1e4])
-def test_scan_decays_from_none_to_at_once(rng, rate):
+def test_scan_decays_from_none_to_at_once(rng, form, rate):
     """No decay at all, the usual ones, and ones whose running sums pass what
     an exponential can hold within a few tokens; some channels keep while others fade."""
     cu = _cu([150, 40])
@@ -233,7 +242,7 @@ def test_scan_decays_from_none_to_at_once(rng, rate):
     _close(st, want_state, 150, torch.float32, f"state {rate}")
 
 
-def test_scan_infinite_decay_clears_a_channel(rng):
+def test_scan_infinite_decay_clears_a_channel(rng, form):
     """decay = -inf: the channel's row is forgotten (e^-inf = 0)."""
     cu = _cu([100])
     a = _scan_inputs(rng, 100, 1, 64, 32, 1)
@@ -246,7 +255,7 @@ def test_scan_infinite_decay_clears_a_channel(rng):
 
 
 @pytest.mark.parametrize("beta", [0.0, 1.0])
-def test_scan_equal_keys_and_beta_at_its_ends(rng, beta):
+def test_scan_equal_keys_and_beta_at_its_ends(rng, form, beta):
     """One key for every token: beta = 1 replaces what it holds each step, beta
     = 0 never writes."""
     cu = _cu([140])
@@ -259,7 +268,7 @@ def test_scan_equal_keys_and_beta_at_its_ends(rng, beta):
     _close(st, want_state, 140, torch.float32, "state")
 
 
-def test_scan_keeps_nan_in_its_own_sequence(rng):
+def test_scan_keeps_nan_in_its_own_sequence(rng, form):
     cu = _cu([70, 20, 75])
     a = _scan_inputs(rng, 165, 2, 128, 64, 3)
     clean, st = _run_scan(a, cu, torch.float32, 1.0)
@@ -272,7 +281,7 @@ def test_scan_keeps_nan_in_its_own_sequence(rng):
     assert torch.isnan(dirty[70:90]).any()
 
 
-def test_scan_is_causal_and_splits_into_pieces(rng):
+def test_scan_is_causal_and_splits_into_pieces(rng, form):
     """A prompt in two pieces, the second from the first's state, and a later
     token's change leaving earlier outputs as they were."""
     from local_kimi_amd.kernels import kda_prefill
@@ -292,7 +301,7 @@ def test_scan_is_causal_and_splits_into_pieces(rng):
     assert torch.equal(whole[:, :150], later[:, :150])
 
 
-def test_scan_state_out_strided_state_and_batches(rng):
+def test_scan_state_out_strided_state_and_batches(rng, form):
     from local_kimi_amd.kernels import kda_prefill
 
     b, s, h, d = 3, 40, 2, 64
@@ -312,7 +321,7 @@ def test_scan_state_out_strided_state_and_batches(rng):
     assert torch.equal(again, out) and torch.equal(view, new) and not wide[..., 1::2].any()
 
 
-def test_scan_offsets_outside_the_rows_are_clamped(rng):
+def test_scan_offsets_outside_the_rows_are_clamped(rng, form):
     """Offsets beyond the rows, decreasing ones and int64 ones."""
     from local_kimi_amd.kernels import kda_prefill
 
@@ -356,7 +365,7 @@ def _prompt(d, conv, state, piece, h, dim, cu=None):
                        cu_seqlens=cu)
 
 
-def test_a_prompt_then_decode_tokens_equals_decoding_all_along(rng):
+def test_a_prompt_then_decode_tokens_equals_decoding_all_along(rng, form):
     """Convolutions, gates and recurrence over a prompt, then single tokens
     from the states they leave, against the one-launch decode layer token by
     token. bf16 convolution outputs may round apart (an ulp, near ties), which moves
@@ -388,7 +397,7 @@ def test_a_prompt_then_decode_tokens_equals_decoding_all_along(rng):
         assert torch.linalg.norm(x - y) <= 2.0 ** -8 * torch.linalg.norm(y)
 
 
-def test_graph_replays_match_eager(rng):
+def test_graph_replays_match_eager(rng, form):
     """The prompt chain captured once, on padded rows with the offsets in a
     static buffer, replayed for other offsets."""
     h, dim, rows = 4, 64, 150
@@ -422,7 +431,7 @@ def test_graph_replays_match_eager(rng):
         assert torch.equal(got, want) and torch.equal(got_state, state), lengths
 
 
-def test_calls_on_another_stream(rng):
+def test_calls_on_another_stream(rng, form):
     a = _scan_inputs(rng, 120, 2, 128, 128, 1)
     cu = _cu([120])
     want, want_state = _run_scan(a, cu, torch.float32, 1.0)
