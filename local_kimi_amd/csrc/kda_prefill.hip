@@ -434,7 +434,7 @@ __device__ inline int after(int at, float x) {
 }
 
 template <int DT, int RT>
-__global__ void __launch_bounds__(kChunkThreads, 4) chunk_prepare_kernel(ScanArgs a, ChunkArgs c) {
+__global__ void __launch_bounds__(kChunkThreads, 3) chunk_prepare_kernel(ScanArgs a, ChunkArgs c) {
   using T = typename Storage<DT>::type;
   using L = ChunkLayout<RT>;
   constexpr int kStride = L::kChannels + 4;  // rows 16 bytes apart in the banks
@@ -452,6 +452,16 @@ __global__ void __launch_bounds__(kChunkThreads, 4) chunk_prepare_kernel(ScanArg
   const int tid = threadIdx.x, i16 = tid >> 4, l = tid & 15;
   const int wave = tid / kWave, lane = tid & (kWave - 1);
 
+  // this thread's first value column (threads behind those of the channels)
+  float v_first[kChunk];
+  {
+    const int vc = tid - L::kChannels;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+      v_first[i] = vc >= 0 && t0 + i < rows.end && vc < a.d_v
+                       ? to_f32<DT>(static_cast<const T*>(a.v)[((t0 + i) * a.heads + h) * a.d_v + vc])
+                       : 0.f;
+  }
   {  // steps behind the sequence's end: no decay, no key, no query
     const int64_t t = t0 + i16;
     const bool ok = t < rows.end;
@@ -550,6 +560,9 @@ __global__ void __launch_bounds__(kChunkThreads, 4) chunk_prepare_kernel(ScanArg
         *reinterpret_cast<float4*>(rec + L::kK + (t * 64 + (col & 15) + 4 * m) * 4) =
             make_float4(kept[m], kept[m + 1], kept[m + 2], kept[m + 3]);
       rec[L::kD + col] = keep;
+    } else if (col == tid) {
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) x[i] = v_first[i];
     } else {
 #pragma unroll
       for (int i = 0; i < kChunk; ++i)
@@ -590,18 +603,37 @@ __global__ void __launch_bounds__(kChunkThreads, 4) chunk_prepare_kernel(ScanArg
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 // Block = one sequence's and head's 16 value columns, through the chunks of the
-// window. Each of the four waves keeps 16 RT key rows of the state as accumulators;
-// the sums over all rows (W S and Q S) meet in LDS once a chunk, in wave order.
-// The next chunk's record is in flight meanwhile.
+// window. Each of four waves keeps 16 RT key rows of the state as accumulators; the
+// sums over all rows (W S - U0, Q S + P U) meet in LDS, in wave order, with one
+// barrier a chunk: W S before it, Q S behind it, where it covers the wait for the
+// other waves' sums, and each wave's quarter of P U at the end. A fifth wave does
+// what is off the path from one state to the next: it brings U0 and the decays,
+// sums and stores the outputs a chunk later.
+//
+// 24 of a record's 27 KB are loaded as operands, 16 cycles of the CU's address
+// unit for each 1 KB, against 25 matrix instructions of 32 cycles on each SIMD.
+// The four waves meet at the barrier, so their loads come at the same time: they
+// are spread over the step, a third behind each of its three products (in one
+// place they held the waves up for 500 cycles of 1900), two chunks ahead, and
+// without a branch (the last record again at the end), so that a wait leaves the
+// younger ones in flight.
+constexpr int kScanWaves = 5;
+
 template <int DT, int RT>
-__global__ void __launch_bounds__(kChunkThreads) chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
+__global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
   using T = typename Storage<DT>::type;
   using L = ChunkLayout<RT>;
-  __shared__ f32x4_t parts[2][2][4][kWave];
-  const int ct = static_cast<int>(blockIdx.x % c.v_tiles);
-  const int64_t sh = blockIdx.x / c.v_tiles;
+  // of the last two chunks: the waves' W S, - U0, the waves' outputs, U; D
+  __shared__ f32x4_t parts[2][10][kWave];
+  __shared__ f32x4_t decay[2][4 * 4 * RT];
+  // the column tiles of a head, which read the same records, lie 8 blocks apart:
+  // on one XCD, whose cache then holds a record for all of them
+  const int64_t span = 8 * c.v_tiles, at = blockIdx.x % span;
+  const int64_t sh = blockIdx.x / span * 8 + at % 8;
+  const int ct = static_cast<int>(at / 8);
   const int h = static_cast<int>(sh % a.heads);
   const int s = static_cast<int>(sh / a.heads);
+  if (s > a.seq.count) return;
   const RowRange rows = sequence_rows(a.seq, s);
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -609,9 +641,8 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_scan_kernel(ScanArgs a, C
   const int col = ct * 16 + m;
   if (s == a.seq.count) {  // rows behind the last sequence
     if (c.first == 0)
-      for (int64_t t = rows.begin + (tid >> 4); t < rows.end; t += 16)
-        if (ct * 16 + (tid & 15) < a.d_v)
-          static_cast<T*>(a.out)[(t * a.heads + h) * a.d_v + ct * 16 + (tid & 15)] = 0;
+      for (int64_t t = rows.begin + (tid >> 4); t < rows.end; t += kScanWaves * 4)
+        if (col < a.d_v) static_cast<T*>(a.out)[(t * a.heads + h) * a.d_v + col] = 0;
     return;
   }
   // the sequence's chunk numbers, at least one, and those of the window
@@ -621,6 +652,97 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_scan_kernel(ScanArgs a, C
   const int64_t lo = number > c.first ? number : c.first;
   const int64_t hi = end_all < c.first + c.count ? end_all : c.first + c.count;
   if (lo >= hi) return;
+  const int steps = chunks > 0 ? static_cast<int>(hi - lo) : 0;
+  const int64_t stride = static_cast<int64_t>(a.heads) * c.record;  // a chunk's record to the next
+  const float* const first = c.records + ((lo - c.first) * a.heads + h) * c.record;
+  const float* const last = first + (hi - lo - 1) * stride;
+  auto advance = [&](const float* rec) { return rec < last ? rec + stride : last; };
+
+  if (wave == kScanWaves - 1) {
+    if (steps == 0) return;
+    const uint32_t values = static_cast<uint32_t>(L::kU + (ct * 64 + lane) * 4);
+    const uint32_t decays = static_cast<uint32_t>(L::kD + lane * RT);
+    typedef float row_t __attribute__((ext_vector_type(RT)));  // channels RT lane, ...
+    const float* ahead = first;
+    f32x4_t u0, u1, u2;
+    row_t d0, d1, d2;
+    auto fetch = [&](f32x4_t& u, row_t& d) {
+      u = *reinterpret_cast<const f32x4_t*>(ahead + values);
+      d = *reinterpret_cast<const row_t*>(ahead + decays);
+      ahead = advance(ahead);
+    };
+    auto hand_over = [&](int i, f32x4_t u, row_t d) {
+      parts[i & 1][4][lane] = -u;
+      reinterpret_cast<row_t*>(decay[i & 1])[lane] = d;
+    };
+    // rows behind the sequence and columns behind the last go past the buffer's
+    // end: stores without a branch, which the compiler can count
+    const int64_t row_values = static_cast<int64_t>(a.heads) * a.d_v;
+    T* out = static_cast<T*>(a.out) + (rows.begin + (lo - number) * kChunk) * row_values + h * a.d_v;
+    int64_t left = rows.end - (rows.begin + (lo - number) * kChunk);
+    int off[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      off[r] = col < a.d_v
+                   ? static_cast<int>(((4 * g + r) * row_values + col) * static_cast<int>(sizeof(T)))
+                   : static_cast<int>(0x80000000u);
+    const float* rec = first;
+    auto finish = [&](int i) {  // chunk i of the window, behind the barrier of i + 1
+      const f32x4_t(*const part)[kWave] = parts[i & 1];
+      f32x4_t o = (part[5][lane] + part[6][lane]) + (part[7][lane] + part[8][lane]);
+      const f32x4_t u = part[9][lane];
+      const bool fine = (u[0] - u[0]) + (u[1] - u[1]) + (u[2] - u[2]) + (u[3] - u[3]) == 0.f;
+      if (__builtin_expect(!__all(fine), 0)) {
+        // infinities and NaNs, which P's zeros would hand to the steps before
+        // their own: the waves left them out of P U, and the steps from
+        // theirs on take them one by one
+#pragma unroll 1
+        for (int j = 0; j < kChunk; ++j) {
+          const float mine = (j & 2) ? ((j & 1) ? u[3] : u[2]) : ((j & 1) ? u[1] : u[0]);
+          const float uj = __shfl(mine, m + 16 * (j >> 2));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float pij = rec[L::kP + ((4 * g + r) + 16 * (j >> 2)) * 4 + (j & 3)];
+            if (j <= 4 * g + r && uj - uj != 0.f) o[r] = fmaf(pij, uj, o[r]);
+          }
+        }
+      }
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(out, 0, 0x7FFFFFFF, 0x00020000);
+      const int live = left < kChunk ? static_cast<int>(left) : kChunk;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int at_r = 4 * g + r < live ? off[r] : static_cast<int>(0x80000000u);
+        if constexpr (DT == LK_DTYPE_F32)
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[r]), rsrc, at_r, 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b16(from_f32<DT>(o[r]), rsrc, at_r, 0, 0);
+      }
+      out += kChunk * row_values;
+      left -= kChunk;
+      rec += stride;
+    };
+    fetch(u0, d0);
+    fetch(u1, d1);
+    // (registers in turn: a copy of one on its way would wait for it)
+    auto turn = [&](int i, f32x4_t u, row_t d, f32x4_t& next_u, row_t& next_d) {
+      hand_over(i, u, d);
+      fetch(next_u, next_d);
+      __syncthreads();
+      if (i > 0) finish(i - 1);
+    };
+    int i = 0;
+    for (; i + 3 <= steps; i += 3) {
+      turn(i, u0, d0, u2, d2);
+      turn(i + 1, u1, d1, u0, d0);
+      turn(i + 2, u2, d2, u1, d1);
+    }
+    if (i < steps) turn(i, u0, d0, u2, d2);
+    if (i + 1 < steps) turn(i + 1, u1, d1, u0, d0);
+    __syncthreads();
+    finish(steps - 1);
+    return;
+  }
+
   const float* const src = lo == number ? a.state : a.state_out;
   const int64_t sbase = sh * a.d_k * a.d_v;
   f32x4_t st[RT];
@@ -631,86 +753,85 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_scan_kernel(ScanArgs a, C
       const int row = 16 * (wave * RT + t) + 4 * g + r;
       st[t][r] = row < a.d_k && col < a.d_v ? src[sbase + static_cast<int64_t>(row) * a.d_v + col] : 0.f;
     }
-
   struct Record {
-    f32x4_t w[RT], q[RT], k[RT], d[RT], u, p;
+    f32x4_t w[RT], q[RT], k[RT];
+    float p;
   };
-  auto fetch = [&](int64_t chunk, Record& f) {
-    const float* const rec = c.records + ((chunk - c.first) * a.heads + h) * c.record;
-    const f32x4_t* const v4 = reinterpret_cast<const f32x4_t*>(rec);
+  const uint32_t tiles = static_cast<uint32_t>((wave * RT * 64 + lane) * 4);
+  const uint32_t plane = static_cast<uint32_t>(L::kP + 4 * lane + wave);
+  const float* ahead = first;
+  auto fetch_w = [&](Record& f) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int tile = wave * RT + t;
-      f.w[t] = v4[L::kW / 4 + tile * 64 + lane];
-      f.q[t] = v4[L::kQ / 4 + tile * 64 + lane];
-      f.k[t] = v4[L::kK / 4 + tile * 64 + lane];
-      f.d[t] = v4[L::kD / 4 + tile * 4 + g];
-    }
-    f.u = v4[L::kU / 4 + ct * 64 + lane];
-    f.p = v4[L::kP / 4 + lane];
+    for (int t = 0; t < RT; ++t)
+      f.w[t] = *reinterpret_cast<const f32x4_t*>(ahead + (tiles + L::kW + 256 * t));
   };
-  if (chunks > 0) {
-    Record cur, next;
-    fetch(lo, cur);
-    for (int64_t ch = lo; ch < hi; ++ch) {
-      if (ch + 1 < hi) fetch(ch + 1, next);
-      const int buf = static_cast<int>(ch & 1);
-      f32x4_t x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+  auto fetch_q = [&](Record& f) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+      f.q[t] = *reinterpret_cast<const f32x4_t*>(ahead + (tiles + L::kQ + 256 * t));
+  };
+  auto fetch_k = [&](Record& f) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+      f.k[t] = *reinterpret_cast<const f32x4_t*>(ahead + (tiles + L::kK + 256 * t));
+    f.p = ahead[plane];
+    ahead = advance(ahead);
+  };
+  auto step = [&](int i, const Record& f, Record& next) {
+    f32x4_t(*const part)[kWave] = parts[i & 1];
+    f32x4_t x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        x = __builtin_amdgcn_mfma_f32_16x16x4f32(f.w[t][r], st[t][r], x, 0, 0, 0);
+    fetch_w(next);
+    part[wave][lane] = x;
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);  // Q S is not to be moved up
+    const f32x4_t x0 = part[0][lane], x1 = part[1][lane], x2 = part[2][lane], x3 = part[3][lane],
+                  x4 = part[4][lane];
+    f32x4_t d[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) d[t] = decay[i & 1][(wave * RT + t) * 4 + g];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        y = __builtin_amdgcn_mfma_f32_16x16x4f32(f.q[t][r], st[t][r], y, 0, 0, 0);
+    fetch_q(next);
+    const f32x4_t u = -(((x0 + x1) + (x2 + x3)) + x4);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) st[t] *= d[t];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.w[t][r], st[t][r], x, 0, 0, 0);
-      parts[buf][0][wave][lane] = x;
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          y = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.q[t][r], st[t][r], y, 0, 0, 0);
-      parts[buf][1][wave][lane] = y;
-      __syncthreads();
-      const f32x4_t u = cur.u - ((parts[buf][0][0][lane] + parts[buf][0][1][lane]) +
-                                 (parts[buf][0][2][lane] + parts[buf][0][3][lane]));
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        st[t] *= cur.d[t];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.k[t][r], u[r], st[t], 0, 0, 0);
-      }
-      if (wave == (ch & 3)) {
-        f32x4_t o = (parts[buf][1][0][lane] + parts[buf][1][1][lane]) +
-                    (parts[buf][1][2][lane] + parts[buf][1][3][lane]);
-        f32x4_t past;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) past[r] = u[r] - u[r] == 0.f ? u[r] : 0.f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          o = __builtin_amdgcn_mfma_f32_16x16x4f32(cur.p[r], past[r], o, 0, 0, 0);
-        const bool fine = (u[0] - u[0]) + (u[1] - u[1]) + (u[2] - u[2]) + (u[3] - u[3]) == 0.f;
-        if (__builtin_expect(!__all(fine), 0)) {
-          // infinities and NaNs, which P's zeros would hand to the steps
-          // before their own: the steps from theirs on take them one by one
-          const float* const rec = c.records + ((ch - c.first) * a.heads + h) * c.record;
-#pragma unroll 1
-          for (int j = 0; j < kChunk; ++j) {
-            const float mine = (j & 2) ? ((j & 1) ? u[3] : u[2]) : ((j & 1) ? u[1] : u[0]);
-            const float uj = __shfl(mine, m + 16 * (j >> 2));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float pij = rec[L::kP + ((4 * g + r) + 16 * (j >> 2)) * 4 + (j & 3)];
-              if (j <= 4 * g + r && uj - uj != 0.f) o[r] = fmaf(pij, uj, o[r]);
-            }
-          }
-        }
-        const int64_t t0 = rows.begin + (ch - number) * kChunk + 4 * g;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (t0 + r < rows.end && col < a.d_v)
-            static_cast<T*>(a.out)[((t0 + r) * a.heads + h) * a.d_v + col] = from_f32<DT>(o[r]);
-      }
-      cur = next;
+        st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.k[t][r], u[r], st[t], 0, 0, 0);
+    const float mine = wave & 2 ? (wave & 1 ? u[3] : u[2]) : (wave & 1 ? u[1] : u[0]);
+    y = __builtin_amdgcn_mfma_f32_16x16x4f32(f.p, mine - mine == 0.f ? mine : 0.f, y, 0, 0, 0);
+    fetch_k(next);
+    part[5 + wave][lane] = y;
+    if (wave == 0) part[9][lane] = u;
+  };
+  if (steps > 0) {
+    Record f0, f1, f2;  // in turn
+    fetch_w(f0);
+    fetch_q(f0);
+    fetch_k(f0);
+    fetch_w(f1);
+    fetch_q(f1);
+    fetch_k(f1);
+    int i = 0;
+    for (; i + 3 <= steps; i += 3) {
+      step(i, f0, f2);
+      step(i + 1, f1, f0);
+      step(i + 2, f2, f1);
     }
+    if (i < steps) step(i, f0, f2);
+    if (i + 1 < steps) step(i + 1, f1, f0);
+    __syncthreads();  // the last chunk's outputs and U, for the fifth wave
   }
 #pragma unroll
   for (int t = 0; t < RT; ++t)
@@ -784,9 +905,10 @@ int64_t chunk_window(int64_t chunks, int64_t heads, int64_t record) {
   return w < chunks ? w : chunks;
 }
 
-bool takes_chunks(int64_t sequences, int64_t tokens, int64_t d_k) {
+bool takes_chunks(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k, int64_t d_v) {
   const int choice = path_choice(kKnobKdaPrefill);
-  if (d_k > 128 || tokens == 0 || choice == 1) return false;
+  // (a chunk's outputs are stored at 31-bit byte offsets)
+  if (d_k > 128 || tokens == 0 || choice == 1 || heads * d_v >= (int64_t{1} << 24)) return false;
   return choice == 2 || tokens >= 32 * sequences;
 }
 
@@ -798,7 +920,7 @@ int launch_chunks(const ScanArgs& a, float* records, hipStream_t s) {
   c.v_tiles = (a.d_v + 15) / 16;
   const int64_t chunks = sequence_tiles(a.seq.rows, a.seq.count, kChunk);
   const int64_t window = chunk_window(chunks, a.heads, c.record);
-  const int64_t scans = (a.seq.count + 1) * static_cast<int64_t>(a.heads) * c.v_tiles;
+  const int64_t scans = ((a.seq.count + 1) * static_cast<int64_t>(a.heads) + 7) / 8 * 8 * c.v_tiles;
   LK_REQUIRE(window * a.heads < (int64_t{1} << 31) && scans < (int64_t{1} << 31),
              "too many sequences x heads for one call");
   for (c.first = 0; c.first < chunks; c.first += window) {
@@ -806,7 +928,7 @@ int launch_chunks(const ScanArgs& a, float* records, hipStream_t s) {
     chunk_prepare_kernel<DT, RT>
         <<<static_cast<unsigned>(c.count * a.heads), kChunkThreads, 0, s>>>(a, c);
     if (const int st = check_launch("lk_kda_prefill")) return st;
-    chunk_scan_kernel<DT, RT><<<static_cast<unsigned>(scans), kChunkThreads, 0, s>>>(a, c);
+    chunk_scan_kernel<DT, RT><<<static_cast<unsigned>(scans), kScanWaves * kWave, 0, s>>>(a, c);
     if (const int st = check_launch("lk_kda_prefill")) return st;
   }
   return LK_OK;
@@ -870,7 +992,7 @@ int lk_kda_short_conv_prefill(const void* q_in, const void* k_in, const void* v_
 int64_t lk_kda_prefill_workspace(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k,
                                  int64_t d_v) {
   if (sequences <= 0 || tokens < 0 || heads <= 0 || d_k <= 0 || d_v <= 0 || d_k > 256) return -1;
-  if (!takes_chunks(sequences, tokens, d_k)) return 0;
+  if (!takes_chunks(sequences, tokens, heads, d_k, d_v)) return 0;
   const int64_t record = chunk_record(d_k, d_v);
   return chunk_window(sequence_tiles(tokens, sequences, kChunk), heads, record) * heads * record * 4;
 }
@@ -900,7 +1022,7 @@ int lk_kda_prefill(const float* state, float* state_out, const float* q, const f
                    static_cast<int>(heads), static_cast<int>(d_k), static_cast<int>(d_v), scale};
   LK_REQUIRE(aligned(workspace, 16), "KDA prefill workspace must be 16-byte aligned");
   const hipStream_t s = as_stream(stream);
-  const bool chunks = takes_chunks(sequences, tokens, d_k);
+  const bool chunks = takes_chunks(sequences, tokens, heads, d_k, d_v);
   if (value_dtype == LK_DTYPE_F32) return launch_scan<LK_DTYPE_F32>(a, chunks, workspace, s);
   if (value_dtype == LK_DTYPE_F16) return launch_scan<LK_DTYPE_F16>(a, chunks, workspace, s);
   return launch_scan<LK_DTYPE_BF16>(a, chunks, workspace, s);
