@@ -223,22 +223,29 @@ __device__ inline float row16_sum(float v) {
   return v;
 }
 
+// p[first .. first + RPL) of a row of d_k values, zeros behind it and where the
+// row is not ok (p is a row that can be read all the same). No branch: loads under
+// one wait for each other.
 template <int RPL>
 __device__ inline void load_rows(const float* p, int first, int d_k, bool ok, float (&r)[RPL]) {
   if ((d_k & 3) == 0) {
+    float4 x[RPL / 4];
+#pragma unroll
+    for (int i = 0; i < RPL; i += 4)
+      x[i / 4] = *reinterpret_cast<const float4*>(p + (first + i < d_k ? first + i : 0));
 #pragma unroll
     for (int i = 0; i < RPL; i += 4) {
       const bool in = ok && first + i < d_k;
-      const float4 x = in ? *reinterpret_cast<const float4*>(p + first + i)
-                          : make_float4(0.f, 0.f, 0.f, 0.f);
-      r[i] = x.x;
-      r[i + 1] = x.y;
-      r[i + 2] = x.z;
-      r[i + 3] = x.w;
+      r[i] = in ? x[i / 4].x : 0.f;
+      r[i + 1] = in ? x[i / 4].y : 0.f;
+      r[i + 2] = in ? x[i / 4].z : 0.f;
+      r[i + 3] = in ? x[i / 4].w : 0.f;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < RPL; ++i) r[i] = ok && first + i < d_k ? p[first + i] : 0.f;
+    for (int i = 0; i < RPL; ++i) r[i] = p[first + i < d_k ? first + i : 0];
+#pragma unroll
+    for (int i = 0; i < RPL; ++i) r[i] = ok && first + i < d_k ? r[i] : 0.f;
   }
 }
 
@@ -281,10 +288,11 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(ScanArgs a,
     load_rows<RPL>(a.k + at, l * RPL, a.d_k, ok, fk);
     load_rows<RPL>(a.decay + at, l * RPL, a.d_k, ok, fg);
     const int vc = cb * kSerialCols + l;
-    fv = ok && vc < a.d_v
-             ? to_f32<DT>(static_cast<const T*>(a.v)[(t * a.heads + h) * a.d_v + vc])
-             : 0.f;
-    fb = ok ? a.beta[t * a.heads + h] : 0.f;
+    const int64_t th = (ok ? t : rows.begin) * a.heads + h;
+    fv = to_f32<DT>(static_cast<const T*>(a.v)[th * a.d_v + (vc < a.d_v ? vc : 0)]);
+    fb = a.beta[th];
+    fv = ok && vc < a.d_v ? fv : 0.f;
+    fb = ok ? fb : 0.f;
   };
   if (rows.begin < rows.end) fetch(rows.begin);
   for (int64_t t0 = rows.begin; t0 < rows.end; t0 += kSerialTokens) {
@@ -456,30 +464,40 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_prepare_kernel(ScanArg
   float v_first[kChunk];
   {
     const int vc = tid - L::kChannels;
+    const int at_v = vc >= 0 && vc < a.d_v ? vc : 0;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) {
+      const int64_t t = t0 + i < rows.end ? t0 + i : t0;
+      v_first[i] = to_f32<DT>(static_cast<const T*>(a.v)[(t * a.heads + h) * a.d_v + at_v]);
+    }
 #pragma unroll
     for (int i = 0; i < kChunk; ++i)
-      v_first[i] = vc >= 0 && t0 + i < rows.end && vc < a.d_v
-                       ? to_f32<DT>(static_cast<const T*>(a.v)[((t0 + i) * a.heads + h) * a.d_v + vc])
-                       : 0.f;
+      v_first[i] = t0 + i < rows.end && at_v == vc ? v_first[i] : 0.f;
   }
   {  // steps behind the sequence's end: no decay, no key, no query
     const int64_t t = t0 + i16;
     const bool ok = t < rows.end;
     const int64_t base = ((ok ? t : t0) * a.heads + h) * a.d_k;
+    float qs[RT][4], ks[RT][4], gs[RT][4];
+    const float beta = a.beta[(ok ? t : t0) * a.heads + h];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      float q[4], k[4], g[4];
       const int d = 4 * (l + 16 * i);
-      load_rows<4>(a.q + base, d, a.d_k, ok, q);
-      load_rows<4>(a.k + base, d, a.d_k, ok, k);
-      load_rows<4>(a.decay + base, d, a.d_k, ok, g);
+      load_rows<4>(a.q + base, d, a.d_k, ok, qs[i]);
+      load_rows<4>(a.k + base, d, a.d_k, ok, ks[i]);
+      load_rows<4>(a.decay + base, d, a.d_k, ok, gs[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int d = 4 * (l + 16 * i);
+      float(&q)[4] = qs[i], (&k)[4] = ks[i], (&g)[4] = gs[i];
 #pragma unroll
       for (int x = 0; x < 4; ++x) g[x] = expf(g[x]);
       *reinterpret_cast<float4*>(&sq[i16][d]) = make_float4(q[0], q[1], q[2], q[3]);
       *reinterpret_cast<float4*>(&sk[i16][d]) = make_float4(k[0], k[1], k[2], k[3]);
       *reinterpret_cast<float4*>(&sg[i16][d]) = make_float4(g[0], g[1], g[2], g[3]);
     }
-    if (l == 0) sb[i16] = ok ? a.beta[t * a.heads + h] : 0.f;
+    if (l == 0) sb[i16] = ok ? beta : 0.f;
   }
   __syncthreads();
 
