@@ -23,6 +23,8 @@ struct AttnArgs {
   int heads, group, d_qk, d_v;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   int64_t tiles;
+  int splits;       // runs of each block's keys
+  float* partial;   // more than one run: their sums, else null
   float scale_log2;  // |scale| * log2(e), 1 where scale is 0
   uint32_t q_keep, q_flip;  // bits of q kept (none where scale is 0), flipped (signs, scale < 0)
 };
@@ -82,13 +84,13 @@ __device__ inline float value_of(uint32_t x) {
 // pass over the banks with their neighbours, and longer ones than 256 start at
 // either half of them, hence the row's upper bits there.
 template <int C>
-__device__ inline int key_swizzle(int r) {
+__host__ __device__ constexpr int key_swizzle(int r) {
   return C % 16 == 0 ? r & 15 : (r >> 1) & 7;
 }
 // V is read down its columns (four rows of 32 bytes by 16 lanes, twice that by a
 // half-wave): four consecutive rows go to four quarters of the banks.
 template <int C>
-__device__ inline int value_swizzle(int r) {
+__host__ __device__ constexpr int value_swizzle(int r) {
   return C % 16 == 0 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
 }
 
@@ -101,6 +103,11 @@ __device__ inline uint2 lds_read_transposed(const uint16_t* p) {
   const i16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
       (lds_i16x4_t*)(const __attribute__((address_space(3))) uint16_t*)(p));
   return __builtin_bit_cast(uint2, v);
+}
+
+__device__ inline SequenceTile attention_tile(const AttnArgs& a, int64_t rank) {
+  return a.sq.count < 64 ? find_longest_tile(a.sq, rank, kAttnQueries)
+                         : find_sequence_tile(a.sq, a.tiles - 1 - rank, kAttnQueries);
 }
 
 // Block = 128 queries of one head, a wave 32 of them. Scores are computed
@@ -120,12 +127,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
   // p is stored as 2^kLift times itself: fp16 keeps 2^-24 at the least
   constexpr float kLift = BF16 ? 0.f : 6.f;
   __shared__ alignas(16) uint16_t stage[2 * kStage];
-  const int64_t total = a.tiles * a.heads;
-  const int64_t id = blockIdx.x;
-  const int h = static_cast<int>(id % a.heads);
-  const int64_t number = a.tiles - 1 - id / a.heads;
-  (void)total;
-  const SequenceTile at = find_sequence_tile(a.sq, number, kAttnQueries);
+  const int h = static_cast<int>(blockIdx.x % a.heads);
+  const int64_t item = blockIdx.x / a.heads;
+  const int split = static_cast<int>(item % a.splits);
+  const SequenceTile at = attention_tile(a, item / a.splits);
+  if (at.sequence < 0) return;
   const RowRange rq = sequence_rows(a.sq, at.sequence);
   const int64_t lq = rq.end - rq.begin;
   const int64_t q0 = at.tile * kAttnQueries;
@@ -148,7 +154,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
     const int64_t ahead = lk - lq;
     // keys seen by the block's last query, and by the wave's
     const int64_t last = q0 + kAttnQueries < lq ? q0 + kAttnQueries : lq;
-    const int64_t keys = last + ahead < 0 ? 0 : last + ahead;
+    const int64_t all = last + ahead < 0 ? 0 : last + ahead;
+    // this block's run of them, and the wave's end of it
+    const int64_t per = ((all + a.splits - 1) / a.splits + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
+    const int64_t from = split * per < all ? split * per : all;
+    const int64_t keys = from + per < all ? from + per : all;
     const int64_t keys_wave = qw + 32 + ahead < keys ? qw + 32 + ahead : keys;
     const int hk = h / a.group;
     const uint16_t* const kb = a.k + rk.begin * a.k_row + hk * a.k_head;
@@ -192,19 +202,34 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
       for (int i = 0; i < kVLoads; ++i)
         lds_direct16(rv_, base + kAttnKeys * DQ * 2 + (wave * kVLoads + i) * kWave * 16, voff[i], 0);
     };
-    // LDS reads of this lane, in values from a stage's start: K row n (+ 32 t), V
-    // rows 4 half + lane % 16 / 4 (+ 8 x), columns 16 (lane / 16 % 2) + 4 (lane % 4)
-    const int vrow = 4 * half + (lane & 15) / 4;
-    const int vcol = 16 * (lane / 16 & 1) + 4 * (lane & 3);
+    // where this lane reads, in values from the start of a tile: K row n (and n +
+    // 32), chunks 2 i + half (the swizzle takes a chunk's low bits alone, so the
+    // reads of later chunks are those of the first at a fixed distance)
+    constexpr int kAddrs = kKChunks % 16 == 0 ? 8 : 4;
+    int kaddr[kAddrs];
+#pragma unroll
+    for (int i = 0; i < kAddrs; ++i)
+      kaddr[i] = n * DQ + 8 * ((2 * i + half) ^ key_swizzle<kKChunks>(n));
+    static_assert(key_swizzle<kKChunks>(32) == 0 && value_swizzle<kVChunks>(8) == 0, "row steps");
+    // V rows 4 half + lane % 16 / 4 (and + 8), columns 16 (lane / 16 % 2) + 4 (lane % 4)
+    int vaddr[2][kVTiles];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int vt = 0; vt < kVTiles; ++vt) {
+        const int row = 8 * x + 4 * half + (lane & 15) / 4;
+        const int col = 32 * vt + 16 * (lane / 16 & 1) + 4 * (lane & 3);
+        vaddr[x][vt] = row * DV + 8 * ((col / 8) ^ value_swizzle<kVChunks>(row)) + col % 8;
+      }
 
-    if (keys > 0) fetch(0, 0);
+    if (from < keys) fetch(from, 0);
     wait_vmcnt<0>();
     __syncthreads();
     int buf = 0;
     bool bad = false;  // V has an infinity or a NaN in a tile that not every query sees
-    for (int64_t k0 = 0; k0 < keys; k0 += kAttnKeys, buf ^= 1) {
+    for (int64_t k0 = from; k0 < keys; k0 += kAttnKeys, buf ^= 1) {
       if (k0 + kAttnKeys < keys) fetch(k0 + kAttnKeys, buf ^ 1);
-      if (k0 < keys_wave) {
+      if (k0 < keys_wave && qw < lq) {
         const uint16_t* const lk_ = stage + buf * kStage;
         const uint16_t* const lv = lk_ + kAttnKeys * DQ;
         f32x16_t s[2];
@@ -212,34 +237,64 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+        // K two steps ahead of its use: read one pair at a time as the matrix
+        // unit wants them, each pair of products waited for LDS
+        u32x4_t kf[3][2];
+        auto read_k = [&](int i) {
 #pragma unroll
-        for (int i = 0; i < kQSteps; ++i)
+          for (int t = 0; t < 2; ++t)
+            kf[i % 3][t] = *reinterpret_cast<const u32x4_t*>(
+                lk_ + kaddr[i % kAddrs] + 8 * (2 * kAddrs) * (i / kAddrs) + 32 * t * DQ);
+        };
+        read_k(0);
+        read_k(1);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const int r = 32 * t + n;
-            const int c = (2 * i + half) ^ key_swizzle<kKChunks>(r);
-            s[t] = mfma32<BF16>(*reinterpret_cast<const u32x4_t*>(lk_ + r * DQ + 8 * c), qf[i], s[t]);
-          }
+        for (int i = 0; i < kQSteps; ++i) {
+          if (i + 2 < kQSteps) read_k(i + 2);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) s[t] = mfma32<BF16>(kf[i % 3][t], qf[i], s[t]);
+        }
+        // the first V rows, on their way through the softmax
+        u32x4_t vf[2][kVTiles];
+        auto read_v = [&](int i) {
+#pragma unroll
+          for (int vt = 0; vt < kVTiles; ++vt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint2 v = lds_read_transposed(lv + vaddr[x][vt] + 16 * i * DV);
+              vf[i & 1][vt][2 * x] = v.x;
+              vf[i & 1][vt][2 * x + 1] = v.y;
+            }
+        };
+        read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
         // register r of tile t: key k0 + 32 t + 8 (r / 4) + 4 half + r % 4. What a
         // query does not see is left out of its maximum and gets p = 0, which
         // an infinity or a NaN in V would turn into one of its own: such values
         // are taken out of the product there and added at the end, for the
         // queries that see them.
         const bool edge = k0 + kAttnKeys - 1 > qw + ahead;  // a query does not see all of them
-        const int seen = static_cast<int>(qi + ahead - k0 < kAttnKeys ? qi + ahead - k0 + 1 : kAttnKeys);
         if (edge) {
+          // keys of this tile that the lane's query sees, from its first register on
+          const int seen =
+              static_cast<int>(qi + ahead - k0 < kAttnKeys ? qi + ahead - k0 + 1 : kAttnKeys) - 4 * half;
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              if (32 * t + 8 * (r / 4) + 4 * half + r % 4 >= seen) s[t][r] = -INFINITY;
+              s[t][r] = 32 * t + 8 * (r / 4) + r % 4 < seen ? s[t][r] : -INFINITY;
         }
         float most = s[0][0];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int r = 0; r < 16; ++r) most = fmaxf(most, s[t][r]);
-        most = fmaxf(most, __shfl_xor(most, 32)) * a.scale_log2;
+        {
+          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most),
+                                                          __float_as_uint(most), false, false);
+          most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.scale_log2;
+        }
         // the maximum only moves when it has grown by more than 2^kSlack: p stays
         // below that, and most passes leave the accumulators alone
         constexpr float kSlack = 8.f;
@@ -270,22 +325,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
           const u32x4_t p = {pack2<BF16>(s[t][r], s[t][r + 1]), pack2<BF16>(s[t][r + 2], s[t][r + 3]),
                              pack2<BF16>(s[t][r + 4], s[t][r + 5]),
                              pack2<BF16>(s[t][r + 6], s[t][r + 7])};
+          if (i < 3) read_v(i + 1);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int vt = 0; vt < kVTiles; ++vt) {
-            u32x4_t vf;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int row = 16 * i + 8 * x + vrow, col = 32 * vt + vcol;
-              const uint2 v = lds_read_transposed(
-                  lv + row * DV + 8 * ((col / 8) ^ value_swizzle<kVChunks>(row)) + col % 8);
-              vf[2 * x] = v.x;
-              vf[2 * x + 1] = v.y;
-            }
-            if (edge && __builtin_expect(__any(any_nonfinite<BF16>(vf)), 0)) {
+            if (edge && __builtin_expect(__any(any_nonfinite<BF16>(vf[i & 1][vt])), 0)) {
               bad = true;
-              vf = finite_only<BF16>(vf);
+              vf[i & 1][vt] = finite_only<BF16>(vf[i & 1][vt]);
             }
-            o[vt] = mfma32<BF16>(vf, p, o[vt]);
+            o[vt] = mfma32<BF16>(vf[i & 1][vt], p, o[vt]);
           }
         }
       }
@@ -296,6 +344,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
     if (__builtin_expect(bad, 0)) {
       // the infinities and NaNs left out above, for the queries that see them
       int64_t key = qw + ahead + 1 < 0 ? 0 : (qw + ahead + 1) / kAttnKeys * kAttnKeys;
+      key = key < from ? from : key;
 #pragma unroll 1
       for (; key < keys_wave; ++key) {
         const uint16_t* const row = vb + key * a.v_row;
@@ -309,6 +358,23 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
           }
       }
     }
+  }
+  if (a.partial) {
+    // the run's sums as they are, with what they are taken against
+    float* const part = a.partial + ((item / a.splits * a.heads + h) * a.splits + split) *
+                                        (kAttnQueries * (DV + 2));
+    const int row = wave * 32 + n;
+#pragma unroll
+    for (int t = 0; t < kVTiles; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<float4*>(part + row * DV + 32 * t + 8 * (r / 4) + 4 * half) =
+            make_float4(o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]);
+    if (half == 0) {
+      part[kAttnQueries * DV + row] = top;
+      part[kAttnQueries * (DV + 1) + row] = sum;
+    }
+    return;
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   // whole rows through the wave's share of LDS (every wave has left the loop)
@@ -332,14 +398,70 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
   }
 }
 
+// The runs of a block's keys joined: a wave takes a query, a lane its columns.
+// Weights 2^(top - largest top) in fp32, the runs in order.
+template <bool BF16, int DV>
+__global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttnArgs a) {
+  const int h = static_cast<int>(blockIdx.x % a.heads);
+  const int64_t rank = blockIdx.x / a.heads;
+  const SequenceTile at = attention_tile(a, rank);
+  if (at.sequence < 0) return;
+  const RowRange rq = sequence_rows(a.sq, at.sequence);
+  const int64_t q0 = at.tile * kAttnQueries;
+  const int lane = threadIdx.x & (kWave - 1);
+  const float* const parts = a.partial + (rank * a.heads + h) * a.splits * (kAttnQueries * (DV + 2));
+  for (int row = threadIdx.x / kWave; row < kAttnQueries; row += kAttnWaves) {
+    const int64_t q = rq.begin + q0 + row;
+    if (q >= rq.end) return;
+    float top = -INFINITY;
+    for (int i = 0; i < a.splits; ++i)
+      top = fmaxf(top, parts[i * (kAttnQueries * (DV + 2)) + kAttnQueries * DV + row]);
+    float sum = 0.f, acc[DV / 64] = {};
+    for (int i = 0; i < a.splits; ++i) {
+      const float* const part = parts + i * (kAttnQueries * (DV + 2));
+      const float own = part[kAttnQueries * DV + row];
+      const float w = own == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own - top);
+      sum = fmaf(w, part[kAttnQueries * (DV + 1) + row], sum);
+#pragma unroll
+      for (int x = 0; x < DV / 64; ++x)
+        acc[x] = fmaf(w, part[row * DV + DV / 64 * lane + x], acc[x]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    uint16_t* const out = a.out + (q * a.heads + h) * a.d_v;
+    if constexpr (DV == 128) {
+      if (2 * lane < a.d_v)
+        *reinterpret_cast<uint32_t*>(out + 2 * lane) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
+    } else {
+      if (lane < a.d_v) out[lane] = static_cast<uint16_t>(pack2<BF16>(acc[0] * inv, 0.f));
+    }
+  }
+}
+
+// Runs of each block's keys. A block alone on a CU leaves its matrix unit idle
+// through every softmax, and a call with fewer blocks than CUs leaves CUs idle: where
+// there are fewer than two blocks a CU, long key ranges are taken in runs, until
+// there are, of 512 keys at least (the runs' sums are written and read again).
+// Counts are estimates from the call's sizes: the lengths are on the device.
+constexpr int kAttnFill = 512;
+int attention_splits(int64_t rows_q, int64_t rows_k, int64_t sequences, int64_t heads) {
+  const int64_t blocks = (rows_q / kAttnQueries + sequences) * heads;
+  const int64_t want = (kAttnFill + blocks - 1) / blocks, most = rows_k / sequences / 512;
+  const int64_t n = want < most ? want : most;
+  return n < 1 ? 1 : (n > 16 ? 16 : static_cast<int>(n));
+}
+
 template <bool BF16>
 int launch_attention(const AttnArgs& a, hipStream_t s) {
-  const int64_t blocks = a.tiles * a.heads;
+  const int64_t blocks = a.tiles * a.heads * a.splits;
   LK_REQUIRE(blocks < (int64_t{1} << 31), "too many query rows and heads for one call");
-  const dim3 grid(static_cast<unsigned>(blocks));
+  const dim3 grid(static_cast<unsigned>(blocks)), join(static_cast<unsigned>(a.tiles * a.heads));
 #define LK_ATTENTION(Q, V)                                          \
   if (a.d_qk <= Q && a.d_v <= V) {                                  \
     attention_kernel<BF16, Q, V><<<grid, kAttnThreads, 0, s>>>(a);  \
+    if (a.partial) {                                                \
+      if (const int st = check_launch("lk_attention_prefill")) return st; \
+      attention_join_kernel<BF16, V><<<join, kAttnThreads, 0, s>>>(a); \
+    }                                                               \
     return check_launch("lk_attention_prefill");                    \
   }
   LK_ATTENTION(64, 64)
@@ -362,7 +484,10 @@ int64_t lk_attention_prefill_workspace(int64_t rows_q, int64_t rows_k, int64_t s
   if (rows_q < 0 || rows_k < 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 ||
       heads % kv_heads || d_qk <= 0 || d_v <= 0 || d_qk > kAttnMaxQk || d_v > kAttnMaxV)
     return -1;
-  return 0;
+  const int64_t splits = attention_splits(rows_q, rows_k, sequences, heads);
+  if (splits == 1) return 0;
+  const int64_t dv = d_qk <= 64 && d_v <= 64 ? 64 : 128;
+  return sequence_tiles(rows_q, sequences, kAttnQueries) * heads * splits * kAttnQueries * (dv + 2) * 4;
 }
 
 int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
@@ -406,6 +531,8 @@ int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
   LK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
              "attention workspace too small: %lld bytes, %lld needed", (long long)workspace_bytes,
              (long long)need);
+  LK_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+             "attention workspace must be 16-byte aligned");
   const int n = static_cast<int>(sequences);
   const AttnArgs a{static_cast<const uint16_t*>(q),
                    static_cast<const uint16_t*>(k),
@@ -420,6 +547,8 @@ int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
                    q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride,
                    v_head_stride,
                    sequence_tiles(rows_q, sequences, kAttnQueries),
+                   attention_splits(rows_q, rows_k, sequences, heads),
+                   need ? static_cast<float*>(workspace) : nullptr,
                    scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f,
                    scale == 0.f ? 0u : 0xFFFFFFFFu,
                    scale < 0.f ? 0x80008000u : 0u};

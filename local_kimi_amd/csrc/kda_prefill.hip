@@ -47,13 +47,14 @@ struct alignas(sizeof(T) * N) Pack {
 //
 // Bound by HBM: 12 operations on a value that is read and written once. A
 // thread owns N neighbouring channels (16 bytes) of one convolution and walks
-// a tile of kConvTile tokens with the three earlier inputs in registers, eight
-// rows' loads in flight; the tile's first three inputs are read again (3 rows
-// in kConvTile, mostly from a cache). The thread with a sequence's first tile
-// has read the state's values, so it is the one that replaces them: the state
-// may be updated in place.
-constexpr int kConvThreads = 256;
-constexpr int kConvTile = 32;
+// a tile of kConvTile tokens with the three earlier inputs in registers,
+// kConvRows rows' loads in flight; the tile's first three inputs are read again (3
+// rows in kConvTile, mostly from a cache). Threads are dealt over the three
+// convolutions' channels as one row, so that only a call's last block has idle
+// ones. The thread with a sequence's first tile has read the state's values, so
+// it is the one that replaces them: the state may be updated in place.
+constexpr int kConvThreads = 128;
+constexpr int kConvTile = 16;  // 4096 tokens x 3 x 4096 bf16: 40 us at 16, 42 at 32, 46 at 64
 constexpr int kConvRows = 8;
 
 struct ConvArgs {
@@ -66,7 +67,6 @@ struct ConvArgs {
   int64_t channels;
   int64_t stride;  // elements from an input row to the next
   int column_blocks;
-  int weight_dtype;
 };
 
 template <typename T>
@@ -74,22 +74,18 @@ __device__ inline T pick(const T (&v)[3], int i) {
   return i == 0 ? v[0] : (i == 1 ? v[1] : v[2]);
 }
 
-__device__ inline float load_weight(const void* p, int64_t i, int dt) {
-  if (dt == LK_DTYPE_F32) return static_cast<const float*>(p)[i];
-  const uint16_t b = static_cast<const uint16_t*>(p)[i];
-  return dt == LK_DTYPE_BF16 ? bf16_to_f32(b) : to_f32<LK_DTYPE_F16>(b);
-}
-
-template <int DT, int N>
+template <int DT, int WDT, int N>
 __global__ void __launch_bounds__(kConvThreads) conv_prefill_kernel(ConvArgs a) {
   using T = typename Storage<DT>::type;
+  using W = typename Storage<WDT>::type;
   using P = Pack<T, N>;
   const int64_t number = blockIdx.x / a.column_blocks;
-  const int cb = blockIdx.x % a.column_blocks;
-  const int conv = blockIdx.y;
-  const int64_t c = (static_cast<int64_t>(cb) * kConvThreads + threadIdx.x) * N;
-  if (c >= a.channels) return;
+  const int64_t item = static_cast<int64_t>(blockIdx.x % a.column_blocks) * kConvThreads + threadIdx.x;
+  const int64_t chunks = a.channels / N;
+  const int conv = item < chunks ? 0 : (item < 2 * chunks ? 1 : 2);
+  const int64_t c = (item - conv * chunks) * N;
   const SequenceTile at = find_sequence_tile(a.seq, number, kConvTile);
+  if (c >= a.channels) return;
   const RowRange rows = sequence_rows(a.seq, at.sequence);
   const int64_t length = rows.end - rows.begin;
   const int64_t t0 = at.tile * kConvTile;
@@ -105,49 +101,49 @@ __global__ void __launch_bounds__(kConvThreads) conv_prefill_kernel(ConvArgs a) 
   }
   if (t0 >= length && at.tile > 0) return;
 
-  float w[4][N];
-  {
-    const void* const wp = pick(a.weight, conv);
+  // every load of the tile's start first
+  P row[kConvRows];
+  auto fetch = [&](int64_t t) {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
+    for (int r = 0; r < kConvRows; ++r) {
+      const int64_t tr = t + r < t1 ? t + r : t1 - 1;
+      row[r] = *reinterpret_cast<const P*>(x + tr * a.stride);
+    }
+  };
+  Pack<W, 4> taps[N];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i][j] = load_weight(wp, (c + j) * 4 + i, a.weight_dtype);
-  }
+  for (int j = 0; j < N; ++j)
+    taps[j] = reinterpret_cast<const Pack<W, 4>*>(pick(a.weight, conv))[c + j];
+  if (t0 < t1) fetch(t0);
   float x1[N], x2[N], x3[N];  // the inputs 3, 2 and 1 tokens back
   if (at.tile == 0) {
-    const int64_t sc = (static_cast<int64_t>(at.sequence) * a.channels + c) * 4;
-    const T* const s = static_cast<const T*>(pick(a.state, conv)) + sc;
-    T* const so = static_cast<T*>(pick(a.state_out, conv)) + sc;
-    T old[N][4];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4>*>(s + 4 * j);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) old[j][i] = p.v[i];
-      x1[j] = to_f32<DT>(old[j][1]);
-      x2[j] = to_f32<DT>(old[j][2]);
-      x3[j] = to_f32<DT>(old[j][3]);
-    }
+    const int64_t sc = static_cast<int64_t>(at.sequence) * a.channels + c;
+    const auto* const s = static_cast<const Pack<T, 4>*>(pick(a.state, conv)) + sc;
+    auto* const so = static_cast<Pack<T, 4>*>(pick(a.state_out, conv)) + sc;
     // entry i of the next state: token length - 4 + i, or entry length + i of
     // this one where that lies before the first token
     P last[4];
+    if (length > 0)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t t = length - 4 + i;
-      if (t >= 0) {
-        last[i] = *reinterpret_cast<const P*>(x + t * a.stride);
-      } else {
+      for (int i = 0; i < 4; ++i)
+        last[i] = *reinterpret_cast<const P*>(x + (length - 4 + i > 0 ? length - 4 + i : 0) * a.stride);
+    Pack<T, 4> old[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          last[i].v[j] = t == -4 ? old[j][0] : (t == -3 ? old[j][1] : (t == -2 ? old[j][2] : old[j][3]));
-      }
-    }
+    for (int j = 0; j < N; ++j) old[j] = s[j];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      Pack<T, 4> p;
+      x1[j] = to_f32<DT>(old[j].v[1]);
+      x2[j] = to_f32<DT>(old[j].v[2]);
+      x3[j] = to_f32<DT>(old[j].v[3]);
+      Pack<T, 4> next;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p.v[i] = last[i].v[j];
-      *reinterpret_cast<Pack<T, 4>*>(so + 4 * j) = p;
+      for (int i = 0; i < 4; ++i) {
+        const int64_t t = length - 4 + i;
+        next.v[i] = t >= 0 ? last[i].v[j]
+                           : (t == -4 ? old[j].v[0]
+                                      : (t == -3 ? old[j].v[1] : (t == -2 ? old[j].v[2] : old[j].v[3])));
+      }
+      so[j] = next;
     }
   } else {
     const P a1 = *reinterpret_cast<const P*>(x + (t0 - 3) * a.stride);
@@ -160,29 +156,31 @@ __global__ void __launch_bounds__(kConvThreads) conv_prefill_kernel(ConvArgs a) 
       x3[j] = to_f32<DT>(a3.v[j]);
     }
   }
+  float w[4][N];
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i][j] = to_f32<WDT>(taps[j].v[i]);
 
   for (int64_t t = t0; t < t1; t += kConvRows) {
-    P row[kConvRows];
+    P res[kConvRows];
 #pragma unroll
     for (int r = 0; r < kConvRows; ++r) {
-      const int64_t tr = t + r < t1 ? t + r : t1 - 1;
-      row[r] = *reinterpret_cast<const P*>(x + tr * a.stride);
-    }
-#pragma unroll
-    for (int r = 0; r < kConvRows; ++r) {
-      P res;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float now = to_f32<DT>(row[r].v[j]);
         const float acc =
             fmaf(now, w[3][j], fmaf(x3[j], w[2][j], fmaf(x2[j], w[1][j], x1[j] * w[0][j])));
-        res.v[j] = from_f32<DT>(silu_fast_f32(acc));
+        res[r].v[j] = from_f32<DT>(silu_fast_f32(acc));
         x1[j] = x2[j];
         x2[j] = x3[j];
         x3[j] = now;
       }
-      if (t + r < t1) *reinterpret_cast<P*>(y + (t + r) * a.channels) = res;
     }
+    if (t + kConvRows < t1) fetch(t + kConvRows);
+#pragma unroll
+    for (int r = 0; r < kConvRows; ++r)
+      if (t + r < t1) *reinterpret_cast<P*>(y + (t + r) * a.channels) = res[r];
   }
 }
 
@@ -875,21 +873,28 @@ int check_sequences(const int32_t* cu, int64_t sequences, int64_t tokens) {
   return LK_OK;
 }
 
-template <int DT>
+template <int DT, int WDT>
 int launch_conv(const ConvArgs& a, bool wide, hipStream_t s) {
   constexpr int kWide = DT == LK_DTYPE_F32 ? 4 : 8;  // 16 bytes
   ConvArgs b = a;
-  const int64_t per = kConvThreads * (wide ? kWide : 1);
-  const int64_t blocks = (a.channels + per - 1) / per;
+  const int64_t items = 3 * (a.channels / (wide ? kWide : 1));
+  const int64_t blocks = (items + kConvThreads - 1) / kConvThreads;
   const int64_t tiles = sequence_tiles(a.seq.rows, a.seq.count, kConvTile);
   LK_REQUIRE(blocks * tiles < (int64_t{1} << 31), "too many tokens and channels for one call");
   b.column_blocks = static_cast<int>(blocks);
-  const dim3 grid(static_cast<unsigned>(blocks * tiles), 3);
+  const dim3 grid(static_cast<unsigned>(blocks * tiles));
   if (wide)
-    conv_prefill_kernel<DT, kWide><<<grid, kConvThreads, 0, s>>>(b);
+    conv_prefill_kernel<DT, WDT, kWide><<<grid, kConvThreads, 0, s>>>(b);
   else
-    conv_prefill_kernel<DT, 1><<<grid, kConvThreads, 0, s>>>(b);
+    conv_prefill_kernel<DT, WDT, 1><<<grid, kConvThreads, 0, s>>>(b);
   return check_launch("lk_kda_short_conv_prefill");
+}
+
+template <int DT>
+int launch_conv_weights(const ConvArgs& a, int weight_dtype, bool wide, hipStream_t s) {
+  if (weight_dtype == LK_DTYPE_F32) return launch_conv<DT, LK_DTYPE_F32>(a, wide, s);
+  if (weight_dtype == LK_DTYPE_F16) return launch_conv<DT, LK_DTYPE_F16>(a, wide, s);
+  return launch_conv<DT, LK_DTYPE_BF16>(a, wide, s);
 }
 
 template <int DT>
@@ -987,6 +992,9 @@ int lk_kda_short_conv_prefill(const void* q_in, const void* k_in, const void* v_
                         static_cast<const void*>(k_state_out),
                         static_cast<const void*>(v_state_out)})
     LK_REQUIRE(aligned(p, 4 * size), "convolution states must be aligned to a channel's entries");
+  for (const void* p : {q_weight, k_weight, v_weight})
+    LK_REQUIRE(aligned(p, weight_dtype == LK_DTYPE_F32 ? 16 : 8),
+               "convolution weights must be aligned to a channel's entries");
   bool wide = channels * size % 16 == 0 && row_stride * size % 16 == 0;
   for (const void* p : {q_in, k_in, v_in, static_cast<const void*>(q_out),
                         static_cast<const void*>(k_out), static_cast<const void*>(v_out)})
@@ -999,12 +1007,11 @@ int lk_kda_short_conv_prefill(const void* q_in, const void* k_in, const void* v_
                    Sequences{cu_seqlens, tokens, tokens / sequences, static_cast<int>(sequences)},
                    channels,
                    row_stride,
-                   0,
-                   weight_dtype};
+                   0};
   const hipStream_t s = as_stream(stream);
-  if (value_dtype == LK_DTYPE_F32) return launch_conv<LK_DTYPE_F32>(a, wide, s);
-  if (value_dtype == LK_DTYPE_F16) return launch_conv<LK_DTYPE_F16>(a, wide, s);
-  return launch_conv<LK_DTYPE_BF16>(a, wide, s);
+  if (value_dtype == LK_DTYPE_F32) return launch_conv_weights<LK_DTYPE_F32>(a, weight_dtype, wide, s);
+  if (value_dtype == LK_DTYPE_F16) return launch_conv_weights<LK_DTYPE_F16>(a, weight_dtype, wide, s);
+  return launch_conv_weights<LK_DTYPE_BF16>(a, weight_dtype, wide, s);
 }
 
 int64_t lk_kda_prefill_workspace(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k,

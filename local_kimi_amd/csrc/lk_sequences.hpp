@@ -50,18 +50,54 @@ struct SequenceTile {
   int64_t tile;
 };
 
+// The tile with this number; called by whole waves. The last s of 0..count with
+// begin(s) / tile + s <= number, 64 candidates at a time, a lane each (one load's
+// latency for up to 63 sequences). Offsets that decrease give some s of that range
+// and perhaps a number before its first.
 __device__ inline SequenceTile find_sequence_tile(const Sequences& q, int64_t number, int tile) {
-  int lo = 0, hi = q.count;  // the last s of 0..count with begin(s) / tile + s <= number
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (sequence_begin(q, mid) / tile + mid <= number)
-      lo = mid;
-    else
-      hi = mid - 1;
+  const int lane = static_cast<int>(threadIdx.x & 63);
+  int lo = 0, span = q.count + 1;
+  while (span > 1) {
+    const int step = (span + 63) / 64, off = lane * step, at = lo + (off < span ? off : 0);
+    const bool before = off < span && sequence_begin(q, at) / tile + at <= number;
+    const int n = __popcll(__ballot(before));
+    const int skip = n > 0 ? (n - 1) * step : 0;
+    lo += skip;
+    span = span - skip < step ? span - skip : step;
   }
-  // decreasing offsets can name a number before the sequence's first
   const int64_t t = number - (sequence_begin(q, lo) / tile + lo);
   return {lo, t < 0 ? 0 : t};
+}
+
+// The same tiles from the longest down: rank 0 is a last tile of the sequence with
+// the most, ties go by sequence, and the rows behind the last sequence come at
+// the end. A tile whose cost grows with its place in its sequence is best
+// started first. For up to 63 sequences, a lane each; called by whole waves.
+// Sequence -1 where there are fewer tiles (of fewer than sequence_tiles()).
+__device__ inline SequenceTile find_longest_tile(const Sequences& q, int64_t rank, int tile) {
+  const int lane = static_cast<int>(threadIdx.x & 63);
+  const RowRange own = sequence_rows(q, lane <= q.count ? lane : 0);
+  const int tiles = lane <= q.count ? static_cast<int>((own.end - own.begin + tile - 1) / tile) : 0;
+  const int mine = lane < q.count ? tiles : 0;
+  int most = mine;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int other = __shfl_xor(most, m);
+    most = other > most ? other : most;
+  }
+  int64_t left = rank;
+  for (int t = __builtin_amdgcn_readfirstlane(most) - 1; t >= 0; --t) {
+    const uint64_t have = __ballot(mine > t);
+    const int n = __popcll(have);
+    if (left < n) {
+      uint64_t rest = have;
+      for (int i = 0; i < static_cast<int>(left); ++i) rest &= rest - 1;
+      return {__ffsll(static_cast<unsigned long long>(rest)) - 1, t};
+    }
+    left -= n;
+  }
+  const int behind = __builtin_amdgcn_readlane(tiles, q.count);
+  return left < behind ? SequenceTile{q.count, left} : SequenceTile{-1, 0};
 }
 
 }  // namespace lk

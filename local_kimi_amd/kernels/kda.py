@@ -389,16 +389,12 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    if t.numel() == 0:
-        return t.data_ptr(), t.data_ptr()
-    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-
-
-def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+def _disjoint(*tensors: torch.Tensor) -> bool:
+    """Whether the dense ones among nonempty tensors share no byte (the others
+    are worked on through copies)."""
+    spans = sorted([(t.data_ptr(), t.numel() * t.element_size()) for t in tensors
+                    if t.is_contiguous()])
+    return all([lo + size <= after for (lo, size), (after, _) in zip(spans, spans[1:])])
 
 
 def _packed_rows(tensors) -> tuple[list[torch.Tensor], int]:
@@ -412,7 +408,7 @@ def _packed_rows(tensors) -> tuple[list[torch.Tensor], int]:
         (batch == 1 or t.stride(0) == rows * stride) for t in tensors)
     if fits and rows > 1:
         return list(tensors), stride
-    return [_w._c(t) for t in tensors], width
+    return [_aligned(t) for t in tensors], width
 
 
 def short_conv_prefill_triple(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torch.Tensor,
@@ -447,41 +443,44 @@ def short_conv_prefill_triple(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torc
     batch, rows, channels = q_in.shape
     if batch == 0 or channels == 0:
         raise ValueError("short convolutions need a nonempty batch and channels")
-    dev = q_in.device
-    if any(t.device != dev for t in (*values[1:], *states, *weights)):
-        raise ValueError("all short convolution tensors must share one device")
+    dev, dtype = q_in.device, q_in.dtype
+    for t in (k_in, v_in, *states, *weights):
+        if t.device != dev:
+            raise ValueError("all short convolution tensors must share one device")
     offsets, count = _offsets(cu_seqlens, batch, dev)
-    if any(tuple(t.shape) != (count, channels, CONV_WIDTH) for t in states):
-        raise ValueError("each short convolution state must have shape [sequences, channels, 4]")
-    if any(tuple(t.shape) not in {(channels, CONV_WIDTH), (channels, 1, CONV_WIDTH)}
-           for t in weights):
-        raise ValueError("each short convolution weight must have shape [channels, 1, 4]")
-    if any(t.dtype != q_in.dtype for t in (*values[1:], *states)):
-        raise TypeError("short convolution inputs and states must share a dtype")
+    shape = (count, channels, CONV_WIDTH)
+    for t in states:
+        if t.shape != shape:
+            raise ValueError("each short convolution state must have shape [sequences, channels, 4]")
+    for t in weights:
+        if t.shape != (channels, 1, CONV_WIDTH) and t.shape != (channels, CONV_WIDTH):
+            raise ValueError("each short convolution weight must have shape [channels, 1, 4]")
+        if not t.is_floating_point():
+            raise TypeError("short convolution weights must be floating point")
+    for t in (k_in, v_in, *states):
+        if t.dtype != dtype:
+            raise TypeError("short convolution inputs and states must share a dtype")
     vcode = _code(q_in, "short convolution inputs and states")
-    if any(not t.is_floating_point() for t in weights):
-        raise TypeError("short convolution weights must be floating point")
     if dev.type != "cuda":
         raise ValueError("prompt short convolutions require CUDA tensors")
-    if any(_overlaps(states[i], states[j]) for i, j in ((0, 1), (0, 2), (1, 2))):
-        raise ValueError("the three convolution states must not overlap")
     targets = states
     if conv_states_out is not None:
         targets = tuple(conv_states_out)
         if len(targets) != 3:
             raise ValueError("conv_states_out must hold the q, k and v states")
-        if any(o.shape != st.shape or o.dtype != st.dtype or o.device != dev
-               for st, o in zip(states, targets)):
-            raise ValueError("each conv_states_out tensor must match its state's shape, dtype "
-                             "and device")
-        for i, o in enumerate(targets):
-            if any(_overlaps(o, t) for t in (*states, *targets[i + 1:])):
-                raise ValueError(f"conv_states_out[{i}] overlaps another state")
+        for t in targets:
+            if t.shape != shape or t.dtype != dtype or t.device != dev:
+                raise ValueError("each conv_states_out tensor must match its state's shape, dtype "
+                                 "and device")
+        if not _disjoint(*states, *targets):
+            raise ValueError("the convolution states and conv_states_out must not overlap")
+    elif not _disjoint(*states):
+        raise ValueError("the three convolution states must not overlap")
     weights = [_weight_view(w) for w in weights]
     if weights[0].dtype not in _DTYPE_CODES or any(w.dtype != weights[0].dtype for w in weights):
         weights = [w.float() for w in weights]
     wcode = _DTYPE_CODES[weights[0].dtype]
-    weights = [_w._c(w) for w in weights]
+    weights = [_aligned(w) for w in weights]
     ins, stride = _packed_rows(values)
     src = [_aligned(st) for st in states]
     if conv_states_out is None:
@@ -548,7 +547,7 @@ def kda_prefill(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.
         if state_out.shape != state.shape or state_out.dtype != state.dtype \
                 or state_out.device != state.device:
             raise ValueError("state_out must match the state's shape, dtype and device")
-        if _overlaps(state_out, state):
+        if not _disjoint(state_out, state):
             raise ValueError("state_out overlaps the state it is computed from")
     if q.device.type != "cuda":
         raise ValueError("KDA prefill requires CUDA inputs")
