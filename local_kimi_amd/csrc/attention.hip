@@ -105,9 +105,27 @@ __device__ inline uint2 lds_read_transposed(const uint16_t* p) {
   return __builtin_bit_cast(uint2, v);
 }
 
-__device__ inline SequenceTile attention_tile(const AttnArgs& a, int64_t rank) {
-  return a.sq.count < 64 ? find_longest_tile(a.sq, rank, kAttnQueries)
-                         : find_sequence_tile(a.sq, a.tiles - 1 - rank, kAttnQueries);
+// A tile of queries, and the rows of its sequence.
+struct AttnTile {
+  SequenceTile at;
+  RowRange q, k;
+};
+
+__device__ inline AttnTile attention_tile(const AttnArgs& a, int64_t rank) {
+  AttnTile t;
+  if (a.sq.count < 64) {  // every sequence's rows at once, a lane each
+    const int lane = threadIdx.x & (kWave - 1), s = lane < a.sq.count ? lane : a.sq.count;
+    const RowRange own = sequence_rows(a.sq, s), own_k = sequence_rows(a.sk, s);
+    t.at = find_longest_tile(own, a.sq.count, rank, kAttnQueries);
+    const int from = t.at.sequence < 0 ? 0 : t.at.sequence;
+    t.q = lane_rows(own, from);
+    t.k = lane_rows(own_k, from);
+  } else {
+    t.at = find_sequence_tile(a.sq, a.tiles - 1 - rank, kAttnQueries);
+    t.q = sequence_rows(a.sq, t.at.sequence);
+    t.k = sequence_rows(a.sk, t.at.sequence);
+  }
+  return t;
 }
 
 // Block = 128 queries of one head, a wave 32 of them. Scores are computed
@@ -130,9 +148,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
   const int h = static_cast<int>(blockIdx.x % a.heads);
   const int64_t item = blockIdx.x / a.heads;
   const int split = static_cast<int>(item % a.splits);
-  const SequenceTile at = attention_tile(a, item / a.splits);
+  const AttnTile tile = attention_tile(a, item / a.splits);
+  const SequenceTile at = tile.at;
   if (at.sequence < 0) return;
-  const RowRange rq = sequence_rows(a.sq, at.sequence);
+  const RowRange rq = tile.q;
   const int64_t lq = rq.end - rq.begin;
   const int64_t q0 = at.tile * kAttnQueries;
   if (q0 >= lq) return;
@@ -149,7 +168,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
   float top = -INFINITY;  // (scaled) maximum that p is taken against
   float sum = 0.f;
   if (at.sequence < a.sq.count) {
-    const RowRange rk = sequence_rows(a.sk, at.sequence);
+    const RowRange rk = tile.k;
     const int64_t lk = rk.end - rk.begin;
     const int64_t ahead = lk - lq;
     // keys seen by the block's last query, and by the wave's
@@ -404,9 +423,10 @@ template <bool BF16, int DV>
 __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttnArgs a) {
   const int h = static_cast<int>(blockIdx.x % a.heads);
   const int64_t rank = blockIdx.x / a.heads;
-  const SequenceTile at = attention_tile(a, rank);
+  const AttnTile tile = attention_tile(a, rank);
+  const SequenceTile at = tile.at;
   if (at.sequence < 0) return;
-  const RowRange rq = sequence_rows(a.sq, at.sequence);
+  const RowRange rq = tile.q;
   const int64_t q0 = at.tile * kAttnQueries;
   const int lane = threadIdx.x & (kWave - 1);
   const float* const parts = a.partial + (rank * a.heads + h) * a.splits * (kAttnQueries * (DV + 2));

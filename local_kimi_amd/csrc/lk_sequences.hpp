@@ -72,13 +72,15 @@ __device__ inline SequenceTile find_sequence_tile(const Sequences& q, int64_t nu
 // The same tiles from the longest down: rank 0 is a last tile of the sequence with
 // the most, ties go by sequence, and the rows behind the last sequence come at
 // the end. A tile whose cost grows with its place in its sequence is best
-// started first. For up to 63 sequences, a lane each; called by whole waves.
-// Sequence -1 where there are fewer tiles (of fewer than sequence_tiles()).
-__device__ inline SequenceTile find_longest_tile(const Sequences& q, int64_t rank, int tile) {
+// started first. For up to 63 sequences, whose rows the wave's lanes hold (`own`
+// of lane s: those of sequence s, of lane count: the ones behind the last);
+// called by whole waves. Sequence -1 where there are fewer tiles (of fewer than
+// sequence_tiles()).
+__device__ inline SequenceTile find_longest_tile(const RowRange& own, int count, int64_t rank,
+                                                 int tile) {
   const int lane = static_cast<int>(threadIdx.x & 63);
-  const RowRange own = sequence_rows(q, lane <= q.count ? lane : 0);
-  const int tiles = lane <= q.count ? static_cast<int>((own.end - own.begin + tile - 1) / tile) : 0;
-  const int mine = lane < q.count ? tiles : 0;
+  const int tiles = static_cast<int>((own.end - own.begin + tile - 1) / tile);
+  const int mine = lane < count ? tiles : 0;
   int most = mine;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
@@ -96,8 +98,14 @@ __device__ inline SequenceTile find_longest_tile(const Sequences& q, int64_t ran
     }
     left -= n;
   }
-  const int behind = __builtin_amdgcn_readlane(tiles, q.count);
-  return left < behind ? SequenceTile{q.count, left} : SequenceTile{-1, 0};
+  const int behind = __builtin_amdgcn_readlane(tiles, count);
+  return left < behind ? SequenceTile{count, left} : SequenceTile{-1, 0};
+}
+
+// What a lane of the wave holds (rows are below 2^31).
+__device__ inline RowRange lane_rows(const RowRange& own, int lane) {
+  return {__builtin_amdgcn_readlane(static_cast<int>(own.begin), lane),
+          __builtin_amdgcn_readlane(static_cast<int>(own.end), lane)};
 }
 
 }  // namespace lk
