@@ -620,19 +620,18 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 // Block = one sequence's and head's 16 value columns, through the chunks of the
 // window. Each of four waves keeps 16 RT key rows of the state as accumulators; the
-// sums over all rows (W S - U0, Q S + P U) meet in LDS, in wave order, with one
-// barrier a chunk: W S before it, Q S behind it, where it covers the wait for the
-// other waves' sums, and each wave's quarter of P U at the end. A fifth wave does
-// what is off the path from one state to the next: it brings U0 and the decays,
-// sums and stores the outputs a chunk later.
+// sums over all rows (W S - U0, Q S) meet in LDS, in wave order, with one barrier a
+// chunk: W S before it, Q S behind it, where it covers the wait for the other
+// waves' sums. A fifth wave does what is off the path from one state to the next: it
+// brings U0 and the decays, and adds up, completes (P U) and stores the outputs a
+// chunk later.
 //
 // 24 of a record's 27 KB are loaded as operands, 16 cycles of the CU's address
-// unit for each 1 KB, against 25 matrix instructions of 32 cycles on each SIMD.
+// unit for each 1 KB, against 24 matrix instructions of 32 cycles on each SIMD.
 // The four waves meet at the barrier, so their loads come at the same time: they
-// are spread over the step, a third behind each of its three products (in one
-// place they held the waves up for 500 cycles of 1900), two chunks ahead, and
-// without a branch (the last record again at the end), so that a wait leaves the
-// younger ones in flight.
+// are put between the products that follow it (in one place they held the waves
+// up for 500 cycles of 1900), two chunks ahead, and without a branch (the last
+// record again at the end), so that a wait leaves the younger ones in flight.
 constexpr int kScanWaves = 5;
 
 template <int DT, int RT>
@@ -677,22 +676,28 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
   if (wave == kScanWaves - 1) {
     if (steps == 0) return;
     const uint32_t values = static_cast<uint32_t>(L::kU + (ct * 64 + lane) * 4);
+    const uint32_t plane = static_cast<uint32_t>(L::kP + 4 * lane);
     const uint32_t decays = static_cast<uint32_t>(L::kD + lane * RT);
     typedef float row_t __attribute__((ext_vector_type(RT)));  // channels RT lane, ...
     const float* ahead = first;
-    f32x4_t u0, u1, u2;
-    row_t d0, d1, d2;
-    auto fetch = [&](f32x4_t& u, row_t& d) {
-      u = *reinterpret_cast<const f32x4_t*>(ahead + values);
-      d = *reinterpret_cast<const row_t*>(ahead + decays);
+    struct Record {
+      f32x4_t u, p;
+      row_t d;
+    };
+    auto fetch = [&](Record& f) {
+      f.u = *reinterpret_cast<const f32x4_t*>(ahead + values);
+      f.p = *reinterpret_cast<const f32x4_t*>(ahead + plane);
+      f.d = *reinterpret_cast<const row_t*>(ahead + decays);
       ahead = advance(ahead);
     };
-    auto hand_over = [&](int i, f32x4_t u, row_t d) {
-      parts[i & 1][4][lane] = -u;
-      reinterpret_cast<row_t*>(decay[i & 1])[lane] = d;
+    auto hand_over = [&](int i, const Record& f) {
+      parts[i & 1][4][lane] = -f.u;
+      reinterpret_cast<row_t*>(decay[i & 1])[lane] = f.d;
     };
-    // rows behind the sequence and columns behind the last go past the buffer's
-    // end: stores without a branch, which the compiler can count
+    // rows behind the sequence, columns behind the last and chunks not begun go
+    // past the buffer's end: stores without a branch. Behind a branch the
+    // compiler has to take them for not issued, and its waits for a record's
+    // loads then wait for the stores as well (0.17 us of 0.88 a chunk).
     const int64_t row_values = static_cast<int64_t>(a.heads) * a.d_v;
     T* out = static_cast<T*>(a.out) + (rows.begin + (lo - number) * kChunk) * row_values + h * a.d_v;
     int64_t left = rows.end - (rows.begin + (lo - number) * kChunk);
@@ -703,15 +708,23 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
                    ? static_cast<int>(((4 * g + r) * row_values + col) * static_cast<int>(sizeof(T)))
                    : static_cast<int>(0x80000000u);
     const float* rec = first;
-    auto finish = [&](int i) {  // chunk i of the window, behind the barrier of i + 1
+    // a chunk's outputs: begun behind the barrier of the next one, stored behind
+    // the one after that, so that no barrier waits for their products
+    auto begin = [&](int i, f32x4_t p, f32x4_t& u) {
       const f32x4_t(*const part)[kWave] = parts[i & 1];
+      u = part[9][lane];
       f32x4_t o = (part[5][lane] + part[6][lane]) + (part[7][lane] + part[8][lane]);
-      const f32x4_t u = part[9][lane];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        o = __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], u[r] - u[r] == 0.f ? u[r] : 0.f, o, 0, 0, 0);
+      return o;
+    };
+    auto store = [&](f32x4_t o, f32x4_t u, bool begun) {
       const bool fine = (u[0] - u[0]) + (u[1] - u[1]) + (u[2] - u[2]) + (u[3] - u[3]) == 0.f;
-      if (__builtin_expect(!__all(fine), 0)) {
+      if (__builtin_expect(begun && !__all(fine), 0)) {
         // infinities and NaNs, which P's zeros would hand to the steps before
-        // their own: the waves left them out of P U, and the steps from
-        // theirs on take them one by one
+        // their own: left out of P U, and taken one by one by the steps
+        // from theirs on
 #pragma unroll 1
         for (int j = 0; j < kChunk; ++j) {
           const float mine = (j & 2) ? ((j & 1) ? u[3] : u[2]) : ((j & 1) ? u[1] : u[0]);
@@ -724,7 +737,7 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
         }
       }
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(out, 0, 0x7FFFFFFF, 0x00020000);
-      const int live = left < kChunk ? static_cast<int>(left) : kChunk;
+      const int live = begun ? (left < kChunk ? static_cast<int>(left) : kChunk) : 0;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int at_r = 4 * g + r < live ? off[r] : static_cast<int>(0x80000000u);
@@ -733,29 +746,38 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
         else
           __builtin_amdgcn_raw_buffer_store_b16(from_f32<DT>(o[r]), rsrc, at_r, 0, 0);
       }
-      out += kChunk * row_values;
-      left -= kChunk;
-      rec += stride;
+      if (begun) {
+        out += kChunk * row_values;
+        left -= kChunk;
+        rec += stride;
+      }
     };
-    fetch(u0, d0);
-    fetch(u1, d1);
-    // (registers in turn: a copy of one on its way would wait for it)
-    auto turn = [&](int i, f32x4_t u, row_t d, f32x4_t& next_u, row_t& next_d) {
-      hand_over(i, u, d);
-      fetch(next_u, next_d);
+    // records three in turn, each until its outputs are begun (a copy of one on
+    // its way would wait for it)
+    Record f0, f1, f2;
+    f32x4_t p = {0.f, 0.f, 0.f, 0.f}, o = p, u = p;
+    fetch(f0);
+    fetch(f1);
+    auto turn = [&](int i, const Record& f, Record& next) {
+      hand_over(i, f);
+      fetch(next);
       __syncthreads();
-      if (i > 0) finish(i - 1);
+      store(o, u, i > 1);
+      o = begin(i - 1, p, u);  // (of nothing for i = 0)
+      p = f.p;
     };
     int i = 0;
     for (; i + 3 <= steps; i += 3) {
-      turn(i, u0, d0, u2, d2);
-      turn(i + 1, u1, d1, u0, d0);
-      turn(i + 2, u2, d2, u1, d1);
+      turn(i, f0, f2);
+      turn(i + 1, f1, f0);
+      turn(i + 2, f2, f1);
     }
-    if (i < steps) turn(i, u0, d0, u2, d2);
-    if (i + 1 < steps) turn(i + 1, u1, d1, u0, d0);
+    if (i < steps) turn(i, f0, f2);
+    if (i + 1 < steps) turn(i + 1, f1, f0);
     __syncthreads();
-    finish(steps - 1);
+    store(o, u, steps > 1);
+    o = begin(steps - 1, p, u);
+    store(o, u, true);
     return;
   }
 
@@ -771,27 +793,23 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
     }
   struct Record {
     f32x4_t w[RT], q[RT], k[RT];
-    float p;
   };
-  const uint32_t tiles = static_cast<uint32_t>((wave * RT * 64 + lane) * 4);
-  const uint32_t plane = static_cast<uint32_t>(L::kP + 4 * lane + wave);
-  const float* ahead = first;
-  auto fetch_w = [&](Record& f) {
+  // byte offsets into a record (32 bits behind a scalar base)
+  const uint32_t tiles = static_cast<uint32_t>((wave * RT * 64 + lane) * 16);
+  const uint32_t w_at = tiles + L::kW * 4, q_at = tiles + L::kQ * 4, k_at = tiles + L::kK * 4;
+  const char* ahead = reinterpret_cast<const char*>(first);
+  auto tile_at = [&](uint32_t off) { return *reinterpret_cast<const f32x4_t*>(ahead + off); };
+  auto fetch_wq = [&](Record& f) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-      f.w[t] = *reinterpret_cast<const f32x4_t*>(ahead + (tiles + L::kW + 256 * t));
-  };
-  auto fetch_q = [&](Record& f) {
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-      f.q[t] = *reinterpret_cast<const f32x4_t*>(ahead + (tiles + L::kQ + 256 * t));
+    for (int t = 0; t < RT; ++t) {
+      f.w[t] = tile_at(w_at + 1024 * t);
+      f.q[t] = tile_at(q_at + 1024 * t);
+    }
   };
   auto fetch_k = [&](Record& f) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-      f.k[t] = *reinterpret_cast<const f32x4_t*>(ahead + (tiles + L::kK + 256 * t));
-    f.p = ahead[plane];
-    ahead = advance(ahead);
+    for (int t = 0; t < RT; ++t) f.k[t] = tile_at(k_at + 1024 * t);
+    ahead = reinterpret_cast<const char*>(advance(reinterpret_cast<const float*>(ahead)));
   };
   auto step = [&](int i, const Record& f, Record& next) {
     f32x4_t(*const part)[kWave] = parts[i & 1];
@@ -801,7 +819,6 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         x = __builtin_amdgcn_mfma_f32_16x16x4f32(f.w[t][r], st[t][r], x, 0, 0, 0);
-    fetch_w(next);
     part[wave][lane] = x;
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);  // Q S is not to be moved up
@@ -814,30 +831,32 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < 4; ++r) {
         y = __builtin_amdgcn_mfma_f32_16x16x4f32(f.q[t][r], st[t][r], y, 0, 0, 0);
-    fetch_q(next);
+        if (r == 1) next.w[t] = tile_at(w_at + 1024 * t);
+        if (r == 3) next.q[t] = tile_at(q_at + 1024 * t);
+        if (r & 1) __builtin_amdgcn_sched_barrier(0);
+      }
     const f32x4_t u = -(((x0 + x1) + (x2 + x3)) + x4);
 #pragma unroll
     for (int t = 0; t < RT; ++t) st[t] *= d[t];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r) {
 #pragma unroll
       for (int t = 0; t < RT; ++t)
         st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.k[t][r], u[r], st[t], 0, 0, 0);
-    const float mine = wave & 2 ? (wave & 1 ? u[3] : u[2]) : (wave & 1 ? u[1] : u[0]);
-    y = __builtin_amdgcn_mfma_f32_16x16x4f32(f.p, mine - mine == 0.f ? mine : 0.f, y, 0, 0, 0);
-    fetch_k(next);
+      if (r < RT) next.k[r] = tile_at(k_at + 1024 * r);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    ahead = reinterpret_cast<const char*>(advance(reinterpret_cast<const float*>(ahead)));
     part[5 + wave][lane] = y;
     if (wave == 0) part[9][lane] = u;
   };
   if (steps > 0) {
     Record f0, f1, f2;  // in turn
-    fetch_w(f0);
-    fetch_q(f0);
+    fetch_wq(f0);
     fetch_k(f0);
-    fetch_w(f1);
-    fetch_q(f1);
+    fetch_wq(f1);
     fetch_k(f1);
     int i = 0;
     for (; i + 3 <= steps; i += 3) {
