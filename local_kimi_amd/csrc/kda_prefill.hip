@@ -351,13 +351,13 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(ScanArgs a,
 }
 
 // ---------------------------------------------------------------------------
-// The recurrence in chunks of 16 steps. Within a chunk with the state S before
+// The recurrence in chunks of 32 steps. Within a chunk with the state S before
 // it, D_i the product of e^g over its steps up to i (per key row) and D_(j,i] that
 // of the steps behind j up to i,
 //   A_ij = beta_j sum_d k_i k_j D_(j,i]   (j < i)
 //   P_ij = scale beta_j sum_d q_i k_j D_(j,i]   (j <= i)
 //   (I + A) [W | U0] = [k D | v]
-//   U = U0 - W S,   o = scale (q D) S + P U,   S = D_15 S + (beta k D_(.,15])^T U,
+//   U = U0 - W S,   o = scale (q D) S + P U,   S = D_31 S + (beta k D_(.,31])^T U,
 // which is the step form with its corrections u solved for together. Only the
 // last line follows from chunk to chunk, so one launch computes W, U0, P and the
 // scaled rows of every chunk (chunk_prepare_kernel) and another takes the
@@ -368,24 +368,33 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(ScanArgs a,
 // product of e^g <= 1 stays in [0, 1] with a relative error of 2^-24 a factor,
 // whatever the decays (a sum of logs of 100 would carry 2^-17 of error into its
 // exponential, a quotient of products overflows where a channel fades within
-// the chunk). That fixes the chunk at 16 steps: A and P cost 120 + 136
-// products of every channel in VALU work, 41 us of a GPU at 8192 tokens x 32 heads
-// of 128, and a longer chunk would square that.
+// the chunk). A and P then cost a product of every channel for every pair of
+// steps in VALU work, so they and W, U0 are computed for halves a, b of 16 steps
+// (120 + 136 pairs each) and the halves joined by matrix products: with
+// M = W_b (beta k D)_a^T over a's decays to its end,
+//   W_b <- W_b D_a - M W_a,  U0_b <- U0_b - M U0_a,  P_ba = (scale q D)_b (beta k D)_a^T,
+//   (q D)_b <- (q D)_b D_a,  (beta k D)_a <- (beta k D)_a D_b.
+// The scan is bound by what a chunk costs beside its products (a barrier and an
+// exchange through LDS, 0.35 us): chunks of 16 took 0.83 us each.
 //
 // Records. A chunk and head has one record in the workspace, its parts in the
 // order in which the second launch's lanes load them (16 bytes a lane, 1 KB a
-// wave): with m = lane % 16, g = lane / 16, r = 0..3,
-//   W, Q (scale q D):  [tile t][lane][r] = row m, channel 16 t + 4 g + r
-//   K (beta k D_(.,15]): [tile t][lane][r] = channel 16 t + m, step 4 g + r
-//   D (D_15):          [channel]
-//   P:                 [lane][r] = row m, column 4 g + r
-//   U0:                [tile t][lane][r] = value column 16 t + m, step 4 g + r
+// wave): with m = lane % 16, g = lane / 16, r = 0..3, half h
+//   W, Q (scale q D):    [h][tile t][lane][r] = row 16 h + m, channel 16 t + 4 g + r
+//   K (beta k D_(.,31]): [h][tile t][lane][r] = channel 16 t + m, step 16 h + 4 g + r
+//   D (D_31):            [channel]
+//   P:                   [aa, ba, bb][lane][r] = row m, column 4 g + r of that block
+//   U0:                  [h][tile t][lane][r] = value column 16 t + m, step 16 h + 4 g + r
 // These are the A operands of v_mfma_f32_16x16x4 for B operands that are the
 // accumulators of an earlier one as they stand: lane (m, g) of a 16 x 16 result
 // holds column m, rows 4 g + r, and register r of it serves as the rows 4 g + r of a
 // product over 16.
-constexpr int kChunk = 16;
-constexpr int kChunkThreads = 256;
+constexpr int kHalf = 16;
+constexpr int kChunk = 2 * kHalf;
+constexpr int kPrepareThreads = 512;  // four waves a half
+constexpr int kPass = 128;            // value columns solved at a time
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 struct ChunkArgs {
   float* records;
@@ -395,25 +404,12 @@ struct ChunkArgs {
 };
 
 template <int RT>
-struct ChunkLayout {  // float offsets of a record's parts; 64 RT channels
+struct ChunkLayout {  // float offsets of a record's parts; 64 RT channels, 4 RT tiles
   static constexpr int kChannels = 64 * RT;
+  static constexpr int kTiles = 4 * RT;
   static constexpr int kW = 0, kQ = kChannels * kChunk, kK = 2 * kChannels * kChunk,
-                       kD = 3 * kChannels * kChunk, kP = kD + kChannels, kU = kP + 256;
+                       kD = 3 * kChannels * kChunk, kP = kD + kChannels, kU = kP + 3 * 256;
 };
-
-// Four values of each lane of a quad, transposed: lane r gets value r of the four.
-__device__ inline void quad_transpose(float (&v)[4], int r) {
-  const bool odd = r & 1, high = r & 2;
-  float t0 = dpp_f32<kQuadXor1>(odd ? v[0] : v[1]), t1 = dpp_f32<kQuadXor1>(odd ? v[2] : v[3]);
-  const float a0 = odd ? t0 : v[0], a1 = odd ? v[1] : t0, a2 = odd ? t1 : v[2],
-              a3 = odd ? v[3] : t1;
-  t0 = dpp_f32<kQuadXor2>(high ? a0 : a2);
-  t1 = dpp_f32<kQuadXor2>(high ? a1 : a3);
-  v[0] = high ? t0 : a0;
-  v[1] = high ? t1 : a1;
-  v[2] = high ? a2 : t0;
-  v[3] = high ? a3 : t1;
-}
 
 // Sums of four values of each lane over the wave's four 16-lane rows: row g is left
 // with that of value (g & 1) + 2 (g >> 1), by two exchanges that each halve what a
@@ -439,14 +435,23 @@ __device__ inline int after(int at, float x) {
   return at;
 }
 
+__device__ inline f32x4_t lds4(const float* p) { return *reinterpret_cast<const f32x4_t*>(p); }
+
 template <int DT, int RT>
-__global__ void __launch_bounds__(kChunkThreads, 3) chunk_prepare_kernel(ScanArgs a, ChunkArgs c) {
+__global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanArgs a, ChunkArgs c) {
   using T = typename Storage<DT>::type;
   using L = ChunkLayout<RT>;
   constexpr int kStride = L::kChannels + 4;  // rows 16 bytes apart in the banks
+  constexpr int kVStride = kPass + 4;
+  // rows of q, k, e^g; then of scale q D, beta k D, W
   __shared__ alignas(16) float sq[kChunk][kStride], sk[kChunk][kStride], sg[kChunk][kStride];
-  __shared__ float part[2][4][kChunk * kChunk];
-  __shared__ alignas(16) float sa[kChunk][kChunk];
+  __shared__ alignas(16) union {
+    float part[2][2][4][kHalf * kHalf];  // the waves' sums for A and P of each half
+    float u[kChunk][kVStride];           // U0 of one pass
+  } sx;
+  __shared__ alignas(16) float sa[2][kHalf][kHalf];
+  __shared__ f32x4_t sm[8][kWave];  // the waves' sums for M and P_ba
+  __shared__ alignas(16) float sd[2][L::kChannels];
   __shared__ float sb[kChunk];
   const int h = static_cast<int>(blockIdx.x % a.heads);
   const int64_t local = blockIdx.x / a.heads;
@@ -455,25 +460,27 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_prepare_kernel(ScanArg
   const RowRange rows = sequence_rows(a.seq, at.sequence);
   const int64_t t0 = rows.begin + at.tile * kChunk;
   if (t0 >= rows.end) return;
-  const int tid = threadIdx.x, i16 = tid >> 4, l = tid & 15;
-  const int wave = tid / kWave, lane = tid & (kWave - 1);
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), l = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int half = wave >> 2, in_half = tid & 255, w4 = wave & 3;
 
-  // this thread's first value column (threads behind those of the channels)
-  float v_first[kChunk];
-  {
-    const int vc = tid - L::kChannels;
-    const int at_v = vc >= 0 && vc < a.d_v ? vc : 0;
+  // this thread's value column of the first pass (the upper threads of a half)
+  float x[kHalf];
+  auto load_values = [&](int vc) {
+    const int from = vc >= 0 && vc < a.d_v ? vc : 0;
+    const int64_t th = t0 + kHalf * half;
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-      const int64_t t = t0 + i < rows.end ? t0 + i : t0;
-      v_first[i] = to_f32<DT>(static_cast<const T*>(a.v)[(t * a.heads + h) * a.d_v + at_v]);
+    for (int i = 0; i < kHalf; ++i) {
+      const int64_t t = th + i < rows.end ? th + i : t0;
+      x[i] = to_f32<DT>(static_cast<const T*>(a.v)[(t * a.heads + h) * a.d_v + from]);
     }
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i)
-      v_first[i] = t0 + i < rows.end && at_v == vc ? v_first[i] : 0.f;
-  }
+    for (int i = 0; i < kHalf; ++i) x[i] = th + i < rows.end && from == vc ? x[i] : 0.f;
+  };
+  load_values(in_half - kPass);
   {  // steps behind the sequence's end: no decay, no key, no query
-    const int64_t t = t0 + i16;
+    const int row = tid >> 4;
+    const int64_t t = t0 + row;
     const bool ok = t < rows.end;
     const int64_t base = ((ok ? t : t0) * a.heads + h) * a.d_k;
     float qs[RT][4], ks[RT][4], gs[RT][4];
@@ -488,159 +495,191 @@ __global__ void __launch_bounds__(kChunkThreads, 3) chunk_prepare_kernel(ScanArg
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       const int d = 4 * (l + 16 * i);
-      float(&q)[4] = qs[i], (&k)[4] = ks[i], (&g)[4] = gs[i];
+      float(&q)[4] = qs[i], (&k)[4] = ks[i], (&e)[4] = gs[i];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) g[x] = expf(g[x]);
-      *reinterpret_cast<float4*>(&sq[i16][d]) = make_float4(q[0], q[1], q[2], q[3]);
-      *reinterpret_cast<float4*>(&sk[i16][d]) = make_float4(k[0], k[1], k[2], k[3]);
-      *reinterpret_cast<float4*>(&sg[i16][d]) = make_float4(g[0], g[1], g[2], g[3]);
+      for (int y = 0; y < 4; ++y) e[y] = expf(e[y]);
+      *reinterpret_cast<float4*>(&sq[row][d]) = make_float4(q[0], q[1], q[2], q[3]);
+      *reinterpret_cast<float4*>(&sk[row][d]) = make_float4(k[0], k[1], k[2], k[3]);
+      *reinterpret_cast<float4*>(&sg[row][d]) = make_float4(e[0], e[1], e[2], e[3]);
     }
-    if (l == 0) sb[i16] = ok ? beta : 0.f;
+    if (l == 0) sb[row] = ok ? beta : 0.f;
   }
   __syncthreads();
 
-  // A and P: lane (j, g) of wave w has key j against every row i >= j, over a
-  // 16th of the channels; its product of decays runs along with i. Rows i < j
-  // are dropped below.
+  // A and P of a half: lane (j, g) of wave w has key j against every row i >= j,
+  // over a 16th of the channels; its product of decays runs along with i. Rows
+  // i < j are dropped below.
   {
-    const float beta = sb[l];
-    const int g = lane >> 4, d0 = wave * 16 * RT + g * 4 * RT;
-    float4 f[RT];
+    const float beta = sb[kHalf * half + l];
+    const int d0 = w4 * 16 * RT + g * 4 * RT;
+    f32x4_t f[RT];
 #pragma unroll 1
-    for (int i0 = 0; i0 < kChunk; i0 += 4) {  // four rows at a time
+    for (int i0 = 0; i0 < kHalf; i0 += 4) {  // four rows at a time
       float kk[4] = {0.f, 0.f, 0.f, 0.f}, qk[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < RT; ++x) {
-        const int d = d0 + 4 * x;
-        const float4 own = *reinterpret_cast<const float4*>(&sk[l][d]);
+      for (int y = 0; y < RT; ++y) {
+        const int d = d0 + 4 * y;
+        const f32x4_t own = lds4(&sk[kHalf * half + l][d]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 e = *reinterpret_cast<const float4*>(&sg[i0 + i][d]);
-          const float4 k = *reinterpret_cast<const float4*>(&sk[i0 + i][d]);
-          const float4 q = *reinterpret_cast<const float4*>(&sq[i0 + i][d]);
+          const int row = kHalf * half + i0 + i;
+          const f32x4_t e = lds4(&sg[row][d]), k = lds4(&sk[row][d]), q = lds4(&sq[row][d]);
           const bool first = i0 + i <= l;
-          f[x].x = first ? own.x * beta : f[x].x * e.x;
-          f[x].y = first ? own.y * beta : f[x].y * e.y;
-          f[x].z = first ? own.z * beta : f[x].z * e.z;
-          f[x].w = first ? own.w * beta : f[x].w * e.w;
-          kk[i] = fmaf(k.x, f[x].x, fmaf(k.y, f[x].y, fmaf(k.z, f[x].z, fmaf(k.w, f[x].w, kk[i]))));
-          qk[i] = fmaf(q.x, f[x].x, fmaf(q.y, f[x].y, fmaf(q.z, f[x].z, fmaf(q.w, f[x].w, qk[i]))));
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            f[y][z] = first ? own[z] * beta : f[y][z] * e[z];
+            kk[i] = fmaf(k[z], f[y][z], kk[i]);
+            qk[i] = fmaf(q[z], f[y][z], qk[i]);
+          }
         }
       }
       const int i = i0 + (g & 1) + 2 * (g >> 1);
-      part[0][wave][i * 16 + l] = rows_reduce(kk);
-      part[1][wave][i * 16 + l] = rows_reduce(qk);
+      sx.part[half][0][w4][i * kHalf + l] = rows_reduce(kk);
+      sx.part[half][1][w4][i * kHalf + l] = rows_reduce(qk);
     }
   }
   __syncthreads();
   float* const rec = c.records + (local * a.heads + h) * c.record;
   {
-    const float kk = (part[0][0][tid] + part[0][1][tid]) + (part[0][2][tid] + part[0][3][tid]);
-    const float qk = (part[1][0][tid] + part[1][1][tid]) + (part[1][2][tid] + part[1][3][tid]);
-    sa[i16][l] = l < i16 ? kk : 0.f;
-    rec[L::kP + (i16 + 16 * (l >> 2)) * 4 + (l & 3)] = l <= i16 ? a.scale * qk : 0.f;
+    const int i = in_half >> 4;
+    const auto& kk = sx.part[half][0];
+    const auto& qk = sx.part[half][1];
+    const float as = (kk[0][in_half] + kk[1][in_half]) + (kk[2][in_half] + kk[3][in_half]);
+    const float ps = (qk[0][in_half] + qk[1][in_half]) + (qk[2][in_half] + qk[3][in_half]);
+    sa[half][i][l] = l < i ? as : 0.f;
+    rec[L::kP + 512 * half + (i + 16 * (l >> 2)) * 4 + (l & 3)] = l <= i ? a.scale * ps : 0.f;
   }
   __syncthreads();
 
-  // columns of [W | U0]: one thread solves a column, row by row
-  const int columns = L::kChannels + 16 * c.v_tiles;
-  for (int col = tid; col < columns; col += kChunkThreads) {
-    float x[kChunk];
-    const bool key = col < L::kChannels;  // uniform in each wave: 64 channels apart
-    const int vc = col - L::kChannels;
-    if (key) {
-      float keep = 1.f;
-      float q[kChunk];
+  // columns of [W | U0] of a half: one thread solves a column, row by row
+  auto solve = [&]() {
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) {
-        keep *= sg[i][col];
-        x[i] = sk[i][col] * keep;
-        q[i] = sq[i][col] * (a.scale * keep);
-      }
-      const int t = col >> 4, g = (col >> 2) & 3, r = col & 3;
-#pragma unroll
-      for (int m = 0; m < kChunk; m += 4) {
-        float y[4] = {q[m], q[m + 1], q[m + 2], q[m + 3]};
-        quad_transpose(y, r);
-        *reinterpret_cast<float4*>(rec + L::kQ + (t * 64 + m + r + 16 * g) * 4) =
-            make_float4(y[0], y[1], y[2], y[3]);
-      }
-      float left = 1.f, kept[kChunk];
-#pragma unroll
-      for (int j = kChunk - 1; j >= 0; --j) {
-        kept[j] = sb[j] * sk[j][col] * left;
-        left *= sg[j][col];
-      }
-#pragma unroll
-      for (int m = 0; m < kChunk; m += 4)
-        *reinterpret_cast<float4*>(rec + L::kK + (t * 64 + (col & 15) + 4 * m) * 4) =
-            make_float4(kept[m], kept[m + 1], kept[m + 2], kept[m + 3]);
-      rec[L::kD + col] = keep;
-    } else if (col == tid) {
-#pragma unroll
-      for (int i = 0; i < kChunk; ++i) x[i] = v_first[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < kChunk; ++i)
-        x[i] = t0 + i < rows.end && vc < a.d_v
-                   ? to_f32<DT>(static_cast<const T*>(a.v)[((t0 + i) * a.heads + h) * a.d_v + vc])
-                   : 0.f;
-    }
-#pragma unroll
-    for (int i = 1; i < kChunk; ++i) {
-      const int at0 = i < 4 ? 0 : after(0, x[i - 4]);  // three rows of A ahead
+    for (int i = 1; i < kHalf; ++i) {
+      const int from = i < 4 ? 0 : after(0, x[i - 4]);  // three rows of A ahead
 #pragma unroll
       for (int j = 0; j < i; j += 4) {
-        const float4 r = *reinterpret_cast<const float4*>(&sa[i][4 * at0 + j]);
-        const float rj[4] = {r.x, r.y, r.z, r.w};
+        const f32x4_t r = lds4(&sa[half][i][4 * from + j]);
 #pragma unroll
         for (int y = 0; y < 4; ++y)
-          if (j + y < i) x[i] = fmaf(-rj[y], x[j + y], x[i]);
+          if (j + y < i) x[i] = fmaf(-r[y], x[j + y], x[i]);
       }
     }
-    if (key) {
-      const int t = col >> 4, g = (col >> 2) & 3, r = col & 3;
+  };
+  const int row0 = kHalf * half;
+  if (in_half < L::kChannels) {
+    const int col = in_half;  // read and replaced by this thread alone
+    float left = 1.f, kept[kHalf];
 #pragma unroll
-      for (int m = 0; m < kChunk; m += 4) {
-        float y[4] = {x[m], x[m + 1], x[m + 2], x[m + 3]};
-        quad_transpose(y, r);
-        *reinterpret_cast<float4*>(rec + L::kW + (t * 64 + m + r + 16 * g) * 4) =
-            make_float4(y[0], y[1], y[2], y[3]);
-      }
-    } else {
-#pragma unroll
-      for (int m = 0; m < kChunk; m += 4)
-        *reinterpret_cast<float4*>(rec + L::kU + ((vc >> 4) * 64 + (vc & 15) + 4 * m) * 4) =
-            make_float4(x[m], x[m + 1], x[m + 2], x[m + 3]);
+    for (int j = kHalf - 1; j >= 0; --j) {
+      kept[j] = sb[row0 + j] * sk[row0 + j][col] * left;
+      left *= sg[row0 + j][col];
     }
+    float keep = 1.f;
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) {
+      keep *= sg[row0 + i][col];
+      x[i] = sk[row0 + i][col] * keep;
+      sq[row0 + i][col] *= a.scale * keep;
+      sk[row0 + i][col] = kept[i];
+    }
+    sd[half][col] = keep;
+    solve();
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) sg[row0 + i][col] = x[i];
+  } else if (in_half >= kPass) {
+    solve();
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) sx.u[row0 + i][in_half - kPass] = x[i];
+  }
+  __syncthreads();
+
+  // M (waves 0 to 3) and P_ba (4 to 7), a quarter of the channels each; both
+  // transposed: lane (row of b, g), register r = step 4 g + r of a
+  {
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int y = 0; y < RT; ++y) {
+      const int d = 16 * (w4 * RT + y) + 4 * g;
+      const f32x4_t ka = lds4(&sk[l][d]);
+      const f32x4_t rb = half ? lds4(&sq[kHalf + l][d]) : lds4(&sg[kHalf + l][d]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(ka[r], rb[r], acc, 0, 0, 0);
+    }
+    sm[wave][lane] = acc;
+  }
+  __syncthreads();
+  const f32x4_t mt = (sm[0][lane] + sm[1][lane]) + (sm[2][lane] + sm[3][lane]);
+  auto put = [&](int off, f32x4_t v) { *reinterpret_cast<f32x4_t*>(rec + off + 4 * lane) = v; };
+  if (wave == 4) put(L::kP + 256, (sm[4][lane] + sm[5][lane]) + (sm[6][lane] + sm[7][lane]));
+  for (int t = wave; t < L::kTiles; t += kPrepareThreads / kWave) {
+    const int d = 16 * t + 4 * g, ch = 16 * t + l;
+    const f32x4_t da = lds4(&sd[0][d]), db = lds4(&sd[1][d]);
+    const float db_ch = sd[1][ch];
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f}, ka, kb;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(sg[4 * g + r][ch], mt[r], acc, 0, 0, 0);
+      ka[r] = sk[4 * g + r][ch] * db_ch;
+      kb[r] = sk[kHalf + 4 * g + r][ch];
+    }
+    put(L::kQ + 256 * t, lds4(&sq[l][d]));
+    put(L::kQ + 256 * (L::kTiles + t), lds4(&sq[kHalf + l][d]) * da);
+    put(L::kK + 256 * t, ka);
+    put(L::kK + 256 * (L::kTiles + t), kb);
+    put(L::kW + 256 * t, lds4(&sg[l][d]));
+    put(L::kW + 256 * (L::kTiles + t), lds4(&sg[kHalf + l][d]) * da - acc);
+    if (l == 0) *reinterpret_cast<f32x4_t*>(rec + L::kD + d) = da * db;
+  }
+  for (int first = 0;;) {
+    const int ct = first / 16 + wave;
+    if (ct < c.v_tiles) {
+      f32x4_t ua, ub, acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        ua[r] = sx.u[4 * g + r][16 * wave + l];
+        ub[r] = sx.u[kHalf + 4 * g + r][16 * wave + l];
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(mt[r], ua[r], acc, 0, 0, 0);
+      }
+      put(L::kU + 256 * ct, ua);
+      put(L::kU + 256 * (c.v_tiles + ct), ub - acc);
+    }
+    first += kPass;
+    if (first >= 16 * c.v_tiles) break;
+    __syncthreads();
+    if (in_half >= kPass) {
+      load_values(first + in_half - kPass);
+      solve();
+#pragma unroll
+      for (int i = 0; i < kHalf; ++i) sx.u[row0 + i][in_half - kPass] = x[i];
+    }
+    __syncthreads();
   }
 }
-
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 // Block = one sequence's and head's 16 value columns, through the chunks of the
 // window. Each of four waves keeps 16 RT key rows of the state as accumulators; the
 // sums over all rows (W S - U0, Q S) meet in LDS, in wave order, with one barrier a
 // chunk: W S before it, Q S behind it, where it covers the wait for the other
-// waves' sums. A fifth wave does what is off the path from one state to the next: it
-// brings U0 and the decays, and adds up, completes (P U) and stores the outputs a
-// chunk later.
+// waves' sums. Two more waves, one for each half, do what is off the path from one
+// state to the next: they bring U0 and the decays, and add up, complete (P U) and
+// store the outputs, a chunk later.
 //
-// 24 of a record's 27 KB are loaded as operands, 16 cycles of the CU's address
-// unit for each 1 KB, against 24 matrix instructions of 32 cycles on each SIMD.
+// 48 of a record's 58 KB are loaded as operands, 16 cycles of the CU's address
+// unit for each 1 KB, against 48 matrix instructions of 32 cycles on each SIMD.
 // The four waves meet at the barrier, so their loads come at the same time: they
 // are put between the products that follow it (in one place they held the waves
 // up for 500 cycles of 1900), two chunks ahead, and without a branch (the last
 // record again at the end), so that a wait leaves the younger ones in flight.
-constexpr int kScanWaves = 5;
+constexpr int kScanWaves = 6;
 
 template <int DT, int RT>
 __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
   using T = typename Storage<DT>::type;
   using L = ChunkLayout<RT>;
-  // of the last two chunks: the waves' W S, - U0, the waves' outputs, U; D
-  __shared__ f32x4_t parts[2][10][kWave];
-  __shared__ f32x4_t decay[2][4 * 4 * RT];
+  // of the last two chunks and each half: the waves' W S, - U0, the waves' Q S, U; D
+  __shared__ f32x4_t parts[2][2][10][kWave];
+  __shared__ f32x4_t decay[2][L::kTiles * 4];
   // the column tiles of a head, which read the same records, lie 8 blocks apart:
   // on one XCD, whose cache then holds a record for all of them
   const int64_t span = 8 * c.v_tiles, at = blockIdx.x % span;
@@ -668,52 +707,64 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
   const int64_t hi = end_all < c.first + c.count ? end_all : c.first + c.count;
   if (lo >= hi) return;
   const int steps = chunks > 0 ? static_cast<int>(hi - lo) : 0;
-  const int64_t stride = static_cast<int64_t>(a.heads) * c.record;  // a chunk's record to the next
-  const float* const first = c.records + ((lo - c.first) * a.heads + h) * c.record;
-  const float* const last = first + (hi - lo - 1) * stride;
-  auto advance = [&](const float* rec) { return rec < last ? rec + stride : last; };
+  const int64_t stride = static_cast<int64_t>(a.heads) * c.record * 4;  // bytes from record to record
+  const char* const first =
+      reinterpret_cast<const char*>(c.records + ((lo - c.first) * a.heads + h) * c.record);
+  const char* const last = first + (hi - lo - 1) * stride;
+  // a record's parts at 32-bit byte offsets behind a scalar base
+  const char* ahead = first;
+  auto part_at = [&](uint32_t off) { return *reinterpret_cast<const f32x4_t*>(ahead + off); };
+  auto advance = [&]() { ahead = ahead < last ? ahead + stride : last; };
 
-  if (wave == kScanWaves - 1) {
+  if (wave >= 4) {
     if (steps == 0) return;
-    const uint32_t values = static_cast<uint32_t>(L::kU + (ct * 64 + lane) * 4);
-    const uint32_t plane = static_cast<uint32_t>(L::kP + 4 * lane);
-    const uint32_t decays = static_cast<uint32_t>(L::kD + lane * RT);
+    const int half = wave - 4;
+    const uint32_t values = static_cast<uint32_t>((L::kU + ((half * c.v_tiles + ct) * 64 + lane) * 4) * 4);
+    const uint32_t planes = static_cast<uint32_t>((L::kP + 4 * lane) * 4);
+    const uint32_t decays = static_cast<uint32_t>((L::kD + lane * RT) * 4);
     typedef float row_t __attribute__((ext_vector_type(RT)));  // channels RT lane, ...
-    const float* ahead = first;
     struct Record {
-      f32x4_t u, p;
+      f32x4_t u, p, pba;
       row_t d;
     };
     auto fetch = [&](Record& f) {
-      f.u = *reinterpret_cast<const f32x4_t*>(ahead + values);
-      f.p = *reinterpret_cast<const f32x4_t*>(ahead + plane);
+      f.u = part_at(values);
+      f.p = part_at(planes + 2048 * half);
+      f.pba = part_at(planes + 1024);
       f.d = *reinterpret_cast<const row_t*>(ahead + decays);
-      ahead = advance(ahead);
+      advance();
     };
     auto hand_over = [&](int i, const Record& f) {
-      parts[i & 1][4][lane] = -f.u;
-      reinterpret_cast<row_t*>(decay[i & 1])[lane] = f.d;
+      parts[i & 1][half][4][lane] = -f.u;
+      if (half == 0) reinterpret_cast<row_t*>(decay[i & 1])[lane] = f.d;
     };
     // rows behind the sequence, columns behind the last and chunks not begun go
     // past the buffer's end: stores without a branch. Behind a branch the
     // compiler has to take them for not issued, and its waits for a record's
-    // loads then wait for the stores as well (0.17 us of 0.88 a chunk).
+    // loads then wait for the stores as well (0.06 us a chunk).
     const int64_t row_values = static_cast<int64_t>(a.heads) * a.d_v;
-    T* out = static_cast<T*>(a.out) + (rows.begin + (lo - number) * kChunk) * row_values + h * a.d_v;
-    int64_t left = rows.end - (rows.begin + (lo - number) * kChunk);
+    const int64_t row0 = rows.begin + (lo - number) * kChunk + kHalf * half;
+    T* out = static_cast<T*>(a.out) + row0 * row_values + h * a.d_v;
+    int64_t left = rows.end - row0;
     int off[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       off[r] = col < a.d_v
                    ? static_cast<int>(((4 * g + r) * row_values + col) * static_cast<int>(sizeof(T)))
                    : static_cast<int>(0x80000000u);
-    const float* rec = first;
+    const char* rec = first;
     // a chunk's outputs: begun behind the barrier of the next one, stored behind
     // the one after that, so that no barrier waits for their products
-    auto begin = [&](int i, f32x4_t p, f32x4_t& u) {
-      const f32x4_t(*const part)[kWave] = parts[i & 1];
+    auto begin = [&](int i, const f32x4_t& p, const f32x4_t& pba, f32x4_t& u) {
+      const f32x4_t(*const part)[kWave] = parts[i & 1][half];
       u = part[9][lane];
       f32x4_t o = (part[5][lane] + part[6][lane]) + (part[7][lane] + part[8][lane]);
+      if (half) {
+        const f32x4_t ua = parts[i & 1][0][9][lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          o = __builtin_amdgcn_mfma_f32_16x16x4f32(pba[r], ua[r], o, 0, 0, 0);
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         o = __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], u[r] - u[r] == 0.f ? u[r] : 0.f, o, 0, 0, 0);
@@ -725,19 +776,20 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
         // infinities and NaNs, which P's zeros would hand to the steps before
         // their own: left out of P U, and taken one by one by the steps
         // from theirs on
+        const float* const p = reinterpret_cast<const float*>(rec) + L::kP + 512 * half;
 #pragma unroll 1
-        for (int j = 0; j < kChunk; ++j) {
+        for (int j = 0; j < kHalf; ++j) {
           const float mine = (j & 2) ? ((j & 1) ? u[3] : u[2]) : ((j & 1) ? u[1] : u[0]);
           const float uj = __shfl(mine, m + 16 * (j >> 2));
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float pij = rec[L::kP + ((4 * g + r) + 16 * (j >> 2)) * 4 + (j & 3)];
+            const float pij = p[((4 * g + r) + 16 * (j >> 2)) * 4 + (j & 3)];
             if (j <= 4 * g + r && uj - uj != 0.f) o[r] = fmaf(pij, uj, o[r]);
           }
         }
       }
       const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(out, 0, 0x7FFFFFFF, 0x00020000);
-      const int live = begun ? (left < kChunk ? static_cast<int>(left) : kChunk) : 0;
+      const int live = begun ? (left < kHalf ? static_cast<int>(left) : kHalf) : 0;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int at_r = 4 * g + r < live ? off[r] : static_cast<int>(0x80000000u);
@@ -755,7 +807,7 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
     // records three in turn, each until its outputs are begun (a copy of one on
     // its way would wait for it)
     Record f0, f1, f2;
-    f32x4_t p = {0.f, 0.f, 0.f, 0.f}, o = p, u = p;
+    f32x4_t p = {0.f, 0.f, 0.f, 0.f}, pba = p, o = p, u = p;
     fetch(f0);
     fetch(f1);
     auto turn = [&](int i, const Record& f, Record& next) {
@@ -763,8 +815,9 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
       fetch(next);
       __syncthreads();
       store(o, u, i > 1);
-      o = begin(i - 1, p, u);  // (of nothing for i = 0)
+      o = begin(i - 1, p, pba, u);  // (of nothing for i = 0)
       p = f.p;
+      pba = f.pba;
     };
     int i = 0;
     for (; i + 3 <= steps; i += 3) {
@@ -776,7 +829,7 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
     if (i + 1 < steps) turn(i + 1, f1, f0);
     __syncthreads();
     store(o, u, steps > 1);
-    o = begin(steps - 1, p, u);
+    o = begin(steps - 1, p, pba, u);
     store(o, u, true);
     return;
   }
@@ -792,39 +845,41 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
       st[t][r] = row < a.d_k && col < a.d_v ? src[sbase + static_cast<int64_t>(row) * a.d_v + col] : 0.f;
     }
   struct Record {
-    f32x4_t w[RT], q[RT], k[RT];
+    f32x4_t w[2][RT], q[2][RT], k[2][RT];
   };
-  // byte offsets into a record (32 bits behind a scalar base)
+  constexpr uint32_t kHalfBytes = L::kTiles * 1024;
   const uint32_t tiles = static_cast<uint32_t>((wave * RT * 64 + lane) * 16);
   const uint32_t w_at = tiles + L::kW * 4, q_at = tiles + L::kQ * 4, k_at = tiles + L::kK * 4;
-  const char* ahead = reinterpret_cast<const char*>(first);
-  auto tile_at = [&](uint32_t off) { return *reinterpret_cast<const f32x4_t*>(ahead + off); };
-  auto fetch_wq = [&](Record& f) {
+  auto fetch = [&](Record& f) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      f.w[t] = tile_at(w_at + 1024 * t);
-      f.q[t] = tile_at(q_at + 1024 * t);
-    }
-  };
-  auto fetch_k = [&](Record& f) {
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-    for (int t = 0; t < RT; ++t) f.k[t] = tile_at(k_at + 1024 * t);
-    ahead = reinterpret_cast<const char*>(advance(reinterpret_cast<const float*>(ahead)));
+      for (int t = 0; t < RT; ++t) {
+        f.w[x][t] = part_at(w_at + kHalfBytes * x + 1024 * t);
+        f.q[x][t] = part_at(q_at + kHalfBytes * x + 1024 * t);
+        f.k[x][t] = part_at(k_at + kHalfBytes * x + 1024 * t);
+      }
+    advance();
   };
   auto step = [&](int i, const Record& f, Record& next) {
-    f32x4_t(*const part)[kWave] = parts[i & 1];
-    f32x4_t x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+    f32x4_t(*const part)[10][kWave] = parts[i & 1];
+    f32x4_t x[2] = {}, y[2] = {};
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        x = __builtin_amdgcn_mfma_f32_16x16x4f32(f.w[t][r], st[t][r], x, 0, 0, 0);
-    part[wave][lane] = x;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          x[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.w[b][t][r], st[t][r], x[b], 0, 0, 0);
+    part[0][wave][lane] = x[0];
+    part[1][wave][lane] = x[1];
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);  // Q S is not to be moved up
-    const f32x4_t x0 = part[0][lane], x1 = part[1][lane], x2 = part[2][lane], x3 = part[3][lane],
-                  x4 = part[4][lane];
-    f32x4_t d[RT];
+    f32x4_t xs[2][5], d[RT];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int w = 0; w < 5; ++w) xs[b][w] = part[b][w][lane];
 #pragma unroll
     for (int t = 0; t < RT; ++t) d[t] = decay[i & 1][(wave * RT + t) * 4 + g];
     __builtin_amdgcn_sched_barrier(0);
@@ -832,32 +887,40 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        y = __builtin_amdgcn_mfma_f32_16x16x4f32(f.q[t][r], st[t][r], y, 0, 0, 0);
-        if (r == 1) next.w[t] = tile_at(w_at + 1024 * t);
-        if (r == 3) next.q[t] = tile_at(q_at + 1024 * t);
-        if (r & 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          y[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.q[b][t][r], st[t][r], y[b], 0, 0, 0);
+        const uint32_t off = kHalfBytes * (r & 1) + 1024 * t;
+        if (r < 2) next.w[r & 1][t] = part_at(w_at + off);
+        else next.q[r & 1][t] = part_at(q_at + off);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    const f32x4_t u = -(((x0 + x1) + (x2 + x3)) + x4);
+    f32x4_t u[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      u[b] = -(((xs[b][0] + xs[b][1]) + (xs[b][2] + xs[b][3])) + xs[b][4]);
 #pragma unroll
     for (int t = 0; t < RT; ++t) st[t] *= d[t];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int t = 0; t < RT; ++t)
-        st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.k[t][r], u[r], st[t], 0, 0, 0);
-      if (r < RT) next.k[r] = tile_at(k_at + 1024 * r);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    ahead = reinterpret_cast<const char*>(advance(reinterpret_cast<const float*>(ahead)));
-    part[5 + wave][lane] = y;
-    if (wave == 0) part[9][lane] = u;
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+          st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.k[b][t][r], u[b][r], st[t], 0, 0, 0);
+        if (r < RT) next.k[b][r] = part_at(k_at + kHalfBytes * b + 1024 * r);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    advance();
+    part[0][5 + wave][lane] = y[0];
+    part[1][5 + wave][lane] = y[1];
+    if (wave == 0) part[0][9][lane] = u[0];
+    if (wave == 1) part[1][9][lane] = u[1];
   };
   if (steps > 0) {
     Record f0, f1, f2;  // in turn
-    fetch_wq(f0);
-    fetch_k(f0);
-    fetch_wq(f1);
-    fetch_k(f1);
+    fetch(f0);
+    fetch(f1);
     int i = 0;
     for (; i + 3 <= steps; i += 3) {
       step(i, f0, f2);
@@ -866,7 +929,7 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
     }
     if (i < steps) step(i, f0, f2);
     if (i + 1 < steps) step(i + 1, f1, f0);
-    __syncthreads();  // the last chunk's outputs and U, for the fifth wave
+    __syncthreads();  // the last chunk's Q S and U, for the last two waves
   }
 #pragma unroll
   for (int t = 0; t < RT; ++t)
@@ -935,12 +998,12 @@ int launch_serial(const ScanArgs& a, hipStream_t s) {
 // Floats of a chunk's and head's record.
 int64_t chunk_record(int64_t d_k, int64_t d_v) {
   const int64_t channels = d_k <= 64 ? 64 : 128;
-  return channels * (3 * kChunk + 1) + 256 + (d_v + 15) / 16 * 16 * kChunk;
+  return channels * (3 * kChunk + 1) + 3 * 256 + (d_v + 15) / 16 * 16 * kChunk;
 }
 
 // Chunks of one window: the records of a window are written by one launch and
 // read by the next, so they are kept within the 256 MB cache in front of HBM.
-constexpr int64_t kWindowBytes = int64_t{128} << 20;
+constexpr int64_t kWindowBytes = int64_t{256} << 20;
 int64_t chunk_window(int64_t chunks, int64_t heads, int64_t record) {
   const int64_t most = kWindowBytes / (heads * record * 4);
   const int64_t w = most < 1 ? 1 : most;
@@ -968,7 +1031,7 @@ int launch_chunks(const ScanArgs& a, float* records, hipStream_t s) {
   for (c.first = 0; c.first < chunks; c.first += window) {
     c.count = window < chunks - c.first ? window : chunks - c.first;
     chunk_prepare_kernel<DT, RT>
-        <<<static_cast<unsigned>(c.count * a.heads), kChunkThreads, 0, s>>>(a, c);
+        <<<static_cast<unsigned>(c.count * a.heads), kPrepareThreads, 0, s>>>(a, c);
     if (const int st = check_launch("lk_kda_prefill")) return st;
     chunk_scan_kernel<DT, RT><<<static_cast<unsigned>(scans), kScanWaves * kWave, 0, s>>>(a, c);
     if (const int st = check_launch("lk_kda_prefill")) return st;
