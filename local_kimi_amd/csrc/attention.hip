@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
           for (int r = 0; r < 16; ++r) {
             const int d = 32 * t + 8 * (r / 4) + 4 * half + r % 4;
             const float x = d < a.d_v && key <= qi + ahead ? value_of<BF16>(row[d]) : 0.f;
-            if (x - x != 0.f) o[t][r] += x;
+            if (!(fabsf(x) < INFINITY)) o[t][r] += x;
           }
       }
     }

@@ -403,13 +403,59 @@ struct ChunkArgs {
   int v_tiles;           // 16-column tiles of d_v
 };
 
-template <int RT>
-struct ChunkLayout {  // float offsets of a record's parts; 64 RT channels, 4 RT tiles
-  static constexpr int kChannels = 64 * RT;
-  static constexpr int kTiles = 4 * RT;
+template <int NW>
+struct ChunkLayout {  // float offsets of a record's parts; 32 NW channels, 2 NW tiles
+  static constexpr int kChannels = 32 * NW;
+  static constexpr int kTiles = 2 * NW;
   static constexpr int kW = 0, kQ = kChannels * kChunk, kK = 2 * kChannels * kChunk,
-                       kD = 3 * kChannels * kChunk, kP = kD + kChannels, kU = kP + 3 * 256;
+                       kD = 3 * kChannels * kChunk, kP = kD + kChannels, kS = kP + 3 * 256,
+                       kU = kS + 2 * kChunk + 16;
 };
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+// Eight fp32 values as the sums of two fp16 each, hi + lo, of 2^k times them.
+struct Split {
+  f16x8_t hi, lo;
+};
+// 2^k that brings the largest magnitude to [2^14, 2^15), as fp32 (at most 2^127),
+// and its inverse. A value down to 2^-16 of the largest keeps 22 bits, a smaller one
+// 2^-39 of the largest.
+struct Scale {
+  float up, down;
+};
+__device__ inline Scale scale_for(float largest) {
+  const uint32_t e = __float_as_uint(largest) & 0x7F800000u;
+  const uint32_t up = e < (15u << 23) ? 253u << 23 : (268u << 23) - e;
+  return {__uint_as_float(up), __uint_as_float((254u << 23) - up)};
+}
+// (v - v == 0 would not do: of a product it is contracted to its rounding error)
+__device__ inline bool is_finite(float v) { return fabsf(v) < INFINITY; }
+__device__ inline float finite_abs(float v) { return is_finite(v) ? fabsf(v) : 0.f; }
+__device__ inline Split split8(const float (&v)[8], float up) {
+  Split s;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = v[i] * up;
+    s.hi[i] = static_cast<_Float16>(x);
+    s.lo[i] = static_cast<_Float16>(x - static_cast<float>(s.hi[i]));
+  }
+  return s;
+}
+// a . b over 32 (four products: the smallest is 2^-22 of the largest)
+__device__ inline f32x4_t mfma_split(const Split& a, const Split& b, f32x4_t c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.lo, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, c, 0, 0, 0);
+}
+// the largest over the four lanes 16 apart
+__device__ inline float column_max(float v) {
+  auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
 
 // Sums of four values of each lane over the wave's four 16-lane rows: row g is left
 // with that of value (g & 1) + 2 (g >> 1), by two exchanges that each halve what a
@@ -437,10 +483,11 @@ __device__ inline int after(int at, float x) {
 
 __device__ inline f32x4_t lds4(const float* p) { return *reinterpret_cast<const f32x4_t*>(p); }
 
-template <int DT, int RT>
+template <int DT, int NW>
 __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanArgs a, ChunkArgs c) {
   using T = typename Storage<DT>::type;
-  using L = ChunkLayout<RT>;
+  using L = ChunkLayout<NW>;
+  constexpr int RT = NW / 2;
   constexpr int kStride = L::kChannels + 4;  // rows 16 bytes apart in the banks
   constexpr int kVStride = kPass + 4;
   // rows of q, k, e^g; then of scale q D, beta k D, W
@@ -453,6 +500,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanA
   __shared__ f32x4_t sm[8][kWave];  // the waves' sums for M and P_ba
   __shared__ alignas(16) float sd[2][L::kChannels];
   __shared__ float sb[kChunk];
+  __shared__ float sl[2][2][NW][kHalf];  // largest of W, Q rows over 32 channels each
   const int h = static_cast<int>(blockIdx.x % a.heads);
   const int64_t local = blockIdx.x / a.heads;
   const SequenceTile at = find_sequence_tile(a.seq, c.first + local, kChunk);
@@ -612,24 +660,81 @@ __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanA
   const f32x4_t mt = (sm[0][lane] + sm[1][lane]) + (sm[2][lane] + sm[3][lane]);
   auto put = [&](int off, f32x4_t v) { *reinterpret_cast<f32x4_t*>(rec + off + 4 * lane) = v; };
   if (wave == 4) put(L::kP + 256, (sm[4][lane] + sm[5][lane]) + (sm[6][lane] + sm[7][lane]));
-  for (int t = wave; t < L::kTiles; t += kPrepareThreads / kWave) {
-    const int d = 16 * t + 4 * g, ch = 16 * t + l;
-    const f32x4_t da = lds4(&sd[0][d]), db = lds4(&sd[1][d]);
-    const float db_ch = sd[1][ch];
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f}, ka, kb;
+  auto put_split = [&](int off, const Split& v) {
+    *reinterpret_cast<f16x8_t*>(rec + off + 4 * lane) = v.hi;
+    *reinterpret_cast<f16x8_t*>(rec + off + 256 + 4 * lane) = v.lo;
+  };
+  // W and Q of half b, channels 32 p to + 31, by wave 2 p + b
+  float wv[8], qv[8];
+  const int p = wave >> 1, b = wave & 1;
+  if (p < NW) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int t = 2 * p + y, d = 16 * t + 4 * g;
+      f32x4_t w = lds4(&sg[kHalf * b + l][d]), q = lds4(&sq[kHalf * b + l][d]);
+      if (b) {
+        const f32x4_t da = lds4(&sd[0][d]);
+        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc = __builtin_amdgcn_mfma_f32_16x16x4f32(sg[4 * g + r][16 * t + l], mt[r], acc, 0, 0, 0);
+        w = w * da - acc;
+        q *= da;
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        wv[4 * y + r] = w[r];
+        qv[4 * y + r] = q[r];
+      }
+    }
+    float mw = 0.f, mq = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      mw = fmaxf(mw, finite_abs(wv[i]));
+      mq = fmaxf(mq, finite_abs(qv[i]));
+    }
+    mw = column_max(mw);
+    mq = column_max(mq);
+    if (g == 0) {
+      sl[0][b][p][l] = mw;
+      sl[1][b][p][l] = mq;
+    }
+  }
+  if (wave < L::kTiles) {
+    const int ch = 16 * wave + l;
+    const float db = sd[1][ch];
+    float kv[8], most = 0.f;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(sg[4 * g + r][ch], mt[r], acc, 0, 0, 0);
-      ka[r] = sk[4 * g + r][ch] * db_ch;
-      kb[r] = sk[kHalf + 4 * g + r][ch];
+      kv[r] = sk[4 * g + r][ch] * db;
+      kv[4 + r] = sk[kHalf + 4 * g + r][ch];
     }
-    put(L::kQ + 256 * t, lds4(&sq[l][d]));
-    put(L::kQ + 256 * (L::kTiles + t), lds4(&sq[kHalf + l][d]) * da);
-    put(L::kK + 256 * t, ka);
-    put(L::kK + 256 * (L::kTiles + t), kb);
-    put(L::kW + 256 * t, lds4(&sg[l][d]));
-    put(L::kW + 256 * (L::kTiles + t), lds4(&sg[kHalf + l][d]) * da - acc);
-    if (l == 0) *reinterpret_cast<f32x4_t*>(rec + L::kD + d) = da * db;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, finite_abs(kv[i]));
+#pragma unroll
+    for (int i = 1; i < kWave; i <<= 1) most = fmaxf(most, __shfl_xor(most, i));
+    const Scale sc = scale_for(most);
+    put_split(L::kK + 512 * wave, split8(kv, sc.up));
+    if (lane == 0) rec[L::kS + 2 * kChunk + wave] = sc.down;
+    if (l == 0)
+      *reinterpret_cast<f32x4_t*>(rec + L::kD + 16 * wave + 4 * g) =
+          lds4(&sd[0][16 * wave + 4 * g]) * lds4(&sd[1][16 * wave + 4 * g]);
+  }
+  __syncthreads();
+  if (p < NW) {  // a row has one scale over all channels
+    float mw = sl[0][b][0][l], mq = sl[1][b][0][l];
+#pragma unroll
+    for (int y = 1; y < NW; ++y) {
+      mw = fmaxf(mw, sl[0][b][y][l]);
+      mq = fmaxf(mq, sl[1][b][y][l]);
+    }
+    const Scale w = scale_for(mw), q = scale_for(mq);
+    put_split(L::kW + 512 * (b * NW + p), split8(wv, w.up));
+    put_split(L::kQ + 512 * (b * NW + p), split8(qv, q.up));
+    if (p == 0 && g == 0) {
+      rec[L::kS + kHalf * b + l] = w.down;
+      rec[L::kS + kChunk + kHalf * b + l] = q.down;
+    }
   }
   for (int first = 0;;) {
     const int ct = first / 16 + wave;
@@ -671,15 +776,17 @@ __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanA
 // are put between the products that follow it (in one place they held the waves
 // up for 500 cycles of 1900), two chunks ahead, and without a branch (the last
 // record again at the end), so that a wait leaves the younger ones in flight.
-constexpr int kScanWaves = 6;
-
-template <int DT, int RT>
-__global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
+template <int DT, int NW>
+__global__ void __launch_bounds__((NW + 2) * kWave) chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
   using T = typename Storage<DT>::type;
-  using L = ChunkLayout<RT>;
-  // of the last two chunks and each half: the waves' W S, - U0, the waves' Q S, U; D
-  __shared__ f32x4_t parts[2][2][10][kWave];
-  __shared__ f32x4_t decay[2][L::kTiles * 4];
+  using L = ChunkLayout<NW>;
+  constexpr int kScanWaves = NW + 2;
+  constexpr int kU0 = NW, kQS = NW + 1, kU = 2 * NW + 1;
+  // of the last two chunks and each half: the waves' W S, - U0, the waves' Q S, U;
+  // D; what the rows of W and the tiles of K are scaled by
+  __shared__ f32x4_t parts[2][2][2 * NW + 2][kWave];
+  __shared__ f32x4_t decay[2][L::kTiles * 4], w_down[2][2][4];
+  __shared__ float k_down[2][L::kTiles];
   // the column tiles of a head, which read the same records, lie 8 blocks apart:
   // on one XCD, whose cache then holds a record for all of them
   const int64_t span = 8 * c.v_tiles, at = blockIdx.x % span;
@@ -716,27 +823,38 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
   auto part_at = [&](uint32_t off) { return *reinterpret_cast<const f32x4_t*>(ahead + off); };
   auto advance = [&]() { ahead = ahead < last ? ahead + stride : last; };
 
-  if (wave >= 4) {
+  if (wave >= NW) {
     if (steps == 0) return;
-    const int half = wave - 4;
+    const int half = wave - NW;
     const uint32_t values = static_cast<uint32_t>((L::kU + ((half * c.v_tiles + ct) * 64 + lane) * 4) * 4);
     const uint32_t planes = static_cast<uint32_t>((L::kP + 4 * lane) * 4);
-    const uint32_t decays = static_cast<uint32_t>((L::kD + lane * RT) * 4);
-    typedef float row_t __attribute__((ext_vector_type(RT)));  // channels RT lane, ...
+    const uint32_t decays = static_cast<uint32_t>((L::kD + lane % (L::kChannels / 2) * 2) * 4);
+    const uint32_t w_scales = static_cast<uint32_t>((L::kS + kHalf * half + m) * 4);
+    const uint32_t q_scales = static_cast<uint32_t>((L::kS + kChunk + kHalf * half + 4 * g) * 4);
+    const uint32_t k_scales = static_cast<uint32_t>((L::kS + 2 * kChunk + lane % L::kTiles) * 4);
     struct Record {
-      f32x4_t u, p, pba;
-      row_t d;
+      f32x4_t u, p, pba, q_down;
+      float2 d;
+      float w_down, k_down;
     };
     auto fetch = [&](Record& f) {
       f.u = part_at(values);
       f.p = part_at(planes + 2048 * half);
       f.pba = part_at(planes + 1024);
-      f.d = *reinterpret_cast<const row_t*>(ahead + decays);
+      f.q_down = part_at(q_scales);
+      f.d = *reinterpret_cast<const float2*>(ahead + decays);
+      f.w_down = *reinterpret_cast<const float*>(ahead + w_scales);
+      f.k_down = *reinterpret_cast<const float*>(ahead + k_scales);
       advance();
     };
     auto hand_over = [&](int i, const Record& f) {
-      parts[i & 1][half][4][lane] = -f.u;
-      if (half == 0) reinterpret_cast<row_t*>(decay[i & 1])[lane] = f.d;
+      parts[i & 1][half][kU0][lane] = -f.u;
+      if (lane < kHalf) reinterpret_cast<float*>(w_down[i & 1][half])[lane] = f.w_down;
+      if (half == 0) {
+        if (lane < L::kChannels / 2) reinterpret_cast<float2*>(decay[i & 1])[lane] = f.d;
+      } else if (lane < L::kTiles) {
+        k_down[i & 1][lane] = f.k_down;
+      }
     };
     // rows behind the sequence, columns behind the last and chunks not begun go
     // past the buffer's end: stores without a branch. Behind a branch the
@@ -755,23 +873,26 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
     const char* rec = first;
     // a chunk's outputs: begun behind the barrier of the next one, stored behind
     // the one after that, so that no barrier waits for their products
-    auto begin = [&](int i, const f32x4_t& p, const f32x4_t& pba, f32x4_t& u) {
+    auto begin = [&](int i, const f32x4_t& p, const f32x4_t& pba, const f32x4_t& q_down,
+                     f32x4_t& u) {
       const f32x4_t(*const part)[kWave] = parts[i & 1][half];
-      u = part[9][lane];
-      f32x4_t o = (part[5][lane] + part[6][lane]) + (part[7][lane] + part[8][lane]);
+      u = part[kU][lane];
+      f32x4_t o = part[kQS][lane] + part[kQS + 1][lane];
+      if constexpr (NW == 4) o += part[kQS + 2][lane] + part[kQS + 3][lane];
+      o *= q_down;
       if (half) {
-        const f32x4_t ua = parts[i & 1][0][9][lane];
+        const f32x4_t ua = parts[i & 1][0][kU][lane];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           o = __builtin_amdgcn_mfma_f32_16x16x4f32(pba[r], ua[r], o, 0, 0, 0);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        o = __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], u[r] - u[r] == 0.f ? u[r] : 0.f, o, 0, 0, 0);
+        o = __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], is_finite(u[r]) ? u[r] : 0.f, o, 0, 0, 0);
       return o;
     };
     auto store = [&](f32x4_t o, f32x4_t u, bool begun) {
-      const bool fine = (u[0] - u[0]) + (u[1] - u[1]) + (u[2] - u[2]) + (u[3] - u[3]) == 0.f;
+      const bool fine = is_finite(u[0]) && is_finite(u[1]) && is_finite(u[2]) && is_finite(u[3]);
       if (__builtin_expect(begun && !__all(fine), 0)) {
         // infinities and NaNs, which P's zeros would hand to the steps before
         // their own: left out of P U, and taken one by one by the steps
@@ -784,7 +905,7 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float pij = p[((4 * g + r) + 16 * (j >> 2)) * 4 + (j & 3)];
-            if (j <= 4 * g + r && uj - uj != 0.f) o[r] = fmaf(pij, uj, o[r]);
+            if (j <= 4 * g + r && !is_finite(uj)) o[r] = fmaf(pij, uj, o[r]);
           }
         }
       }
@@ -807,7 +928,7 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
     // records three in turn, each until its outputs are begun (a copy of one on
     // its way would wait for it)
     Record f0, f1, f2;
-    f32x4_t p = {0.f, 0.f, 0.f, 0.f}, pba = p, o = p, u = p;
+    f32x4_t p = {0.f, 0.f, 0.f, 0.f}, pba = p, q_down = p, o = p, u = p;
     fetch(f0);
     fetch(f1);
     auto turn = [&](int i, const Record& f, Record& next) {
@@ -815,9 +936,10 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
       fetch(next);
       __syncthreads();
       store(o, u, i > 1);
-      o = begin(i - 1, p, pba, u);  // (of nothing for i = 0)
+      o = begin(i - 1, p, pba, q_down, u);  // (of nothing for i = 0)
       p = f.p;
       pba = f.pba;
+      q_down = f.q_down;
     };
     int i = 0;
     for (; i + 3 <= steps; i += 3) {
@@ -829,93 +951,101 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
     if (i + 1 < steps) turn(i + 1, f1, f0);
     __syncthreads();
     store(o, u, steps > 1);
-    o = begin(steps - 1, p, pba, u);
+    o = begin(steps - 1, p, pba, q_down, u);
     store(o, u, true);
     return;
   }
 
+  // the state's rows 32 wave + 16 t + 4 g + r, and as the operand of the next chunk
   const float* const src = lo == number ? a.state : a.state_out;
   const int64_t sbase = sh * a.d_k * a.d_v;
-  f32x4_t st[RT];
+  f32x4_t st[2];
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = 16 * (wave * RT + t) + 4 * g + r;
+      const int row = 32 * wave + 16 * t + 4 * g + r;
       st[t][r] = row < a.d_k && col < a.d_v ? src[sbase + static_cast<int64_t>(row) * a.d_v + col] : 0.f;
     }
-  struct Record {
-    f32x4_t w[2][RT], q[2][RT], k[2][RT];
+  // both tiles (halves) of a column as an operand with one scale
+  auto split_column = [&](const f32x4_t& v0, const f32x4_t& v1, Split& out) {
+    const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
+    const Scale sc = scale_for(column_max(most));
+    out = split8(v, sc.up);
+    return sc.down;
   };
-  constexpr uint32_t kHalfBytes = L::kTiles * 1024;
-  const uint32_t tiles = static_cast<uint32_t>((wave * RT * 64 + lane) * 16);
-  const uint32_t w_at = tiles + L::kW * 4, q_at = tiles + L::kQ * 4, k_at = tiles + L::kK * 4;
+  Split ss;
+  float s_down = split_column(st[0], st[1], ss);
+  struct Record {
+    Split w[2], q[2], k[2];  // [half], [half], [tile]
+  };
+  // 2 KB a fragment; W and Q: half NW + wave, K: tile 2 wave + t
+  const uint32_t w_at = static_cast<uint32_t>((L::kW + 512 * wave + 4 * lane) * 4);
+  const uint32_t q_at = w_at + L::kQ * 4;
+  const uint32_t k_at = static_cast<uint32_t>((L::kK + 1024 * wave + 4 * lane) * 4);
+  constexpr uint32_t kHalfBytes = 2048 * NW;
+  auto half_at = [&](uint32_t off) { return *reinterpret_cast<const f16x8_t*>(ahead + off); };
   auto fetch = [&](Record& f) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        f.w[x][t] = part_at(w_at + kHalfBytes * x + 1024 * t);
-        f.q[x][t] = part_at(q_at + kHalfBytes * x + 1024 * t);
-        f.k[x][t] = part_at(k_at + kHalfBytes * x + 1024 * t);
-      }
+    for (int x = 0; x < 2; ++x) {
+      f.w[x] = {half_at(w_at + kHalfBytes * x), half_at(w_at + kHalfBytes * x + 1024)};
+      f.q[x] = {half_at(q_at + kHalfBytes * x), half_at(q_at + kHalfBytes * x + 1024)};
+      f.k[x] = {half_at(k_at + 2048 * x), half_at(k_at + 2048 * x + 1024)};
+    }
     advance();
   };
   auto step = [&](int i, const Record& f, Record& next) {
-    f32x4_t(*const part)[10][kWave] = parts[i & 1];
-    f32x4_t x[2] = {}, y[2] = {};
+    f32x4_t(*const part)[2 * NW + 2][kWave] = parts[i & 1];
+    const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          x[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.w[b][t][r], st[t][r], x[b], 0, 0, 0);
-    part[0][wave][lane] = x[0];
-    part[1][wave][lane] = x[1];
+    for (int b = 0; b < 2; ++b) part[b][wave][lane] = mfma_split(f.w[b], ss, zero) * s_down;
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);  // Q S is not to be moved up
-    f32x4_t xs[2][5], d[RT];
+    f32x4_t xs[2][NW + 1], down[2], d[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < 2; ++b) {
 #pragma unroll
-      for (int w = 0; w < 5; ++w) xs[b][w] = part[b][w][lane];
+      for (int w = 0; w < NW + 1; ++w) xs[b][w] = part[b][w][lane];
+      down[b] = w_down[i & 1][b][g];
+    }
+    float kd[2];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) d[t] = decay[i & 1][(wave * RT + t) * 4 + g];
+    for (int t = 0; t < 2; ++t) {
+      d[t] = decay[i & 1][(2 * wave + t) * 4 + g];
+      kd[t] = k_down[i & 1][2 * wave + t];
+    }
     __builtin_amdgcn_sched_barrier(0);
+    f32x4_t y[2];
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          y[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.q[b][t][r], st[t][r], y[b], 0, 0, 0);
-        const uint32_t off = kHalfBytes * (r & 1) + 1024 * t;
-        if (r < 2) next.w[r & 1][t] = part_at(w_at + off);
-        else next.q[r & 1][t] = part_at(q_at + off);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int b = 0; b < 2; ++b) {
+      y[b] = mfma_split(f.q[b], ss, zero);
+      next.w[b] = {half_at(w_at + kHalfBytes * b), half_at(w_at + kHalfBytes * b + 1024)};
+      __builtin_amdgcn_sched_barrier(0);
+    }
     f32x4_t u[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-      u[b] = -(((xs[b][0] + xs[b][1]) + (xs[b][2] + xs[b][3])) + xs[b][4]);
+    for (int b = 0; b < 2; ++b) {
+      f32x4_t x = xs[b][0] + xs[b][1];
+      if constexpr (NW == 4) x += xs[b][2] + xs[b][3];
+      u[b] = -(x * down[b] + xs[b][kU0]);
+    }
+    Split us;
+    const float u_down = split_column(u[0], u[1], us);
 #pragma unroll
-    for (int t = 0; t < RT; ++t) st[t] *= d[t];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-          st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(f.k[b][t][r], u[b][r], st[t], 0, 0, 0);
-        if (r < RT) next.k[b][r] = part_at(k_at + kHalfBytes * b + 1024 * r);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int t = 0; t < 2; ++t) {
+      const f32x4_t acc = mfma_split(f.k[t], us, zero);
+      next.q[t] = {half_at(q_at + kHalfBytes * t), half_at(q_at + kHalfBytes * t + 1024)};
+      next.k[t] = {half_at(k_at + 2048 * t), half_at(k_at + 2048 * t + 1024)};
+      part[t][kQS + wave][lane] = y[t] * s_down;
+      __builtin_amdgcn_sched_barrier(0);
+      st[t] = st[t] * d[t] + acc * (kd[t] * u_down);
+    }
     advance();
-    part[0][5 + wave][lane] = y[0];
-    part[1][5 + wave][lane] = y[1];
-    if (wave == 0) part[0][9][lane] = u[0];
-    if (wave == 1) part[1][9][lane] = u[1];
+    if (wave < 2) part[wave][kU][lane] = wave == 0 ? u[0] : u[1];
+    s_down = split_column(st[0], st[1], ss);
   };
   if (steps > 0) {
     Record f0, f1, f2;  // in turn
@@ -932,10 +1062,10 @@ __global__ void __launch_bounds__(kScanWaves * kWave) chunk_scan_kernel(ScanArgs
     __syncthreads();  // the last chunk's Q S and U, for the last two waves
   }
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = 16 * (wave * RT + t) + 4 * g + r;
+      const int row = 32 * wave + 16 * t + 4 * g + r;
       if (row < a.d_k && col < a.d_v)
         a.state_out[sbase + static_cast<int64_t>(row) * a.d_v + col] = st[t][r];
     }
@@ -998,7 +1128,7 @@ int launch_serial(const ScanArgs& a, hipStream_t s) {
 // Floats of a chunk's and head's record.
 int64_t chunk_record(int64_t d_k, int64_t d_v) {
   const int64_t channels = d_k <= 64 ? 64 : 128;
-  return channels * (3 * kChunk + 1) + 3 * 256 + (d_v + 15) / 16 * 16 * kChunk;
+  return channels * (3 * kChunk + 1) + 3 * 256 + 2 * kChunk + 16 + (d_v + 15) / 16 * 16 * kChunk;
 }
 
 // Chunks of one window: the records of a window are written by one launch and
@@ -1017,7 +1147,7 @@ bool takes_chunks(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k,
   return choice == 2 || tokens >= 32 * sequences;
 }
 
-template <int DT, int RT>
+template <int DT, int NW>
 int launch_chunks(const ScanArgs& a, float* records, hipStream_t s) {
   ChunkArgs c;
   c.records = records;
@@ -1030,10 +1160,10 @@ int launch_chunks(const ScanArgs& a, float* records, hipStream_t s) {
              "too many sequences x heads for one call");
   for (c.first = 0; c.first < chunks; c.first += window) {
     c.count = window < chunks - c.first ? window : chunks - c.first;
-    chunk_prepare_kernel<DT, RT>
+    chunk_prepare_kernel<DT, NW>
         <<<static_cast<unsigned>(c.count * a.heads), kPrepareThreads, 0, s>>>(a, c);
     if (const int st = check_launch("lk_kda_prefill")) return st;
-    chunk_scan_kernel<DT, RT><<<static_cast<unsigned>(scans), kScanWaves * kWave, 0, s>>>(a, c);
+    chunk_scan_kernel<DT, NW><<<static_cast<unsigned>(scans), (NW + 2) * kWave, 0, s>>>(a, c);
     if (const int st = check_launch("lk_kda_prefill")) return st;
   }
   return LK_OK;
@@ -1043,7 +1173,7 @@ template <int DT>
 int launch_scan(const ScanArgs& a, bool chunks, void* workspace, hipStream_t s) {
   if (!chunks) return launch_serial<DT>(a, s);
   float* const records = static_cast<float*>(workspace);
-  return a.d_k <= 64 ? launch_chunks<DT, 1>(a, records, s) : launch_chunks<DT, 2>(a, records, s);
+  return a.d_k <= 64 ? launch_chunks<DT, 2>(a, records, s) : launch_chunks<DT, 4>(a, records, s);
 }
 
 }  // namespace
