@@ -776,22 +776,23 @@ __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanA
 // are put between the products that follow it (in one place they held the waves
 // up for 500 cycles of 1900), two chunks ahead, and without a branch (the last
 // record again at the end), so that a wait leaves the younger ones in flight.
-template <int DT, int NW>
-__global__ void __launch_bounds__((NW + 2) * kWave) chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
+template <int DT, int NW, int CT>
+__global__ void __launch_bounds__((NW + 2 * CT) * kWave)
+chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
   using T = typename Storage<DT>::type;
   using L = ChunkLayout<NW>;
-  constexpr int kScanWaves = NW + 2;
+  constexpr int kScanWaves = NW + 2 * CT;
   constexpr int kU0 = NW, kQS = NW + 1, kU = 2 * NW + 1;
   // of the last two chunks and each half: the waves' W S, - U0, the waves' Q S, U;
   // D; what the rows of W and the tiles of K are scaled by
-  __shared__ f32x4_t parts[2][2][2 * NW + 2][kWave];
+  __shared__ f32x4_t parts[2][CT][2][2 * NW + 2][kWave];
   __shared__ f32x4_t decay[2][L::kTiles * 4], w_down[2][2][4];
   __shared__ float k_down[2][L::kTiles];
   // the column tiles of a head, which read the same records, lie 8 blocks apart:
   // on one XCD, whose cache then holds a record for all of them
-  const int64_t span = 8 * c.v_tiles, at = blockIdx.x % span;
+  const int64_t span = 8 * ((c.v_tiles + CT - 1) / CT), at = blockIdx.x % span;
   const int64_t sh = blockIdx.x / span * 8 + at % 8;
-  const int ct = static_cast<int>(at / 8);
+  const int ct = static_cast<int>(at / 8) * CT;  // the first of the block's tiles
   const int h = static_cast<int>(sh % a.heads);
   const int s = static_cast<int>(sh / a.heads);
   if (s > a.seq.count) return;
@@ -799,11 +800,13 @@ __global__ void __launch_bounds__((NW + 2) * kWave) chunk_scan_kernel(ScanArgs a
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int m = lane & 15, g = lane >> 4;
-  const int col = ct * 16 + m;
   if (s == a.seq.count) {  // rows behind the last sequence
     if (c.first == 0)
       for (int64_t t = rows.begin + (tid >> 4); t < rows.end; t += kScanWaves * 4)
-        if (col < a.d_v) static_cast<T*>(a.out)[(t * a.heads + h) * a.d_v + col] = 0;
+        for (int x = 0; x < CT; ++x) {
+          const int col = (ct + x) * 16 + m;
+          if (col < a.d_v) static_cast<T*>(a.out)[(t * a.heads + h) * a.d_v + col] = 0;
+        }
     return;
   }
   // the sequence's chunk numbers, at least one, and those of the window
@@ -825,8 +828,10 @@ __global__ void __launch_bounds__((NW + 2) * kWave) chunk_scan_kernel(ScanArgs a
 
   if (wave >= NW) {
     if (steps == 0) return;
-    const int half = wave - NW;
-    const uint32_t values = static_cast<uint32_t>((L::kU + ((half * c.v_tiles + ct) * 64 + lane) * 4) * 4);
+    const int half = (wave - NW) & 1, tile = (wave - NW) >> 1;  // of the block
+    const int vt = ct + tile < c.v_tiles ? ct + tile : ct;      // (no such tile: no column of it)
+    const int col = (ct + tile) * 16 + m;
+    const uint32_t values = static_cast<uint32_t>((L::kU + ((half * c.v_tiles + vt) * 64 + lane) * 4) * 4);
     const uint32_t planes = static_cast<uint32_t>((L::kP + 4 * lane) * 4);
     const uint32_t decays = static_cast<uint32_t>((L::kD + lane % (L::kChannels / 2) * 2) * 4);
     const uint32_t w_scales = static_cast<uint32_t>((L::kS + kHalf * half + m) * 4);
@@ -848,7 +853,8 @@ __global__ void __launch_bounds__((NW + 2) * kWave) chunk_scan_kernel(ScanArgs a
       advance();
     };
     auto hand_over = [&](int i, const Record& f) {
-      parts[i & 1][half][kU0][lane] = -f.u;
+      parts[i & 1][tile][half][kU0][lane] = -f.u;
+      if (tile > 0) return;
       if (lane < kHalf) reinterpret_cast<float*>(w_down[i & 1][half])[lane] = f.w_down;
       if (half == 0) {
         if (lane < L::kChannels / 2) reinterpret_cast<float2*>(decay[i & 1])[lane] = f.d;
@@ -875,13 +881,13 @@ __global__ void __launch_bounds__((NW + 2) * kWave) chunk_scan_kernel(ScanArgs a
     // the one after that, so that no barrier waits for their products
     auto begin = [&](int i, const f32x4_t& p, const f32x4_t& pba, const f32x4_t& q_down,
                      f32x4_t& u) {
-      const f32x4_t(*const part)[kWave] = parts[i & 1][half];
+      const f32x4_t(*const part)[kWave] = parts[i & 1][tile][half];
       u = part[kU][lane];
       f32x4_t o = part[kQS][lane] + part[kQS + 1][lane];
       if constexpr (NW == 4) o += part[kQS + 2][lane] + part[kQS + 3][lane];
       o *= q_down;
       if (half) {
-        const f32x4_t ua = parts[i & 1][0][kU][lane];
+        const f32x4_t ua = parts[i & 1][tile][0][kU][lane];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           o = __builtin_amdgcn_mfma_f32_16x16x4f32(pba[r], ua[r], o, 0, 0, 0);
@@ -959,14 +965,17 @@ __global__ void __launch_bounds__((NW + 2) * kWave) chunk_scan_kernel(ScanArgs a
   // the state's rows 32 wave + 16 t + 4 g + r, and as the operand of the next chunk
   const float* const src = lo == number ? a.state : a.state_out;
   const int64_t sbase = sh * a.d_k * a.d_v;
-  f32x4_t st[2];
+  f32x4_t st[CT][2];
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int x = 0; x < CT; ++x)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 32 * wave + 16 * t + 4 * g + r;
-      st[t][r] = row < a.d_k && col < a.d_v ? src[sbase + static_cast<int64_t>(row) * a.d_v + col] : 0.f;
-    }
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 32 * wave + 16 * t + 4 * g + r, col = (ct + x) * 16 + m;
+        st[x][t][r] =
+            row < a.d_k && col < a.d_v ? src[sbase + static_cast<int64_t>(row) * a.d_v + col] : 0.f;
+      }
   // both tiles (halves) of a column as an operand with one scale
   auto split_column = [&](const f32x4_t& v0, const f32x4_t& v1, Split& out) {
     const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
@@ -977,8 +986,10 @@ __global__ void __launch_bounds__((NW + 2) * kWave) chunk_scan_kernel(ScanArgs a
     out = split8(v, sc.up);
     return sc.down;
   };
-  Split ss;
-  float s_down = split_column(st[0], st[1], ss);
+  Split ss[CT];
+  float s_down[CT];
+#pragma unroll
+  for (int x = 0; x < CT; ++x) s_down[x] = split_column(st[x][0], st[x][1], ss[x]);
   struct Record {
     Split w[2], q[2], k[2];  // [half], [half], [tile]
   };
@@ -998,54 +1009,66 @@ __global__ void __launch_bounds__((NW + 2) * kWave) chunk_scan_kernel(ScanArgs a
     advance();
   };
   auto step = [&](int i, const Record& f, Record& next) {
-    f32x4_t(*const part)[2 * NW + 2][kWave] = parts[i & 1];
+    f32x4_t(*const part)[2][2 * NW + 2][kWave] = parts[i & 1];
     const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int b = 0; b < 2; ++b) part[b][wave][lane] = mfma_split(f.w[b], ss, zero) * s_down;
+    for (int x = 0; x < CT; ++x)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        part[x][b][wave][lane] = mfma_split(f.w[b], ss[x], zero) * s_down[x];
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);  // Q S is not to be moved up
-    f32x4_t xs[2][NW + 1], down[2], d[2];
+    f32x4_t down[2], d[2], y[CT][2], u[CT][2];
+    float kd[2], u_down[CT];
+    Split us[CT];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int x = 0; x < CT; ++x) {
+      f32x4_t xs[2][NW + 1];
 #pragma unroll
-      for (int w = 0; w < NW + 1; ++w) xs[b][w] = part[b][w][lane];
-      down[b] = w_down[i & 1][b][g];
-    }
-    float kd[2];
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      d[t] = decay[i & 1][(2 * wave + t) * 4 + g];
-      kd[t] = k_down[i & 1][2 * wave + t];
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    f32x4_t y[2];
+        for (int w = 0; w < NW + 1; ++w) xs[b][w] = part[x][b][w][lane];
+      if (x == 0)
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      y[b] = mfma_split(f.q[b], ss, zero);
-      next.w[b] = {half_at(w_at + kHalfBytes * b), half_at(w_at + kHalfBytes * b + 1024)};
+        for (int b = 0; b < 2; ++b) {
+          down[b] = w_down[i & 1][b][g];
+          d[b] = decay[i & 1][(2 * wave + b) * 4 + g];
+          kd[b] = k_down[i & 1][2 * wave + b];
+        }
       __builtin_amdgcn_sched_barrier(0);
-    }
-    f32x4_t u[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      f32x4_t x = xs[b][0] + xs[b][1];
-      if constexpr (NW == 4) x += xs[b][2] + xs[b][3];
-      u[b] = -(x * down[b] + xs[b][kU0]);
+      for (int b = 0; b < 2; ++b) {
+        y[x][b] = mfma_split(f.q[b], ss[x], zero);
+        if (x == 0) next.w[b] = {half_at(w_at + kHalfBytes * b), half_at(w_at + kHalfBytes * b + 1024)};
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        f32x4_t sum = xs[b][0] + xs[b][1];
+        if constexpr (NW == 4) sum += xs[b][2] + xs[b][3];
+        u[x][b] = -(sum * down[b] + xs[b][kU0]);
+      }
+      u_down[x] = split_column(u[x][0], u[x][1], us[x]);
     }
-    Split us;
-    const float u_down = split_column(u[0], u[1], us);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const f32x4_t acc = mfma_split(f.k[t], us, zero);
+      f32x4_t acc[CT];
+#pragma unroll
+      for (int x = 0; x < CT; ++x) acc[x] = mfma_split(f.k[t], us[x], zero);
       next.q[t] = {half_at(q_at + kHalfBytes * t), half_at(q_at + kHalfBytes * t + 1024)};
       next.k[t] = {half_at(k_at + 2048 * t), half_at(k_at + 2048 * t + 1024)};
-      part[t][kQS + wave][lane] = y[t] * s_down;
+#pragma unroll
+      for (int x = 0; x < CT; ++x) part[x][t][kQS + wave][lane] = y[x][t] * s_down[x];
       __builtin_amdgcn_sched_barrier(0);
-      st[t] = st[t] * d[t] + acc * (kd[t] * u_down);
+#pragma unroll
+      for (int x = 0; x < CT; ++x) st[x][t] = st[x][t] * d[t] + acc[x] * (kd[t] * u_down[x]);
     }
     advance();
-    if (wave < 2) part[wave][kU][lane] = wave == 0 ? u[0] : u[1];
-    s_down = split_column(st[0], st[1], ss);
+    if (wave < 2)
+#pragma unroll
+      for (int x = 0; x < CT; ++x) part[x][wave][kU][lane] = wave == 0 ? u[x][0] : u[x][1];
+#pragma unroll
+    for (int x = 0; x < CT; ++x) s_down[x] = split_column(st[x][0], st[x][1], ss[x]);
   };
   if (steps > 0) {
     Record f0, f1, f2;  // in turn
@@ -1059,16 +1082,18 @@ __global__ void __launch_bounds__((NW + 2) * kWave) chunk_scan_kernel(ScanArgs a
     }
     if (i < steps) step(i, f0, f2);
     if (i + 1 < steps) step(i + 1, f1, f0);
-    __syncthreads();  // the last chunk's Q S and U, for the last two waves
+    __syncthreads();  // the last chunk's Q S and U, for the other waves
   }
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int x = 0; x < CT; ++x)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 32 * wave + 16 * t + 4 * g + r;
-      if (row < a.d_k && col < a.d_v)
-        a.state_out[sbase + static_cast<int64_t>(row) * a.d_v + col] = st[t][r];
-    }
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 32 * wave + 16 * t + 4 * g + r, col = (ct + x) * 16 + m;
+        if (row < a.d_k && col < a.d_v)
+          a.state_out[sbase + static_cast<int64_t>(row) * a.d_v + col] = st[x][t][r];
+      }
 }
 
 bool known_dtype(int d) { return d == LK_DTYPE_F32 || d == LK_DTYPE_F16 || d == LK_DTYPE_BF16; }
@@ -1131,6 +1156,8 @@ int64_t chunk_record(int64_t d_k, int64_t d_v) {
   return channels * (3 * kChunk + 1) + 3 * 256 + 2 * kChunk + 16 + (d_v + 15) / 16 * 16 * kChunk;
 }
 
+constexpr int64_t kTwoTiles = 1024;
+
 // Chunks of one window: the records of a window are written by one launch and
 // read by the next, so they are kept within the 256 MB cache in front of HBM.
 constexpr int64_t kWindowBytes = int64_t{256} << 20;
@@ -1144,7 +1171,7 @@ bool takes_chunks(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k,
   const int choice = path_choice(kKnobKdaPrefill);
   // (a chunk's outputs are stored at 31-bit byte offsets)
   if (d_k > 128 || tokens == 0 || choice == 1 || heads * d_v >= (int64_t{1} << 24)) return false;
-  return choice == 2 || tokens >= 32 * sequences;
+  return choice == 2 || tokens >= 48 * sequences;
 }
 
 template <int DT, int NW>
@@ -1155,7 +1182,11 @@ int launch_chunks(const ScanArgs& a, float* records, hipStream_t s) {
   c.v_tiles = (a.d_v + 15) / 16;
   const int64_t chunks = sequence_tiles(a.seq.rows, a.seq.count, kChunk);
   const int64_t window = chunk_window(chunks, a.heads, c.record);
-  const int64_t scans = ((a.seq.count + 1) * static_cast<int64_t>(a.heads) + 7) / 8 * 8 * c.v_tiles;
+  // a block reads a head's records for one tile of value columns, or for two where
+  // there are enough of them to fill the CUs twice
+  const int64_t pairs = (a.seq.count + 1) * static_cast<int64_t>(a.heads);
+  const bool two = c.v_tiles > 1 && a.seq.count * static_cast<int64_t>(a.heads) * c.v_tiles >= kTwoTiles;
+  const int64_t scans = (pairs + 7) / 8 * 8 * (two ? (c.v_tiles + 1) / 2 : c.v_tiles);
   LK_REQUIRE(window * a.heads < (int64_t{1} << 31) && scans < (int64_t{1} << 31),
              "too many sequences x heads for one call");
   for (c.first = 0; c.first < chunks; c.first += window) {
@@ -1163,7 +1194,10 @@ int launch_chunks(const ScanArgs& a, float* records, hipStream_t s) {
     chunk_prepare_kernel<DT, NW>
         <<<static_cast<unsigned>(c.count * a.heads), kPrepareThreads, 0, s>>>(a, c);
     if (const int st = check_launch("lk_kda_prefill")) return st;
-    chunk_scan_kernel<DT, NW><<<static_cast<unsigned>(scans), (NW + 2) * kWave, 0, s>>>(a, c);
+    if (two)
+      chunk_scan_kernel<DT, NW, 2><<<static_cast<unsigned>(scans), (NW + 4) * kWave, 0, s>>>(a, c);
+    else
+      chunk_scan_kernel<DT, NW, 1><<<static_cast<unsigned>(scans), (NW + 2) * kWave, 0, s>>>(a, c);
     if (const int st = check_launch("lk_kda_prefill")) return st;
   }
   return LK_OK;

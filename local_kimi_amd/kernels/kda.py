@@ -392,23 +392,27 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 def _disjoint(*tensors: torch.Tensor) -> bool:
     """Whether the dense ones among nonempty tensors share no byte (the others
     are worked on through copies)."""
-    spans = sorted([(t.data_ptr(), t.numel() * t.element_size()) for t in tensors
-                    if t.is_contiguous()])
-    return all([lo + size <= after for (lo, size), (after, _) in zip(spans, spans[1:])])
+    spans = sorted([(t.data_ptr(), t.nbytes) for t in tensors if t.is_contiguous()])
+    end = 0
+    for lo, size in spans:
+        if lo < end:
+            return False
+        end = lo + size
+    return True
 
 
 def _packed_rows(tensors) -> tuple[list[torch.Tensor], int]:
     """[B, S, C] tensors as rows one stride apart (the same for all of them):
     views of one projection's rows as they are, other layouts copied."""
-    first = tensors[0]
-    batch, rows, width = first.shape
-    stride = first.stride(1)
-    fits = stride >= width and all(
-        (width == 1 or t.stride(2) == 1) and t.stride(1) == stride and
-        (batch == 1 or t.stride(0) == rows * stride) for t in tensors)
-    if fits and rows > 1:
-        return list(tensors), stride
-    return [_aligned(t) for t in tensors], width
+    batch, rows, width = tensors[0].shape
+    stride = tensors[0].stride(1)
+    if rows < 2 or stride < width:
+        return [_aligned(t) for t in tensors], width
+    strides = (rows * stride if batch > 1 else None, stride, 1 if width > 1 else None)
+    for t in tensors:
+        if any([want is not None and have != want for have, want in zip(t.stride(), strides)]):
+            return [_aligned(t) for t in tensors], width
+    return list(tensors), stride
 
 
 def short_conv_prefill_triple(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torch.Tensor,
@@ -476,11 +480,10 @@ def short_conv_prefill_triple(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torc
             raise ValueError("the convolution states and conv_states_out must not overlap")
     elif not _disjoint(*states):
         raise ValueError("the three convolution states must not overlap")
-    weights = [_weight_view(w) for w in weights]
-    if weights[0].dtype not in _DTYPE_CODES or any(w.dtype != weights[0].dtype for w in weights):
-        weights = [w.float() for w in weights]
-    wcode = _DTYPE_CODES[weights[0].dtype]
-    weights = [_aligned(w) for w in weights]
+    wcode = _DTYPE_CODES.get(q_weight.dtype)
+    if wcode is None or k_weight.dtype != q_weight.dtype or v_weight.dtype != q_weight.dtype:
+        weights, wcode = [w.float() for w in weights], 0
+    weights = [_aligned(w) for w in weights]  # [C, 1, 4] and [C, 4] lie alike
     ins, stride = _packed_rows(values)
     src = [_aligned(st) for st in states]
     if conv_states_out is None:
@@ -488,11 +491,10 @@ def short_conv_prefill_triple(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torc
     else:
         work = [o if o.is_contiguous() and o.data_ptr() % 16 == 0 else
                 torch.empty(o.shape, dtype=o.dtype, device=dev) for o in targets]
-    outs = [torch.empty((batch, rows, channels), dtype=q_in.dtype, device=dev) for _ in range(3)]
+    outs = [torch.empty((batch, rows, channels), dtype=dtype, device=dev) for _ in range(3)]
     with _w._on(dev):
-        _lib.call("lk_kda_short_conv_prefill", *(t.data_ptr() for t in ins),
-                  *(t.data_ptr() for t in src), *(t.data_ptr() for t in work),
-                  *(t.data_ptr() for t in weights), *(t.data_ptr() for t in outs),
+        _lib.call("lk_kda_short_conv_prefill",
+                  *[t.data_ptr() for t in (*ins, *src, *work, *weights, *outs)],
                   None if offsets is None else offsets.data_ptr(), count, batch * rows, channels,
                   stride, vcode, wcode, _w._stream(dev))
     for target, w in zip(targets, work):
