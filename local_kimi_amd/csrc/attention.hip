@@ -13,6 +13,7 @@ constexpr int kAttnThreads = 256;
 constexpr int kAttnWaves = kAttnThreads / kWave;
 constexpr int kAttnQueries = 32 * kAttnWaves;  // per block
 constexpr int kAttnKeys = 64;                  // per pass of the loop
+constexpr int kJoinBlocks = kAttnQueries / kAttnWaves;  // of a block's queries
 constexpr int kAttnMaxQk = 192;
 constexpr int kAttnMaxV = 128;
 
@@ -111,20 +112,13 @@ struct AttnTile {
   RowRange q, k;
 };
 
+// From the last one back: a sequence's later tiles see more keys, and are begun first.
 __device__ inline AttnTile attention_tile(const AttnArgs& a, int64_t rank) {
   AttnTile t;
-  if (a.sq.count < 64) {  // every sequence's rows at once, a lane each
-    const int lane = threadIdx.x & (kWave - 1), s = lane < a.sq.count ? lane : a.sq.count;
-    const RowRange own = sequence_rows(a.sq, s), own_k = sequence_rows(a.sk, s);
-    t.at = find_longest_tile(own, a.sq.count, rank, kAttnQueries);
-    const int from = t.at.sequence < 0 ? 0 : t.at.sequence;
-    t.q = lane_rows(own, from);
-    t.k = lane_rows(own_k, from);
-  } else {
-    t.at = find_sequence_tile(a.sq, a.tiles - 1 - rank, kAttnQueries);
-    t.q = sequence_rows(a.sq, t.at.sequence);
-    t.k = sequence_rows(a.sk, t.at.sequence);
-  }
+  t.at = find_sequence_tile(a.sq, a.tiles - 1 - rank, kAttnQueries);
+  const int from = t.at.sequence < 0 ? 0 : t.at.sequence;
+  t.q = sequence_rows(a.sq, from);
+  t.k = sequence_rows(a.sk, from);
   return t;
 }
 
@@ -383,6 +377,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
     float* const part = a.partial + ((item / a.splits * a.heads + h) * a.splits + split) *
                                         (kAttnQueries * (DV + 2));
     const int row = wave * 32 + n;
+    if (qi >= lq) return;
 #pragma unroll
     for (int t = 0; t < kVTiles; ++t)
 #pragma unroll
@@ -417,64 +412,75 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
   }
 }
 
-// The runs of a block's keys joined: a wave takes a query, a lane its columns.
-// Weights 2^(top - largest top) in fp32, the runs in order.
+// The runs of a block's keys joined: a wave takes a query, a lane a run's maximum
+// and sum, then columns. Weights 2^(top - largest top) in fp32, the runs in order.
 template <bool BF16, int DV>
 __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttnArgs a) {
-  const int h = static_cast<int>(blockIdx.x % a.heads);
-  const int64_t rank = blockIdx.x / a.heads;
+  const int64_t block = blockIdx.x / kJoinBlocks, rank = block / a.heads;
+  const int h = static_cast<int>(block % a.heads);
   const AttnTile tile = attention_tile(a, rank);
-  const SequenceTile at = tile.at;
-  if (at.sequence < 0) return;
-  const RowRange rq = tile.q;
-  const int64_t q0 = at.tile * kAttnQueries;
+  if (tile.at.sequence < 0) return;
   const int lane = threadIdx.x & (kWave - 1);
-  const float* const parts = a.partial + (rank * a.heads + h) * a.splits * (kAttnQueries * (DV + 2));
-  for (int row = threadIdx.x / kWave; row < kAttnQueries; row += kAttnWaves) {
-    const int64_t q = rq.begin + q0 + row;
-    if (q >= rq.end) return;
-    float top = -INFINITY;
-    for (int i = 0; i < a.splits; ++i)
-      top = fmaxf(top, parts[i * (kAttnQueries * (DV + 2)) + kAttnQueries * DV + row]);
-    float sum = 0.f, acc[DV / 64] = {};
-    for (int i = 0; i < a.splits; ++i) {
-      const float* const part = parts + i * (kAttnQueries * (DV + 2));
-      const float own = part[kAttnQueries * DV + row];
-      const float w = own == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own - top);
-      sum = fmaf(w, part[kAttnQueries * (DV + 1) + row], sum);
+  const int row = blockIdx.x % kJoinBlocks * kAttnWaves + threadIdx.x / kWave;
+  const int64_t q = tile.q.begin + tile.at.tile * kAttnQueries + row;
+  if (q >= tile.q.end) return;
+  constexpr int kRun = kAttnQueries * (DV + 2), kCols = DV / 64;
+  const float* const parts = a.partial + block * a.splits * kRun;
+  const float* const tops = parts + (lane < a.splits ? lane : 0) * kRun + kAttnQueries * DV + row;
+  const float own = lane < a.splits ? tops[0] : -INFINITY;
+  float total = lane < a.splits ? tops[kAttnQueries] : 0.f, top = own;
 #pragma unroll
-      for (int x = 0; x < DV / 64; ++x)
-        acc[x] = fmaf(w, part[row * DV + DV / 64 * lane + x], acc[x]);
+  for (int m = 1; m < kWave; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+  const float weight = own == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own - top);
+  total *= weight;
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m);
+  float acc[kCols] = {};
+  for (int i0 = 0; i0 < a.splits; i0 += 8) {  // eight runs' loads at a time
+    float x[8][kCols];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+        x[i][c] = parts[(i0 + i < a.splits ? i0 + i : i0) * kRun + row * DV + kCols * lane + c];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float w = __shfl(weight, i0 + i);
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) acc[c] = i0 + i < a.splits ? fmaf(w, x[i][c], acc[c]) : acc[c];
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    uint16_t* const out = a.out + (q * a.heads + h) * a.d_v;
-    if constexpr (DV == 128) {
-      if (2 * lane < a.d_v)
-        *reinterpret_cast<uint32_t*>(out + 2 * lane) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
-    } else {
-      if (lane < a.d_v) out[lane] = static_cast<uint16_t>(pack2<BF16>(acc[0] * inv, 0.f));
-    }
+  }
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  uint16_t* const out = a.out + (q * a.heads + h) * a.d_v;
+  if constexpr (DV == 128) {
+    if (2 * lane < a.d_v)
+      *reinterpret_cast<uint32_t*>(out + 2 * lane) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
+  } else {
+    if (lane < a.d_v) out[lane] = static_cast<uint16_t>(pack2<BF16>(acc[0] * inv, 0.f));
   }
 }
 
 // Runs of each block's keys. A block alone on a CU leaves its matrix unit idle
 // through every softmax, and a call with fewer blocks than CUs leaves CUs idle: where
 // there are fewer than two blocks a CU, long key ranges are taken in runs, until
-// there are, of 512 keys at least (the runs' sums are written and read again).
+// there are, of kAttnRun keys at least (the runs' sums are written and read again).
 // Counts are estimates from the call's sizes: the lengths are on the device.
 constexpr int kAttnFill = 512;
+constexpr int kAttnRun = 384;
 int attention_splits(int64_t rows_q, int64_t rows_k, int64_t sequences, int64_t heads) {
   const int64_t blocks = (rows_q / kAttnQueries + sequences) * heads;
-  const int64_t want = (kAttnFill + blocks - 1) / blocks, most = rows_k / sequences / 512;
-  const int64_t n = want < most ? want : most;
-  return n < 1 ? 1 : (n > 16 ? 16 : static_cast<int>(n));
+  const int64_t want = (kAttnFill + blocks - 1) / blocks;
+  const int64_t seen = (rows_k - rows_q / 2) / sequences;  // keys of a query, about
+  const int64_t n = want < seen / kAttnRun ? want : seen / kAttnRun;
+  return n < 1 ? 1 : (n > kWave ? kWave : static_cast<int>(n));  // the join has a lane for each
 }
 
 template <bool BF16>
 int launch_attention(const AttnArgs& a, hipStream_t s) {
   const int64_t blocks = a.tiles * a.heads * a.splits;
-  LK_REQUIRE(blocks < (int64_t{1} << 31), "too many query rows and heads for one call");
-  const dim3 grid(static_cast<unsigned>(blocks)), join(static_cast<unsigned>(a.tiles * a.heads));
+  LK_REQUIRE(blocks < (int64_t{1} << 31) && a.tiles * a.heads * kJoinBlocks < (int64_t{1} << 31),
+             "too many query rows and heads for one call");
+  const dim3 grid(static_cast<unsigned>(blocks)), join(static_cast<unsigned>(a.tiles * a.heads * kJoinBlocks));
 #define LK_ATTENTION(Q, V)                                          \
   if (a.d_qk <= Q && a.d_v <= V) {                                  \
     attention_kernel<BF16, Q, V><<<grid, kAttnThreads, 0, s>>>(a);  \

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_prefill_kernel(ConvArgs a) 
   const int conv = item < chunks ? 0 : (item < 2 * chunks ? 1 : 2);
   const int64_t c = (item - conv * chunks) * N;
   const SequenceTile at = find_sequence_tile(a.seq, number, kConvTile);
-  if (c >= a.channels) return;
+  if (c >= a.channels || at.sequence < 0) return;
   const RowRange rows = sequence_rows(a.seq, at.sequence);
   const int64_t length = rows.end - rows.begin;
   const int64_t t0 = at.tile * kConvTile;
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanA
   const int h = static_cast<int>(blockIdx.x % a.heads);
   const int64_t local = blockIdx.x / a.heads;
   const SequenceTile at = find_sequence_tile(a.seq, c.first + local, kChunk);
-  if (at.sequence == a.seq.count) return;
+  if (at.sequence < 0 || at.sequence == a.seq.count) return;
   const RowRange rows = sequence_rows(a.seq, at.sequence);
   const int64_t t0 = rows.begin + at.tile * kChunk;
   if (t0 >= rows.end) return;
@@ -1167,6 +1167,11 @@ int64_t chunk_window(int64_t chunks, int64_t heads, int64_t record) {
   return w < chunks ? w : chunks;
 }
 
+int64_t chunk_bytes(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k, int64_t d_v) {
+  const int64_t record = chunk_record(d_k, d_v);
+  return chunk_window(sequence_tiles(tokens, sequences, kChunk), heads, record) * heads * record * 4;
+}
+
 bool takes_chunks(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k, int64_t d_v) {
   const int choice = path_choice(kKnobKdaPrefill);
   // (a chunk's outputs are stored at 31-bit byte offsets)
@@ -1264,8 +1269,7 @@ int64_t lk_kda_prefill_workspace(int64_t sequences, int64_t tokens, int64_t head
                                  int64_t d_v) {
   if (sequences <= 0 || tokens < 0 || heads <= 0 || d_k <= 0 || d_v <= 0 || d_k > 256) return -1;
   if (!takes_chunks(sequences, tokens, heads, d_k, d_v)) return 0;
-  const int64_t record = chunk_record(d_k, d_v);
-  return chunk_window(sequence_tiles(tokens, sequences, kChunk), heads, record) * heads * record * 4;
+  return chunk_bytes(sequences, tokens, heads, d_k, d_v);
 }
 
 int lk_kda_prefill(const float* state, float* state_out, const float* q, const float* k,
@@ -1284,7 +1288,9 @@ int lk_kda_prefill(const float* state, float* state_out, const float* q, const f
                         static_cast<const void*>(q), static_cast<const void*>(k), v,
                         static_cast<const void*>(decay), static_cast<const void*>(out)})
     LK_REQUIRE(aligned(p, 16), "KDA prefill tensors must start on a 16-byte boundary");
-  const int64_t need = lk_kda_prefill_workspace(sequences, tokens, heads, d_k, d_v);
+  // the choice is read once: the knob may change in the middle of a call
+  const bool chunks = takes_chunks(sequences, tokens, heads, d_k, d_v);
+  const int64_t need = chunks ? chunk_bytes(sequences, tokens, heads, d_k, d_v) : 0;
   LK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
              "KDA prefill workspace too small: %lld bytes, %lld needed",
              (long long)workspace_bytes, (long long)need);
@@ -1293,7 +1299,6 @@ int lk_kda_prefill(const float* state, float* state_out, const float* q, const f
                    static_cast<int>(heads), static_cast<int>(d_k), static_cast<int>(d_v), scale};
   LK_REQUIRE(aligned(workspace, 16), "KDA prefill workspace must be 16-byte aligned");
   const hipStream_t s = as_stream(stream);
-  const bool chunks = takes_chunks(sequences, tokens, heads, d_k, d_v);
   if (value_dtype == LK_DTYPE_F32) return launch_scan<LK_DTYPE_F32>(a, chunks, workspace, s);
   if (value_dtype == LK_DTYPE_F16) return launch_scan<LK_DTYPE_F16>(a, chunks, workspace, s);
   return launch_scan<LK_DTYPE_BF16>(a, chunks, workspace, s);

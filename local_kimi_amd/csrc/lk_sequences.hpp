@@ -7,9 +7,10 @@
 namespace lk {
 
 // `count` sequences over `rows` rows: row cu[s] to cu[s + 1] - 1 of sequence s,
-// or without offsets equal sequences of rows / count. Offsets are read on the
-// device and clamped to the rows (a decreasing pair is an empty sequence), so
-// no offset leads outside the tensors.
+// or without offsets equal sequences of rows / count. Offsets start with 0 and
+// do not decrease. They are read on the device and clamped to the rows (a
+// decreasing pair is an empty sequence), so that no offset leads outside the
+// tensors; what other offsets give is left open.
 struct Sequences {
   const int32_t* cu;
   int64_t rows;
@@ -52,8 +53,8 @@ struct SequenceTile {
 
 // The tile with this number; called by whole waves. The last s of 0..count with
 // begin(s) / tile + s <= number, 64 candidates at a time, a lane each (one load's
-// latency for up to 63 sequences). Offsets that decrease give some s of that range
-// and perhaps a number before its first.
+// latency for up to 63 sequences). Sequence -1 for a number before the found
+// one's first, which only offsets that decrease or do not start with 0 give.
 __device__ inline SequenceTile find_sequence_tile(const Sequences& q, int64_t number, int tile) {
   const int lane = static_cast<int>(threadIdx.x & 63);
   int lo = 0, span = q.count + 1;
@@ -66,46 +67,7 @@ __device__ inline SequenceTile find_sequence_tile(const Sequences& q, int64_t nu
     span = span - skip < step ? span - skip : step;
   }
   const int64_t t = number - (sequence_begin(q, lo) / tile + lo);
-  return {lo, t < 0 ? 0 : t};
-}
-
-// The same tiles from the longest down: rank 0 is a last tile of the sequence with
-// the most, ties go by sequence, and the rows behind the last sequence come at
-// the end. A tile whose cost grows with its place in its sequence is best
-// started first. For up to 63 sequences, whose rows the wave's lanes hold (`own`
-// of lane s: those of sequence s, of lane count: the ones behind the last);
-// called by whole waves. Sequence -1 where there are fewer tiles (of fewer than
-// sequence_tiles()).
-__device__ inline SequenceTile find_longest_tile(const RowRange& own, int count, int64_t rank,
-                                                 int tile) {
-  const int lane = static_cast<int>(threadIdx.x & 63);
-  const int tiles = static_cast<int>((own.end - own.begin + tile - 1) / tile);
-  const int mine = lane < count ? tiles : 0;
-  int most = mine;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int other = __shfl_xor(most, m);
-    most = other > most ? other : most;
-  }
-  int64_t left = rank;
-  for (int t = __builtin_amdgcn_readfirstlane(most) - 1; t >= 0; --t) {
-    const uint64_t have = __ballot(mine > t);
-    const int n = __popcll(have);
-    if (left < n) {
-      uint64_t rest = have;
-      for (int i = 0; i < static_cast<int>(left); ++i) rest &= rest - 1;
-      return {__ffsll(static_cast<unsigned long long>(rest)) - 1, t};
-    }
-    left -= n;
-  }
-  const int behind = __builtin_amdgcn_readlane(tiles, count);
-  return left < behind ? SequenceTile{count, left} : SequenceTile{-1, 0};
-}
-
-// What a lane of the wave holds (rows are below 2^31).
-__device__ inline RowRange lane_rows(const RowRange& own, int lane) {
-  return {__builtin_amdgcn_readlane(static_cast<int>(own.begin), lane),
-          __builtin_amdgcn_readlane(static_cast<int>(own.end), lane)};
+  return {t < 0 ? -1 : lo, t};
 }
 
 }  // namespace lk

@@ -379,7 +379,9 @@ def _offsets(cu_seqlens: torch.Tensor | None, batch: int, device: torch.device,
         raise ValueError(f"{what} must be on the inputs' device")
     if batch != 1:
         raise ValueError(f"{what} takes inputs of batch one that hold the packed sequences")
-    return _w._c(cu_seqlens.to(torch.int32)), cu_seqlens.shape[0] - 1
+    if cu_seqlens.dtype == torch.int64:  # beyond int32 is behind every row
+        cu_seqlens = cu_seqlens.clamp(0, 2 ** 31 - 1).to(torch.int32)
+    return _w._c(cu_seqlens), cu_seqlens.shape[0] - 1
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
