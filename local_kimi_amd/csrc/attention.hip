@@ -11,9 +11,9 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kAttnThreads = 256;
 constexpr int kAttnWaves = kAttnThreads / kWave;
-constexpr int kAttnQueries = 32 * kAttnWaves;  // per block
+constexpr int kAttnRows = 32 * kAttnWaves;  // queries x heads of a block
 constexpr int kAttnKeys = 64;                  // per pass of the loop
-constexpr int kJoinBlocks = kAttnQueries / kAttnWaves;  // of a block's queries
+constexpr int kJoinBlocks = kAttnRows / kAttnWaves;  // of a block's rows
 constexpr int kAttnMaxQk = 192;
 constexpr int kAttnMaxV = 128;
 
@@ -22,6 +22,9 @@ struct AttnArgs {
   uint16_t* out;
   Sequences sq, sk;
   int heads, group, d_qk, d_v;
+  // A block's rows: `tokens` queries of `pack` heads that share a key head, row r
+  // query r / pack (r inv_pack >> 16), head r % pack. Blocks for a query: `packs`.
+  int pack, inv_pack, tokens, packs;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   int64_t tiles;
   int splits;       // runs of each block's keys
@@ -115,7 +118,7 @@ struct AttnTile {
 // From the last one back: a sequence's later tiles see more keys, and are begun first.
 __device__ inline AttnTile attention_tile(const AttnArgs& a, int64_t rank) {
   AttnTile t;
-  t.at = find_sequence_tile(a.sq, a.tiles - 1 - rank, kAttnQueries);
+  t.at = find_sequence_tile(a.sq, a.tiles - 1 - rank, a.tokens);
   const int from = t.at.sequence < 0 ? 0 : t.at.sequence;
   t.q = sequence_rows(a.sq, from);
   t.k = sequence_rows(a.sk, from);
@@ -139,21 +142,24 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
   // p is stored as 2^kLift times itself: fp16 keeps 2^-24 at the least
   constexpr float kLift = BF16 ? 0.f : 6.f;
   __shared__ alignas(16) uint16_t stage[2 * kStage];
-  const int h = static_cast<int>(blockIdx.x % a.heads);
-  const int64_t item = blockIdx.x / a.heads;
+  const int pack = static_cast<int>(blockIdx.x % a.packs);
+  const int64_t item = blockIdx.x / a.packs;
   const int split = static_cast<int>(item % a.splits);
   const AttnTile tile = attention_tile(a, item / a.splits);
   const SequenceTile at = tile.at;
   if (at.sequence < 0) return;
   const RowRange rq = tile.q;
   const int64_t lq = rq.end - rq.begin;
-  const int64_t q0 = at.tile * kAttnQueries;
+  const int64_t q0 = at.tile * a.tokens;
   if (q0 >= lq) return;
+  const int64_t last = q0 + a.tokens < lq ? q0 + a.tokens : lq;  // the block's, exclusive
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int n = lane & 31, half = lane >> 5;
-  const int64_t qw = q0 + wave * 32;  // the wave's first query
-  const int64_t qi = qw + n;          // the lane's
+  const int64_t qw = q0 + (wave * 32 * a.inv_pack >> 16);  // the wave's first query
+  const int row = wave * 32 + n, token = row * a.inv_pack >> 16;
+  const int64_t qi = q0 + token;  // the lane's, of this head
+  const int h = pack * a.pack + row - token * a.pack;
   f32x16_t o[kVTiles];
 #pragma unroll
   for (int t = 0; t < kVTiles; ++t)
@@ -166,14 +172,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
     const int64_t lk = rk.end - rk.begin;
     const int64_t ahead = lk - lq;
     // keys seen by the block's last query, and by the wave's
-    const int64_t last = q0 + kAttnQueries < lq ? q0 + kAttnQueries : lq;
     const int64_t all = last + ahead < 0 ? 0 : last + ahead;
     // this block's run of them, and the wave's end of it
     const int64_t per = ((all + a.splits - 1) / a.splits + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
     const int64_t from = split * per < all ? split * per : all;
     const int64_t keys = from + per < all ? from + per : all;
-    const int64_t keys_wave = qw + 32 + ahead < keys ? qw + 32 + ahead : keys;
-    const int hk = h / a.group;
+    const int64_t end_wave = q0 + ((wave * 32 + 31) * a.inv_pack >> 16) + 1 + ahead;
+    const int64_t keys_wave = end_wave < keys ? end_wave : keys;
+    const int hk = pack * a.pack / a.group;
     const uint16_t* const kb = a.k + rk.begin * a.k_row + hk * a.k_head;
     const uint16_t* const vb = a.v + rk.begin * a.v_row + hk * a.v_head;
     u32x4_t qf[kQSteps];
@@ -374,10 +380,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
   }
   if (a.partial) {
     // the run's sums as they are, with what they are taken against
-    float* const part = a.partial + ((item / a.splits * a.heads + h) * a.splits + split) *
-                                        (kAttnQueries * (DV + 2));
-    const int row = wave * 32 + n;
-    if (qi >= lq) return;
+    float* const part = a.partial + ((item / a.splits * a.packs + pack) * a.splits + split) *
+                                        (kAttnRows * (DV + 2));
+    if (qi >= last) return;
 #pragma unroll
     for (int t = 0; t < kVTiles; ++t)
 #pragma unroll
@@ -385,8 +390,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
         *reinterpret_cast<float4*>(part + row * DV + 32 * t + 8 * (r / 4) + 4 * half) =
             make_float4(o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]);
     if (half == 0) {
-      part[kAttnQueries * DV + row] = top;
-      part[kAttnQueries * (DV + 1) + row] = sum;
+      part[kAttnRows * DV + row] = top;
+      part[kAttnRows * (DV + 1) + row] = sum;
     }
     return;
   }
@@ -406,8 +411,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
 #pragma unroll
   for (int i = 0; i < 32 * kVChunks / kWave; ++i) {
     const int slot = i * kWave + lane, r = slot / kVChunks, d = slot % kVChunks * 8;
-    if (qw + r < lq && d < a.d_v)
-      *reinterpret_cast<u32x4_t*>(a.out + ((rq.begin + qw + r) * a.heads + h) * a.d_v + d) =
+    const int to = wave * 32 + r, q = to * a.inv_pack >> 16;
+    const int64_t head = pack * a.pack + to - q * a.pack;
+    if (q0 + q < last && d < a.d_v)
+      *reinterpret_cast<u32x4_t*>(a.out + ((rq.begin + q0 + q) * a.heads + head) * a.d_v + d) =
           *reinterpret_cast<const u32x4_t*>(rows + r * kOutStride + d);
   }
 }
@@ -416,19 +423,20 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
 // and sum, then columns. Weights 2^(top - largest top) in fp32, the runs in order.
 template <bool BF16, int DV>
 __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttnArgs a) {
-  const int64_t block = blockIdx.x / kJoinBlocks, rank = block / a.heads;
-  const int h = static_cast<int>(block % a.heads);
-  const AttnTile tile = attention_tile(a, rank);
+  const int64_t block = blockIdx.x / kJoinBlocks;
+  const AttnTile tile = attention_tile(a, block / a.packs);
   if (tile.at.sequence < 0) return;
   const int lane = threadIdx.x & (kWave - 1);
   const int row = blockIdx.x % kJoinBlocks * kAttnWaves + threadIdx.x / kWave;
-  const int64_t q = tile.q.begin + tile.at.tile * kAttnQueries + row;
-  if (q >= tile.q.end) return;
-  constexpr int kRun = kAttnQueries * (DV + 2), kCols = DV / 64;
+  const int token = row * a.inv_pack >> 16;
+  const int64_t q = tile.q.begin + tile.at.tile * a.tokens + token;
+  const int64_t h = block % a.packs * a.pack + row - token * a.pack;
+  if (token >= a.tokens || q >= tile.q.end) return;
+  constexpr int kRun = kAttnRows * (DV + 2), kCols = DV / 64;
   const float* const parts = a.partial + block * a.splits * kRun;
-  const float* const tops = parts + (lane < a.splits ? lane : 0) * kRun + kAttnQueries * DV + row;
+  const float* const tops = parts + (lane < a.splits ? lane : 0) * kRun + kAttnRows * DV + row;
   const float own = lane < a.splits ? tops[0] : -INFINITY;
-  float total = lane < a.splits ? tops[kAttnQueries] : 0.f, top = own;
+  float total = lane < a.splits ? tops[kAttnRows] : 0.f, top = own;
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
   const float weight = own == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own - top);
@@ -460,6 +468,17 @@ __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttnArgs a
   }
 }
 
+// Heads of a block: as many as divide those of a key head, up to 16, so that a
+// key is read once for all of them and a few queries fill more of a block's rows.
+// (With more, the rows that 128 leaves over weigh more than what is saved.)
+constexpr int kAttnPack = 16;
+int attention_pack(int64_t heads, int64_t kv_heads) {
+  int pack = 1;
+  for (int p = 2; p <= kAttnPack; ++p)
+    if (heads / kv_heads % p == 0) pack = p;
+  return pack;
+}
+
 // Runs of each block's keys. A block alone on a CU leaves its matrix unit idle
 // through every softmax, and a call with fewer blocks than CUs leaves CUs idle: where
 // there are fewer than two blocks a CU, long key ranges are taken in runs, until
@@ -467,8 +486,8 @@ __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttnArgs a
 // Counts are estimates from the call's sizes: the lengths are on the device.
 constexpr int kAttnFill = 512;
 constexpr int kAttnRun = 384;
-int attention_splits(int64_t rows_q, int64_t rows_k, int64_t sequences, int64_t heads) {
-  const int64_t blocks = (rows_q / kAttnQueries + sequences) * heads;
+int attention_splits(int64_t rows_q, int64_t rows_k, int64_t sequences, int64_t heads, int pack) {
+  const int64_t blocks = (rows_q / (kAttnRows / pack) + sequences) * (heads / pack);
   const int64_t want = (kAttnFill + blocks - 1) / blocks;
   const int64_t seen = (rows_k - rows_q / 2) / sequences;  // keys of a query, about
   const int64_t n = want < seen / kAttnRun ? want : seen / kAttnRun;
@@ -477,10 +496,10 @@ int attention_splits(int64_t rows_q, int64_t rows_k, int64_t sequences, int64_t 
 
 template <bool BF16>
 int launch_attention(const AttnArgs& a, hipStream_t s) {
-  const int64_t blocks = a.tiles * a.heads * a.splits;
-  LK_REQUIRE(blocks < (int64_t{1} << 31) && a.tiles * a.heads * kJoinBlocks < (int64_t{1} << 31),
+  const int64_t items = a.tiles * a.packs, blocks = items * a.splits;
+  LK_REQUIRE(blocks < (int64_t{1} << 31) && items * kJoinBlocks < (int64_t{1} << 31),
              "too many query rows and heads for one call");
-  const dim3 grid(static_cast<unsigned>(blocks)), join(static_cast<unsigned>(a.tiles * a.heads * kJoinBlocks));
+  const dim3 grid(static_cast<unsigned>(blocks)), join(static_cast<unsigned>(items * kJoinBlocks));
 #define LK_ATTENTION(Q, V)                                          \
   if (a.d_qk <= Q && a.d_v <= V) {                                  \
     attention_kernel<BF16, Q, V><<<grid, kAttnThreads, 0, s>>>(a);  \
@@ -510,10 +529,12 @@ int64_t lk_attention_prefill_workspace(int64_t rows_q, int64_t rows_k, int64_t s
   if (rows_q < 0 || rows_k < 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 ||
       heads % kv_heads || d_qk <= 0 || d_v <= 0 || d_qk > kAttnMaxQk || d_v > kAttnMaxV)
     return -1;
-  const int64_t splits = attention_splits(rows_q, rows_k, sequences, heads);
+  const int pack = attention_pack(heads, kv_heads);
+  const int64_t splits = attention_splits(rows_q, rows_k, sequences, heads, pack);
   if (splits == 1) return 0;
   const int64_t dv = d_qk <= 64 && d_v <= 64 ? 64 : 128;
-  return sequence_tiles(rows_q, sequences, kAttnQueries) * heads * splits * kAttnQueries * (dv + 2) * 4;
+  const int64_t tiles = sequence_tiles(rows_q, sequences, kAttnRows / pack);
+  return tiles * (heads / pack) * splits * kAttnRows * (dv + 2) * 4;
 }
 
 int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
@@ -559,7 +580,7 @@ int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
              (long long)need);
   LK_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
              "attention workspace must be 16-byte aligned");
-  const int n = static_cast<int>(sequences);
+  const int n = static_cast<int>(sequences), pack = attention_pack(heads, kv_heads);
   const AttnArgs a{static_cast<const uint16_t*>(q),
                    static_cast<const uint16_t*>(k),
                    static_cast<const uint16_t*>(v),
@@ -570,10 +591,14 @@ int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
                    static_cast<int>(heads / kv_heads),
                    static_cast<int>(d_qk),
                    static_cast<int>(d_v),
+                   pack,
+                   65536 / pack + 1,
+                   kAttnRows / pack,
+                   static_cast<int>(heads) / pack,
                    q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride,
                    v_head_stride,
-                   sequence_tiles(rows_q, sequences, kAttnQueries),
-                   attention_splits(rows_q, rows_k, sequences, heads),
+                   sequence_tiles(rows_q, sequences, kAttnRows / pack),
+                   attention_splits(rows_q, rows_k, sequences, heads, pack),
                    need ? static_cast<float*>(workspace) : nullptr,
                    scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f,
                    scale == 0.f ? 0u : 0xFFFFFFFFu,
