@@ -29,8 +29,9 @@ extern "C" {
  * cu_q[s + 1] - 1 and key rows cu_k[s] to cu_k[s + 1] - 1; a null cu_q (cu_k)
  * means equal sequences of rows_q (rows_k) / sequences. A sequence's queries
  * are its last rows: query i of lq sees keys 0 .. i + lk - lq of lk. One that
- * sees none gets zeros, as do the rows behind the last sequence. Offsets are
- * clamped to the rows.
+ * sees none gets zeros, as do the rows behind the last sequence. Offsets start
+ * with 0 and do not decrease; they are clamped to the rows, so that others lead
+ * nowhere outside the tensors. out overlaps nothing.
  *   o_i = sum_j p_ij v_j,  p_i = softmax over the keys seen of scale * q_i . k_j
  * Scores and sums in fp32; p is rounded to dtype for its product with v. A key
  * or value row that a query does not see has no part in its result, NaN and

@@ -108,10 +108,12 @@ LK_API int lk_kda_decode_layer_split(const void* q_in, const void* k_in, const v
  *
  * Sequences are packed one behind the other over the rows of a call: sequence
  * s has rows cu_seqlens[s] to cu_seqlens[s + 1] - 1 (int32 [sequences + 1] on
- * the device, starting with 0; clamped to the rows), or with a null cu_seqlens
- * tokens / sequences rows each. A sequence may be empty: its state is kept.
- * Output rows behind the last sequence are set to zero. A state may be
- * updated in place (state_out = state) or written elsewhere. */
+ * the device, starting with 0 and not decreasing; clamped to the rows, so that
+ * others lead nowhere outside the tensors), or with a null cu_seqlens tokens /
+ * sequences rows each. A sequence may be empty: its state is kept. Output
+ * rows behind the last sequence are set to zero. A state may be updated in
+ * place (state_out = state) or written elsewhere; nothing else that is
+ * written may overlap anything. Reruns are bit-identical. */
 
 /* the three width-4 convolutions of a prompt: what lk_kda_short_conv_triple
  * computes token by token. inputs [tokens, C] in value_dtype, row_stride
@@ -134,8 +136,12 @@ LK_API int lk_kda_short_conv_prefill(const void* q_in, const void* k_in, const v
  * writes them for any number of rows), v [tokens, H, d_v] and out
  * [tokens, H, d_v] in value_dtype, state fp32 [sequences, H, d_k, d_v].
  * decay <= 0 (a log decay). d_k <= 256; tensors start on 16 bytes. All sums
- * and the state are fp32; out is rounded once. workspace:
- * lk_kda_prefill_workspace() bytes on 16 bytes (may be null where that is 0). */
+ * and the state are fp32; out is rounded once. From 48 tokens a sequence on and
+ * up to d_k = 128, chunks of 32 steps are solved together, in which the operands
+ * of the state's products are sums of two fp16 (22 bits of the largest beside
+ * them); otherwise steps follow one another in fp32. The knob kda_prefill
+ * (lk_set_path) asks for one form. workspace: lk_kda_prefill_workspace() bytes
+ * on 16 bytes (may be null where that is 0), by the knob's setting of the call. */
 LK_API int64_t lk_kda_prefill_workspace(int64_t sequences, int64_t tokens, int64_t heads,
                                         int64_t d_k, int64_t d_v);
 

@@ -125,12 +125,23 @@ __device__ inline AttnTile attention_tile(const AttnArgs& a, int64_t rank) {
   return t;
 }
 
-// Block = 128 queries of one head, a wave 32 of them. Scores are computed
-// transposed, S^T = K Q^T (32x32 MFMA tiles, keys down, queries across), so a
-// lane holds one query's scores in its registers: the softmax needs one
-// exchange between the half-waves per 64 keys, the running maximum and sum are
+// o_i = sum_j p_ij v_j / sum_j p_ij, p_ij = 2^(s_ij - top_i), in one pass over the
+// keys: s in units of log2, top_i the running maximum, what is summed scaled down
+// where it moves.
+//
+// Block = 128 rows (queries x heads of one key head), a wave 32 of them. Scores
+// are computed transposed, S^T = K Q^T (32x32 MFMA tiles, keys down, queries
+// across), so a lane holds one query's scores in its registers: the softmax needs
+// one exchange between the half-waves per 64 keys, the running maximum and sum are
 // a scalar per lane, and the score registers, rounded, are the B operand of
-// O^T += V^T P^T as they stand.
+// O^T += V^T P^T as they stand. That rounding of p to the inputs' type is the one
+// before the output's: the products need it, the sums of p are of the unrounded.
+//
+// Two stages of 64 keys are up to 80 KB of LDS, so two blocks share a CU and one's
+// products run beside the other's softmax. Long prompts are bound by the matrix
+// unit and VALU together (53% and 31% of the cycles, at the 1.8 GHz that the power
+// allows): 8192 tokens x 32 heads of 192/128 take 690 us, 996 TFLOP/s, where a bf16
+// 8192^3 library product reaches 1139. Short calls are bound by latency.
 template <bool BF16, int DQ, int DV>
 __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) {
   constexpr int kQSteps = DQ / 16;
@@ -484,6 +495,9 @@ int attention_pack(int64_t heads, int64_t kv_heads) {
 // there are fewer than two blocks a CU, long key ranges are taken in runs, until
 // there are, of kAttnRun keys at least (the runs' sums are written and read again).
 // Counts are estimates from the call's sizes: the lengths are on the device.
+// With one run / by this rule, bf16 heads of 128: one query x 16384 keys x 8 heads
+// 329 / 21 us, 512 x 4096 x 32 93 / 58, 4096 x 4096 x 4 91 / 44, 16 x 800 x 32 23 / 18.
+// 1024 queries x 1024 keys x 32 took 30 in one and 40 in two runs (of 256 keys).
 constexpr int kAttnFill = 512;
 constexpr int kAttnRun = 384;
 int attention_splits(int64_t rows_q, int64_t rows_k, int64_t sequences, int64_t heads, int pack) {

@@ -45,11 +45,13 @@ struct alignas(sizeof(T) * N) Pack {
 // per channel, with x before a sequence's first token from its state; the
 // state becomes the last four of (state, tokens).
 //
-// Bound by HBM: 12 operations on a value that is read and written once. A
+// Bound by HBM: 12 operations on a value that is read and written once (16384
+// tokens x 3 x 2304 fp16: 89 us, 5.1 TB/s, as fast as a large copy). A
 // thread owns N neighbouring channels (16 bytes) of one convolution and walks
 // a tile of kConvTile tokens with the three earlier inputs in registers,
 // kConvRows rows' loads in flight; the tile's first three inputs are read again (3
-// rows in kConvTile, mostly from a cache). Threads are dealt over the three
+// rows in kConvTile, mostly from a cache). Where rows do not start on 16 bytes, N
+// is one. Threads are dealt over the three
 // convolutions' channels as one row, so that only a call's last block has idle
 // ones. The thread with a sequence's first tile has read the state's values, so
 // it is the one that replaces them: the state may be updated in place.
@@ -194,7 +196,9 @@ __global__ void __launch_bounds__(kConvThreads) conv_prefill_kernel(ConvArgs a) 
 // column l / 16, sums over the 16 lanes of a DPP row. A block of four waves
 // takes 16 columns and stages kSerialTokens steps of q, k, e^g and k . q in
 // LDS (one lane of the staging per 16th of a row, as the steps use them) while
-// the batch before it runs.
+// the batch before it runs. Bound by the chain from step to step: LDS reads, the
+// products, 8 DPP additions, 0.4 us a step (heads of 128 x 128: 20 steps 10 us,
+// 256 steps 90 us).
 constexpr int kSerialThreads = 256;
 constexpr int kSerialCols = 16;
 constexpr int kSerialTokens = 16;
@@ -361,8 +365,10 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(ScanArgs a,
 // which is the step form with its corrections u solved for together. Only the
 // last line follows from chunk to chunk, so one launch computes W, U0, P and the
 // scaled rows of every chunk (chunk_prepare_kernel) and another takes the
-// states through them (chunk_scan_kernel), on fp32 matrix instructions: state and
-// sums keep fp32, as the step form has them.
+// states through them (chunk_scan_kernel). State, sums and everything that leaves
+// the second launch are fp32; what multiplies there, W, Q, K, S and U, goes in as
+// sums of two fp16 (22 bits, with powers of two beside them: see Scale), since an
+// fp32 matrix instruction takes 8 times the time of four fp16 products.
 //
 // Decays are multiplied up, never divided or taken as differences of sums: every
 // product of e^g <= 1 stays in [0, 1] with a relative error of 2^-24 a factor,
@@ -374,21 +380,23 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(ScanArgs a,
 // M = W_b (beta k D)_a^T over a's decays to its end,
 //   W_b <- W_b D_a - M W_a,  U0_b <- U0_b - M U0_a,  P_ba = (scale q D)_b (beta k D)_a^T,
 //   (q D)_b <- (q D)_b D_a,  (beta k D)_a <- (beta k D)_a D_b.
-// The scan is bound by what a chunk costs beside its products (a barrier and an
-// exchange through LDS, 0.35 us): chunks of 16 took 0.83 us each.
+// The scan is bound by the way from one chunk's state to the next (products, a
+// barrier, an exchange through LDS, 1.2 us), hence not 16 steps a chunk: 8192 tokens
+// x 32 heads took 707 us in chunks of 16, 605 in chunks of 32.
 //
 // Records. A chunk and head has one record in the workspace, its parts in the
 // order in which the second launch's lanes load them (16 bytes a lane, 1 KB a
 // wave): with m = lane % 16, g = lane / 16, r = 0..3, half h
-//   W, Q (scale q D):    [h][tile t][lane][r] = row 16 h + m, channel 16 t + 4 g + r
-//   K (beta k D_(.,31]): [h][tile t][lane][r] = channel 16 t + m, step 16 h + 4 g + r
+//   W, Q (scale q D):    [h][p][hi, lo][lane][i] = row 16 h + m, channel 32 p + c(i)
+//   K (beta k D_(.,31]): [t][hi, lo][lane][i] = channel 16 t + m, step c(i)
+//                        (i = 0..7, c(i) = 16 (i / 4) + 4 g + i % 4)
 //   D (D_31):            [channel]
 //   P:                   [aa, ba, bb][lane][r] = row m, column 4 g + r of that block
+//   the inverse scales of W's rows, Q's rows and K's tiles
 //   U0:                  [h][tile t][lane][r] = value column 16 t + m, step 16 h + 4 g + r
-// These are the A operands of v_mfma_f32_16x16x4 for B operands that are the
-// accumulators of an earlier one as they stand: lane (m, g) of a 16 x 16 result
-// holds column m, rows 4 g + r, and register r of it serves as the rows 4 g + r of a
-// product over 16.
+// These are A operands for B operands that are the accumulators of an earlier
+// product as they stand: lane (m, g) of a 16 x 16 result holds column m, rows 4 g + r,
+// and two such tiles, split, serve as 32 rows of a product over 32.
 constexpr int kHalf = 16;
 constexpr int kChunk = 2 * kHalf;
 constexpr int kPrepareThreads = 512;  // four waves a half
@@ -483,6 +491,10 @@ __device__ inline int after(int at, float x) {
 
 __device__ inline f32x4_t lds4(const float* p) { return *reinterpret_cast<const f32x4_t*>(p); }
 
+// Block = one chunk and head. LDS reads fill 65% of the time and VALU 54%, of which
+// A and P are most; 3840 records of 32 steps x 128 x 128 take 148 us, 370 MB read
+// and written. Two blocks share a CU (80 KB of LDS each) and cover each other's
+// loads and barriers.
 template <int DT, int NW>
 __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanArgs a, ChunkArgs c) {
   using T = typename Storage<DT>::type;
@@ -762,20 +774,21 @@ __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanA
   }
 }
 
-// Block = one sequence's and head's 16 value columns, through the chunks of the
-// window. Each of four waves keeps 16 RT key rows of the state as accumulators; the
+// Block = one sequence's and head's 16 CT value columns, through the chunks of the
+// window. Each of NW waves keeps 32 key rows of the state as accumulators; the
 // sums over all rows (W S - U0, Q S) meet in LDS, in wave order, with one barrier a
 // chunk: W S before it, Q S behind it, where it covers the wait for the other
-// waves' sums. Two more waves, one for each half, do what is off the path from one
-// state to the next: they bring U0 and the decays, and add up, complete (P U) and
-// store the outputs, a chunk later.
+// waves' sums. Two more waves for each 16 columns, one for each half, do what is
+// off the path from one state to the next: they bring U0 and the decays, and
+// add up, complete (P U) and store the outputs, a chunk later.
 //
-// 48 of a record's 58 KB are loaded as operands, 16 cycles of the CU's address
-// unit for each 1 KB, against 48 matrix instructions of 32 cycles on each SIMD.
-// The four waves meet at the barrier, so their loads come at the same time: they
-// are put between the products that follow it (in one place they held the waves
-// up for 500 cycles of 1900), two chunks ahead, and without a branch (the last
-// record again at the end), so that a wait leaves the younger ones in flight.
+// Bound by that path: 1.2 us a chunk for 32 heads of 128 x 128, where the matrix
+// unit is busy for a sixth of the time and VALU for a third. 48 of a record's 68 KB
+// are loaded as operands by the blocks of each 16 columns. The waves meet at the
+// barrier, so their loads come at the same time: they are put between the
+// products that follow it (in one place they held the waves up for 500 cycles of
+// 1900), two chunks ahead, and without a branch (the last record again at the
+// end), so that a wait leaves the younger ones in flight.
 template <int DT, int NW, int CT>
 __global__ void __launch_bounds__((NW + 2 * CT) * kWave)
 chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
@@ -1156,10 +1169,16 @@ int64_t chunk_record(int64_t d_k, int64_t d_v) {
   return channels * (3 * kChunk + 1) + 3 * 256 + 2 * kChunk + 16 + (d_v + 15) / 16 * 16 * kChunk;
 }
 
+// From this many 16-column tiles of a call on (twice as many as keep two blocks on
+// each CU), a block takes two: half the blocks load the same records. 4096 tokens
+// of 11 sequences x 32 heads x 8 tiles: 361 us with one, 335 with two; a single
+// prompt's 256 tiles, which fill the CUs once: 587 with one, 705 with two.
 constexpr int64_t kTwoTiles = 1024;
 
 // Chunks of one window: the records of a window are written by one launch and
-// read by the next, so they are kept within the 256 MB cache in front of HBM.
+// read by the next, partly from the 256 MB cache in front of HBM. Smaller windows
+// leave more of them there, but begin and end more launches: 32, 64 and 128 MB
+// were slower for 8192 tokens x 32 heads. It bounds the workspace as well.
 constexpr int64_t kWindowBytes = int64_t{256} << 20;
 int64_t chunk_window(int64_t chunks, int64_t heads, int64_t record) {
   const int64_t most = kWindowBytes / (heads * record * 4);
@@ -1174,7 +1193,10 @@ int64_t chunk_bytes(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_
 
 bool takes_chunks(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k, int64_t d_v) {
   const int choice = path_choice(kKnobKdaPrefill);
-  // (a chunk's outputs are stored at 31-bit byte offsets)
+  // (a chunk's outputs are stored at 31-bit byte offsets.) Chunks from 48 tokens a
+  // sequence on: 32 heads of 128 x 128 took, in steps / in chunks, for one sequence of
+  // 32 tokens 15 / 18 us, of 48 19 / 19, of 128 48 / 22, for 32 sequences of 32 tokens
+  // 150 / 172, of 64 269 / 241.
   if (d_k > 128 || tokens == 0 || choice == 1 || heads * d_v >= (int64_t{1} << 24)) return false;
   return choice == 2 || tokens >= 48 * sequences;
 }
@@ -1187,8 +1209,6 @@ int launch_chunks(const ScanArgs& a, float* records, hipStream_t s) {
   c.v_tiles = (a.d_v + 15) / 16;
   const int64_t chunks = sequence_tiles(a.seq.rows, a.seq.count, kChunk);
   const int64_t window = chunk_window(chunks, a.heads, c.record);
-  // a block reads a head's records for one tile of value columns, or for two where
-  // there are enough of them to fill the CUs twice
   const int64_t pairs = (a.seq.count + 1) * static_cast<int64_t>(a.heads);
   const bool two = c.v_tiles > 1 && a.seq.count * static_cast<int64_t>(a.heads) * c.v_tiles >= kTwoTiles;
   const int64_t scans = (pairs + 7) / 8 * 8 * (two ? (c.v_tiles + 1) / 2 : c.v_tiles);

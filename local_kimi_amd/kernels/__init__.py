@@ -145,7 +145,8 @@ _register_mxfp4()
 
 __all__ = [
     "registry", "kda_decode_step", "kda_decode_layer", "fused_short_conv_triple",
-    "fused_kda_gates", "kda_prefill", "short_conv_prefill_triple", "attention_prefill", "rms_norm", "add_rms_norm", "rms_gated_norm",
+    "fused_kda_gates", "kda_prefill", "short_conv_prefill_triple", "attention_prefill",
+    "rms_norm", "add_rms_norm", "rms_gated_norm",
     "W4A16_GROUPED", "W4A16_DENSE", "W4A16_SWIGLU", "W4A16_FUSED_QKV",
     "W4A16_W2_COMBINE", "W4A16_MOE_BLOCK", "moe_router", "router_logits",
     "shape_stable_expert_indices",

@@ -46,8 +46,8 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     d_v up to 128. The queries are the last S of the S_k positions: query i
     sees keys 0 .. i + S_k - S, and one that sees none gets zeros.
 
-    With ``cu_seqlens`` [N + 1] (int32 or int64, on the device, from 0) B is one
-    and the S rows hold N packed sequences, whose keys are the same rows of
+    With ``cu_seqlens`` [N + 1] (int32 or int64, on the device, from 0, not
+    decreasing) B is one and the S rows hold N packed sequences, whose keys are the same rows of
     ``k`` and ``v``, or with ``cu_seqlens_k`` [N + 1] the rows that it gives.
     Offsets are clamped to the rows; output rows behind the last sequence are
     zero.

@@ -430,7 +430,7 @@ def short_conv_prefill_triple(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torc
     ``q_in``, ``k_in``, ``v_in`` [B, S, C]; states [B, C, 4] and weights
     [C, 1, 4] (or [C, 4]) as ``fused_short_conv_triple`` takes them, which
     this equals token by token. With ``cu_seqlens`` [N + 1] (int32 or int64, on
-    the device, from 0) B is one, the S rows hold N packed sequences and the
+    the device, from 0, not decreasing) B is one, the S rows hold N packed sequences and the
     states are [N, C, 4]; offsets are clamped to the rows, and output rows
     behind the last sequence are zero. A sequence may be empty (its state
     stays). A fresh prompt's state is zeros.
@@ -515,14 +515,15 @@ def kda_prefill(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.
     ``q``, ``k``, ``decay`` [B, S, H, d_k] and ``beta`` [B, S, H] float32 (as
     ``fused_kda_gates`` returns them, ``decay`` <= 0), ``v`` [B, S, H, d_v] float32,
     float16 or bfloat16, ``state`` float32 [B, H, d_k, d_v]. With
-    ``cu_seqlens`` [N + 1] (int32 or int64, on the device, from 0) B is one,
-    the S rows hold N packed sequences and ``state`` is [N, H, d_k, d_v];
-    offsets are clamped to the rows, and output rows behind the last sequence
-    are zero. A sequence may be empty (its state stays). A fresh prompt's
-    state is zeros.
+    ``cu_seqlens`` [N + 1] (int32 or int64, on the device, from 0, not
+    decreasing) B is one, the S rows hold N packed sequences and ``state`` is
+    [N, H, d_k, d_v]; offsets are clamped to the rows, and output rows behind
+    the last sequence are zero. A sequence may be empty (its state stays). A
+    fresh prompt's state is zeros.
 
-    Returns the output [B, S, H, d_v] in v's dtype (sums and state are fp32,
-    one rounding at the end); ``state`` is updated in place, or with
+    Returns the output [B, S, H, d_v] in v's dtype (sums and state are fp32, the
+    output is rounded once; from 48 tokens a sequence on, operands of the
+    state's products have 22 bits); ``state`` is updated in place, or with
     ``state_out`` left as it is and the new one written there. d_k up to 256.
     """
     if q.ndim != 4:

@@ -1,10 +1,11 @@
-"""Kimi Delta Attention decode kernels, restated in numpy (test infrastructure).
+"""Kimi Delta Attention kernels, restated in numpy (test infrastructure).
 
 Only the tests, ``__graft_entry__.smoke()`` and the bench's CPU leg use this
 module, as the checker of the HIP kernels; nothing in the product path calls it.
 
-Three functions, each in float64 so it serves as the exact answer the fp32
-kernels are held to:
+Three functions of one token, each in float64 so it serves as the exact answer
+the fp32 kernels are held to, and at the end of the file the same over whole
+prompts:
 
 * ``decode_step``  — engine/kernels/kda_step.py:173-196 (the eager recurrence):
   S ← S·exp(decay) row-wise; pred = Sᵀk; S ← S + β·k·(v − pred)ᵀ;
