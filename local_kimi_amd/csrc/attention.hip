@@ -13,7 +13,8 @@ constexpr int kAttnThreads = 256;
 constexpr int kAttnWaves = kAttnThreads / kWave;
 constexpr int kAttnRows = 32 * kAttnWaves;  // queries x heads of a block
 constexpr int kAttnKeys = 64;                  // per pass of the loop
-constexpr int kJoinBlocks = kAttnRows / kAttnWaves;  // of a block's rows
+constexpr int kJoinRows = 2;  // of a wave of the join
+constexpr int kJoinBlocks = kAttnRows / (kAttnWaves * kJoinRows);
 constexpr int kAttnMaxQk = 192;
 constexpr int kAttnMaxV = 128;
 
@@ -430,52 +431,89 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
   }
 }
 
-// The runs of a block's keys joined: a wave takes a query, a lane a run's maximum
-// and sum, then columns. Weights 2^(top - largest top) in fp32, the runs in order.
+// A sum (or maximum) over the wave's lanes, in every lane.
+template <typename Op>
+__device__ inline float over_wave(float v, Op op) {
+  v = op(v, dpp_f32<kQuadXor1>(v));
+  v = op(v, dpp_f32<kQuadXor2>(v));
+  v = op(v, dpp_f32<kRowHalfMirror>(v));
+  v = op(v, dpp_f32<kRowMirror>(v));
+  auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+
+// The runs of a block's keys joined: a wave takes kJoinRows rows, a lane a run's
+// maxima and sums of them, then columns. Weights 2^(top - largest top) in fp32, the
+// runs in order. Bound by latency, a chain of five loads: with one row a wave there
+// were more rounds of them (777 queries x 32 heads in two runs: 151 us with the runs
+// themselves, 146 with two rows or four), with four a single query waited for
+// rows that it does not have (1 x 16384 keys: 24 us, 26 with four).
 template <bool BF16, int DV>
 __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttnArgs a) {
   const int64_t block = blockIdx.x / kJoinBlocks;
   const AttnTile tile = attention_tile(a, block / a.packs);
   if (tile.at.sequence < 0) return;
+  constexpr int kRun = kAttnRows * (DV + 2), kCols = DV / 64, kRuns = 4;
   const int lane = threadIdx.x & (kWave - 1);
-  const int row = blockIdx.x % kJoinBlocks * kAttnWaves + threadIdx.x / kWave;
-  const int token = row * a.inv_pack >> 16;
-  const int64_t q = tile.q.begin + tile.at.tile * a.tokens + token;
-  const int64_t h = block % a.packs * a.pack + row - token * a.pack;
-  if (token >= a.tokens || q >= tile.q.end) return;
-  constexpr int kRun = kAttnRows * (DV + 2), kCols = DV / 64;
+  const int row0 = (blockIdx.x % kJoinBlocks * kAttnWaves + threadIdx.x / kWave) * kJoinRows;
+  const int64_t q0 = tile.q.begin + tile.at.tile * a.tokens;
+  const int64_t head0 = block % a.packs * a.pack;
+  auto exists = [&](int row) {
+    const int token = row * a.inv_pack >> 16;
+    return token < a.tokens && q0 + token < tile.q.end;
+  };
+  if (!exists(row0)) return;
   const float* const parts = a.partial + block * a.splits * kRun;
-  const float* const tops = parts + (lane < a.splits ? lane : 0) * kRun + kAttnRows * DV + row;
-  const float own = lane < a.splits ? tops[0] : -INFINITY;
-  float total = lane < a.splits ? tops[kAttnRows] : 0.f, top = own;
+  const float* const tops = parts + (lane < a.splits ? lane : 0) * kRun + kAttnRows * DV;
+  float weight[kJoinRows], total[kJoinRows], acc[kJoinRows][kCols] = {};
+  int from[kJoinRows];  // rows that do not exist read the first
 #pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-  const float weight = own == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own - top);
-  total *= weight;
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) total += __shfl_xor(total, m);
-  float acc[kCols] = {};
-  for (int i0 = 0; i0 < a.splits; i0 += 8) {  // eight runs' loads at a time
-    float x[8][kCols];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int c = 0; c < kCols; ++c)
-        x[i][c] = parts[(i0 + i < a.splits ? i0 + i : i0) * kRun + row * DV + kCols * lane + c];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float w = __shfl(weight, i0 + i);
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) acc[c] = i0 + i < a.splits ? fmaf(w, x[i][c], acc[c]) : acc[c];
-    }
+  for (int r = 0; r < kJoinRows; ++r) {
+    from[r] = exists(row0 + r) ? row0 + r : row0;
+    weight[r] = lane < a.splits ? tops[from[r]] : -INFINITY;
+    total[r] = lane < a.splits ? tops[kAttnRows + from[r]] : 0.f;
   }
-  const float inv = total == 0.f ? 0.f : 1.0f / total;
-  uint16_t* const out = a.out + (q * a.heads + h) * a.d_v;
-  if constexpr (DV == 128) {
-    if (2 * lane < a.d_v)
-      *reinterpret_cast<uint32_t*>(out + 2 * lane) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
-  } else {
-    if (lane < a.d_v) out[lane] = static_cast<uint16_t>(pack2<BF16>(acc[0] * inv, 0.f));
+#pragma unroll
+  for (int r = 0; r < kJoinRows; ++r) {
+    const float top = over_wave(weight[r], [](float x, float y) { return fmaxf(x, y); });
+    weight[r] = weight[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(weight[r] - top);
+    total[r] = over_wave(total[r] * weight[r], [](float x, float y) { return x + y; });
+  }
+  for (int i0 = 0; i0 < a.splits; i0 += kRuns) {
+    float x[kJoinRows][kRuns][kCols];
+#pragma unroll
+    for (int r = 0; r < kJoinRows; ++r)
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          x[r][i][c] = parts[(i0 + i < a.splits ? i0 + i : i0) * kRun + from[r] * DV + kCols * lane + c];
+#pragma unroll
+    for (int r = 0; r < kJoinRows; ++r)
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i) {
+        const float w = __uint_as_float(
+            __builtin_amdgcn_readlane(__float_as_uint(weight[r]), (i0 + i) & (kWave - 1)));
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          acc[r][c] = i0 + i < a.splits ? fmaf(w, x[r][i][c], acc[r][c]) : acc[r][c];
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < kJoinRows; ++r) {
+    if (!exists(row0 + r)) return;
+    const int token = (row0 + r) * a.inv_pack >> 16;
+    const float inv = total[r] == 0.f ? 0.f : 1.0f / total[r];
+    uint16_t* const out =
+        a.out + ((q0 + token) * a.heads + head0 + row0 + r - token * a.pack) * a.d_v;
+    if constexpr (DV == 128) {
+      if (2 * lane < a.d_v)
+        *reinterpret_cast<uint32_t*>(out + 2 * lane) = pack2<BF16>(acc[r][0] * inv, acc[r][1] * inv);
+    } else {
+      if (lane < a.d_v) out[lane] = static_cast<uint16_t>(pack2<BF16>(acc[r][0] * inv, 0.f));
+    }
   }
 }
 
