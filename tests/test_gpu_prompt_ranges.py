@@ -252,3 +252,90 @@ def test_conv_and_attention_on_another_stream(rng):
     stream.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_no_tokens_and_no_keys(rng):
+    """Calls without a row: states are kept (or handed on), queries without keys get zeros."""
+    from local_kimi_amd.kernels import attention_prefill, kda_prefill, short_conv_prefill_triple
+
+    def made(*shape, dtype=torch.float32):
+        return _t(rng.normal(size=shape), dtype)
+
+    state, new = made(2, 3, 16, 8), torch.zeros((2, 3, 16, 8), device=DEV)
+    kept = state.clone()
+    none = [torch.zeros((2, 0, 3, w), device=DEV) for w in (16, 16, 8, 16)]
+    out = kda_prefill(state, *none, torch.zeros((2, 0, 3), device=DEV), scale=1.0, state_out=new)
+    assert out.shape == (2, 0, 3, 8) and torch.equal(state, kept) and torch.equal(new, kept)
+
+    states = [made(2, 24, 4, dtype=torch.float16) for _ in range(3)]
+    before = [s.clone() for s in states]
+    x = torch.zeros((2, 0, 24), device=DEV, dtype=torch.float16)
+    w = [made(24, 4, dtype=torch.float16) for _ in range(3)]
+    outs = short_conv_prefill_triple(x, x, x, *states, *w)
+    assert all(o.shape == x.shape for o in outs)
+    assert all(torch.equal(a, b) for a, b in zip(states, before))
+
+    q, kv = made(2, 5, 4, 64, dtype=torch.float16), torch.zeros((2, 0, 2, 64), device=DEV, dtype=torch.float16)
+    assert not attention_prefill(q, kv, kv).any()
+    assert attention_prefill(q[:, :0], kv, kv).shape == (2, 0, 4, 64)
+
+
+def test_graph_of_runs_and_windows_replays(rng):
+    """A prompt of several windows and a query in runs of the keys, captured
+    together; replayed on other values between eager work."""
+    from local_kimi_amd.kernels import attention_prefill, kda_prefill
+
+    a = [_t(x) for x in _scan_inputs(rng, 5000, 32, 128, 128, 1, rate=0.02)]
+    state, args = a[0], [x[None] for x in a[1:]]
+    q = _t(rng.normal(size=(1, 3, 8, 128)), torch.bfloat16)
+    k, v = (_t(rng.normal(size=(1, 4000, 2, 128)), torch.bfloat16) for _ in range(2))
+    start = state.clone()
+
+    def run():
+        return kda_prefill(state, *args, scale=0.1), attention_prefill(q, k, v)
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for i in range(3):
+        for t in (q, k, args[2]):
+            t.mul_(0.75)
+        state.copy_(start)
+        want = [t.clone() for t in run()] + [state.clone()]
+        for t in got:
+            t.zero_()
+        state.copy_(start)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip([*got, state], want):
+            assert torch.equal(x, y), i
+
+
+def test_two_calls_at_once(rng, form):
+    """Each of two streams has a workspace of its own."""
+    from local_kimi_amd.kernels import attention_prefill, kda_prefill
+
+    calls = []
+    for n in (700, 900):
+        a = [_t(x) for x in _scan_inputs(rng, n, 16, 64, 64, 1)]
+        q = _t(rng.normal(size=(1, 2, 8, 64)), torch.float16)
+        kv = _t(rng.normal(size=(1, 3000 + n, 4, 64)), torch.float16)
+        calls.append((a, q, kv))
+
+    def run(a, q, kv):
+        state = a[0].clone()
+        return kda_prefill(state, *(x[None] for x in a[1:]), scale=0.2), state, attention_prefill(q, kv, kv)
+
+    want = [run(*c) for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [None, None]
+    for _ in range(3):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i] = run(*calls[i])
+    torch.cuda.synchronize()
+    for x, y in zip(got, want):
+        assert all(torch.equal(s, t) for s, t in zip(x, y))
