@@ -420,6 +420,8 @@ struct ChunkLayout {  // float offsets of a record's parts; 32 NW channels, 2 NW
                        kU = kS + 2 * kChunk + 16;
 };
 
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 // Eight fp32 values as the sums of two fp16 each, hi + lo, of 2^k times them.
@@ -443,10 +445,13 @@ __device__ inline float finite_abs(float v) { return is_finite(v) ? fabsf(v) : 0
 __device__ inline Split split8(const float (&v)[8], float up) {
   Split s;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = v[i] * up;
-    s.hi[i] = static_cast<_Float16>(x);
-    s.lo[i] = static_cast<_Float16>(x - static_cast<float>(s.hi[i]));
+  for (int i = 0; i < 8; i += 2) {  // (two at a time: packed conversions)
+    const f32x2_t x = {v[i] * up, v[i + 1] * up};
+    const f16x2_t hi = __builtin_convertvector(x, f16x2_t);
+    s.hi[i] = hi[0];
+    s.hi[i + 1] = hi[1];
+    s.lo[i] = static_cast<_Float16>(fmaf(v[i], up, -static_cast<float>(hi[0])));
+    s.lo[i + 1] = static_cast<_Float16>(fmaf(v[i + 1], up, -static_cast<float>(hi[1])));
   }
   return s;
 }
