@@ -462,12 +462,12 @@ __device__ inline f32x4_t mfma_split(const Split& a, const Split& b, f32x4_t c) 
   c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, c, 0, 0, 0);
 }
-// the largest over the four lanes 16 apart
+// the largest over the four lanes 16 apart of values >= 0, whose bits order as they do
 __device__ inline float column_max(float v) {
   auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-  x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  const uint32_t m = x[0] > x[1] ? x[0] : x[1];
+  x = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  return __uint_as_float(x[0] > x[1] ? x[0] : x[1]);
 }
 
 // Sums of four values of each lane over the wave's four 16-lane rows: row g is left
@@ -801,7 +801,7 @@ chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
   using L = ChunkLayout<NW>;
   constexpr int kScanWaves = NW + 2 * CT;
   constexpr int kU0 = NW, kQS = NW + 1, kU = 2 * NW + 1;
-  // of the last two chunks and each half: the waves' W S, - U0, the waves' Q S, U;
+  // of the last two chunks and each half: the waves' W S, - U0, the waves' Q S, - U;
   // D; what the rows of W and the tiles of K are scaled by
   __shared__ f32x4_t parts[2][CT][2][2 * NW + 2][kWave];
   __shared__ f32x4_t decay[2][L::kTiles * 4], w_down[2][2][4];
@@ -900,12 +900,12 @@ chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
     auto begin = [&](int i, const f32x4_t& p, const f32x4_t& pba, const f32x4_t& q_down,
                      f32x4_t& u) {
       const f32x4_t(*const part)[kWave] = parts[i & 1][tile][half];
-      u = part[kU][lane];
+      u = -part[kU][lane];
       f32x4_t o = part[kQS][lane] + part[kQS + 1][lane];
       if constexpr (NW == 4) o += part[kQS + 2][lane] + part[kQS + 3][lane];
       o *= q_down;
       if (half) {
-        const f32x4_t ua = parts[i & 1][tile][0][kU][lane];
+        const f32x4_t ua = -parts[i & 1][tile][0][kU][lane];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           o = __builtin_amdgcn_mfma_f32_16x16x4f32(pba[r], ua[r], o, 0, 0, 0);
@@ -1064,7 +1064,7 @@ chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
       for (int b = 0; b < 2; ++b) {
         f32x4_t sum = xs[b][0] + xs[b][1];
         if constexpr (NW == 4) sum += xs[b][2] + xs[b][3];
-        u[x][b] = -(sum * down[b] + xs[b][kU0]);
+        u[x][b] = sum * down[b] + xs[b][kU0];  // - U
       }
       u_down[x] = split_column(u[x][0], u[x][1], us[x]);
     }
@@ -1073,13 +1073,19 @@ chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
       f32x4_t acc[CT];
 #pragma unroll
       for (int x = 0; x < CT; ++x) acc[x] = mfma_split(f.k[t], us[x], zero);
+#pragma unroll
+      for (int x = 0; x < CT; ++x) st[x][t] *= d[t];  // beside those products
       next.q[t] = {half_at(q_at + kHalfBytes * t), half_at(q_at + kHalfBytes * t + 1024)};
       next.k[t] = {half_at(k_at + 2048 * t), half_at(k_at + 2048 * t + 1024)};
 #pragma unroll
       for (int x = 0; x < CT; ++x) part[x][t][kQS + wave][lane] = y[x][t] * s_down[x];
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x < CT; ++x) st[x][t] = st[x][t] * d[t] + acc[x] * (kd[t] * u_down[x]);
+      for (int x = 0; x < CT; ++x) {
+        const float down_x = -(kd[t] * u_down[x]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[x][t][r] = fmaf(acc[x][r], down_x, st[x][t][r]);
+      }
     }
     advance();
     if (wave < 2)
