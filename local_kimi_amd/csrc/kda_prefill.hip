@@ -1012,17 +1012,22 @@ chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
     Split w[2], q[2], k[2];  // [half], [half], [tile]
   };
   // 2 KB a fragment; W and Q: half NW + wave, K: tile 2 wave + t
-  const uint32_t w_at = static_cast<uint32_t>((L::kW + 512 * wave + 4 * lane) * 4);
-  const uint32_t q_at = w_at + L::kQ * 4;
-  const uint32_t k_at = static_cast<uint32_t>((L::kK + 1024 * wave + 4 * lane) * 4);
-  constexpr uint32_t kHalfBytes = 2048 * NW;
-  auto half_at = [&](uint32_t off) { return *reinterpret_cast<const f16x8_t*>(ahead + off); };
+  const int w_at = (512 * wave + 4 * lane) * 4, k_at = (1024 * wave + 4 * lane) * 4;
+  constexpr int kHalfBytes = 2048 * NW;
+  auto split_at = [&](int at, int part) {  // (buffer loads: no 64-bit address for each)
+    const auto rec = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(ahead), 0, 0x7FFFFFFF, 0x00020000);
+    return Split{__builtin_bit_cast(f16x8_t, __builtin_amdgcn_raw_buffer_load_b128(rec, at, part, 0)),
+                 __builtin_bit_cast(f16x8_t, __builtin_amdgcn_raw_buffer_load_b128(rec, at + 1024, part, 0))};
+  };
+  auto w_of = [&](int b) { return split_at(w_at, L::kW * 4 + kHalfBytes * b); };
+  auto q_of = [&](int b) { return split_at(w_at, L::kQ * 4 + kHalfBytes * b); };
+  auto k_of = [&](int t) { return split_at(k_at + 2048 * t, L::kK * 4); };
   auto fetch = [&](Record& f) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      f.w[x] = {half_at(w_at + kHalfBytes * x), half_at(w_at + kHalfBytes * x + 1024)};
-      f.q[x] = {half_at(q_at + kHalfBytes * x), half_at(q_at + kHalfBytes * x + 1024)};
-      f.k[x] = {half_at(k_at + 2048 * x), half_at(k_at + 2048 * x + 1024)};
+      f.w[x] = w_of(x);
+      f.q[x] = q_of(x);
+      f.k[x] = k_of(x);
     }
     advance();
   };
@@ -1057,7 +1062,7 @@ chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         y[x][b] = mfma_split(f.q[b], ss[x], zero);
-        if (x == 0) next.w[b] = {half_at(w_at + kHalfBytes * b), half_at(w_at + kHalfBytes * b + 1024)};
+        if (x == 0) next.w[b] = w_of(b);
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
@@ -1075,8 +1080,8 @@ chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
       for (int x = 0; x < CT; ++x) acc[x] = mfma_split(f.k[t], us[x], zero);
 #pragma unroll
       for (int x = 0; x < CT; ++x) st[x][t] *= d[t];  // beside those products
-      next.q[t] = {half_at(q_at + kHalfBytes * t), half_at(q_at + kHalfBytes * t + 1024)};
-      next.k[t] = {half_at(k_at + 2048 * t), half_at(k_at + 2048 * t + 1024)};
+      next.q[t] = q_of(t);
+      next.k[t] = k_of(t);
 #pragma unroll
       for (int x = 0; x < CT; ++x) part[x][t][kQS + wave][lane] = y[x][t] * s_down[x];
       __builtin_amdgcn_sched_barrier(0);
