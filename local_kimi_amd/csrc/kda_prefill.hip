@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(ScanArgs a,
 //   (q D)_b <- (q D)_b D_a,  (beta k D)_a <- (beta k D)_a D_b.
 // The scan is bound by the way from one chunk's state to the next (products, a
 // barrier, an exchange through LDS, 1.2 us), hence not 16 steps a chunk: 8192 tokens
-// x 32 heads took 707 us in chunks of 16, 605 in chunks of 32.
+// x 32 heads took 707 us in chunks of 16, 605 in chunks of 32 (of then).
 //
 // Records. A chunk and head has one record in the workspace, its parts in the
 // order in which the second launch's lanes load them (16 bytes a lane, 1 KB a
@@ -496,10 +496,11 @@ __device__ inline int after(int at, float x) {
 
 __device__ inline f32x4_t lds4(const float* p) { return *reinterpret_cast<const f32x4_t*>(p); }
 
-// Block = one chunk and head. LDS reads fill 65% of the time and VALU 54%, of which
-// A and P are most; 3840 records of 32 steps x 128 x 128 take 148 us, 370 MB read
-// and written. Two blocks share a CU (80 KB of LDS each) and cover each other's
-// loads and barriers.
+// Block = one chunk and head; two share a CU (80 KB of LDS each) and cover each
+// other's loads and barriers. 3840 records of 32 steps x 128 x 128 take 141 us, 370 MB
+// read and written. No one thing bounds it: of 164 us (traced) 30 went without A and
+// P, 27 with a third of the stores, none without the solve, and none with the next
+// chunk's loads under way or with half the LDS reads of A and P.
 template <int DT, int NW>
 __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanArgs a, ChunkArgs c) {
   using T = typename Storage<DT>::type;
@@ -1187,8 +1188,8 @@ int64_t chunk_record(int64_t d_k, int64_t d_v) {
 
 // From this many 16-column tiles of a call on (twice as many as keep two blocks on
 // each CU), a block takes two: half the blocks load the same records. 4096 tokens
-// of 11 sequences x 32 heads x 8 tiles: 361 us with one, 335 with two; a single
-// prompt's 256 tiles, which fill the CUs once: 587 with one, 705 with two.
+// of 11 sequences x 32 heads x 8 tiles: 350 us with one, 316 with two; a single
+// prompt's 256 tiles (8192 tokens), which fill the CUs once: 570 and 655.
 constexpr int64_t kTwoTiles = 1024;
 
 // Chunks of one window: the records of a window are written by one launch and
@@ -1211,8 +1212,8 @@ bool takes_chunks(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k,
   const int choice = path_choice(kKnobKdaPrefill);
   // (a chunk's outputs are stored at 31-bit byte offsets.) Chunks from 48 tokens a
   // sequence on: 32 heads of 128 x 128 took, in steps / in chunks, for one sequence of
-  // 32 tokens 15 / 18 us, of 48 19 / 19, of 128 48 / 22, for 32 sequences of 32 tokens
-  // 150 / 172, of 64 269 / 241.
+  // 32 tokens 15 / 18 us, of 48 20 / 19, of 128 48 / 22, for 32 sequences of 32 tokens
+  // 149 / 127; 16 heads of 64 x 64 for 16 sequences of 32 tokens 19 / 23.
   if (d_k > 128 || tokens == 0 || choice == 1 || heads * d_v >= (int64_t{1} << 24)) return false;
   return choice == 2 || tokens >= 48 * sequences;
 }
