@@ -95,7 +95,7 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
         raise ValueError("scale must be finite")
     if q.device.type != "cuda":
         raise ValueError("the HIP attention kernel requires CUDA tensors")
-    out = torch.empty((batch, rows, heads, d_v), dtype=q.dtype, device=q.device)
+    out = q.new_empty((batch, rows, heads, d_v))
     if rows == 0:
         return out
     qc, kc, vc = _rows(q), _rows(k), _rows(v)

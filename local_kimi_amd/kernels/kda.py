@@ -392,21 +392,19 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 
 def _disjoint(*tensors: torch.Tensor) -> bool:
-    """Whether the dense ones among nonempty tensors share no byte (the others
-    are worked on through copies)."""
-    spans = sorted([(t.data_ptr(), t.nbytes) for t in tensors if t.is_contiguous()])
-    end = 0
-    for lo, size in spans:
-        if lo < end:
-            return False
-        end = lo + size
-    return True
+    """Whether the dense ones among nonempty tensors of one shape and dtype share
+    no byte (the others are worked on through copies)."""
+    size = tensors[0].nbytes
+    starts = sorted([t.data_ptr() for t in tensors if t.is_contiguous()])
+    return all([hi - lo >= size for lo, hi in zip(starts, starts[1:])])
 
 
 def _packed_rows(tensors) -> tuple[list[torch.Tensor], int]:
     """[B, S, C] tensors as rows one stride apart (the same for all of them):
     views of one projection's rows as they are, other layouts copied."""
     batch, rows, width = tensors[0].shape
+    if all([t.is_contiguous() for t in tensors]):
+        return list(tensors), width
     stride = tensors[0].stride(1)
     if rows < 2 or stride < width:
         return [_aligned(t) for t in tensors], width
@@ -493,7 +491,8 @@ def short_conv_prefill_triple(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torc
     else:
         work = [o if o.is_contiguous() and o.data_ptr() % 16 == 0 else
                 torch.empty(o.shape, dtype=o.dtype, device=dev) for o in targets]
-    outs = [torch.empty((batch, rows, channels), dtype=dtype, device=dev) for _ in range(3)]
+    first = torch.empty_like(q_in, memory_format=torch.contiguous_format)
+    outs = [first, torch.empty_like(first), torch.empty_like(first)]
     with _w._on(dev):
         _lib.call("lk_kda_short_conv_prefill",
                   *[t.data_ptr() for t in (*ins, *src, *work, *weights, *outs)],
@@ -567,7 +566,7 @@ def kda_prefill(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.
         work = target
     else:
         work = torch.empty(target.shape, dtype=torch.float32, device=q.device)
-    out = torch.empty(v.shape, dtype=v.dtype, device=q.device)
+    out = torch.empty_like(vc)
     need = _lib.query("lk_kda_prefill_workspace", count, batch * rows, heads, d_k, d_v)
     ws = _w.workspace(need, q.device) if need else None
     with _w._on(q.device):
