@@ -326,11 +326,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
                                                           __float_as_uint(most), false, false);
           most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.scale_log2;
         }
-        // the maximum only moves when it has grown by more than 2^kSlack: p stays
-        // below that, and most passes leave the accumulators alone
+        // a query's maximum only moves when it has grown by more than 2^kSlack: p
+        // stays below that, and most passes leave the accumulators alone. Each query
+        // decides for itself, though the wave branches together: the others' keys
+        // may be ones that it does not see.
         constexpr float kSlack = 8.f;
-        if (__any(most > top + kSlack || (top == -INFINITY && most > top))) {
-          const float next = fmaxf(top, most);
+        const bool moves = most > top + kSlack || (top == -INFINITY && most > top);
+        if (__any(moves)) {
+          const float next = moves ? most : top;
           const float fade = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
           top = next;
           sum *= fade;

@@ -1,0 +1,85 @@
+"""What the prompt operators promise beyond their sums: a query's result does not
+depend on what it does not see, finite inputs whose result the type holds give finite
+results, states that are only read may be shared, and calls that mix one prompt with
+many short sequences.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kda as K
+
+from .test_gpu_attention import _check, _inputs
+from .test_gpu_kda_prefill import (DEV, _close, _conv_check, _conv_inputs, _cu, _np, _require_gpu,
+                                   _run_scan, _scan_inputs, _t, form)
+
+pytestmark = pytest.mark.gpu
+
+_ = _require_gpu, form  # fixtures
+
+
+# ---------------------------------------------------------------------------
+# attention
+
+
+@pytest.mark.parametrize("h,hk,d,lk", [(2, 2, 128, 150), (4, 1, 64, 150), (2, 1, 192, 1500)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_later_finite_keys_change_nothing(h, hk, d, lk, dtype):
+    """A key of ordinary values that only the later queries of a wave see, large
+    enough to be their maximum by far: the earlier queries' results stay as they
+    are, bit for bit (their sums have the same terms in the same order), over many
+    draws."""
+    from local_kimi_amd.kernels import attention_prefill
+
+    lq = 150
+    for seed in range(20):
+        a = [_t(x[None], dtype) for x in _inputs(np.random.default_rng(seed), lq, lk, h, hk, d, 64, dtype)]
+        clean = attention_prefill(*a, scale=0.2)
+        for back in (1, 17, 70, 118):  # seen by the last `back` queries
+            k = a[1].clone()
+            k[:, lk - back] = 8 * a[0][:, lq - 1, ::h // hk, :]
+            got = attention_prefill(a[0], k, a[2], scale=0.2)
+            assert not torch.equal(got[:, lq - back:], clean[:, lq - back:])
+            assert torch.equal(got[:, :lq - back], clean[:, :lq - back]), (seed, back)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_another_heads_queries_change_nothing(dtype):
+    """Heads of one key head share a block's rows: a head's result does not
+    depend on the other heads' queries."""
+    from local_kimi_amd.kernels import attention_prefill
+
+    for seed in range(20):
+        a = [_t(x[None], dtype) for x in _inputs(np.random.default_rng(seed), 20, 400, 8, 2, 64, 64, dtype)]
+        clean = attention_prefill(*a, scale=0.2)
+        q = a[0].clone()
+        q[:, :, 1::4] *= 8
+        got = attention_prefill(q, *a[1:], scale=0.2)
+        for head in (0, 2, 3, 4, 6, 7):
+            assert torch.equal(got[:, :, head], clean[:, :, head]), (seed, head)
+
+
+@pytest.mark.parametrize("cu_k", [False, True])
+def test_attention_of_one_prompt_among_short_ones(rng, cu_k):
+    from local_kimi_amd.kernels import attention_prefill
+
+    lengths = [1] * 9 + [700] + [1, 0, 2] * 5
+    keys = [n + (5 if n == 1 else 900 if n == 700 else 0) for n in lengths] if cu_k else lengths
+    dtype = torch.bfloat16
+    a = _inputs(rng, sum(lengths), sum(keys), 4, 2, 64, 64, dtype)
+    offsets = {"cu_seqlens": _t(_cu(lengths), torch.int32)}
+    if cu_k:
+        offsets["cu_seqlens_k"] = _t(_cu(keys), torch.int32)
+    got = attention_prefill(*(_t(x[None], dtype) for x in a), **offsets)
+    _check(got, a, 0.125, dtype, len(lengths), _cu(lengths), _cu(keys), "mixed")
+
+
+# ---------------------------------------------------------------------------
+# recurrence
+
+
+# ---------------------------------------------------------------------------
+# states
