@@ -55,6 +55,15 @@ __device__ inline uint32_t pack2(float a, float b) {
   }
 }
 
+// A finite mean of V's values, within the type: p is rounded before its product and
+// not in the sum that divides it, so that a mean of 65504 can come out as much as
+// 2^-11 above it, where fp16 has infinity from 2^-12 on. (bf16 ends where fp32 does.)
+template <bool BF16>
+__device__ inline float within_type(float x) {
+  if constexpr (BF16) return x;
+  else return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
+}
+
 // Whether any of the eight values is an infinity or a NaN (exponent all ones:
 // one more carries into the sign's place).
 template <bool BF16>
@@ -420,8 +429,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
 #pragma unroll
     for (int r = 0; r < 16; r += 4)
       *reinterpret_cast<uint2*>(rows + n * kOutStride + 32 * t + 8 * (r / 4) + 4 * half) =
-          make_uint2(pack2<BF16>(o[t][r] * inv, o[t][r + 1] * inv),
-                     pack2<BF16>(o[t][r + 2] * inv, o[t][r + 3] * inv));
+          make_uint2(pack2<BF16>(within_type<BF16>(o[t][r] * inv), within_type<BF16>(o[t][r + 1] * inv)),
+                     pack2<BF16>(within_type<BF16>(o[t][r + 2] * inv),
+                                 within_type<BF16>(o[t][r + 3] * inv)));
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 32 * kVChunks / kWave; ++i) {
@@ -513,9 +523,11 @@ __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttnArgs a
         a.out + ((q0 + token) * a.heads + head0 + row0 + r - token * a.pack) * a.d_v;
     if constexpr (DV == 128) {
       if (2 * lane < a.d_v)
-        *reinterpret_cast<uint32_t*>(out + 2 * lane) = pack2<BF16>(acc[r][0] * inv, acc[r][1] * inv);
+        *reinterpret_cast<uint32_t*>(out + 2 * lane) =
+            pack2<BF16>(within_type<BF16>(acc[r][0] * inv), within_type<BF16>(acc[r][1] * inv));
     } else {
-      if (lane < a.d_v) out[lane] = static_cast<uint16_t>(pack2<BF16>(acc[r][0] * inv, 0.f));
+      if (lane < a.d_v)
+        out[lane] = static_cast<uint16_t>(pack2<BF16>(within_type<BF16>(acc[r][0] * inv), 0.f));
     }
   }
 }

@@ -62,6 +62,46 @@ def test_another_heads_queries_change_nothing(dtype):
             assert torch.equal(got[:, :, head], clean[:, :, head]), (seed, head)
 
 
+@pytest.mark.parametrize("keys", [41, 2001])
+def test_largest_fp16_values_under_weights_that_round_up(keys):
+    """One key of weight 1 and the others just above 1/2, which fp16 rounds up by
+    0.9 * 2^-12 each: of forty, 40 * 0.9 * 2^-12 / 21 = 1.7 steps of 2^-12 in their mean,
+    where 65504 has one to the next exponent (65520 rounds to infinity). The mean of
+    equal values at the type's end is that value; an infinity among them stays one."""
+    from local_kimi_amd.kernels import attention_prefill
+
+    q = torch.zeros((1, 41, 1, 64), device=DEV, dtype=torch.float16)
+    q[..., 0] = 1
+    k = torch.zeros((1, keys, 1, 64), device=DEV, dtype=torch.float16)
+    k[:, 1:, :, 0] = -1
+    v = torch.full_like(k, 65504.0)
+    v[..., 1::2] = -65504.0
+    scale = -float(np.log(0.5 + 1.1 * 2.0 ** -12))
+    assert torch.equal(attention_prefill(q, k, v, scale=scale), v[:, :41])
+    v[:, 0, :, 3] = float("inf")
+    got = attention_prefill(q, k, v, scale=scale)
+    assert bool((got[..., 3] == float("inf")).all()) and torch.equal(got[..., 4:], v[:, :41, :, 4:])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_many_weights_far_below_the_largest(rng, dtype):
+    """4000 keys whose p is 2^-21 or so of the largest one's, below fp16's normal
+    range as it is stored: they count, in the sum of the weights as in that of
+    the values."""
+    from local_kimi_amd.kernels import attention_prefill
+
+    a = _inputs(rng, 1, 4001, 1, 1, 64, 64, dtype)
+    a[0][:] = 0.0
+    a[0][..., 0] = 1.0
+    a[1][:] = 0.0
+    a[1][1:, :, 0] = -8.0
+    a[2] = np.abs(a[2])
+    a[2][0] = 0.0
+    scale = 20.6 * float(np.log(2.0)) / 8.0
+    got = attention_prefill(*(_t(x[None], dtype) for x in a), scale=scale)
+    _check(got, a, scale, dtype, what="far below")
+
+
 @pytest.mark.parametrize("cu_k", [False, True])
 def test_attention_of_one_prompt_among_short_ones(rng, cu_k):
     from local_kimi_amd.kernels import attention_prefill
