@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kSerialThreads) scan_serial_kernel(ScanArgs a,
 //                        (i = 0..7, c(i) = 16 (i / 4) + 4 g + i % 4)
 //   D (D_31):            [channel]
 //   P:                   [aa, ba, bb][lane][r] = row m, column 4 g + r of that block
-//   the inverse scales of W's rows, Q's rows and K's tiles
+//   the inverse scales of W's rows, Q's rows (both by kRowsUp) and K's tiles
 //   U0:                  [h][tile t][lane][r] = value column 16 t + m, step 16 h + 4 g + r
 // These are A operands for B operands that are the accumulators of an earlier
 // product as they stand: lane (m, g) of a 16 x 16 result holds column m, rows 4 g + r,
@@ -428,12 +428,16 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 struct Split {
   f16x8_t hi, lo;
 };
-// 2^k that brings the largest magnitude to [2^14, 2^15), as fp32 (at most 2^127),
+// 2^k that brings the largest magnitude to [2^14, 2^15), as fp32 (at most 2^126),
 // and its inverse. A value down to 2^-16 of the largest keeps 22 bits, a smaller one
 // 2^-39 of the largest.
 struct Scale {
   float up, down;
 };
+// Of the products with W and Q, what takes the state's scale back takes the rows' 2^14
+// back as well, and the rows' inverse scales are kept 2^14 times as large: between the
+// two the sums are at most 64 times the state's largest value, not 2^21 times.
+constexpr float kRowsDown = 0x1p-14f, kRowsUp = 0x1p14f;
 __device__ inline Scale scale_for(float largest) {
   const uint32_t e = __float_as_uint(largest) & 0x7F800000u;
   const uint32_t up = e < (15u << 23) ? 253u << 23 : (268u << 23) - e;
@@ -750,8 +754,8 @@ __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanA
     put_split(L::kW + 512 * (b * NW + p), split8(wv, w.up));
     put_split(L::kQ + 512 * (b * NW + p), split8(qv, q.up));
     if (p == 0 && g == 0) {
-      rec[L::kS + kHalf * b + l] = w.down;
-      rec[L::kS + kChunk + kHalf * b + l] = q.down;
+      rec[L::kS + kHalf * b + l] = w.down * kRowsUp;
+      rec[L::kS + kChunk + kHalf * b + l] = q.down * kRowsUp;
     }
   }
   for (int first = 0;;) {
@@ -1008,7 +1012,7 @@ chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
   Split ss[CT];
   float s_down[CT];
 #pragma unroll
-  for (int x = 0; x < CT; ++x) s_down[x] = split_column(st[x][0], st[x][1], ss[x]);
+  for (int x = 0; x < CT; ++x) s_down[x] = kRowsDown * split_column(st[x][0], st[x][1], ss[x]);
   struct Record {
     Split w[2], q[2], k[2];  // [half], [half], [tile]
   };
@@ -1098,7 +1102,7 @@ chunk_scan_kernel(ScanArgs a, ChunkArgs c) {
 #pragma unroll
       for (int x = 0; x < CT; ++x) part[x][wave][kU][lane] = wave == 0 ? u[x][0] : u[x][1];
 #pragma unroll
-    for (int x = 0; x < CT; ++x) s_down[x] = split_column(st[x][0], st[x][1], ss[x]);
+    for (int x = 0; x < CT; ++x) s_down[x] = kRowsDown * split_column(st[x][0], st[x][1], ss[x]);
   };
   if (steps > 0) {
     Record f0, f1, f2;  // in turn

@@ -121,5 +121,34 @@ def test_attention_of_one_prompt_among_short_ones(rng, cu_k):
 # recurrence
 
 
+@pytest.mark.parametrize("size", [1e-30, 1e30, 1e34, 1e36])
+def test_states_of_any_size_that_fp32_holds(rng, form, size):
+    """The sums of a step are of a state's size, so a state up to a hundredth of
+    fp32's range goes through."""
+    cu = _cu([150, 40])
+    a = _scan_inputs(rng, 190, 2, 128, 64, 2)
+    a[0] *= np.float32(size)
+    a[3] *= np.float32(size)
+    want_state, want = K.prefill(*a, 0.1, cu)
+    out, st = _run_scan(a, cu, torch.float32, 0.1)
+    _close(out, want, 150, torch.float32, f"out {size}")
+    _close(st, want_state, 150, torch.float32, f"state {size}")
+
+
+@pytest.mark.parametrize("which", [1, 2])  # q, k
+@pytest.mark.parametrize("size", [1e-25, 1e-12, 30.0])
+def test_queries_and_keys_of_other_sizes(rng, form, which, size):
+    """(Keys above 1 with beta <= 1 / |k|^2, where a step does not enlarge.)"""
+    cu = _cu([100, 40])
+    a = _scan_inputs(rng, 140, 2, 64, 48, 2)
+    a[which] *= np.float32(size)
+    if which == 2 and size > 1:
+        a[5] /= np.float32(size * size)
+    want_state, want = K.prefill(*a, 0.1, cu)
+    out, st = _run_scan(a, cu, torch.float32, 0.1)
+    _close(out, want, 100, torch.float32, f"out {size}")
+    _close(st, want_state, 100, torch.float32, f"state {size}")
+
+
 # ---------------------------------------------------------------------------
 # states
