@@ -391,12 +391,17 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _disjoint(*tensors: torch.Tensor) -> bool:
-    """Whether the dense ones among nonempty tensors of one shape and dtype share
-    no byte (the others are worked on through copies)."""
-    size = tensors[0].nbytes
-    starts = sorted([t.data_ptr() for t in tensors if t.is_contiguous()])
-    return all([hi - lo >= size for lo, hi in zip(starts, starts[1:])])
+def _disjoint(written, read=()) -> bool:
+    """Whether no written tensor shares a byte with another one, written or read: of
+    nonempty tensors of one shape and dtype, the dense ones (the others are
+    worked on through copies). What is only read may be one tensor."""
+    size = written[0].nbytes
+    to = [t.data_ptr() for t in written if t.is_contiguous()]
+    others = [t.data_ptr() for t in read if t.is_contiguous()]
+    starts = sorted(to + others)
+    if all([hi - lo >= size for lo, hi in zip(starts, starts[1:])]):
+        return True
+    return all(abs(a - b) >= size for i, a in enumerate(to) for b in to[i + 1:] + others)
 
 
 def _packed_rows(tensors) -> tuple[list[torch.Tensor], int]:
@@ -434,8 +439,8 @@ def short_conv_prefill_triple(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torc
     stays). A fresh prompt's state is zeros.
 
     Returns the outputs in the input dtype; the states are updated in place,
-    or with ``conv_states_out`` left as they are and the new ones written
-    there. Equal row strides (views of one fused projection) are read in
+    or with ``conv_states_out`` left as they are (they may then be one tensor)
+    and the new ones written there. Equal row strides (views of one fused projection) are read in
     place.
     """
     values, states = (q_in, k_in, v_in), (q_state, k_state, v_state)
@@ -476,9 +481,9 @@ def short_conv_prefill_triple(q_in: torch.Tensor, k_in: torch.Tensor, v_in: torc
             if t.shape != shape or t.dtype != dtype or t.device != dev:
                 raise ValueError("each conv_states_out tensor must match its state's shape, dtype "
                                  "and device")
-        if not _disjoint(*states, *targets):
-            raise ValueError("the convolution states and conv_states_out must not overlap")
-    elif not _disjoint(*states):
+        if not _disjoint(targets, states):
+            raise ValueError("conv_states_out must not overlap the states or each other")
+    elif not _disjoint(states):
         raise ValueError("the three convolution states must not overlap")
     wcode = _DTYPE_CODES.get(q_weight.dtype)
     if wcode is None or k_weight.dtype != q_weight.dtype or v_weight.dtype != q_weight.dtype:
@@ -551,7 +556,7 @@ def kda_prefill(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.
         if state_out.shape != state.shape or state_out.dtype != state.dtype \
                 or state_out.device != state.device:
             raise ValueError("state_out must match the state's shape, dtype and device")
-        if not _disjoint(state_out, state):
+        if not _disjoint([state_out], [state]):
             raise ValueError("state_out overlaps the state it is computed from")
     if q.device.type != "cuda":
         raise ValueError("KDA prefill requires CUDA inputs")

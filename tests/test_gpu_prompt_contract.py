@@ -152,3 +152,27 @@ def test_queries_and_keys_of_other_sizes(rng, form, which, size):
 
 # ---------------------------------------------------------------------------
 # states
+
+
+def _conv_call(x, states, w, **kw):
+    from local_kimi_amd.kernels import short_conv_prefill_triple
+
+    return short_conv_prefill_triple(*x, *states, *w, **kw)
+
+
+def test_one_fresh_state_for_the_three_convolutions(rng):
+    """States that are only read may be one tensor (and one row for all
+    sequences)."""
+    n, s, c = 2, 21, 32
+    x, st, w = _conv_inputs(rng, n * s, n, c, torch.bfloat16)
+    xs = [_t(a.reshape(n, s, c), torch.bfloat16) for a in x]
+    ws = [_t(a, torch.bfloat16) for a in w]
+    zero = torch.zeros((n, c, 4), device=DEV, dtype=torch.bfloat16)
+    for state in (zero, zero[:1].expand(n, c, 4)):
+        new = [torch.empty_like(zero) for _ in range(3)]
+        outs = _conv_call(xs, [state] * 3, ws, conv_states_out=tuple(new))
+        assert not state.any()
+        for i in range(3):
+            none = np.zeros_like(st[i])
+            _conv_check(outs[i].reshape(n * s, c), x[i], none, w[i], torch.bfloat16, None, f"conv {i}")
+            assert np.array_equal(_np(new[i]), K.short_conv_prefill(x[i], none, w[i], "float32")[1])
