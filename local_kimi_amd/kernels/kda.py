@@ -391,17 +391,46 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _disjoint(written, read=()) -> bool:
-    """Whether no written tensor shares a byte with another one, written or read: of
-    nonempty tensors of one shape and dtype, the dense ones (the others are
-    worked on through copies). What is only read may be one tensor."""
-    size = written[0].nbytes
-    to = [t.data_ptr() for t in written if t.is_contiguous()]
-    others = [t.data_ptr() for t in read if t.is_contiguous()]
-    starts = sorted(to + others)
-    if all([hi - lo >= size for lo, hi in zip(starts, starts[1:])]):
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two nonempty tensors of one shape and dtype share a byte. Exact for
+    equal strides; other views count as sharing where the bytes they span meet."""
+    size = a.element_size()
+
+    def steps(t):
+        return sorted([(s * size, n) for s, n in zip(t.stride(), t.shape) if n > 1], reverse=True)
+
+    def span(dims):
+        return sum(s * (n - 1) for s, n in dims) + size
+
+    gap = b.data_ptr() - a.data_ptr()
+    if gap >= span(steps(a)) or -gap >= span(steps(b)):
+        return False
+    if steps(a) != steps(b):
         return True
-    return all(abs(a - b) >= size for i, a in enumerate(to) for b in to[i + 1:] + others)
+
+    def meets(gap, dims):  # an element of each, `gap` bytes apart over these dimensions
+        if not dims:
+            return abs(gap) < size
+        (step, n), rest = dims[0], dims[1:]
+        if step == 0:
+            return meets(gap, rest)
+        reach = span(rest) - 1
+        first, last = -((reach - gap) // step), (gap + reach) // step
+        return any(meets(gap - d * step, rest) for d in range(max(first, 1 - n), min(last, n - 1) + 1))
+
+    return meets(gap, steps(a))
+
+
+def _disjoint(written, read=()) -> bool:
+    """Whether no written tensor shares a byte with another one, written or read, of
+    nonempty tensors of one shape and dtype. What is only read may be one tensor."""
+    tensors = (*written, *read)
+    if all([t.is_contiguous() for t in tensors]):
+        size = written[0].nbytes
+        starts = sorted([t.data_ptr() for t in tensors])
+        if all([hi - lo >= size for lo, hi in zip(starts, starts[1:])]):
+            return True
+    return not any(_share(a, b) for i, a in enumerate(written) for b in tensors[i + 1:])
 
 
 def _packed_rows(tensors) -> tuple[list[torch.Tensor], int]:

@@ -176,3 +176,45 @@ def test_one_fresh_state_for_the_three_convolutions(rng):
             none = np.zeros_like(st[i])
             _conv_check(outs[i].reshape(n * s, c), x[i], none, w[i], torch.bfloat16, None, f"conv {i}")
             assert np.array_equal(_np(new[i]), K.short_conv_prefill(x[i], none, w[i], "float32")[1])
+
+
+def test_states_that_share_memory_are_refused(rng):
+    """A written state that shares a byte with another one, dense or strided."""
+    from local_kimi_amd.kernels import kda_prefill
+
+    n, s, c = 2, 5, 32
+    x, _, w = _conv_inputs(rng, n * s, n, c, torch.bfloat16)
+    xs = [_t(a.reshape(n, s, c), torch.bfloat16) for a in x]
+    ws = [_t(a, torch.bfloat16) for a in w]
+    wide = torch.zeros((n, 4 * c, 8), device=DEV, dtype=torch.bfloat16)
+    one = wide[:, :c, ::2]
+    dense = [torch.zeros((n, c, 4), device=DEV, dtype=torch.bfloat16) for _ in range(3)]
+    for states, out in (([one] * 3, None), ([dense[0], one, one], None),
+                        ([wide[:, i:c + i, ::2] for i in range(3)], None),
+                        ([one, *dense[1:]], (one, *dense[1:])), (dense, (one, one, wide[:, c:2 * c, ::2])),
+                        (dense, (dense[0], one, wide[:, c:2 * c, ::2])), ([dense[0]] * 3, None)):
+        with pytest.raises(ValueError, match="overlap"):
+            _conv_call(xs, states, ws, conv_states_out=out)
+    state = torch.zeros((n, 2, 16, 16), device=DEV)[..., ::2]
+    args = [torch.zeros((n, s, 2, width), device=DEV) for width in (16, 16, 8, 16)]
+    with pytest.raises(ValueError, match="overlap"):
+        kda_prefill(state, *args, torch.zeros((n, s, 2), device=DEV), scale=1.0, state_out=state)
+
+
+def test_states_beside_each_other_in_one_buffer(rng):
+    """Interleaved and neighbouring views of one buffer share no byte."""
+    n, s, c = 3, 9, 24
+    x, st, w = _conv_inputs(rng, n * s, n, c, torch.bfloat16)
+    xs = [_t(a.reshape(n, s, c), torch.bfloat16) for a in x]
+    ws = [_t(a, torch.bfloat16) for a in w]
+    for views in (lambda b: [b[:, i * c:(i + 1) * c, :4] for i in range(3)],
+                  lambda b: [b[:, i:3 * c:3, :4] for i in range(3)],
+                  lambda b: [b[:, :c, ::2], b[:, :c, 1::2], b[:, c:2 * c, ::2]]):
+        buffer = torch.zeros((n, 3 * c, 8), device=DEV, dtype=torch.bfloat16)
+        states = views(buffer)
+        for t, a in zip(states, st):
+            t.copy_(_t(a, torch.bfloat16))
+        _conv_call(xs, states, ws)
+        for i in range(3):
+            want = K.short_conv_prefill(x[i], st[i], w[i], "float32")[1]
+            assert np.array_equal(_np(states[i]), want)
