@@ -565,7 +565,8 @@ int attention_splits(int64_t rows_q, int64_t rows_k, int64_t sequences, int64_t 
 template <bool BF16>
 int launch_attention(const AttnArgs& a, hipStream_t s) {
   const int64_t items = a.tiles * a.packs, blocks = items * a.splits;
-  LK_REQUIRE(blocks < (int64_t{1} << 31) && items * kJoinBlocks < (int64_t{1} << 31),
+  LK_REQUIRE(grid_fits(blocks, kAttnThreads) &&
+                 (!a.partial || grid_fits(items * kJoinBlocks, kAttnThreads)),
              "too many query rows and heads for one call");
   const dim3 grid(static_cast<unsigned>(blocks)), join(static_cast<unsigned>(items * kJoinBlocks));
 #define LK_ATTENTION(Q, V)                                          \

@@ -1151,7 +1151,7 @@ int launch_conv(const ConvArgs& a, bool wide, hipStream_t s) {
   const int64_t items = 3 * (a.channels / (wide ? kWide : 1));
   const int64_t blocks = (items + kConvThreads - 1) / kConvThreads;
   const int64_t tiles = sequence_tiles(a.seq.rows, a.seq.count, kConvTile);
-  LK_REQUIRE(blocks * tiles < (int64_t{1} << 31), "too many tokens and channels for one call");
+  LK_REQUIRE(grid_fits(blocks * tiles, kConvThreads), "too many tokens and channels for one call");
   b.column_blocks = static_cast<int>(blocks);
   const dim3 grid(static_cast<unsigned>(blocks * tiles));
   if (wide)
@@ -1172,7 +1172,7 @@ template <int DT>
 int launch_serial(const ScanArgs& a, hipStream_t s) {
   const int64_t col_blocks = (a.d_v + kSerialCols - 1) / kSerialCols;
   const int64_t blocks = (a.seq.count + 1) * static_cast<int64_t>(a.heads) * col_blocks;
-  LK_REQUIRE(blocks < (int64_t{1} << 31), "too many sequences x heads for one call");
+  LK_REQUIRE(grid_fits(blocks, kSerialThreads), "too many sequences x heads for one call");
   const dim3 grid(static_cast<unsigned>(blocks));
   const int cb = static_cast<int>(col_blocks);
   if (a.d_k <= 64)
@@ -1233,7 +1233,8 @@ int launch_chunks(const ScanArgs& a, float* records, hipStream_t s) {
   const int64_t pairs = (a.seq.count + 1) * static_cast<int64_t>(a.heads);
   const bool two = c.v_tiles > 1 && a.seq.count * static_cast<int64_t>(a.heads) * c.v_tiles >= kTwoTiles;
   const int64_t scans = (pairs + 7) / 8 * 8 * (two ? (c.v_tiles + 1) / 2 : c.v_tiles);
-  LK_REQUIRE(window * a.heads < (int64_t{1} << 31) && scans < (int64_t{1} << 31),
+  LK_REQUIRE(grid_fits(window * a.heads, kPrepareThreads) &&
+                 grid_fits(scans, (NW + (two ? 4 : 2)) * kWave),
              "too many sequences x heads for one call");
   for (c.first = 0; c.first < chunks; c.first += window) {
     c.count = window < chunks - c.first ? window : chunks - c.first;

@@ -18,6 +18,11 @@ struct Sequences {
   int count;
 };
 
+// Whether a launch takes this many blocks: the threads of a grid are counted in 32 bits.
+inline bool grid_fits(int64_t blocks, int64_t threads) {
+  return blocks < (int64_t{1} << 31) && blocks * threads < (int64_t{1} << 32);
+}
+
 struct RowRange {
   int64_t begin, end;
 };
