@@ -150,6 +150,21 @@ def test_queries_and_keys_of_other_sizes(rng, form, which, size):
     _close(st, want_state, 100, torch.float32, f"state {size}")
 
 
+@pytest.mark.parametrize("lengths", [[1] * 8 + [500] + [1] * 8, [47], [48], [48, 48, 47], [96, 0],
+                                     [300] + [0] * 20])
+@pytest.mark.parametrize("dk", [64, 129])
+def test_scan_as_it_chooses_its_form(rng, lengths, dk):
+    """The form that a call takes by itself, on both sides of its rules."""
+    from local_kimi_amd import _lib
+
+    assert _lib.get_path("kda_prefill") == "auto"
+    a = _scan_inputs(rng, sum(lengths), 2, dk, 40, len(lengths))
+    want_state, want = K.prefill(*a, 0.1, _cu(lengths))
+    out, st = _run_scan(a, _cu(lengths), torch.float32, 0.1)
+    _close(out, want, max(lengths), torch.float32, "out")
+    _close(st, want_state, max(lengths), torch.float32, "state")
+
+
 # ---------------------------------------------------------------------------
 # states
 

@@ -7,6 +7,11 @@ import pytest
 
 from local_kimi_amd import _lib
 
+from .test_kernel_resources import kernels
+from .test_prompt_resources import _found
+
+_ = kernels  # fixture
+
 
 @pytest.fixture(scope="module", autouse=True)
 def _require_lib():
@@ -42,3 +47,48 @@ def test_grids_of_2_to_the_32_threads_are_refused():
         _scan(1 << 23, 1 << 23, 4, 64, 64, 16, 1 << 40)
     with pytest.raises(RuntimeError, match="too many query rows and heads"):
         _attention(1, 1 << 29, 1 << 29, 4, 2, 64)
+
+
+@pytest.mark.parametrize("sequences,tokens,heads,d_k,d_v,chunks", [
+    (1, 47, 4, 64, 64, False), (1, 48, 4, 64, 64, True), (3, 143, 4, 64, 64, False),
+    (3, 144, 4, 64, 64, True), (1, 500, 4, 128, 64, True), (1, 500, 4, 129, 64, False),
+    (1, 500, 4, 256, 64, False), (1, 500, 1 << 14, 16, (1 << 10) - 1, True),
+    (1, 500, 1 << 14, 16, 1 << 10, False), (1, 0, 4, 64, 64, False)])
+def test_the_form_that_a_scan_chooses(sequences, tokens, heads, d_k, d_v, chunks):
+    """Chunks have a workspace, steps none: from 48 tokens a sequence on, up to d_k
+    = 128, below 2^24 values a row."""
+    size = _lib.query("lk_kda_prefill_workspace", sequences, tokens, heads, d_k, d_v)
+    assert (size > 0) == chunks
+    with _lib.forced_path("kda_prefill", "steps"):
+        assert _lib.query("lk_kda_prefill_workspace", sequences, tokens, heads, d_k, d_v) == 0
+
+
+def test_workspaces_a_byte_short_or_off_16_bytes_are_refused():
+    need = _lib.query("lk_kda_prefill_workspace", 2, 500, 4, 64, 64)
+    for size in (0, need - 1):
+        with pytest.raises(RuntimeError, match="KDA prefill workspace too small"):
+            _scan(2, 500, 4, 64, 64, 16, size)
+    with pytest.raises(RuntimeError, match="KDA prefill workspace too small"):
+        _scan(2, 500, 4, 64, 64, None, need)
+    with pytest.raises(RuntimeError, match="workspace must be 16-byte aligned"):
+        _scan(2, 500, 4, 64, 64, 8, need)
+    need = _lib.query("lk_attention_prefill_workspace", 1, 5000, 1, 4, 2, 64, 64)
+    assert need > 0
+    for size in (0, need - 1):
+        with pytest.raises(RuntimeError, match="attention workspace too small"):
+            _attention(1, 1, 5000, 4, 2, 64, 16, size)
+    with pytest.raises(RuntimeError, match="workspace must be 16-byte aligned"):
+        _attention(1, 1, 5000, 4, 2, 64, 8, need)
+
+
+def test_scalars_and_scratch_memory(kernels):
+    """No kernel of a prompt has scratch memory; scalars that do not fit are kept in
+    lanes of a vector register or two, as many as they are now."""
+    limits = {"attention_kernel": 72, "attention_join_kernel": 0, "chunk_prepare_kernel": 8,
+              "chunk_scan_kernel": 0, "scan_serial_kernel": 56, "conv_prefill_kernel": 0}
+    for name, spills in limits.items():
+        found = _found(kernels, name)
+        assert found, name
+        for args, k in found.items():
+            assert k[".private_segment_fixed_size"] == 0 and k[".vgpr_spill_count"] == 0, (name, args)
+            assert k[".sgpr_spill_count"] <= spills, (name, args)
