@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
         // decides for itself, though the wave branches together: the others' keys
         // may be ones that it does not see.
         constexpr float kSlack = 8.f;
-        const bool moves = most > top + kSlack || (top == -INFINITY && most > top);
+        const bool moves = most > top + kSlack;  // (any at all from -infinity)
         if (__any(moves)) {
           const float next = moves ? most : top;
           const float fade = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
