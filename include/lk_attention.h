@@ -35,7 +35,8 @@ extern "C" {
  *   o_i = sum_j p_ij v_j,  p_i = softmax over the keys seen of scale * q_i . k_j
  * Scores and sums in fp32; p is rounded to dtype for its product with v. A key
  * or value row that a query does not see has no part in its result, NaN and
- * infinities included. Reruns are bit-identical.
+ * infinities included. A query whose every score is -infinity gets zeros too. fp16
+ * results of finite values stay finite. Reruns are bit-identical.
  *
  * workspace: lk_attention_prefill_workspace() bytes on 16 bytes (may be null
  * where that is 0). */

@@ -136,12 +136,13 @@ LK_API int lk_kda_short_conv_prefill(const void* q_in, const void* k_in, const v
  * writes them for any number of rows), v [tokens, H, d_v] and out
  * [tokens, H, d_v] in value_dtype, state fp32 [sequences, H, d_k, d_v].
  * decay <= 0 (a log decay). d_k <= 256; tensors start on 16 bytes. All sums
- * and the state are fp32; out is rounded once. From 48 tokens a sequence on and
- * up to d_k = 128, chunks of 32 steps are solved together, in which the operands
- * of the state's products are sums of two fp16 (22 bits of the largest beside
- * them); otherwise steps follow one another in fp32. The knob kda_prefill
- * (lk_set_path) asks for one form. workspace: lk_kda_prefill_workspace() bytes
- * on 16 bytes (may be null where that is 0), by the knob's setting of the call. */
+ * and the state are fp32; out is rounded once. From 48 tokens a sequence on (the
+ * call's mean) and up to d_k = 128, chunks of 32 steps are solved together, in which
+ * the operands of the state's products are sums of two fp16 (22 bits of the largest
+ * beside them), for states up to 1e36; otherwise steps follow one another in fp32.
+ * The knob kda_prefill (lk_set_path) asks for one form. workspace:
+ * lk_kda_prefill_workspace() bytes on 16 bytes (may be null where that is 0), by
+ * the knob's setting of the call. */
 LK_API int64_t lk_kda_prefill_workspace(int64_t sequences, int64_t tokens, int64_t heads,
                                         int64_t d_k, int64_t d_v);
 

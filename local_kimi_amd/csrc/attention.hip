@@ -149,9 +149,9 @@ __device__ inline AttnTile attention_tile(const AttnArgs& a, int64_t rank) {
 //
 // Two stages of 64 keys are up to 80 KB of LDS, so two blocks share a CU and one's
 // products run beside the other's softmax. Long prompts are bound by the matrix
-// unit and VALU together (53% and 31% of the cycles, at the 1.8 GHz that the power
-// allows): 8192 tokens x 32 heads of 192/128 take 690 us, 996 TFLOP/s, where a bf16
-// 8192^3 library product reaches 1139. Short calls are bound by latency.
+// unit and VALU together (53% and 31% of the cycles, at the 1.77 GHz that the card
+// runs at meanwhile): 8192 tokens x 32 heads of 192/128 take 690 to 705 us, 975 to 996
+// TFLOP/s, where a bf16 8192^3 library product reaches 1139. Short calls are bound by latency.
 template <bool BF16, int DQ, int DV>
 __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) {
   constexpr int kQSteps = DQ / 16;
@@ -547,8 +547,11 @@ int attention_pack(int64_t heads, int64_t kv_heads) {
 // Runs of each block's keys. A block alone on a CU leaves its matrix unit idle
 // through every softmax, and a call with fewer blocks than CUs leaves CUs idle: where
 // there are fewer than two blocks a CU, long key ranges are taken in runs, until
-// there are, of kAttnRun keys at least (the runs' sums are written and read again).
-// Counts are estimates from the call's sizes: the lengths are on the device.
+// there are, of kAttnRun keys at least in the mean (the runs' sums are written and read
+// again). Counts are estimates from the call's sizes: the lengths are on the device. A
+// sequence far longer than the mean is in fewer runs than it could be, a shorter one in
+// shorter runs: 64 queries x 8 heads, one on 16384 keys and 63 on 16, take 337 us, the
+// one alone 25.
 // With one run / by this rule, bf16 heads of 128: one query x 16384 keys x 8 heads
 // 329 / 21 us, 512 x 4096 x 32 93 / 58, 4096 x 4096 x 4 91 / 44, 16 x 800 x 32 23 / 18.
 // 1024 queries x 1024 keys x 32 took 30 in one and 40 in two runs (of 256 keys).

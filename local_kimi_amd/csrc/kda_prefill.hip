@@ -51,7 +51,8 @@ struct alignas(sizeof(T) * N) Pack {
 // a tile of kConvTile tokens with the three earlier inputs in registers,
 // kConvRows rows' loads in flight; the tile's first three inputs are read again (3
 // rows in kConvTile, mostly from a cache). Where rows do not start on 16 bytes, N
-// is one. Threads are dealt over the three
+// is one: 4096 tokens x 3 x 4095 bf16 48 us, 4096 channels 38, eight times the loads
+// and stores of a 16th each, which the caches join. Threads are dealt over the three
 // convolutions' channels as one row, so that only a call's last block has idle
 // ones. The thread with a sequence's first tile has read the state's values, so
 // it is the one that replaces them: the state may be updated in place.
@@ -196,9 +197,11 @@ __global__ void __launch_bounds__(kConvThreads) conv_prefill_kernel(ConvArgs a) 
 // column l / 16, sums over the 16 lanes of a DPP row. A block of four waves
 // takes 16 columns and stages kSerialTokens steps of q, k, e^g and k . q in
 // LDS (one lane of the staging per 16th of a row, as the steps use them) while
-// the batch before it runs. Bound by the chain from step to step: LDS reads, the
-// products, 8 DPP additions, 0.4 us a step (heads of 128 x 128: 20 steps 10 us,
-// 256 steps 90 us).
+// the batch before it runs. Bound by the chain from step to step, in which a wave
+// has nothing else to do: six LDS reads, RPL products after one another for each of
+// the two sums, four DPP additions, RPL more products. 32 heads take 0.28 us a step at
+// d_k = 64, 0.35 at 128 (256 steps 90 us), 0.67 to 0.70 at 256 (256 steps 179 us, 1024
+// steps 680).
 constexpr int kSerialThreads = 256;
 constexpr int kSerialCols = 16;
 constexpr int kSerialTokens = 16;
@@ -792,8 +795,12 @@ __global__ void __launch_bounds__(kPrepareThreads, 4) chunk_prepare_kernel(ScanA
 // off the path from one state to the next: they bring U0 and the decays, and
 // add up, complete (P U) and store the outputs, a chunk later.
 //
-// Bound by that path: 1.2 us a chunk for 32 heads of 128 x 128, where the matrix
-// unit is busy for a sixth of the time and VALU for a third. 48 of a record's 68 KB
+// One prompt is bound by that path: 1.2 us a chunk for 32 heads of 128 x 128, where
+// the matrix unit is busy for a sixth of the time and VALU for a third. So are many
+// prompts, though their chunks are independent: with the records on their way a block's
+// registers (204 a lane, 246 for two tiles) leave room for no second block on its CU,
+// which could use the waits (4096 tokens of 11 prompts: 180 us, the longest prompt's
+// chunks 41). 48 of a record's 68 KB
 // are loaded as operands by the blocks of each 16 columns. The waves meet at the
 // barrier, so their loads come at the same time: they are put between the
 // products that follow it (in one place they held the waves up for 500 cycles of
@@ -1190,10 +1197,13 @@ int64_t chunk_record(int64_t d_k, int64_t d_v) {
   return channels * (3 * kChunk + 1) + 3 * 256 + 2 * kChunk + 16 + (d_v + 15) / 16 * 16 * kChunk;
 }
 
-// From this many 16-column tiles of a call on (twice as many as keep two blocks on
-// each CU), a block takes two: half the blocks load the same records. 4096 tokens
-// of 11 sequences x 32 heads x 8 tiles: 350 us with one, 316 with two; a single
-// prompt's 256 tiles (8192 tokens), which fill the CUs once: 570 and 655.
+// From this many 16-column tiles of a call on (four for each CU, which holds one
+// block), a block takes two: half the blocks load the same records. With one / with two
+// tiles a block, us a call: 32 heads of 128 x 128, equal prompts, 4096 tokens in all,
+// 256 tiles 298 / 337, 512 304 / 274, 1024 310 / 278, 2048 324 / 295, 4096 358 / 305;
+// prompts of 512 tokens, 256 tiles 46 / 52, 512 75 / 68, 768 107 / 106, 1024 146 / 132,
+// 4096 651 / 567. 16 heads of 64 x 64, prompts of 512 tokens, 1024 tiles 135 / 142, 2048
+// 302 / 312. (Half as many tiles would do at d_k = 128; at 64 one is better.)
 constexpr int64_t kTwoTiles = 1024;
 
 // Chunks of one window: the records of a window are written by one launch and
@@ -1214,10 +1224,15 @@ int64_t chunk_bytes(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_
 
 bool takes_chunks(int64_t sequences, int64_t tokens, int64_t heads, int64_t d_k, int64_t d_v) {
   const int choice = path_choice(kKnobKdaPrefill);
-  // (a chunk's outputs are stored at 31-bit byte offsets.) Chunks from 48 tokens a
-  // sequence on: 32 heads of 128 x 128 took, in steps / in chunks, for one sequence of
-  // 32 tokens 15 / 18 us, of 48 20 / 19, of 128 48 / 22, for 32 sequences of 32 tokens
-  // 149 / 127; 16 heads of 64 x 64 for 16 sequences of 32 tokens 19 / 23.
+  // (a chunk's outputs are stored at 31-bit byte offsets. Beyond d_k = 128 there are
+  // no chunks: prepare's rows of q, k and e^g alone would take 100 of a CU's 160 KB of
+  // LDS at 256.) Chunks from 48 tokens a sequence on: 32 heads of 128 x 128 took, in
+  // steps / in chunks, for one sequence of 32 tokens 15 / 18 us, of 48 20 / 19, of 128
+  // 48 / 22; 16 heads of 64 x 64 for 16 sequences of 32 tokens 19 / 23. The tokens a
+  // sequence are the call's mean, since the lengths are on the device; that takes the
+  // slower form for 32 sequences of 32 tokens (150 / 127) and where one prompt is
+  // among many short sequences: 1000 tokens beside 32 single ones 396 / 176, 2048
+  // beside 64 880 / 390. The knob is for those.
   if (d_k > 128 || tokens == 0 || choice == 1 || heads * d_v >= (int64_t{1} << 24)) return false;
   return choice == 2 || tokens >= 48 * sequences;
 }

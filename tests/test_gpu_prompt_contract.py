@@ -102,6 +102,25 @@ def test_many_weights_far_below_the_largest(rng, dtype):
     _check(got, a, scale, dtype, what="far below")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("keys", [150, 2500])
+def test_scores_of_minus_infinity(rng, dtype, keys):
+    """Keys whose score is -infinity have no weight, and a query that sees no other
+    gets zeros; every query here has the sign that makes it so."""
+    from local_kimi_amd.kernels import attention_prefill
+
+    a = _inputs(rng, 40, keys, 2, 1, 64, 64, dtype)
+    a[0][:, :, 0] = 1.0
+    masked = [x.copy() for x in a]
+    masked[1][::3, :, 0] = -np.inf
+    a[1], a[2] = (np.delete(x, np.arange(0, keys, 3), axis=0) for x in a[1:])
+    t = [_t(x[None], dtype) for x in masked]
+    got = attention_prefill(t[0][:, -1:], *t[1:])  # (a query that sees every key)
+    _check(got, [a[0][-1:], *a[1:]], 0.125, dtype, what="some")
+    t[1][..., 0] = -float("inf")
+    assert not attention_prefill(*t).any()
+
+
 @pytest.mark.parametrize("cu_k", [False, True])
 def test_attention_of_one_prompt_among_short_ones(rng, cu_k):
     from local_kimi_amd.kernels import attention_prefill
