@@ -639,7 +639,8 @@ int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
              "attention strides must not be negative");
   LK_REQUIRE(k_row_stride < (int64_t{1} << 24) && v_row_stride < (int64_t{1} << 24),
              "attention row strides must be below 2^24 elements");
-  LK_REQUIRE(scale == scale && scale - scale == 0.f, "the attention scale must be finite");
+  const float scale_log2 = fabsf(scale) * 1.4426950408889634f;
+  LK_REQUIRE(scale_log2 < INFINITY, "the attention scale must be finite, below 2^127");
   if (rows_q == 0) return LK_OK;
   LK_REQUIRE(q && out && (rows_k == 0 || (k && v)), "null pointer argument");
   for (const void* p : {q, k, v, static_cast<const void*>(out)})
@@ -672,7 +673,7 @@ int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
                    sequence_tiles(rows_q, sequences, kAttnRows / pack),
                    attention_splits(rows_q, rows_k, sequences, heads, pack),
                    need ? static_cast<float*>(workspace) : nullptr,
-                   scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f,
+                   scale == 0.f ? 1.f : scale_log2,
                    scale == 0.f ? 0u : 0xFFFFFFFFu,
                    scale < 0.f ? 0x80008000u : 0u};
   const hipStream_t s = as_stream(stream);

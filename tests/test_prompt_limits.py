@@ -29,10 +29,10 @@ def _scan(sequences, tokens, heads, d_k, d_v, workspace=None, size=0):
               workspace, size, None)
 
 
-def _attention(sequences, rows_q, rows_k, heads, kv_heads, d, workspace=None, size=0):
+def _attention(sequences, rows_q, rows_k, heads, kv_heads, d, workspace=None, size=0, scale=1.0):
     _lib.call("lk_attention_prefill", 16, 16, 16, 16, None, None, sequences, rows_q, rows_k, heads,
-              kv_heads, d, d, heads * d, d, kv_heads * d, d, kv_heads * d, d, 1.0, 2, workspace, size,
-              None)
+              kv_heads, d, d, heads * d, d, kv_heads * d, d, kv_heads * d, d, scale, 2, workspace,
+              size, None)
 
 
 def test_grids_of_2_to_the_32_threads_are_refused():
@@ -47,6 +47,13 @@ def test_grids_of_2_to_the_32_threads_are_refused():
         _scan(1 << 23, 1 << 23, 4, 64, 64, 16, 1 << 40)
     with pytest.raises(RuntimeError, match="too many query rows and heads"):
         _attention(1, 1 << 29, 1 << 29, 4, 2, 64)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38, -3e38])
+def test_scales_that_log2_e_takes_to_infinity_are_refused(scale):
+    """Scores are scaled by scale * log2(e) in fp32: NaN for every result beyond it."""
+    with pytest.raises(RuntimeError, match="scale must be finite"):
+        _attention(1, 1, 1, 4, 2, 64, scale=scale)
 
 
 @pytest.mark.parametrize("sequences,tokens,heads,d_k,d_v,chunks", [
