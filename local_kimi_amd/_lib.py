@@ -83,6 +83,11 @@ SIGNATURES: dict[str, list] = {
                        _P, _I64, _P],
     "lk_attention_prefill": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                              _I64, _I64, _I64, _I64, _I64, _I64, _F, _I, _P, _I64, _P],
+    "lk_qk_norm_rope": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                        _I64, _I64, _I64, _I, _I64, _I, _F, _I, _I, _P],
+    "lk_paged_append": [*[_P] * 12, *[_I64] * 24, _I, _I64, _F, _I, _I, _P],
+    "lk_attention_paged": [*[_P] * 7, *[_I64] * 18, _F, _I, _P, _I64, _P],
+    "lk_copy_pages": [_P, _P, _P, _I64, _P, _P, _I64, _I64, _P],
     "lk_rms_norm": [_P, _P, _P, _I64, _I64, _F, _I, _I, _P],
     "lk_add_rms_norm": [_P, _P, _P, _P, _P, _I64, _I64, _F, _I, _I, _P],
     "lk_rms_gated_norm": [_P, _P, _P, _P, _I64, _I64, _F, _I, _I, _I, _I, _P],
@@ -99,6 +104,7 @@ QUERIES: dict[str, list] = {
     "lk_mxfp4_moe_forward_workspace": [_I64, _I64, _I64, _I64, _I64],
     "lk_kda_prefill_workspace": [_I64, _I64, _I64, _I64, _I64],
     "lk_attention_prefill_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I64],
+    "lk_attention_paged_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I64],
 }
 
 _lock = threading.Lock()

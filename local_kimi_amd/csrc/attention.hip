@@ -2,7 +2,7 @@
 
 #include "lk_attention.h"
 #include "lk_gemm.hpp"
-#include "lk_sequences.hpp"
+#include "lk_pages.hpp"
 
 namespace lk {
 namespace {
@@ -44,17 +44,6 @@ __device__ inline f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
                                                   __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-template <bool BF16>
-__device__ inline uint32_t pack2(float a, float b) {
-  if constexpr (BF16) {
-    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, v2{static_cast<__bf16>(a), static_cast<__bf16>(b)});
-  } else {
-    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, v2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
-  }
-}
-
 // A finite mean of V's values, within the type: p is rounded before its product and
 // not in the sum that divides it, so that a mean of 65504 can come out as much as
 // 2^-11 above it, where fp16 has infinity from 2^-12 on. (bf16 ends where fp32 does.)
@@ -82,12 +71,6 @@ __device__ inline u32x4_t finite_only(u32x4_t x) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] &= ~((((x[i] & kExp) + kOne) >> 15 & 0x00010001u) * 0xFFFFu);
   return x;
-}
-
-template <bool BF16>
-__device__ inline float value_of(uint32_t x) {
-  if constexpr (BF16) return bf16_to_f32(static_cast<uint16_t>(x));
-  else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(x)));
 }
 
 // Staging. A tile of K (V) in LDS is kAttnKeys rows of C 16-byte chunks, filled

@@ -27,6 +27,8 @@ from .moe import (moe_router, moe_schedule, router_logits, shape_stable_expert_i
 from .mxfp4 import (grouped_mxfp4_gemm, grouped_mxfp4_reference, grouped_mxfp4_swiglu_gemm,
                     mxfp4_expert_mlp, mxfp4_gemm, mxfp4_gemm_reference, mxfp4_linear,
                     mxfp4_moe_block, mxfp4_moe_block_reference, split_activations_fp8)
+from .paged import (attention_paged, copy_pages, paged_append, qk_norm_rope, qk_norm_rope_append,
+                    rope_table)
 from .w4a16 import (fused_qkv_w4a16, fused_qkv_w4a16_reference, fused_w2_combine,
                     fused_w2_combine_reference, grouped_w4a16_gemm, grouped_w4a16_gemv,
                     grouped_w4a16_reference, grouped_w4a16_swiglu_gemm,
@@ -146,7 +148,8 @@ _register_mxfp4()
 __all__ = [
     "registry", "kda_decode_step", "kda_decode_layer", "fused_short_conv_triple",
     "fused_kda_gates", "kda_prefill", "short_conv_prefill_triple", "attention_prefill",
-    "rms_norm", "add_rms_norm", "rms_gated_norm",
+    "attention_paged", "qk_norm_rope", "qk_norm_rope_append", "paged_append", "copy_pages",
+    "rope_table", "rms_norm", "add_rms_norm", "rms_gated_norm",
     "W4A16_GROUPED", "W4A16_DENSE", "W4A16_SWIGLU", "W4A16_FUSED_QKV",
     "W4A16_W2_COMBINE", "W4A16_MOE_BLOCK", "moe_router", "router_logits",
     "shape_stable_expert_indices",
