@@ -1,106 +1,22 @@
 // Causal softmax attention over packed prompts, for gfx950.
 
 #include "lk_attention.h"
-#include "lk_gemm.hpp"
-#include "lk_pages.hpp"
+#include "lk_attention_tile.hpp"
 
 namespace lk {
 namespace {
 
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-
-constexpr int kAttnThreads = 256;
-constexpr int kAttnWaves = kAttnThreads / kWave;
-constexpr int kAttnRows = 32 * kAttnWaves;  // queries x heads of a block
-constexpr int kAttnKeys = 64;                  // per pass of the loop
 constexpr int kJoinRows = 2;  // of a wave of the join
 constexpr int kJoinBlocks = kAttnRows / (kAttnWaves * kJoinRows);
-constexpr int kAttnMaxQk = 192;
-constexpr int kAttnMaxV = 128;
 
-struct AttnArgs {
-  const uint16_t *q, *k, *v;
-  uint16_t* out;
+struct AttnArgs : AttnShape {
+  const uint16_t *k, *v;
   Sequences sq, sk;
-  int heads, group, d_qk, d_v;
-  // A block's rows: `tokens` queries of `pack` heads that share a key head, row r
-  // query r / pack (r inv_pack >> 16), head r % pack. Blocks for a query: `packs`.
-  int pack, inv_pack, tokens, packs;
-  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  int64_t k_row, k_head, v_row, v_head;
   int64_t tiles;
   int splits;       // runs of each block's keys
   float* partial;   // more than one run: their sums, else null
-  float scale_log2;  // |scale| * log2(e), 1 where scale is 0
-  uint32_t q_keep, q_flip;  // bits of q kept (none where scale is 0), flipped (signs, scale < 0)
 };
-
-template <bool BF16>
-__device__ inline f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
-  if constexpr (BF16)
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
-                                                   __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
-                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-}
-
-// A finite mean of V's values, within the type: p is rounded before its product and
-// not in the sum that divides it, so that a mean of 65504 can come out as much as
-// 2^-11 above it, where fp16 has infinity from 2^-12 on. (bf16 ends where fp32 does.)
-template <bool BF16>
-__device__ inline float within_type(float x) {
-  if constexpr (BF16) return x;
-  else return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
-}
-
-// Whether any of the eight values is an infinity or a NaN (exponent all ones:
-// one more carries into the sign's place).
-template <bool BF16>
-__device__ inline bool any_nonfinite(u32x4_t x) {
-  constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
-  uint32_t hit = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) hit |= (x[i] & kExp) + kOne;
-  return (hit & 0x80008000u) != 0;
-}
-
-// The eight values with those set to zero.
-template <bool BF16>
-__device__ inline u32x4_t finite_only(u32x4_t x) {
-  constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] &= ~((((x[i] & kExp) + kOne) >> 15 & 0x00010001u) * 0xFFFFu);
-  return x;
-}
-
-// Staging. A tile of K (V) in LDS is kAttnKeys rows of C 16-byte chunks, filled
-// by direct loads (a wave-wide load fills 1 KB in slot order), row r's chunk c
-// in slot r C + (c ^ swizzle(r)). A matrix row's chunks are read by 16 or 32 lanes
-// with consecutive rows at once, so the swizzle spreads 16 consecutive rows over
-// all 16-byte columns of the 64 banks; rows shorter than 256 bytes share one
-// pass over the banks with their neighbours, and longer ones than 256 start at
-// either half of them, hence the row's upper bits there.
-template <int C>
-__host__ __device__ constexpr int key_swizzle(int r) {
-  return C % 16 == 0 ? r & 15 : (r >> 1) & 7;
-}
-// V is read down its columns (four rows of 32 bytes by 16 lanes, twice that by a
-// half-wave): four consecutive rows go to four quarters of the banks.
-template <int C>
-__host__ __device__ constexpr int value_swizzle(int r) {
-  return C % 16 == 0 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
-}
-
-typedef short i16x4_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
-
-// Four rows of 16 columns, by 16 lanes: lane l gives the address of row l / 4,
-// columns 4 (l % 4) to + 3, and gets column l of the four rows.
-__device__ inline uint2 lds_read_transposed(const uint16_t* p) {
-  const i16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lds_i16x4_t*)(const __attribute__((address_space(3))) uint16_t*)(p));
-  return __builtin_bit_cast(uint2, v);
-}
 
 // A tile of queries, and the rows of its sequence.
 struct AttnTile {
@@ -118,17 +34,8 @@ __device__ inline AttnTile attention_tile(const AttnArgs& a, int64_t rank) {
   return t;
 }
 
-// o_i = sum_j p_ij v_j / sum_j p_ij, p_ij = 2^(s_ij - top_i), in one pass over the
-// keys: s in units of log2, top_i the running maximum, what is summed scaled down
-// where it moves.
-//
-// Block = 128 rows (queries x heads of one key head), a wave 32 of them. Scores
-// are computed transposed, S^T = K Q^T (32x32 MFMA tiles, keys down, queries
-// across), so a lane holds one query's scores in its registers: the softmax needs
-// one exchange between the half-waves per 64 keys, the running maximum and sum are
-// a scalar per lane, and the score registers, rounded, are the B operand of
-// O^T += V^T P^T as they stand. That rounding of p to the inputs' type is the one
-// before the output's: the products need it, the sums of p are of the unrounded.
+// A block's rows against its sequence's keys (attend_rows), to the output or, in runs,
+// to the workspace.
 //
 // Two stages of 64 keys are up to 80 KB of LDS, so two blocks share a CU and one's
 // products run beside the other's softmax. Long prompts are bound by the matrix
@@ -137,33 +44,19 @@ __device__ inline AttnTile attention_tile(const AttnArgs& a, int64_t rank) {
 // TFLOP/s, where a bf16 8192^3 library product reaches 1139. Short calls are bound by latency.
 template <bool BF16, int DQ, int DV>
 __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) {
-  constexpr int kQSteps = DQ / 16;
   constexpr int kVTiles = DV / 32;
-  constexpr int kKChunks = DQ / 8, kVChunks = DV / 8;
-  constexpr int kKLoads = kAttnKeys * kKChunks / kAttnThreads;
-  constexpr int kVLoads = kAttnKeys * kVChunks / kAttnThreads;
-  constexpr int kStage = kAttnKeys * (DQ + DV);  // values of one stage
-  // p is stored as 2^kLift times itself: fp16 keeps 2^-24 at the least
-  constexpr float kLift = BF16 ? 0.f : 6.f;
-  __shared__ alignas(16) uint16_t stage[2 * kStage];
+  __shared__ alignas(16) uint16_t stage[2 * kAttnKeys * (DQ + DV)];
   const int pack = static_cast<int>(blockIdx.x % a.packs);
   const int64_t item = blockIdx.x / a.packs;
   const int split = static_cast<int>(item % a.splits);
   const AttnTile tile = attention_tile(a, item / a.splits);
   const SequenceTile at = tile.at;
   if (at.sequence < 0) return;
-  const RowRange rq = tile.q;
-  const int64_t lq = rq.end - rq.begin;
+  const int64_t lq = tile.q.end - tile.q.begin;
   const int64_t q0 = at.tile * a.tokens;
   if (q0 >= lq) return;
   const int64_t last = q0 + a.tokens < lq ? q0 + a.tokens : lq;  // the block's, exclusive
-  const int tid = threadIdx.x, lane = tid & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int n = lane & 31, half = lane >> 5;
-  const int64_t qw = q0 + (wave * 32 * a.inv_pack >> 16);  // the wave's first query
-  const int row = wave * 32 + n, token = row * a.inv_pack >> 16;
-  const int64_t qi = q0 + token;  // the lane's, of this head
-  const int h = pack * a.pack + row - token * a.pack;
+  const AttnBlock b{tile.q, tile.k.end - tile.k.begin, q0, last, pack, split, a.splits};
   f32x16_t o[kVTiles];
 #pragma unroll
   for (int t = 0; t < kVTiles; ++t)
@@ -172,272 +65,18 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
   float top = -INFINITY;  // (scaled) maximum that p is taken against
   float sum = 0.f;
   if (at.sequence < a.sq.count) {
-    const RowRange rk = tile.k;
-    const int64_t lk = rk.end - rk.begin;
-    const int64_t ahead = lk - lq;
-    // keys seen by the block's last query, and by the wave's
-    const int64_t all = last + ahead < 0 ? 0 : last + ahead;
-    // this block's run of them, and the wave's end of it
-    const int64_t per = ((all + a.splits - 1) / a.splits + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
-    const int64_t from = split * per < all ? split * per : all;
-    const int64_t keys = from + per < all ? from + per : all;
-    const int64_t end_wave = q0 + ((wave * 32 + 31) * a.inv_pack >> 16) + 1 + ahead;
-    const int64_t keys_wave = end_wave < keys ? end_wave : keys;
     const int hk = pack * a.pack / a.group;
-    const uint16_t* const kb = a.k + rk.begin * a.k_row + hk * a.k_head;
-    const uint16_t* const vb = a.v + rk.begin * a.v_row + hk * a.v_head;
-    u32x4_t qf[kQSteps];
-    {
-      const uint16_t* const qp = a.q + (rq.begin + (qi < lq ? qi : lq - 1)) * a.q_row + h * a.q_head;
-#pragma unroll
-      for (int i = 0; i < kQSteps; ++i) {
-        const int d = 16 * i + 8 * half;
-        const u32x4_t z = {0u, 0u, 0u, 0u};
-        qf[i] = d < a.d_qk ? *reinterpret_cast<const u32x4_t*>(qp + d) : z;
-        qf[i] = (qf[i] & a.q_keep) ^ a.q_flip;
-      }
-    }
-    // byte offsets of this lane's chunks from a tile's first row
-    uint32_t koff[kKLoads], voff[kVLoads];
-#pragma unroll
-    for (int i = 0; i < kKLoads; ++i) {
-      const int slot = (wave * kKLoads + i) * kWave + lane, r = slot / kKChunks;
-      const int c = slot % kKChunks ^ key_swizzle<kKChunks>(r);
-      koff[i] = 8 * c < a.d_qk ? static_cast<uint32_t>(r * a.k_row + 8 * c) * 2u : 0xFFFFFFF0u;
-    }
-#pragma unroll
-    for (int i = 0; i < kVLoads; ++i) {
-      const int slot = (wave * kVLoads + i) * kWave + lane, r = slot / kVChunks;
-      const int c = slot % kVChunks ^ value_swizzle<kVChunks>(r);
-      voff[i] = 8 * c < a.d_v ? static_cast<uint32_t>(r * a.v_row + 8 * c) * 2u : 0xFFFFFFF0u;
-    }
-    const uint32_t lds = lds_offset(stage);
-    auto fetch = [&](int64_t k0, int buf) {
-      // rows behind the sequence's last read as zeros
-      const int64_t rows = lk - k0 < kAttnKeys ? lk - k0 : kAttnKeys;
-      const u32x4_t rk_ = buffer_rsrc(kb + k0 * a.k_row, ((rows - 1) * a.k_row + a.d_qk) * 2);
-      const u32x4_t rv_ = buffer_rsrc(vb + k0 * a.v_row, ((rows - 1) * a.v_row + a.d_v) * 2);
-      const uint32_t base = lds + buf * kStage * 2;
-#pragma unroll
-      for (int i = 0; i < kKLoads; ++i)
-        lds_direct16(rk_, base + (wave * kKLoads + i) * kWave * 16, koff[i], 0);
-#pragma unroll
-      for (int i = 0; i < kVLoads; ++i)
-        lds_direct16(rv_, base + kAttnKeys * DQ * 2 + (wave * kVLoads + i) * kWave * 16, voff[i], 0);
-    };
-    // where this lane reads, in values from the start of a tile: K row n (and n +
-    // 32), chunks 2 i + half (the swizzle takes a chunk's low bits alone, so the
-    // reads of later chunks are those of the first at a fixed distance)
-    constexpr int kAddrs = kKChunks % 16 == 0 ? 8 : 4;
-    int kaddr[kAddrs];
-#pragma unroll
-    for (int i = 0; i < kAddrs; ++i)
-      kaddr[i] = n * DQ + 8 * ((2 * i + half) ^ key_swizzle<kKChunks>(n));
-    static_assert(key_swizzle<kKChunks>(32) == 0 && value_swizzle<kVChunks>(8) == 0, "row steps");
-    // V rows 4 half + lane % 16 / 4 (and + 8), columns 16 (lane / 16 % 2) + 4 (lane % 4)
-    int vaddr[2][kVTiles];
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int vt = 0; vt < kVTiles; ++vt) {
-        const int row = 8 * x + 4 * half + (lane & 15) / 4;
-        const int col = 32 * vt + 16 * (lane / 16 & 1) + 4 * (lane & 3);
-        vaddr[x][vt] = row * DV + 8 * ((col / 8) ^ value_swizzle<kVChunks>(row)) + col % 8;
-      }
-
-    if (from < keys) fetch(from, 0);
-    wait_vmcnt<0>();
-    __syncthreads();
-    int buf = 0;
-    bool bad = false;  // V has an infinity or a NaN in a tile that not every query sees
-    for (int64_t k0 = from; k0 < keys; k0 += kAttnKeys, buf ^= 1) {
-      if (k0 + kAttnKeys < keys) fetch(k0 + kAttnKeys, buf ^ 1);
-      if (k0 < keys_wave && qw < lq) {
-        const uint16_t* const lk_ = stage + buf * kStage;
-        const uint16_t* const lv = lk_ + kAttnKeys * DQ;
-        f32x16_t s[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
-        // K two steps ahead of its use: read one pair at a time as the matrix
-        // unit wants them, each pair of products waited for LDS
-        u32x4_t kf[3][2];
-        auto read_k = [&](int i) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            kf[i % 3][t] = *reinterpret_cast<const u32x4_t*>(
-                lk_ + kaddr[i % kAddrs] + 8 * (2 * kAddrs) * (i / kAddrs) + 32 * t * DQ);
-        };
-        read_k(0);
-        read_k(1);
-#pragma unroll
-        for (int i = 0; i < kQSteps; ++i) {
-          if (i + 2 < kQSteps) read_k(i + 2);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int t = 0; t < 2; ++t) s[t] = mfma32<BF16>(kf[i % 3][t], qf[i], s[t]);
-        }
-        // the first V rows, on their way through the softmax
-        u32x4_t vf[2][kVTiles];
-        auto read_v = [&](int i) {
-#pragma unroll
-          for (int vt = 0; vt < kVTiles; ++vt)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const uint2 v = lds_read_transposed(lv + vaddr[x][vt] + 16 * i * DV);
-              vf[i & 1][vt][2 * x] = v.x;
-              vf[i & 1][vt][2 * x + 1] = v.y;
-            }
-        };
-        read_v(0);
-        __builtin_amdgcn_sched_barrier(0);
-        // register r of tile t: key k0 + 32 t + 8 (r / 4) + 4 half + r % 4. What a
-        // query does not see is left out of its maximum and gets p = 0, which
-        // an infinity or a NaN in V would turn into one of its own: such values
-        // are taken out of the product there and added at the end, for the
-        // queries that see them.
-        const bool edge = k0 + kAttnKeys - 1 > qw + ahead;  // a query does not see all of them
-        if (edge) {
-          // keys of this tile that the lane's query sees, from its first register on
-          const int seen =
-              static_cast<int>(qi + ahead - k0 < kAttnKeys ? qi + ahead - k0 + 1 : kAttnKeys) - 4 * half;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[t][r] = 32 * t + 8 * (r / 4) + r % 4 < seen ? s[t][r] : -INFINITY;
-        }
-        float most = s[0][0];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) most = fmaxf(most, s[t][r]);
-        {
-          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most),
-                                                          __float_as_uint(most), false, false);
-          most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.scale_log2;
-        }
-        // a query's maximum only moves when it has grown by more than 2^kSlack: p
-        // stays below that, and most passes leave the accumulators alone. Each query
-        // decides for itself, though the wave branches together: the others' keys
-        // may be ones that it does not see.
-        constexpr float kSlack = 8.f;
-        const bool moves = most > top + kSlack;  // (any at all from -infinity)
-        if (__any(moves)) {
-          const float next = moves ? most : top;
-          const float fade = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
-          top = next;
-          sum *= fade;
-#pragma unroll
-          for (int t = 0; t < kVTiles; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[t][r] *= fade;
-        }
-        const float base = kLift - (top == -INFINITY ? 0.f : top);
-        float part[2] = {0.f, 0.f};
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2, base));
-            part[t] += s[t][r];
-          }
-        sum += part[0] + part[1];
-        // k-slots of MFMA step i: keys 16 i + 4 half + {0..3} and + 8
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = i / 2, r = 8 * (i & 1);
-          const u32x4_t p = {pack2<BF16>(s[t][r], s[t][r + 1]), pack2<BF16>(s[t][r + 2], s[t][r + 3]),
-                             pack2<BF16>(s[t][r + 4], s[t][r + 5]),
-                             pack2<BF16>(s[t][r + 6], s[t][r + 7])};
-          if (i < 3) read_v(i + 1);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int vt = 0; vt < kVTiles; ++vt) {
-            if (edge && __builtin_expect(__any(any_nonfinite<BF16>(vf[i & 1][vt])), 0)) {
-              bad = true;
-              vf[i & 1][vt] = finite_only<BF16>(vf[i & 1][vt]);
-            }
-            o[vt] = mfma32<BF16>(vf[i & 1][vt], p, o[vt]);
-          }
-        }
-      }
-      wait_vmcnt<0>();  // the next tile has landed
-      __syncthreads();
-    }
-    sum += __shfl_xor(sum, 32);
-    if (__builtin_expect(bad, 0)) {
-      // the infinities and NaNs left out above, for the queries that see them
-      int64_t key = qw + ahead + 1 < 0 ? 0 : (qw + ahead + 1) / kAttnKeys * kAttnKeys;
-      key = key < from ? from : key;
-#pragma unroll 1
-      for (; key < keys_wave; ++key) {
-        const uint16_t* const row = vb + key * a.v_row;
-#pragma unroll
-        for (int t = 0; t < kVTiles; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int d = 32 * t + 8 * (r / 4) + 4 * half + r % 4;
-            const float x = d < a.d_v && key <= qi + ahead ? value_of<BF16>(row[d]) : 0.f;
-            if (!(fabsf(x) < INFINITY)) o[t][r] += x;
-          }
-      }
-    }
+    DenseKeys<DQ, DV> keys(a.k + tile.k.begin * a.k_row + hk * a.k_head,
+                           a.v + tile.k.begin * a.v_row + hk * a.v_head, a.k_row, a.v_row, b.lk, a,
+                           stage);
+    attend_rows<BF16, DQ, DV>(a, b, keys, stage, o, top, sum);
   }
   if (a.partial) {
-    // the run's sums as they are, with what they are taken against
-    float* const part = a.partial + ((item / a.splits * a.packs + pack) * a.splits + split) *
-                                        (kAttnRows * (DV + 2));
-    if (qi >= last) return;
-#pragma unroll
-    for (int t = 0; t < kVTiles; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4)
-        *reinterpret_cast<float4*>(part + row * DV + 32 * t + 8 * (r / 4) + 4 * half) =
-            make_float4(o[t][r], o[t][r + 1], o[t][r + 2], o[t][r + 3]);
-    if (half == 0) {
-      part[kAttnRows * DV + row] = top;
-      part[kAttnRows * (DV + 1) + row] = sum;
-    }
+    store_sums<DV>(a, b, a.partial + ((item / a.splits * a.packs + pack) * a.splits + split) *
+                                         (kAttnRows * (DV + 2)), o, top, sum);
     return;
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  // whole rows through the wave's share of LDS (every wave has left the loop)
-  constexpr int kOutStride = DV + 8;
-  static_assert(kAttnWaves * 32 * kOutStride <= 2 * kStage, "output tile in LDS");
-  uint16_t* const rows = stage + wave * 32 * kOutStride;
-#pragma unroll
-  for (int t = 0; t < kVTiles; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      *reinterpret_cast<uint2*>(rows + n * kOutStride + 32 * t + 8 * (r / 4) + 4 * half) =
-          make_uint2(pack2<BF16>(within_type<BF16>(o[t][r] * inv), within_type<BF16>(o[t][r + 1] * inv)),
-                     pack2<BF16>(within_type<BF16>(o[t][r + 2] * inv),
-                                 within_type<BF16>(o[t][r + 3] * inv)));
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 32 * kVChunks / kWave; ++i) {
-    const int slot = i * kWave + lane, r = slot / kVChunks, d = slot % kVChunks * 8;
-    const int to = wave * 32 + r, q = to * a.inv_pack >> 16;
-    const int64_t head = pack * a.pack + to - q * a.pack;
-    if (q0 + q < last && d < a.d_v)
-      *reinterpret_cast<u32x4_t*>(a.out + ((rq.begin + q0 + q) * a.heads + head) * a.d_v + d) =
-          *reinterpret_cast<const u32x4_t*>(rows + r * kOutStride + d);
-  }
-}
-
-// A sum (or maximum) over the wave's lanes, in every lane.
-template <typename Op>
-__device__ inline float over_wave(float v, Op op) {
-  v = op(v, dpp_f32<kQuadXor1>(v));
-  v = op(v, dpp_f32<kQuadXor2>(v));
-  v = op(v, dpp_f32<kRowHalfMirror>(v));
-  v = op(v, dpp_f32<kRowMirror>(v));
-  auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = op(__uint_as_float(x[0]), __uint_as_float(x[1]));
-  x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return op(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  store_rows<BF16, DQ, DV>(a, b, stage, o, sum);
 }
 
 // The runs of a block's keys joined: a wave takes kJoinRows rows, a lane a run's
@@ -513,18 +152,6 @@ __global__ void __launch_bounds__(kAttnThreads) attention_join_kernel(AttnArgs a
         out[lane] = static_cast<uint16_t>(pack2<BF16>(within_type<BF16>(acc[r][0] * inv), 0.f));
     }
   }
-}
-
-// Heads of a block: as many as divide those of a key head, up to 16, so that a
-// key is read once for all of them and a few queries fill more of a block's rows
-// (one query x 16384 keys, 32 heads on 8: 48 us with a head a block, 24 with four;
-// 2 x 2048 queries 92 and 90). Up to 16, 112 of the 128 rows are in use at least.
-constexpr int kAttnPack = 16;
-int attention_pack(int64_t heads, int64_t kv_heads) {
-  int pack = 1;
-  for (int p = 2; p <= kAttnPack; ++p)
-    if (heads / kv_heads % p == 0) pack = p;
-  return pack;
 }
 
 // Runs of each block's keys. A block alone on a CU leaves its matrix unit idle
@@ -637,28 +264,22 @@ int lk_attention_prefill(const void* q, const void* k, const void* v, void* out,
   LK_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
              "attention workspace must be 16-byte aligned");
   const int n = static_cast<int>(sequences), pack = attention_pack(heads, kv_heads);
-  const AttnArgs a{static_cast<const uint16_t*>(q),
-                   static_cast<const uint16_t*>(k),
-                   static_cast<const uint16_t*>(v),
-                   static_cast<uint16_t*>(out),
-                   Sequences{cu_q, rows_q, rows_q / sequences, n},
-                   Sequences{cu_k, rows_k, rows_k / sequences, n},
-                   static_cast<int>(heads),
-                   static_cast<int>(heads / kv_heads),
-                   static_cast<int>(d_qk),
-                   static_cast<int>(d_v),
-                   pack,
-                   65536 / pack + 1,
-                   kAttnRows / pack,
-                   static_cast<int>(heads) / pack,
-                   q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride,
-                   v_head_stride,
-                   sequence_tiles(rows_q, sequences, kAttnRows / pack),
-                   attention_splits(rows_q, rows_k, sequences, heads, pack),
-                   need ? static_cast<float*>(workspace) : nullptr,
-                   scale == 0.f ? 1.f : scale_log2,
-                   scale == 0.f ? 0u : 0xFFFFFFFFu,
-                   scale < 0.f ? 0x80008000u : 0u};
+  AttnArgs a{};
+  a.q = static_cast<const uint16_t*>(q), a.out = static_cast<uint16_t*>(out);
+  a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.sq = Sequences{cu_q, rows_q, rows_q / sequences, n};
+  a.sk = Sequences{cu_k, rows_k, rows_k / sequences, n};
+  a.heads = static_cast<int>(heads), a.group = static_cast<int>(heads / kv_heads);
+  a.d_qk = static_cast<int>(d_qk), a.d_v = static_cast<int>(d_v);
+  a.pack = pack, a.inv_pack = 65536 / pack + 1, a.tokens = kAttnRows / pack;
+  a.packs = static_cast<int>(heads) / pack;
+  a.q_row = q_row_stride, a.q_head = q_head_stride, a.k_row = k_row_stride;
+  a.k_head = k_head_stride, a.v_row = v_row_stride, a.v_head = v_head_stride;
+  a.tiles = sequence_tiles(rows_q, sequences, a.tokens);
+  a.splits = attention_splits(rows_q, rows_k, sequences, heads, pack);
+  a.partial = need ? static_cast<float*>(workspace) : nullptr;
+  a.scale_log2 = scale == 0.f ? 1.f : scale_log2;
+  a.q_keep = scale == 0.f ? 0u : 0xFFFFFFFFu, a.q_flip = scale < 0.f ? 0x80008000u : 0u;
   const hipStream_t s = as_stream(stream);
   return dtype == LK_DTYPE_BF16 ? launch_attention<true>(a, s) : launch_attention<false>(a, s);
 }

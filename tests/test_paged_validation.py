@@ -173,11 +173,16 @@ def test_c_abi_refusals_come_before_any_launch(lib):
     append(rows=0)
 
     def attention(seqs=1, rows=8, h=4, hk=2, d=64, dv=64, pages=5, page_rows=16, width=3, stride=3, page=4096,
-                  row=128, scale=1.0, dt=2, p=16, qs=256):
+                  row=128, scale=1.0, dt=2, p=16, qs=256, ws=None, size=0):
         _lib.call("lk_attention_paged", p, p, p, p, p, p, None, seqs, rows, h, hk, d, dv, qs, d, pages, page_rows,
-                  width, stride, page, row, d, page, row, dv, scale, dt, None, 0, None)
+                  width, stride, page, row, d, page, row, dv, scale, dt, ws, size, None)
 
-    for args, match in (*shared, ({"hk": 3}, "multiple of the key heads"), ({"d": 200}, "d_qk"), ({"dv": 136}, "d_v"),
+    long = {"width": 100, "stride": 100}
+    need = lib.lk_attention_paged_workspace(8, 1, 1600, 4, 2, 64, 64)
+    assert need > 0 and lib.lk_attention_paged_workspace(8, 1, 64, 4, 2, 64, 64) == 0
+    for args, match in (*shared, ({**long}, "workspace too small"), ({**long, "ws": 16, "size": need - 1}, "workspace too"),
+                        ({**long, "size": need}, "workspace too"), ({**long, "ws": 8, "size": need}, "16-byte aligned"),
+                        ({"seqs": 65537, "rows": 65537}, "up to 65536"), ({"hk": 3}, "multiple of the key heads"), ({"d": 200}, "d_qk"), ({"dv": 136}, "d_v"),
                         ({"scale": float("nan")}, "finite"), ({"scale": 3e38}, "finite"), ({"qs": 12}, "multiples of 8"),
                         ({"row": 1 << 24}, "2\\^24"), ({"rows": (1 << 31) - 1, "h": 32768}, "too many query rows")):
         with pytest.raises(RuntimeError, match=match):
