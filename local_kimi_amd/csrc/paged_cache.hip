@@ -2,7 +2,7 @@
 // queries and keys, their write to the pages, copies of pages.
 
 #include <algorithm>
-#include <new>
+#include <cstdlib>
 
 #include "lk_common.hpp"
 #include "lk_paged.h"
@@ -28,204 +28,289 @@ struct HeadArgs {
   Sequences sq;
   int64_t table_rows;
   int heads, kv_heads, d, d_v, rotary, offset;
-  int slots, parts;  // of a token: heads of q, k (and v); blocks
+  int slots;  // rows of a token: heads of q, k (and v)
   float eps;
   int interleaved, positions_64, weight_dtype;
 };
 
-template <int DT>
-struct Four;  // four neighbouring values as stored
-template <>
-struct Four<LK_DTYPE_F32> {
-  float4 v;
-};
-template <>
-struct Four<LK_DTYPE_F16> {
-  uint2 v;
-};
-template <>
-struct Four<LK_DTYPE_BF16> {
-  uint2 v;
+// G neighbouring values as stored: 16 bytes, or 8 of the 16-bit types at G = 4.
+template <int DT, int G>
+struct Group {
+  static constexpr int kWords = G * (DT == LK_DTYPE_F32 ? 4 : 2) / 4;
+  uint32_t w[kWords];
 };
 
-template <int DT>
-__device__ inline void unpack4(const Four<DT>& x, float (&f)[4]) {
-  if constexpr (DT == LK_DTYPE_F32) {
-    f[0] = x.v.x, f[1] = x.v.y, f[2] = x.v.z, f[3] = x.v.w;
-  } else {
-    const uint32_t w[4] = {x.v.x & 0xFFFFu, x.v.x >> 16, x.v.y & 0xFFFFu, x.v.y >> 16};
+template <int DT, int G>
+__device__ inline void unpack(const Group<DT, G>& x, float (&f)[G]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = value_of<DT == LK_DTYPE_BF16>(w[i]);
+  for (int i = 0; i < G; ++i) {
+    if constexpr (DT == LK_DTYPE_F32) f[i] = __uint_as_float(x.w[i]);
+    else f[i] = value_of<DT == LK_DTYPE_BF16>(i % 2 ? x.w[i / 2] >> 16 : x.w[i / 2] & 0xFFFFu);
   }
 }
 
-template <int DT>
-__device__ inline Four<DT> pack4(const float (&f)[4]) {
-  if constexpr (DT == LK_DTYPE_F32)
-    return {make_float4(f[0], f[1], f[2], f[3])};
-  else
-    return {make_uint2(pack2<DT == LK_DTYPE_BF16>(f[0], f[1]), pack2<DT == LK_DTYPE_BF16>(f[2], f[3]))};
+template <int DT, int G>
+__device__ inline Group<DT, G> pack(const float (&f)[G]) {
+  Group<DT, G> x;
+#pragma unroll
+  for (int i = 0; i < Group<DT, G>::kWords; ++i) {
+    if constexpr (DT == LK_DTYPE_F32) x.w[i] = __float_as_uint(f[i]);
+    else x.w[i] = pack2<DT == LK_DTYPE_BF16>(f[2 * i], f[2 * i + 1]);
+  }
+  return x;
 }
 
-template <int DT>
-__device__ inline Four<DT> load4(const void* base, int64_t at) {
-  return *reinterpret_cast<const Four<DT>*>(
-      static_cast<const char*>(base) + at * static_cast<int64_t>(sizeof(Four<DT>) / 4));
-}
-template <int DT>
-__device__ inline void store4(void* base, int64_t at, const Four<DT>& x) {
-  *reinterpret_cast<Four<DT>*>(static_cast<char*>(base) +
-                               at * static_cast<int64_t>(sizeof(Four<DT>) / 4)) = x;
+// `at` counts values; groups start on their own size (strides and offsets are multiples of 8
+// values, bases of 16 bytes).
+template <int DT, int G>
+__device__ inline Group<DT, G> load_group(const void* base, int64_t at) {
+  constexpr int kWords = Group<DT, G>::kWords;
+  Group<DT, G> x;
+  const char* const p = static_cast<const char*>(base) + at * (DT == LK_DTYPE_F32 ? 4 : 2);
+  if constexpr (kWords == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x.w[0] = v.x, x.w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
+      x.w[i] = v.x, x.w[i + 1] = v.y, x.w[i + 2] = v.z, x.w[i + 3] = v.w;
+    }
+  }
+  return x;
 }
 
-__device__ inline void weights4(const void* base, int at, int dtype, float (&f)[4]) {
-  if (dtype == LK_DTYPE_F32) unpack4(load4<LK_DTYPE_F32>(base, at), f);
-  else if (dtype == LK_DTYPE_F16) unpack4(load4<LK_DTYPE_F16>(base, at), f);
-  else unpack4(load4<LK_DTYPE_BF16>(base, at), f);
+template <int DT, int G>
+__device__ inline void store_group(void* base, int64_t at, const Group<DT, G>& x) {
+  constexpr int kWords = Group<DT, G>::kWords;
+  char* const p = static_cast<char*>(base) + at * (DT == LK_DTYPE_F32 ? 4 : 2);
+  if constexpr (kWords == 2) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(x.w[0], x.w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4)
+      *reinterpret_cast<uint4*>(p + 4 * i) = make_uint4(x.w[i], x.w[i + 1], x.w[i + 2], x.w[i + 3]);
+  }
+}
+
+template <int G>
+__device__ inline void load_weights(const void* base, int at, int dtype, float (&f)[G]) {
+  if (dtype == LK_DTYPE_F32) unpack<LK_DTYPE_F32, G>(load_group<LK_DTYPE_F32, G>(base, at), f);
+  else if (dtype == LK_DTYPE_F16) unpack<LK_DTYPE_F16, G>(load_group<LK_DTYPE_F16, G>(base, at), f);
+  else unpack<LK_DTYPE_BF16, G>(load_group<LK_DTYPE_BF16, G>(base, at), f);
 }
 
 template <int LPR>
 __device__ inline float lanes_sum(float v) {
   v += dpp_f32<kQuadXor1>(v);
   v += dpp_f32<kQuadXor2>(v);
-  v += dpp_f32<kRowHalfMirror>(v);
+  if constexpr (LPR >= 8) v += dpp_f32<kRowHalfMirror>(v);
   if constexpr (LPR >= 16) v += dpp_f32<kRowMirror>(v);
   if constexpr (LPR >= 32) v += __shfl_xor(v, 16);
   return v;
 }
 
-// A row (a head of a token) is LPR lanes' (8, 16 or 32), a lane has two groups of
-// four of its values: the partners of a rotation, so that nothing is exchanged but
-// the sum of squares.
-template <int DT, int LPR, bool PAGED>
+// A row (a head of a token) is LPR lanes', a lane has two groups of G of its values: the
+// partners of a rotation, so that nothing is exchanged but the sum of squares. A
+// block takes 256 / LPR x R rows of the call's tokens x (heads of q, of k, of v), each LPR
+// lanes R that follow one another, mostly of one token: its angles are read once.
+// The block's rows are on their way while its threads find the places of its tokens.
+template <int DT, int G, int LPR, int R, bool PAGED>
 __global__ void __launch_bounds__(kHeadThreads) head_rope_kernel(HeadArgs a) {
-  constexpr int kRows = kHeadThreads / LPR;
-  const int64_t t = blockIdx.x / a.parts;
-  const int part = static_cast<int>(blockIdx.x % a.parts);
+  constexpr int kRows = kHeadThreads / LPR * R, kTokens = kRows / 2 + 2;
+  __shared__ int64_t k_place[PAGED ? kTokens : 1], v_place[PAGED ? kTokens : 1];  // -1: none
+  __shared__ int position[kTokens];                                             // -1: behind
+  const uint32_t slots = a.slots, first = blockIdx.x * static_cast<uint32_t>(kRows);
+  const uint32_t t0 = first / slots, slot0 = first - t0 * slots;
   const int lane = threadIdx.x % LPR;
-  int64_t pos = 0;
-  bool behind = false, place = false;
-  int64_t page = 0;
-  int in_page = 0;
-  if constexpr (PAGED) {
-    const int s = find_sequence(a.sq, t);
-    const RowRange rows = sequence_rows(a.sq, s);
-    behind = s >= a.sq.count || t < rows.begin || t >= rows.end;
-    if (!behind) {
-      pos = cached_length(a.table, s) - (rows.end - t);
-      if (pos >= 0) {
-        const int64_t block = pos / a.table.page_rows;
-        in_page = static_cast<int>(pos - block * a.table.page_rows);
-        page = a.table.pages_of[s * a.table.stride + block];
-        place = page >= 0 && page < a.table.pages;
-      }
-    }
-  } else {
-    pos = a.positions_64 ? static_cast<const int64_t*>(a.positions)[t]
-                         : static_cast<const int32_t*>(a.positions)[t];
-  }
-  pos = pos < 0 ? 0 : (pos >= a.table_rows ? a.table_rows - 1 : pos);
+  const uint32_t row0 = slot0 + threadIdx.x / LPR * R;  // from the block's first token's
+  const uint32_t tokens = static_cast<uint32_t>(a.sq.rows) - t0;
+  const uint32_t token0 = row0 / slots;
   // where this lane's two groups start, and whether they are turned
-  int ga, gb, angle = 0;
+  int ga, gb, angle;
   bool turned;
   if (a.interleaved) {
-    ga = 8 * lane, gb = ga + 4;
+    ga = 2 * G * lane, gb = ga + G;
     turned = ga >= a.offset && ga < a.offset + a.rotary;
     angle = (ga - a.offset) / 2;
   } else {
-    turned = 8 * lane < a.rotary;
-    ga = turned ? a.offset + 4 * lane : 8 * lane - a.rotary;
+    turned = 2 * G * lane < a.rotary;
+    ga = turned ? a.offset + G * lane : 2 * G * lane - a.rotary;
     if (!turned && ga >= a.offset) ga += a.rotary;
-    gb = turned ? ga + a.rotary / 2 : ga + 4;
-    angle = 4 * lane;
+    gb = turned ? ga + a.rotary / 2 : ga + G;
+    angle = G * lane;
   }
-  float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-  if (turned) {
-    const float* const row = a.cos_sin + pos * a.rotary + angle;
-    unpack4(load4<LK_DTYPE_F32>(row, 0), c);
-    unpack4(load4<LK_DTYPE_F32>(row, a.rotary / 2), s);
+  const bool in_head = 2 * G * lane < a.d, in_value = PAGED && 2 * G * lane < a.d_v;
+  Group<DT, G> xa[R], xb[R];
+  {
+    uint32_t token = token0, slot = row0 - token0 * slots;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t t = t0 + token;
+      const bool is_q = static_cast<int>(slot) < a.heads;
+      const bool is_v = PAGED && static_cast<int>(slot) >= a.heads + a.kv_heads;
+      if (token < tokens && (is_v ? in_value : in_head)) {
+        const int head = static_cast<int>(slot) - (is_q ? 0 : a.heads) - (is_v ? a.kv_heads : 0);
+        const void* const from = is_q ? a.q : (is_v ? a.v : a.k);
+        const int64_t at = is_q ? t * a.q_row + head * a.q_head
+                                : (is_v ? t * a.v_row + head * a.v_head : t * a.k_row + head * a.k_head);
+        xa[r] = load_group<DT, G>(from, at + (is_v ? 2 * G * lane : ga));
+        xb[r] = load_group<DT, G>(from, at + (is_v ? 2 * G * lane + G : gb));
+      }
+      if (++slot == slots) slot = 0, ++token;
+    }
   }
-  for (int slot = part * kRows + threadIdx.x / LPR; slot < a.slots; slot += a.parts * kRows) {
-    if (PAGED && slot >= a.heads + a.kv_heads) {  // v, as it is
-      const int head = slot - a.heads - a.kv_heads;
-      if (8 * lane < a.d_v && place) {
-        const int64_t from = t * a.v_row + head * a.v_head + 8 * lane;
-        const int64_t to = page * a.v_page + in_page * a.v_page_row + head * a.v_page_head + 8 * lane;
-        const Four<DT> x = load4<DT>(a.v, from), y = load4<DT>(a.v, from + 4);
-        store4(a.v_out, to, x);
-        store4(a.v_out, to + 4, y);
+  const uint32_t last = slot0 + kRows - 1 < tokens * slots ? (slot0 + kRows - 1) / slots : tokens - 1;
+  if constexpr (PAGED) {
+    int s = find_sequence(a.sq, t0);  // by whole waves, of the block's first token
+    for (uint32_t i = threadIdx.x; i <= last; i += kHeadThreads) {
+      const int64_t t = static_cast<int64_t>(t0) + i;
+      while (s < a.sq.count && sequence_rows(a.sq, s).end <= t) ++s;
+      const RowRange rows = sequence_rows(a.sq, s);
+      int pos = -1;
+      int64_t kp = -1, vp = -1;
+      if (s < a.sq.count && t >= rows.begin && t < rows.end) {
+        const int64_t at = cached_length(a.table, s) - (rows.end - t);
+        pos = at < 0 ? 0 : static_cast<int>(at);
+        if (at >= 0) {
+          const uint32_t block = static_cast<uint32_t>(pos) / static_cast<uint32_t>(a.table.page_rows);
+          const int64_t page = a.table.pages_of[s * a.table.stride + block];
+          const int64_t row = pos - static_cast<int64_t>(block) * a.table.page_rows;
+          if (page >= 0 && page < a.table.pages) {
+            kp = page * a.k_page + row * a.k_page_row;
+            vp = page * a.v_page + row * a.v_page_row;
+          }
+        }
       }
-      continue;
+      position[i] = pos, k_place[i] = kp, v_place[i] = vp;
     }
-    const bool is_q = slot < a.heads;
-    const int head = is_q ? slot : slot - a.heads;
-    const bool mine = 8 * lane < a.d;
-    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-    if (mine) {
-      const void* const from = is_q ? a.q : a.k;
-      const int64_t at = is_q ? t * a.q_row + head * a.q_head : t * a.k_row + head * a.k_head;
-      unpack4(load4<DT>(from, at + ga), x);
-      unpack4(load4<DT>(from, at + gb), y);
+  } else {
+    for (uint32_t i = threadIdx.x; i <= last; i += kHeadThreads) {
+      const int64_t t = static_cast<int64_t>(t0) + i;
+      int64_t pos = a.rotary == 0 ? 0
+                    : a.positions_64 ? static_cast<const int64_t*>(a.positions)[t]
+                                     : static_cast<const int32_t*>(a.positions)[t];
+      pos = pos < 0 ? 0 : (pos >= a.table_rows ? a.table_rows - 1 : pos);
+      position[i] = static_cast<int>(pos);
     }
-    const void* const weight = is_q ? a.q_weight : a.k_weight;
-    if (weight) {
-      float sq = 0.f;
+  }
+  __syncthreads();
+  float c[G], s[G];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sq = fmaf(x[i], x[i], sq);
+  for (int i = 0; i < G; ++i) c[i] = 1.f, s[i] = 0.f;
+  uint32_t token = token0, slot = row0 - token0 * slots;
+  int known = -1;  // the token that c and s are of
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sq = fmaf(y[i], y[i], sq);
-      const float r = 1.0f / sqrtf(lanes_sum<LPR>(sq) / static_cast<float>(a.d) + a.eps);
-      if (mine) {
-        float w[4], u[4];
-        weights4(weight, ga, a.weight_dtype, w);
-        weights4(weight, gb, a.weight_dtype, u);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = x[i] * r * w[i], y[i] = y[i] * r * u[i];
-      }
-    }
-    if (turned) {
-      if (a.interleaved) {
-        const float p[4] = {x[0], x[2], y[0], y[2]}, q[4] = {x[1], x[3], y[1], y[3]};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float* const to = i < 2 ? x + 2 * i : y + 2 * (i - 2);
-          to[0] = p[i] * c[i] - q[i] * s[i];
-          to[1] = q[i] * c[i] + p[i] * s[i];
+  for (int r = 0; r < R; ++r) {
+    if (token < tokens) {
+      const int64_t t = t0 + token;
+      const int pos = position[token];
+      const bool is_q = static_cast<int>(slot) < a.heads;
+      const bool is_v = PAGED && static_cast<int>(slot) >= a.heads + a.kv_heads;
+      const int head = static_cast<int>(slot) - (is_q ? 0 : a.heads) - (is_v ? a.kv_heads : 0);
+      if (is_v) {  // as it is
+        if (PAGED && in_value && v_place[token] >= 0) {
+          const int64_t to = v_place[token] + head * a.v_page_head + 2 * G * lane;
+          store_group<DT, G>(a.v_out, to, xa[r]);
+          store_group<DT, G>(a.v_out, to + G, xb[r]);
         }
       } else {
+        if (turned && known != static_cast<int>(token)) {
+          known = static_cast<int>(token);
+          const int row = pos < 0 ? 0 : (pos < a.table_rows ? pos : static_cast<int>(a.table_rows) - 1);
+          const float* const angles = a.cos_sin + static_cast<int64_t>(row) * a.rotary + angle;
+          unpack<LK_DTYPE_F32, G>(load_group<LK_DTYPE_F32, G>(angles, 0), c);
+          unpack<LK_DTYPE_F32, G>(load_group<LK_DTYPE_F32, G>(angles, a.rotary / 2), s);
+        }
+        const void* const weight = is_q ? a.q_weight : a.k_weight;
+        if (weight || a.rotary) {
+          float x[G], y[G];
+          if (in_head) {
+            unpack<DT, G>(xa[r], x);
+            unpack<DT, G>(xb[r], y);
+          } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = x[i], q = y[i];
-          x[i] = p * c[i] - q * s[i];
-          y[i] = q * c[i] + p * s[i];
+            for (int i = 0; i < G; ++i) x[i] = y[i] = 0.f;
+          }
+          if (weight) {
+            float sq = 0.f;
+#pragma unroll
+            for (int i = 0; i < G; ++i) sq = fmaf(x[i], x[i], sq);
+#pragma unroll
+            for (int i = 0; i < G; ++i) sq = fmaf(y[i], y[i], sq);
+            const float inv = 1.0f / sqrtf(lanes_sum<LPR>(sq) / static_cast<float>(a.d) + a.eps);
+            if (in_head) {
+              float w[G], u[G];
+              load_weights<G>(weight, ga, a.weight_dtype, w);
+              load_weights<G>(weight, gb, a.weight_dtype, u);
+#pragma unroll
+              for (int i = 0; i < G; ++i) x[i] = x[i] * inv * w[i], y[i] = y[i] * inv * u[i];
+            }
+          }
+          if (turned) {
+// interleaved: pair i lies at values 2 i and 2 i + 1 of the two groups
+            float p[G], q[G];
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+              const float first_of = a.interleaved ? (2 * i < G ? x[2 * i % G] : y[2 * i % G]) : x[i];
+              const float second = a.interleaved ? (2 * i < G ? x[2 * i % G + 1] : y[2 * i % G + 1]) : y[i];
+              p[i] = first_of * c[i] - second * s[i];
+              q[i] = second * c[i] + first_of * s[i];
+            }
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+              x[i] = a.interleaved ? (i % 2 ? q[i / 2] : p[i / 2]) : p[i];
+              y[i] = a.interleaved ? (i % 2 ? q[(i + G) / 2] : p[(i + G) / 2]) : q[i];
+            }
+          }
+          xa[r] = pack<DT, G>(x);
+          xb[r] = pack<DT, G>(y);
+        }
+        if (in_head && (!PAGED || is_q || k_place[token] >= 0)) {
+          if (PAGED && is_q && pos < 0) xa[r] = xb[r] = Group<DT, G>{};
+          int64_t to = (t * (is_q ? a.heads : a.kv_heads) + head) * a.d;
+          if (PAGED && !is_q) to = k_place[token] + head * a.k_page_head;
+          store_group<DT, G>(is_q ? a.q_out : a.k_out, to + ga, xa[r]);
+          store_group<DT, G>(is_q ? a.q_out : a.k_out, to + gb, xb[r]);
         }
       }
     }
-    if (PAGED && behind) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = y[i] = 0.f;
-    }
-    if (!mine || (PAGED && !is_q && !place)) continue;
-    void* const out = is_q ? a.q_out : a.k_out;
-    int64_t to = (t * (is_q ? a.heads : a.kv_heads) + head) * a.d;
-    if (PAGED && !is_q) to = page * a.k_page + in_page * a.k_page_row + head * a.k_page_head;
-    store4(out, to + ga, pack4<DT>(x));
-    store4(out, to + gb, pack4<DT>(y));
+    if (++slot == slots) slot = 0, ++token;
   }
 }
 
-template <int DT, bool PAGED>
-int launch_heads(HeadArgs& a, int64_t rows, const char* name, hipStream_t s) {
-  const int width = PAGED && a.d_v > a.d ? a.d_v : a.d;
-  const int lanes = width <= 64 ? 8 : (width <= 128 ? 16 : 32);
-  a.parts = (a.slots + kHeadThreads / lanes - 1) / (kHeadThreads / lanes);
-  const int64_t blocks = rows * a.parts;
-  LK_REQUIRE(grid_fits(blocks, kHeadThreads), "too many rows and heads for one call");
+constexpr int kHeadRun = 4;        // rows of a lane's in large calls
+constexpr int kHeadFill = 1024;    // blocks from which a call is large
+
+template <int DT, int G, bool PAGED>
+int launch_heads(const HeadArgs& a, const char* name, hipStream_t s) {
+  const int width = PAGED && a.d_v > a.d ? a.d_v : a.d, need = (width + 2 * G - 1) / (2 * G);
+  const int lanes = need <= 32 / G ? 32 / G : (need <= 64 / G ? 64 / G : 128 / G);
+  const int64_t rows = a.sq.rows * a.slots, one = kHeadThreads / lanes;  // of a block at R = 1
+  const bool large = rows >= one * kHeadRun * kHeadFill;
+  const int64_t blocks = (rows + one * (large ? kHeadRun : 1) - 1) / (one * (large ? kHeadRun : 1));
+  LK_REQUIRE(grid_fits(blocks, kHeadThreads) && rows < (int64_t{1} << 32),
+             "too many rows and heads for one call");
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (lanes == 8) head_rope_kernel<DT, 8, PAGED><<<grid, kHeadThreads, 0, s>>>(a);
-  else if (lanes == 16) head_rope_kernel<DT, 16, PAGED><<<grid, kHeadThreads, 0, s>>>(a);
-  else head_rope_kernel<DT, 32, PAGED><<<grid, kHeadThreads, 0, s>>>(a);
+#define LK_HEADS(L)                                                                        \
+  if (lanes == L) {                                                                        \
+    if (large) head_rope_kernel<DT, G, L, kHeadRun, PAGED><<<grid, kHeadThreads, 0, s>>>(a); \
+    else head_rope_kernel<DT, G, L, 1, PAGED><<<grid, kHeadThreads, 0, s>>>(a);            \
+  }
+  LK_HEADS(32 / G)
+  LK_HEADS(64 / G)
+  LK_HEADS(128 / G)
+#undef LK_HEADS
   return check_launch(name);
+}
+
+// Groups of eight 16-bit values (16 bytes) where the widths and the slice divide.
+template <int DT, bool PAGED>
+int launch_heads(const HeadArgs& a, const char* name, hipStream_t s) {
+  if constexpr (DT != LK_DTYPE_F32)
+    if ((a.d | a.rotary | a.offset | (PAGED ? a.d_v : 0)) % 16 == 0)
+      return launch_heads<DT, 8, PAGED>(a, name, s);
+  return launch_heads<DT, 4, PAGED>(a, name, s);
 }
 
 bool on_16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -284,23 +369,17 @@ int check_pairs(const int32_t* src, const int32_t* dst, int64_t pairs, int64_t p
     LK_REQUIRE(src[i] >= 0 && src[i] < pages && dst[i] >= 0 && dst[i] < pages,
                "pair %lld copies page %d to %d of a cache of %lld", (long long)i, src[i], dst[i],
                (long long)pages);
-  int32_t* const sorted = new (std::nothrow) int32_t[2 * pairs];
-  LK_REQUIRE(sorted, "no memory for the list of pages");
-  int32_t *const to = sorted, *const from = sorted + pairs;
-  int64_t n = 0;
-  for (int64_t i = 0; i < pairs; ++i)
-    if (src[i] != dst[i]) to[n] = dst[i], from[n++] = src[i];
-  std::sort(to, to + n);
-  std::sort(from, from + n);
+  uint8_t* const written = static_cast<uint8_t*>(std::calloc(pages / 8 + 1, 1));  // a bit a page
+  LK_REQUIRE(written, "no memory for the list of pages");
   int32_t twice = -1, both = -1;
-  for (int64_t i = 1; i < n; ++i)
-    if (to[i] == to[i - 1]) twice = to[i];
-  for (int64_t i = 0, j = 0; i < n && j < n;) {
-    if (to[i] == from[j]) both = to[i];
-    if (to[i] <= from[j]) ++i;
-    else ++j;
+  for (int64_t i = 0; i < pairs; ++i) {
+    if (src[i] == dst[i]) continue;
+    if (written[dst[i] / 8] >> dst[i] % 8 & 1) twice = dst[i];
+    written[dst[i] / 8] |= static_cast<uint8_t>(1u << dst[i] % 8);
   }
-  delete[] sorted;
+  for (int64_t i = 0; i < pairs; ++i)
+    if (src[i] != dst[i] && written[src[i] / 8] >> src[i] % 8 & 1) both = src[i];
+  std::free(written);
   LK_REQUIRE(twice < 0, "page %d is written twice", twice);
   LK_REQUIRE(both < 0, "page %d is both read and written", both);
   return LK_OK;
@@ -339,12 +418,13 @@ int lk_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
   a.heads = static_cast<int>(heads), a.kv_heads = static_cast<int>(kv_heads);
   a.d = static_cast<int>(d), a.rotary = static_cast<int>(rotary), a.offset = static_cast<int>(offset);
   a.slots = a.heads + a.kv_heads;
+  a.sq.rows = rows;
   a.eps = eps, a.interleaved = interleaved != 0, a.weight_dtype = weight_dtype;
   const hipStream_t s = as_stream(stream);
   constexpr const char* kName = "lk_qk_norm_rope";
-  if (dtype == LK_DTYPE_F32) return launch_heads<LK_DTYPE_F32, false>(a, rows, kName, s);
-  if (dtype == LK_DTYPE_F16) return launch_heads<LK_DTYPE_F16, false>(a, rows, kName, s);
-  return launch_heads<LK_DTYPE_BF16, false>(a, rows, kName, s);
+  if (dtype == LK_DTYPE_F32) return launch_heads<LK_DTYPE_F32, false>(a, kName, s);
+  if (dtype == LK_DTYPE_F16) return launch_heads<LK_DTYPE_F16, false>(a, kName, s);
+  return launch_heads<LK_DTYPE_BF16, false>(a, kName, s);
 }
 
 int lk_paged_append(const void* q, const void* k, const void* v, const void* q_weight,
@@ -398,8 +478,8 @@ int lk_paged_append(const void* q, const void* k, const void* v, const void* q_w
   a.eps = eps, a.interleaved = interleaved != 0, a.weight_dtype = weight_dtype;
   const hipStream_t s = as_stream(stream);
   constexpr const char* kName = "lk_paged_append";
-  if (dtype == LK_DTYPE_F16) return launch_heads<LK_DTYPE_F16, true>(a, rows, kName, s);
-  return launch_heads<LK_DTYPE_BF16, true>(a, rows, kName, s);
+  if (dtype == LK_DTYPE_F16) return launch_heads<LK_DTYPE_F16, true>(a, kName, s);
+  return launch_heads<LK_DTYPE_BF16, true>(a, kName, s);
 }
 
 int lk_copy_pages(void* const* tensors, const int64_t* page_strides, const int64_t* page_bytes,

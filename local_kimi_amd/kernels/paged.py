@@ -20,8 +20,8 @@ entries that name no page (-1, say) lead nowhere.
 
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
 from collections.abc import Sequence
 
 import torch
@@ -53,88 +53,113 @@ def rope_table(positions: int, rotary_dim: int, theta: float = 10000.0, *,
 # checks
 
 
-def _check_angles(cos_sin, d, rotary_offset, device) -> tuple[torch.Tensor, int]:
-    if cos_sin.ndim != 2 or cos_sin.shape[0] == 0:
+def _check_angles(cos_sin, d, rotary_offset, device) -> tuple[torch.Tensor, int, int]:
+    """The table as the kernels read it, its positions and its width."""
+    shape = cos_sin.shape
+    if len(shape) != 2 or shape[0] == 0:
         raise ValueError("cos_sin must have shape [positions, rotary_dim]")
-    if cos_sin.dtype != torch.float32:
+    if cos_sin.dtype is not torch.float32:
         raise TypeError(f"cos_sin must be float32, got {cos_sin.dtype}")
     if cos_sin.device != device:
         raise ValueError("cos_sin must be on the inputs' device")
-    rotary = cos_sin.shape[1]
+    rows, rotary = shape
     if rotary == 0 or rotary % 8 or rotary_offset % 8 or rotary_offset < 0 or rotary_offset + rotary > d:
         raise ValueError(f"the rotated slice [{rotary_offset}, {rotary_offset + rotary}) must lie "
                          f"within the head's {d} values, in multiples of 8")
-    return _aligned(cos_sin), rotary
+    return _aligned(cos_sin), rows, rotary
 
 
 def _check_weights(q_weight, k_weight, d, device, eps):
-    if (q_weight is None) != (k_weight is None):
-        raise ValueError("q_weight and k_weight must both be given, or neither")
     if not eps >= 0:
         raise ValueError("eps must be non-negative")
-    if q_weight is None:
+    if q_weight is None and k_weight is None:
         return None, None, 0
+    if q_weight is None or k_weight is None:
+        raise ValueError("q_weight and k_weight must both be given, or neither")
     for w in (q_weight, k_weight):
-        if w.ndim != 1 or w.shape[0] != d:
+        if w.shape != (d,):
             raise ValueError(f"the norm weights must have shape [{d}]")
         if w.device != device:
             raise ValueError("norm weights must be on the inputs' device")
-    if q_weight.dtype not in _DTYPE_CODES or k_weight.dtype != q_weight.dtype:
+    code = _DTYPE_CODES.get(q_weight.dtype)
+    if code is None or k_weight.dtype != q_weight.dtype:
         raise TypeError("the norm weights must share one dtype: float32, float16 or bfloat16")
-    return _aligned(q_weight), _aligned(k_weight), _DTYPE_CODES[q_weight.dtype]
+    return _aligned(q_weight), _aligned(k_weight), code
 
 
-def _check_heads(q, k, max_dim=HEAD_MAX_DIM):
-    if q.ndim != 4 or k.ndim != 4:
+def _check_heads(q, k):
+    """(batch, sequence, query heads, key heads, head_dim, dtype, device)."""
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4:
         raise ValueError("queries and keys must have shape [batch, sequence, heads, head_dim]")
-    if k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+    batch, rows, heads, d = qs
+    kbatch, krows, kv_heads, kd = ks
+    if kbatch != batch or krows != rows or kd != d:
         raise ValueError("queries and keys must agree in batch, sequence and head_dim")
-    if k.dtype != q.dtype:
+    dtype, device = q.dtype, q.device
+    if k.dtype is not dtype:
         raise TypeError("queries and keys must share one dtype")
-    if k.device != q.device:
+    if k.device != device:
         raise ValueError("queries and keys must share one device")
-    if q.shape[2] == 0 or k.shape[2] == 0 or q.shape[0] == 0:
+    if heads == 0 or kv_heads == 0 or batch == 0:
         raise ValueError("batch and heads must be nonzero")
-    d = q.shape[3]
-    if d == 0 or d % 8 or d > max_dim:
-        raise ValueError(f"head_dim must be a positive multiple of 8 up to {max_dim}, got {d}")
+    if d == 0 or d % 8 or d > HEAD_MAX_DIM:
+        raise ValueError(f"head_dim must be a positive multiple of 8 up to {HEAD_MAX_DIM}, got {d}")
+    return batch, rows, heads, kv_heads, d, dtype, device
 
 
 def _check_cache(k_pages, v_pages, page_table, lengths, kv_heads, d_qk, dtype, device):
-    """(d_v, the strides of both, the table, the lengths) of a cache that fits."""
-    if k_pages.ndim != 4 or v_pages.ndim != 4 or k_pages.shape[:3] != v_pages.shape[:3]:
+    """(d_v, table, lengths, [pages, rows, the table's width and stride, and the strides of
+    keys' and values' pages, rows and heads]) of a cache that fits."""
+    ks, vs = k_pages.shape, v_pages.shape
+    if len(ks) != 4 or len(vs) != 4 or ks[:3] != vs[:3]:
         raise ValueError("k_pages and v_pages must have shape [pages, rows, kv_heads, head_dim]")
-    pages, rows, heads, width = k_pages.shape
-    d_v = v_pages.shape[3]
+    pages, rows, heads, width = ks
+    d_v = vs[3]
     if heads != kv_heads or width != d_qk:
         raise ValueError(f"the cache holds {heads} heads of {width}, the call has {kv_heads} of {d_qk}")
     if rows == 0 or rows % PAGE_ROWS_STEP or rows > 65536:
         raise ValueError(f"a page must have a multiple of {PAGE_ROWS_STEP} rows up to 65536, got {rows}")
-    if k_pages.dtype != dtype or v_pages.dtype != dtype:
+    if k_pages.dtype is not dtype or v_pages.dtype is not dtype:
         raise TypeError("the cache must have the inputs' dtype")
-    if page_table.ndim != 2 or lengths.ndim != 1 or lengths.shape[0] != page_table.shape[0]:
+    ts, ls = page_table.shape, lengths.shape
+    if len(ts) != 2 or len(ls) != 1 or ls[0] != ts[0]:
         raise ValueError("page_table must have shape [sequences, pages a sequence], lengths "
                          "[sequences]")
-    if page_table.dtype != torch.int32 or lengths.dtype not in (torch.int32, torch.int64):
+    lengths_type = lengths.dtype
+    if page_table.dtype is not torch.int32 or lengths_type not in (torch.int32, torch.int64):
         raise TypeError("page_table must be int32, lengths int32 or int64")
-    if any(t.device != device for t in (k_pages, v_pages, page_table, lengths)):
+    if k_pages.device != device or v_pages.device != device or page_table.device != device \
+            or lengths.device != device:
         raise ValueError("the cache, its table and the lengths must be on the inputs' device")
-    strides = []
-    for t in (k_pages, v_pages):
-        if t.shape[3] > 1 and t.stride(3) != 1 or any(s % 8 or s < 0 for s in t.stride()[:3]) \
-                or t.data_ptr() % 16:
-            raise ValueError("cached heads must be dense, and pages, rows and heads on 16 bytes")
-        strides += t.stride()[:3]
-    n, width = page_table.shape
-    if width > 1 and page_table.stride(1) != 1 or n > 1 and page_table.stride(0) < width:
-        page_table = page_table.contiguous()
-    if lengths.dtype == torch.int64:  # beyond int32 is beyond every table
+    a, b, c, x = k_pages.stride()
+    e, f, g, y = v_pages.stride()
+    if x != 1 and width > 1 or y != 1 and d_v > 1 or (a | b | c | e | f | g) % 8 \
+            or min(a, b, c, e, f, g) < 0 or (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
+        raise ValueError("cached heads must be dense, and pages, rows and heads on 16 bytes")
+    n, width = ts
+    step, one = page_table.stride()
+    if width > 1 and one != 1 or n > 1 and step < width:
+        page_table, step = page_table.contiguous(), width
+    if lengths_type is torch.int64:  # beyond int32 is beyond every table
         lengths = lengths.clamp(0, 2 ** 31 - 1).to(torch.int32)
-    return d_v, strides, page_table, _w._c(lengths)
+    return (d_v, page_table, _w._c(lengths),
+            (pages, rows, width, step if n > 1 else width, a, b, c, e, f, g))
 
 
-def _table_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _heads_of(t: torch.Tensor, batch: int, rows: int) -> tuple[torch.Tensor, int, int]:
+    """``t`` [batch, rows, heads, d] as the kernels address it, copied where its layout is
+    another, and the strides of its rows and heads."""
+    a, b, c, one = t.stride()
+    if one == 1 and (batch == 1 or a == rows * b) and (b | c) % 8 == 0 and b < 1 << 24 \
+            and t.data_ptr() % 16 == 0:
+        return t, b, c
+    t = _rows(t)
+    return t, t.stride(1), t.stride(2)
+
+
+def _pointer(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 # ---------------------------------------------------------------------------
@@ -154,74 +179,70 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos_sin: torch.Tensor, positi
     8 up to 256, rotary_dim and rotary_offset multiples of 8. Strided inputs (slices of a
     fused projection) are read in place where rows and heads start on 16 bytes. Returns
     dense (q, k)."""
-    _check_heads(q, k)
-    code = _DTYPE_CODES.get(q.dtype)
+    batch, rows, heads, kv_heads, d, dtype, device = _check_heads(q, k)
+    code = _DTYPE_CODES.get(dtype)
     if code is None:
-        raise TypeError(f"queries and keys must be float32, float16 or bfloat16, got {q.dtype}")
-    batch, rows, heads, d = q.shape
-    cs, rotary = _check_angles(cos_sin, d, rotary_offset, q.device)
-    qw, kw, wcode = _check_weights(q_weight, k_weight, d, q.device, eps)
-    if tuple(positions.shape) != (batch, rows):
+        raise TypeError(f"queries and keys must be float32, float16 or bfloat16, got {dtype}")
+    cs, table_rows, rotary = _check_angles(cos_sin, d, rotary_offset, device)
+    qw, kw, wcode = _check_weights(q_weight, k_weight, d, device, eps)
+    if positions.shape != (batch, rows):
         raise ValueError("positions must have shape [batch, sequence]")
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-    if positions.device != q.device:
+    at_type = positions.dtype
+    if at_type is not torch.int32 and at_type is not torch.int64:
+        raise TypeError(f"positions must be int32 or int64, got {at_type}")
+    if positions.device != device:
         raise ValueError("positions must be on the inputs' device")
-    if q.device.type != "cuda":
+    if device.type != "cuda":
         raise ValueError("the HIP head kernels require CUDA tensors")
-    q_out = q.new_empty(q.shape)
-    k_out = k.new_empty(k.shape)
+    q_out = torch.empty((batch, rows, heads, d), dtype=dtype, device=device)
+    k_out = torch.empty((batch, rows, kv_heads, d), dtype=dtype, device=device)
     if rows:
-        qc, kc, at = _rows(q), _rows(k), _w._c(positions)
-        with _w._on(q.device):
-            _lib.call("lk_qk_norm_rope", qc.data_ptr(), kc.data_ptr(),
-                      None if qw is None else qw.data_ptr(), None if kw is None else kw.data_ptr(),
+        (q, q_row, q_head), (k, k_row, k_head) = _heads_of(q, batch, rows), _heads_of(k, batch, rows)
+        at = _w._c(positions)
+        with _w._on(device):
+            _lib.call("lk_qk_norm_rope", q.data_ptr(), k.data_ptr(), _pointer(qw), _pointer(kw),
                       cs.data_ptr(), at.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
-                      batch * rows, heads, k.shape[2], d, qc.stride(1), qc.stride(2), kc.stride(1),
-                      kc.stride(2), rotary, rotary_offset, int(interleaved), cs.shape[0],
-                      int(at.dtype == torch.int64), eps, code, wcode, _w._stream(q.device))
+                      batch * rows, heads, kv_heads, d, q_row, q_head, k_row, k_head, rotary,
+                      rotary_offset, bool(interleaved), table_rows, at_type is torch.int64, eps,
+                      code, wcode, _w._stream(device))
     return q_out, k_out
 
 
-def _append(q, k, v, k_pages, v_pages, page_table, lengths, cos_sin, q_weight, k_weight, eps,
-            cu_seqlens, rotary_offset, interleaved):
-    batch, rows, kv_heads, d = k.shape
-    if v.ndim != 4 or v.shape[:3] != k.shape[:3]:
+def _append(q, heads, k, v, batch, rows, kv_heads, d, dtype, device, k_pages, v_pages, page_table,
+            lengths, cos_sin, q_weight, k_weight, eps, cu_seqlens, rotary_offset, interleaved):
+    vs = v.shape
+    if len(vs) != 4 or vs[:3] != (batch, rows, kv_heads):
         raise ValueError("v must have shape [batch, sequence, kv_heads, d_v]")
-    code = _DTYPE_CODES.get(k.dtype)
-    if code not in (1, 2):
-        raise TypeError(f"cached values must be float16 or bfloat16, got {k.dtype}")
-    if v.dtype != k.dtype:
+    code = _DTYPE_CODES.get(dtype)
+    if code != 1 and code != 2:
+        raise TypeError(f"cached values must be float16 or bfloat16, got {dtype}")
+    if v.dtype is not dtype:
         raise TypeError("keys and values must share one dtype")
-    if v.device != k.device:
+    if v.device != device:
         raise ValueError("keys and values must share one device")
-    d_v, strides, table, lengths = _check_cache(k_pages, v_pages, page_table, lengths, kv_heads, d,
-                                                k.dtype, k.device)
-    if v.shape[3] != d_v or d_v == 0 or d_v % 8 or d_v > HEAD_MAX_DIM:
+    d_v, table, lengths, layout = _check_cache(k_pages, v_pages, page_table, lengths, kv_heads, d,
+                                               dtype, device)
+    if vs[3] != d_v or d_v == 0 or d_v % 8 or d_v > HEAD_MAX_DIM:
         raise ValueError(f"values must have the cache's width, a multiple of 8 up to {HEAD_MAX_DIM}")
-    cs, rotary = (None, 0) if cos_sin is None else _check_angles(cos_sin, d, rotary_offset, k.device)
-    qw, kw, wcode = _check_weights(q_weight, k_weight, d, k.device, eps)
-    offsets, count = _offsets(cu_seqlens, batch, k.device)
+    cs, table_rows, rotary = (None, 0, 0) if cos_sin is None else \
+        _check_angles(cos_sin, d, rotary_offset, device)
+    qw, kw, wcode = _check_weights(q_weight, k_weight, d, device, eps)
+    offsets, count = _offsets(cu_seqlens, batch, device)
     if count != table.shape[0]:
         raise ValueError(f"the table has {table.shape[0]} sequences, the call {count}")
-    if k.device.type != "cuda":
+    if device.type != "cuda":
         raise ValueError("the HIP cache kernels require CUDA tensors")
-    q_out = None if q is None else q.new_empty(q.shape)
+    q_out = torch.empty((batch, rows, heads, d), dtype=dtype, device=device) if heads else None
     if rows:
-        qc, kc, vc = None if q is None else _rows(q), _rows(k), _rows(v)
-        with _w._on(k.device):
-            _lib.call("lk_paged_append", None if q is None else qc.data_ptr(), kc.data_ptr(),
-                      vc.data_ptr(), None if qw is None else qw.data_ptr(),
-                      None if kw is None else kw.data_ptr(), None if cs is None else cs.data_ptr(),
-                      table.data_ptr(), lengths.data_ptr(),
-                      None if offsets is None else offsets.data_ptr(),
-                      None if q is None else q_out.data_ptr(), k_pages.data_ptr(),
-                      v_pages.data_ptr(), count, batch * rows, 0 if q is None else q.shape[2],
-                      kv_heads, d, d_v, 0 if q is None else qc.stride(1),
-                      0 if q is None else qc.stride(2), kc.stride(1), kc.stride(2), vc.stride(1),
-                      vc.stride(2), k_pages.shape[0], k_pages.shape[1], table.shape[1],
-                      _table_stride(table), *strides, rotary, rotary_offset, int(interleaved),
-                      0 if cs is None else cs.shape[0], eps, code, wcode, _w._stream(k.device))
+        q, q_row, q_head = _heads_of(q, batch, rows) if heads else (None, 0, 0)
+        (k, k_row, k_head), (v, v_row, v_head) = _heads_of(k, batch, rows), _heads_of(v, batch, rows)
+        with _w._on(device):
+            _lib.call("lk_paged_append", _pointer(q), k.data_ptr(), v.data_ptr(), _pointer(qw),
+                      _pointer(kw), _pointer(cs), table.data_ptr(), lengths.data_ptr(),
+                      _pointer(offsets), _pointer(q_out), k_pages.data_ptr(), v_pages.data_ptr(),
+                      count, batch * rows, heads, kv_heads, d, d_v, q_row, q_head, k_row, k_head,
+                      v_row, v_head, *layout, rotary, rotary_offset, bool(interleaved), table_rows,
+                      eps, code, wcode, _w._stream(device))
     return q_out
 
 
@@ -241,9 +262,10 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pag
     below 0; rows behind the last sequence write nothing and return zeros. Two sequences'
     new tokens must not share a page: copy a forked sequence's last page first
     (``PagedCache.extend`` does)."""
-    _check_heads(q, k)
-    return _append(q, k, v, k_pages, v_pages, page_table, lengths, cos_sin, q_weight, k_weight, eps,
-                   cu_seqlens, rotary_offset, interleaved)
+    batch, rows, heads, kv_heads, d, dtype, device = _check_heads(q, k)
+    return _append(q, heads, k, v, batch, rows, kv_heads, d, dtype, device, k_pages, v_pages,
+                   page_table, lengths, cos_sin, q_weight, k_weight, eps, cu_seqlens, rotary_offset,
+                   interleaved)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -251,9 +273,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                  cu_seqlens: torch.Tensor | None = None) -> None:
     """``k`` [B, S, H_kv, d_qk] and ``v`` [B, S, H_kv, d_v] written to the cache as they
     are (layers without rotation); places as in ``qk_norm_rope_append``."""
-    _check_heads(k, k)
-    _append(None, k, v, k_pages, v_pages, page_table, lengths, None, None, None, 0.0, cu_seqlens, 0,
-            False)
+    batch, rows, kv_heads, _, d, dtype, device = _check_heads(k, k)
+    _append(None, 0, k, v, batch, rows, kv_heads, d, dtype, device, k_pages, v_pages, page_table,
+            lengths, None, None, None, 0.0, cu_seqlens, 0, False)
 
 
 # ---------------------------------------------------------------------------
@@ -277,45 +299,44 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Returns [B, S, H, d_v] in q's dtype. ``scale`` defaults to d_qk ** -0.5. Scores and
     sums are fp32; the probabilities are rounded to the inputs' dtype for their product
     with the values."""
-    code = _DTYPE_CODES.get(q.dtype)
-    if code not in (1, 2):
-        raise TypeError(f"attention inputs must be float16 or bfloat16, got {q.dtype}")
-    if q.ndim != 4:
+    dtype, shape, device = q.dtype, q.shape, q.device
+    code = _DTYPE_CODES.get(dtype)
+    if code != 1 and code != 2:
+        raise TypeError(f"attention inputs must be float16 or bfloat16, got {dtype}")
+    if len(shape) != 4:
         raise ValueError("q must have shape [batch, sequence, heads, head_dim]")
-    batch, rows, heads, d_qk = q.shape
+    batch, rows, heads, d_qk = shape
     kv_heads = k_pages.shape[2] if k_pages.ndim == 4 else 0
     if batch == 0 or heads == 0 or kv_heads == 0 or heads % kv_heads:
         raise ValueError("the query heads must be a positive multiple of the key heads")
     if d_qk == 0 or d_qk % 8 or d_qk > ATTENTION_MAX_QK_DIM:
         raise ValueError(f"d_qk must be a positive multiple of 8 up to {ATTENTION_MAX_QK_DIM}, "
                          f"got {d_qk}")
-    d_v, strides, table, lengths = _check_cache(k_pages, v_pages, page_table, lengths, kv_heads,
-                                                d_qk, q.dtype, q.device)
+    d_v, table, lengths, layout = _check_cache(k_pages, v_pages, page_table, lengths, kv_heads, d_qk,
+                                               dtype, device)
     if d_v == 0 or d_v % 8 or d_v > ATTENTION_MAX_V_DIM:
         raise ValueError(f"d_v must be a positive multiple of 8 up to {ATTENTION_MAX_V_DIM}, "
                          f"got {d_v}")
-    offsets, count = _offsets(cu_seqlens, batch, q.device)
+    offsets, count = _offsets(cu_seqlens, batch, device)
     if count != table.shape[0]:
         raise ValueError(f"the table has {table.shape[0]} sequences, the call {count}")
     scale = d_qk ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
-    if q.device.type != "cuda":
+    if device.type != "cuda":
         raise ValueError("the HIP attention kernel requires CUDA tensors")
-    out = q.new_empty((batch, rows, heads, d_v))
+    out = torch.empty((batch, rows, heads, d_v), dtype=dtype, device=device)
     if rows == 0:
         return out
-    qc = _rows(q)
-    need = _lib.query("lk_attention_paged_workspace", batch * rows, count,
-                      table.shape[1] * k_pages.shape[1], heads, kv_heads, d_qk, d_v)
-    ws = _w.workspace(need, q.device) if need else None
-    with _w._on(q.device):
-        _lib.call("lk_attention_paged", qc.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                  out.data_ptr(), table.data_ptr(), lengths.data_ptr(),
-                  None if offsets is None else offsets.data_ptr(), count, batch * rows, heads,
-                  kv_heads, d_qk, d_v, qc.stride(1), qc.stride(2), k_pages.shape[0],
-                  k_pages.shape[1], table.shape[1], _table_stride(table), *strides, scale, code,
-                  None if ws is None else ws.data_ptr(), need, _w._stream(q.device))
+    q, q_row, q_head = _heads_of(q, batch, rows)
+    need = _lib.query("lk_attention_paged_workspace", batch * rows, count, layout[1] * layout[2],
+                      heads, kv_heads, d_qk, d_v)
+    ws = _w.workspace(need, device) if need else None
+    with _w._on(device):
+        _lib.call("lk_attention_paged", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                  out.data_ptr(), table.data_ptr(), lengths.data_ptr(), _pointer(offsets), count,
+                  batch * rows, heads, kv_heads, d_qk, d_v, q_row, q_head, *layout, scale, code,
+                  _pointer(ws), need, _w._stream(device))
     return out
 
 
@@ -323,57 +344,77 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 # copies
 
 
-def _page_bytes(t: torch.Tensor) -> int:
-    """Bytes of one page where a page is dense in some order of its dimensions."""
-    dims = sorted((s, n) for s, n in zip(t.stride()[1:], t.shape[1:]) if n != 1)
-    size = 1
-    for s, n in dims:
-        if s != size:
+def _page_layout(shape, strides, size: int) -> tuple[int, int]:
+    """Bytes from a page to the next and of one page, which is dense in some order of its
+    dimensions."""
+    page = 1
+    for step, n in sorted(x for x in zip(strides[1:], shape[1:]) if x[1] != 1):
+        if step != page:
             raise ValueError("the pages of a copied tensor must be dense")
-        size *= n
-    return size * t.element_size()
+        page *= n
+    page, step = page * size, strides[0] * size
+    if shape[0] > 1 and step < page:
+        raise ValueError("the pages of a copied tensor must not overlap")
+    step = max(step, page)
+    if page % 16 or step % 16:
+        raise ValueError("pages must be multiples of 16 bytes, on 16 bytes")
+    return step, page
 
 
-def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
+def _page_list(pages: Sequence[int] | torch.Tensor, what: str) -> array:
+    if isinstance(pages, torch.Tensor):
+        if pages.device.type != "cpu" or pages.ndim != 1 or pages.is_floating_point():
+            raise ValueError(f"{what} must be a list of integers on the host")
+        pages = pages.tolist()
+    try:
+        return array("i", pages)
+    except OverflowError:
+        raise ValueError(f"{what} has page numbers beyond 2^31 - 1") from None
+
+
+def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int] | torch.Tensor,
+               dst: Sequence[int] | torch.Tensor) -> None:
     """Page ``src[i]`` to page ``dst[i]`` (dimension 0) of every tensor: all layers' caches,
     in one launch per 192 pairs of 64 tensors.
 
     ``src`` and ``dst`` are sequences of integers or integer tensors on the host; a page is
     written once at most, and is no other pair's source (ValueError). A captured graph
     keeps the lists it was captured with. Pages must be dense, in any order of their
-    dimensions, and multiples of 16 bytes."""
-    tensors = list(tensors)
-    a, b = (torch.as_tensor(x, dtype=torch.int64, device="cpu") if len(x) else
-            torch.empty(0, dtype=torch.int64) for x in (src, dst))
-    if a.ndim != 1 or a.shape != b.shape:
+    dimensions, and multiples of 16 bytes; the tensors must not overlap each other."""
+    a, b = _page_list(src, "src"), _page_list(dst, "dst")
+    if len(a) != len(b):
         raise ValueError("src and dst must be lists of one length")
     if not tensors:
         return
-    pages, device = tensors[0].shape[0], tensors[0].device
-    sizes = []
+    pages, device = (tensors[0].shape or (0,))[0], tensors[0].device
+    known: dict = {}  # most tensors are laid out alike
+    pointers, steps, sizes = [], [], []
     for t in tensors:
-        if t.ndim < 2 or t.shape[0] != pages:
-            raise ValueError("copied tensors must have shape [pages, ...], all of one number of pages")
+        key = t.shape, t.stride(), t.dtype
+        layout = known.get(key)
+        if layout is None:
+            if len(key[0]) < 2 or key[0][0] != pages:
+                raise ValueError("copied tensors must have shape [pages, ...], all of one number of "
+                                 "pages")
+            layout = known[key] = _page_layout(key[0], key[1], t.element_size())
         if t.device != device:
             raise ValueError("copied tensors must share one device")
-        sizes.append(_page_bytes(t))
-        if sizes[-1] % 16 or t.data_ptr() % 16 or t.stride(0) * t.element_size() % 16:
+        pointers.append(t.data_ptr())
+        if pointers[-1] % 16:
             raise ValueError("pages must be multiples of 16 bytes, on 16 bytes")
-        if pages > 1 and t.stride(0) * t.element_size() < sizes[-1]:
-            raise ValueError("the pages of a copied tensor must not overlap")
+        steps.append(layout[0])
+        sizes.append(layout[1])
     if device.type != "cuda":
         raise ValueError("the HIP copy requires CUDA tensors")
-    n = a.shape[0]
-    if n == 0:
+    if not a:
         return
-    if bool(((a < 0) | (a >= pages) | (b < 0) | (b >= pages)).any()):
+    if min(a) < 0 or max(a) >= pages or min(b) < 0 or max(b) >= pages:
         raise ValueError(f"page numbers must be in 0 .. {pages - 1}")
-    a, b = a.to(torch.int32), b.to(torch.int32)
-    count = len(tensors)
-    pointers = (ctypes.c_void_p * count)(*(t.data_ptr() for t in tensors))
-    steps = (ctypes.c_int64 * count)(*(max(t.stride(0) * t.element_size(), s)
-                                       for t, s in zip(tensors, sizes)))
-    bytes_ = (ctypes.c_int64 * count)(*sizes)
+    moved = [x for x in zip(a, b) if x[0] != x[1]]
+    written = {y for _, y in moved}
+    if len(written) != len(moved) or not written.isdisjoint(x for x, _ in moved):
+        raise ValueError("a page may be written once, and not be another pair's source")
+    tables = [array("q", x) for x in (pointers, steps, sizes)]
     with _w._on(device):
-        _lib.call("lk_copy_pages", pointers, steps, bytes_, count, a.data_ptr(), b.data_ptr(), n,
-                  pages, _w._stream(device))
+        _lib.call("lk_copy_pages", *(t.buffer_info()[0] for t in tables), len(pointers),
+                  a.buffer_info()[0], b.buffer_info()[0], len(a), pages, _w._stream(device))

@@ -397,6 +397,19 @@ def test_copies_of_pages(rng, pairs):
     assert all(bool((t == -i).all()) for i, t in enumerate(many))
 
 
+def test_copies_that_depend_on_each_other_are_refused():
+    from local_kimi_amd.kernels import copy_pages
+
+    t = torch.randn((8, 16, 2, 8), device=DEV)
+    want = t.clone()
+    for src, dst, match in (([0, 1], [2, 2], "written once"), ([0, 2], [2, 3], "source"), ([0, 1], [1, 0], "source"),
+                            ([8], [1], "0 .. 7"), ([0], [-1], "0 .. 7"), (torch.tensor([1]), [9], "0 .. 7")):
+        with pytest.raises(ValueError, match=match):
+            copy_pages([t], src, dst)
+    copy_pages([t], [3, 4], [3, 4])
+    assert torch.equal(t, want)
+
+
 def test_a_conversation_through_the_cache(rng):
     """Prompts, single tokens, a fork that diverges, a freed sequence, a compaction: at
     each step every layer's attention equals dense attention over the same tokens, and the

@@ -124,9 +124,13 @@ def test_copy_refusals():
                         (([t[..., :4]], [0], [1]), "dense"), (([t[:, :, 0]], [0], [1]), "dense"),
                         (([torch.zeros(6, 3)], [0], [1]), "16 bytes"),
                         (([torch.zeros(1, 16, 2, 8).expand(6, 16, 2, 8)], [0], [1]), "must not overlap"),
-                        (([torch.zeros(6)], [0], [1]), "shape")):
+                        (([torch.zeros(6)], [0], [1]), "shape"), (([torch.tensor(0.0)], [0], [1]), "shape"),
+                        (([t], [2 ** 31], [1]), "beyond"), (([t], torch.zeros(1), [1]), "integers on the host"),
+                        (([t], torch.zeros(1, 1, dtype=torch.int64), [1]), "integers on the host")):
         with pytest.raises(ValueError, match=match):
             copy_pages(*args)
+    with pytest.raises(TypeError):
+        copy_pages([t], [0.5], [1])
 
 
 @pytest.fixture(scope="module")
