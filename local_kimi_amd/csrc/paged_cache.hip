@@ -80,16 +80,20 @@ __device__ inline Group<DT, G> load_group(const void* base, int64_t at) {
   return x;
 }
 
-template <int DT, int G>
+// STREAM: past the caches, for outputs that are larger than them.
+template <int DT, int G, bool STREAM>
 __device__ inline void store_group(void* base, int64_t at, const Group<DT, G>& x) {
-  constexpr int kWords = Group<DT, G>::kWords;
+  constexpr int kWords = Group<DT, G>::kWords, kStep = kWords == 2 ? 2 : 4;
+  typedef uint32_t words_t __attribute__((ext_vector_type(kStep)));
   char* const p = static_cast<char*>(base) + at * (DT == LK_DTYPE_F32 ? 4 : 2);
-  if constexpr (kWords == 2) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(x.w[0], x.w[1]);
-  } else {
 #pragma unroll
-    for (int i = 0; i < kWords; i += 4)
-      *reinterpret_cast<uint4*>(p + 4 * i) = make_uint4(x.w[i], x.w[i + 1], x.w[i + 2], x.w[i + 3]);
+  for (int i = 0; i < kWords; i += kStep) {
+    words_t v;
+#pragma unroll
+    for (int k = 0; k < kStep; ++k) v[k] = x.w[i + k];
+    words_t* const to = reinterpret_cast<words_t*>(p + 4 * i);
+    if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+    else *to = v;
   }
 }
 
@@ -211,8 +215,8 @@ __global__ void __launch_bounds__(kHeadThreads) head_rope_kernel(HeadArgs a) {
       if (is_v) {  // as it is
         if (PAGED && in_value && v_place[token] >= 0) {
           const int64_t to = v_place[token] + head * a.v_page_head + 2 * G * lane;
-          store_group<DT, G>(a.v_out, to, xa[r]);
-          store_group<DT, G>(a.v_out, to + G, xb[r]);
+          store_group<DT, G, (R > 1)>(a.v_out, to, xa[r]);
+          store_group<DT, G, (R > 1)>(a.v_out, to + G, xb[r]);
         }
       } else {
         if (turned && known != static_cast<int>(token)) {
@@ -270,8 +274,8 @@ __global__ void __launch_bounds__(kHeadThreads) head_rope_kernel(HeadArgs a) {
           if (PAGED && is_q && pos < 0) xa[r] = xb[r] = Group<DT, G>{};
           int64_t to = (t * (is_q ? a.heads : a.kv_heads) + head) * a.d;
           if (PAGED && !is_q) to = k_place[token] + head * a.k_page_head;
-          store_group<DT, G>(is_q ? a.q_out : a.k_out, to + ga, xa[r]);
-          store_group<DT, G>(is_q ? a.q_out : a.k_out, to + gb, xb[r]);
+          store_group<DT, G, (R > 1)>(is_q ? a.q_out : a.k_out, to + ga, xa[r]);
+          store_group<DT, G, (R > 1)>(is_q ? a.q_out : a.k_out, to + gb, xb[r]);
         }
       }
     }
@@ -279,8 +283,13 @@ __global__ void __launch_bounds__(kHeadThreads) head_rope_kernel(HeadArgs a) {
   }
 }
 
-constexpr int kHeadRun = 4;        // rows of a lane's in large calls
-constexpr int kHeadFill = 1024;    // blocks from which a call is large
+// Large calls (kHeadFill blocks at least) take two rows a lane group, and their
+// outputs go past the caches. Both by 8192 tokens x 40 heads of 128 / 4096 packed tokens x
+// 96 heads of 192 and 128: 36 / 55 us (4.8 and 4.9 TB/s; a large copy moves 5.1), with
+// ordinary stores 37 / 63, of those with three rows 36 / 70, four 37 / 63, eight 40 / 64; loads
+// past the caches 45 / 71 (a row's two halves share its lines).
+constexpr int kHeadRun = 2;
+constexpr int kHeadFill = 512;
 
 template <int DT, int G, bool PAGED>
 int launch_heads(const HeadArgs& a, const char* name, hipStream_t s) {
