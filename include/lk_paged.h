@@ -92,9 +92,9 @@ LK_API int lk_paged_append(const void* q, const void* k, const void* v, const vo
  * is 0). Calls that overlap in time take one each. */
 LK_API int64_t lk_attention_paged_workspace(int64_t rows, int64_t sequences, int64_t capacity,
                                             int64_t heads, int64_t kv_heads, int64_t d_qk,
-                                            int64_t d_v);
+                                            int64_t d_v, int packed);
 
-/* capacity above is table_width * page_rows */
+/* above: capacity is table_width * page_rows, packed whether cu is given */
 LK_API int lk_attention_paged(const void* q, const void* k_pages, const void* v_pages, void* out,
                               const int32_t* page_table, const int32_t* lengths,
                               const int32_t* cu, int64_t sequences, int64_t rows, int64_t heads,

@@ -104,7 +104,7 @@ QUERIES: dict[str, list] = {
     "lk_mxfp4_moe_forward_workspace": [_I64, _I64, _I64, _I64, _I64],
     "lk_kda_prefill_workspace": [_I64, _I64, _I64, _I64, _I64],
     "lk_attention_prefill_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I64],
-    "lk_attention_paged_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I64],
+    "lk_attention_paged_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I],
 }
 
 _lock = threading.Lock()

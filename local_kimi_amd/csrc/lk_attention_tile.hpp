@@ -110,9 +110,9 @@ __device__ inline uint2 lds_read_transposed(const uint16_t* p) {
 // (one query x 16384 keys, 32 heads on 8: 48 us with a head a block, 24 with four;
 // 2 x 2048 queries 92 and 90). Up to 16, 112 of the 128 rows are in use at least.
 constexpr int kAttnPack = 16;
-inline int attention_pack(int64_t heads, int64_t kv_heads) {
+inline int attention_pack(int64_t heads, int64_t kv_heads, int most = kAttnPack) {
   int pack = 1;
-  for (int p = 2; p <= kAttnPack; ++p)
+  for (int p = 2; p <= most; ++p)
     if (heads / kv_heads % p == 0) pack = p;
   return pack;
 }

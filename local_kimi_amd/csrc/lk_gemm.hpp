@@ -215,11 +215,19 @@ __device__ inline u32x4_t uniform_rsrc(u32x4_t r) {
   for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
   return r;
 }
+// ONCE: a hint that nothing else will read the bytes (past the caches).
+template <bool ONCE = false>
 __device__ inline void lds_direct16(u32x4_t rs, uint32_t lds, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_rsrc(rs)),
-                 "s"(__builtin_amdgcn_readfirstlane(soff))
-               : "memory");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
+                 ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_rsrc(rs)),
+                   "s"(__builtin_amdgcn_readfirstlane(soff))
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_rsrc(rs)),
+                   "s"(__builtin_amdgcn_readfirstlane(soff))
+                 : "memory");
 }
 __device__ inline void lds_direct4(u32x4_t rs, uint32_t lds, uint32_t voff, uint32_t soff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, %3 offen lds"

@@ -1,16 +1,18 @@
 // Causal softmax attention of new rows on a paged cache, for gfx950.
 
+#include <algorithm>
+
 #include "lk_attention_tile.hpp"
 #include "lk_paged.h"
 
 namespace lk {
 namespace {
 
-constexpr int kFewRows = 16;  // queries x heads of a block for single tokens
-constexpr int kFill = 512;    // blocks that fill the chip: two a CU
+constexpr int kFewRows = 16;  // queries x heads of a block for single tokens, or twice that
+constexpr int kPagedPack = 32;
+constexpr int kFill = 1024;   // runs that a call's keys are dealt in: four a CU
 constexpr int kMinRun = 256;  // keys of a run, at the least
-constexpr int kJoinRows = 2;  // of a wave of the join
-constexpr int kJoinBlockRows = kAttnWaves * kJoinRows;
+constexpr int kJoinFew = 4, kJoinMany = 16;  // rows of a block of the join
 constexpr int64_t kMaxSequences = 65536;
 
 struct PagedArgs : AttnShape {
@@ -18,8 +20,22 @@ struct PagedArgs : AttnShape {
   Sequences sq;
   PageTable table;
   int64_t k_page, k_row, k_head, v_page, v_row, v_head;
-  float* partial;  // sums of rows whose keys are in runs; null where none can be
-  uint32_t units;  // of kFewRows rows that it holds
+  // where keys can be in runs, else null: their number and tiles, then their rows' sums
+  struct SplitTiles* split;
+  float* partial;
+  uint32_t units;  // of kFewRows rows that `partial` holds
+};
+
+// A tile whose keys are in runs, for the join.
+struct SplitTile {
+  int64_t row;  // its first
+  int rows, pack, runs, units;
+  uint32_t unit;
+  int unused;
+};
+struct SplitTiles {
+  int count;
+  SplitTile tile[kFill];
 };
 
 // Rows in pages: a wave stages 16 rows of each tile, which lie in one page. The
@@ -80,6 +96,8 @@ struct PagedKeys {
   }
 
   // Rows without a page, and those behind the sequence's last, read as zeros.
+  // ONCE: past the caches, for keys that no other block reads.
+  template <bool ONCE = false>
   __device__ __forceinline__ void fetch(int64_t at, int buf) {
     const int k0 = static_cast<int>(at);
     if (k0 >= first + kAttnKeys * kWave) find_pages(k0);
@@ -94,10 +112,10 @@ struct PagedKeys {
     const uint32_t base = lds + buf * kAttnKeys * (DQ + DV) * 2;
 #pragma unroll
     for (int i = 0; i < kKLoads; ++i)
-      lds_direct16(rk, base + (wave * kKLoads + i) * kWave * 16, koff[i], 0);
+      lds_direct16<ONCE>(rk, base + (wave * kKLoads + i) * kWave * 16, koff[i], 0);
 #pragma unroll
     for (int i = 0; i < kVLoads; ++i)
-      lds_direct16(rv, base + kAttnKeys * DQ * 2 + (wave * kVLoads + i) * kWave * 16, voff[i], 0);
+      lds_direct16<ONCE>(rv, base + kAttnKeys * DQ * 2 + (wave * kVLoads + i) * kWave * 16, voff[i], 0);
   }
 
   __device__ __forceinline__ const uint16_t* value_row(int64_t key) const {
@@ -131,13 +149,13 @@ __device__ inline f32x4_t mfma16_half(uint2 a, uint2 b, f32x4_t c) {
   }
 }
 
-// Up to 16 rows (queries x heads of one key head) against the run's keys: the four
+// Up to 16 GROUPS rows (queries x heads of one key head) against the run's keys: the four
 // waves take 16 keys of each 64, every wave with a maximum and sums of its own and no
 // barrier between them, since a wave reads what it staged itself; at the end the four
 // are joined. S^T = K Q^T and O^T += V^T P^T as in attend_rows, on 16 x 16 tiles: a
 // lane holds four scores of a row, which rounded are its part of the next
 // product's operand.
-template <bool BF16, int DQ, int DV>
+template <bool BF16, int DQ, int DV, int GROUPS>
 __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& b,
                                            PagedKeys<DQ, DV>& keys_of, uint16_t* stage,
                                            float* part) {
@@ -149,29 +167,36 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int n = lane & 15, g = lane >> 4;
   const int lq = static_cast<int>(b.q.end - b.q.begin), lk = static_cast<int>(b.lk);
-  const int token = n * a.inv_pack >> 16;
+  int token[GROUPS];
+#pragma unroll
+  for (int j = 0; j < GROUPS; ++j) token[j] = (kFewRows * j + n) * a.inv_pack >> 16;
   const int ahead = lk - lq;  // query i sees the keys up to ahead + i
   const int per = ((lk + b.splits - 1) / b.splits + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
   const int64_t from64 = static_cast<int64_t>(b.split) * per;
   const int from = from64 < lk ? static_cast<int>(from64) : lk;
   const int to = lk - from < per ? lk : from + per;
-  u32x4_t qf[kQSteps];
-  {
-    const int64_t head = b.pack * a.pack + n - token * a.pack;
+  u32x4_t qf[GROUPS][kQSteps];
+#pragma unroll
+  for (int j = 0; j < GROUPS; ++j) {
+    const int64_t head = b.pack * a.pack + kFewRows * j + n - token[j] * a.pack;
     const uint16_t* const qp =
-        a.q + (b.q.begin + (token < lq ? token : lq - 1)) * a.q_row + head * a.q_head;
+        a.q + (b.q.begin + (token[j] < lq ? token[j] : lq - 1)) * a.q_row + head * a.q_head;
 #pragma unroll
     for (int i = 0; i < kQSteps; ++i) {
       const int d = 32 * i + 8 * g;
       const u32x4_t z = {0u, 0u, 0u, 0u};
-      qf[i] = d < a.d_qk ? *reinterpret_cast<const u32x4_t*>(qp + d) : z;
-      qf[i] = (qf[i] & a.q_keep) ^ a.q_flip;
+      qf[j][i] = d < a.d_qk ? *reinterpret_cast<const u32x4_t*>(qp + d) : z;
+      qf[j][i] = (qf[j][i] & a.q_keep) ^ a.q_flip;
     }
   }
-  f32x4_t o[kVTiles];
+  f32x4_t o[GROUPS][kVTiles];
+  float top[GROUPS], sum[GROUPS];
 #pragma unroll
-  for (int t = 0; t < kVTiles; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float top = -INFINITY, sum = 0.f;
+  for (int j = 0; j < GROUPS; ++j) {
+    top[j] = -INFINITY, sum[j] = 0.f;
+#pragma unroll
+    for (int t = 0; t < kVTiles; ++t) o[j][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
   // where this lane reads in its wave's rows of a tile: K row n, chunks 4 i + g; V row
   // 4 g + lane % 16 / 4, columns 16 t + 4 (lane % 4)
   constexpr int kAddrs = kKChunks % 16 == 0 ? 4 : 2;
@@ -187,61 +212,29 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
                8 * ((col / 8) ^ value_swizzle<kVChunks>(row)) + col % 8;
   }
   bool bad = false;
-  if (from < to) keys_of.fetch(from, 0);
-  if (from + kAttnKeys < to) keys_of.fetch(from + kAttnKeys, 1);
+  if (from < to) keys_of.template fetch<true>(from, 0);
+  if (from + kAttnKeys < to) keys_of.template fetch<true>(from + kAttnKeys, 1);
   int buf = 0;
   for (int k0 = from; k0 < to; k0 += kAttnKeys, buf ^= 1) {
     if (k0 + kAttnKeys < to) wait_vmcnt<kLoads>();
     else wait_vmcnt<0>();
     const uint16_t* const tile = stage + buf * kStage;
     const int p0 = k0 + kPageStep * wave;
+    u32x4_t kf[kQSteps];
+    uint2 vf[kVTiles];
+#pragma unroll
+    for (int i = 0; i < kQSteps; ++i)
+      kf[i] = *reinterpret_cast<const u32x4_t*>(tile + kaddr[i % kAddrs] + 32 * kAddrs * (i / kAddrs));
+#pragma unroll
+    for (int t = 0; t < kVTiles; ++t) vf[t] = lds_read_transposed(tile + vaddr[t]);
+    // once it is all in registers, its place may be filled again
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (k0 + 2 * kAttnKeys < to) keys_of.template fetch<true>(k0 + 2 * kAttnKeys, buf);
     if (p0 < lk) {
-      u32x4_t kf[kQSteps];
-#pragma unroll
-      for (int i = 0; i < kQSteps; ++i)
-        kf[i] = *reinterpret_cast<const u32x4_t*>(tile + kaddr[i % kAddrs] +
-                                                  32 * kAddrs * (i / kAddrs));
-      uint2 vf[kVTiles];
-#pragma unroll
-      for (int t = 0; t < kVTiles; ++t) vf[t] = lds_read_transposed(tile + vaddr[t]);
-      f32x4_t s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < kQSteps; ++i) s = mfma16<BF16>(kf[i], qf[i], s);
       const bool edge = p0 + kPageStep - 1 > ahead;  // not seen by every query
       if (edge) {
-        const int seen = token + ahead + 1 - p0 - 4 * g;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = i < seen ? s[i] : -INFINITY;
-      }
-      float most = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-      {
-        auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(most), __float_as_uint(most),
-                                                  false, false);
-        most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-        x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false,
-                                             false);
-        most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.scale_log2;
-      }
-      constexpr float kSlack = 8.f;  // as in attend_rows
-      const bool moves = most > top + kSlack;
-      if (__any(moves)) {
-        const float next = moves ? most : top;
-        const float fade = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
-        top = next;
-        sum *= fade;
-#pragma unroll
-        for (int t = 0; t < kVTiles; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[t][i] *= fade;
-      }
-      const float base = kLift - (top == -INFINITY ? 0.f : top);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, base));
-      sum += (s[0] + s[1]) + (s[2] + s[3]);
-      const uint2 p = make_uint2(pack2<BF16>(s[0], s[1]), pack2<BF16>(s[2], s[3]));
-#pragma unroll
-      for (int t = 0; t < kVTiles; ++t) {
-        if (edge) {
+        for (int t = 0; t < kVTiles; ++t) {
           const u32x4_t both = {vf[t].x, vf[t].y, 0u, 0u};
           if (__builtin_expect(__any(any_nonfinite<BF16>(both)), 0)) {
             bad = true;
@@ -249,97 +242,140 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
             vf[t] = make_uint2(kept[0], kept[1]);
           }
         }
-        o[t] = mfma16_half<BF16>(vf[t], p, o[t]);
+      }
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) {
+        f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kQSteps; ++i) s = mfma16<BF16>(kf[i], qf[j][i], s);
+        if (edge) {
+          const int seen = token[j] + ahead + 1 - p0 - 4 * g;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[i] = i < seen ? s[i] : -INFINITY;
+        }
+        float most = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        {
+          auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(most), __float_as_uint(most),
+                                                    false, false);
+          most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+          x = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false,
+                                               false);
+          most = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.scale_log2;
+        }
+        constexpr float kSlack = 8.f;  // as in attend_rows
+        const bool moves = most > top[j] + kSlack;
+        if (__any(moves)) {
+          const float next = moves ? most : top[j];
+          const float fade = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[j] - next);
+          top[j] = next;
+          sum[j] *= fade;
+#pragma unroll
+          for (int t = 0; t < kVTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[j][t][i] *= fade;
+        }
+        const float base = kLift - (top[j] == -INFINITY ? 0.f : top[j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale_log2, base));
+        sum[j] += (s[0] + s[1]) + (s[2] + s[3]);
+        const uint2 p = make_uint2(pack2<BF16>(s[0], s[1]), pack2<BF16>(s[2], s[3]));
+#pragma unroll
+        for (int t = 0; t < kVTiles; ++t) o[j][t] = mfma16_half<BF16>(vf[t], p, o[j][t]);
       }
     }
-    // what was read above is in registers: its place may be filled again
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (k0 + 2 * kAttnKeys < to) keys_of.fetch(k0 + 2 * kAttnKeys, buf);
   }
-  {
-    auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-    sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-    x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-    sum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+#pragma unroll
+  for (int j = 0; j < GROUPS; ++j) {
+    auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[j]), __float_as_uint(sum[j]), false, false);
+    sum[j] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    x = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[j]), __float_as_uint(sum[j]), false, false);
+    sum[j] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
   }
   if (__builtin_expect(bad, 0)) {
     // the infinities and NaNs left out above, for the queries that see them
+    int left = a.d_v - 4 * g;
 #pragma unroll 1
     for (int key = from; key < to; ++key) {
       const int p0 = key / kPageStep * kPageStep;
       if ((p0 - from) / kPageStep % kAttnWaves != wave || p0 + kPageStep - 1 <= ahead) continue;
       const uint16_t* const row = keys_of.value_row(key);
       if (!row) continue;
+      asm volatile("" : "+v"(left));  // (as in attend_rows)
 #pragma unroll
-      for (int t = 0; t < kVTiles; ++t)
+      for (int j = 0; j < GROUPS; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int d = 16 * t + 4 * g + i;
-          const float x = d < a.d_v && key <= token + ahead ? value_of<BF16>(row[d]) : 0.f;
-          if (!(fabsf(x) < INFINITY)) o[t][i] += x;
-        }
+        for (int t = 0; t < kVTiles; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = 16 * t + i;
+            const float x = d < left && key <= token[j] + ahead ? value_of<BF16>(row[4 * g + d]) : 0.f;
+            if (!(fabsf(x) < INFINITY)) o[j][t][i] += x;
+          }
     }
   }
-  // the four waves' sums, through LDS
+  // the four waves' sums, through LDS, 16 rows at a time
   constexpr int kRow = DV + 4, kCols = DV / 16;
   float* const sums = reinterpret_cast<float*>(stage);
   float* const tops = sums + kAttnWaves * kFewRows * kRow;  // then the sums of p
   static_assert(kAttnWaves * kFewRows * (kRow + 2) * 4 <= 2 * kStage * 2, "sums in LDS");
-  __syncthreads();
 #pragma unroll
-  for (int t = 0; t < kVTiles; ++t)
-    *reinterpret_cast<f32x4_t*>(sums + (wave * kFewRows + n) * kRow + 16 * t + 4 * g) = o[t];
-  if (g == 0) {
-    tops[wave * kFewRows + n] = top;
-    tops[(kAttnWaves + wave) * kFewRows + n] = sum;
-  }
-  __syncthreads();
-  const int row = tid / 16, col = tid % 16 * kCols, query = row * a.inv_pack >> 16;
-  if (query >= lq) return;
-  float all = -INFINITY, total = 0.f, acc[kCols] = {};
+  for (int j = 0; j < GROUPS; ++j) {
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kAttnWaves; ++w) all = fmaxf(all, tops[w * kFewRows + row]);
+    for (int t = 0; t < kVTiles; ++t)
+      *reinterpret_cast<f32x4_t*>(sums + (wave * kFewRows + n) * kRow + 16 * t + 4 * g) = o[j][t];
+    if (g == 0) {
+      tops[wave * kFewRows + n] = top[j];
+      tops[(kAttnWaves + wave) * kFewRows + n] = sum[j];
+    }
+    __syncthreads();
+    const int mine = tid / 16, col = tid % 16 * kCols;
+    const int row = kFewRows * j + mine, query = row * a.inv_pack >> 16;
+    if (query >= lq) continue;
+    float all = -INFINITY, total = 0.f, acc[kCols] = {};
 #pragma unroll
-  for (int w = 0; w < kAttnWaves; ++w) {
-    const float t = tops[w * kFewRows + row];
-    const float weight = t == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t - all);
-    total = fmaf(weight, tops[(kAttnWaves + w) * kFewRows + row], total);
-    const float* const from_wave = sums + (w * kFewRows + row) * kRow + col;
-    // (a wave that saw nothing has zeros; one whose weight is 0 may have none)
+    for (int w = 0; w < kAttnWaves; ++w) all = fmaxf(all, tops[w * kFewRows + mine]);
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] = fmaf(weight, from_wave[c], acc[c]);
-  }
-  if (part) {
+    for (int w = 0; w < kAttnWaves; ++w) {
+      const float t = tops[w * kFewRows + mine];
+      const float weight = t == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t - all);
+      total = fmaf(weight, tops[(kAttnWaves + w) * kFewRows + mine], total);
+      const float* const from_wave = sums + (w * kFewRows + mine) * kRow + col;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) acc[c] = fmaf(weight, from_wave[c], acc[c]);
+    }
+    if (part) {
+#pragma unroll
+      for (int c = 0; c < kCols; c += 4)
+        *reinterpret_cast<float4*>(part + row * DV + col + c) =
+            make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+      if (col == 0) {
+        part[kFewRows * GROUPS * DV + row] = all;
+        part[kFewRows * GROUPS * (DV + 1) + row] = total;
+      }
+      continue;
+    }
+    const float inv = total == 0.f ? 0.f : 1.0f / total;
+    const int64_t head = b.pack * a.pack + row - query * a.pack;
+    uint16_t* const out = a.out + ((b.q.begin + query) * a.heads + head) * a.d_v + col;
 #pragma unroll
     for (int c = 0; c < kCols; c += 4)
-      *reinterpret_cast<float4*>(part + row * DV + col + c) =
-          make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-    if (col == 0) {
-      part[kFewRows * DV + row] = all;
-      part[kFewRows * (DV + 1) + row] = total;
-    }
-    return;
+      if (col + c < a.d_v)
+        *reinterpret_cast<uint2*>(out + c) =
+            make_uint2(pack2<BF16>(within_type<BF16>(acc[c] * inv), within_type<BF16>(acc[c + 1] * inv)),
+                       pack2<BF16>(within_type<BF16>(acc[c + 2] * inv),
+                                   within_type<BF16>(acc[c + 3] * inv)));
   }
-  const float inv = total == 0.f ? 0.f : 1.0f / total;
-  const int64_t head = b.pack * a.pack + row - query * a.pack;
-  uint16_t* const out = a.out + ((b.q.begin + query) * a.heads + head) * a.d_v + col;
-#pragma unroll
-  for (int c = 0; c < kCols; c += 4)
-    if (col + c < a.d_v)
-      *reinterpret_cast<uint2*>(out + c) =
-          make_uint2(pack2<BF16>(within_type<BF16>(acc[c] * inv), within_type<BF16>(acc[c + 1] * inv)),
-                     pack2<BF16>(within_type<BF16>(acc[c + 2] * inv),
-                                 within_type<BF16>(acc[c + 3] * inv)));
 }
 
 // ---------------------------------------------------------------------------
 // Who does what. A call's work is found on the device, from the lengths as they are:
-// sequence s has ceil(n / tokens) tiles of rows (one of up to 16 rows where its new
-// tokens fit) for each pack of heads, and every tile's keys are taken in runs of about
+// sequence s has ceil(n / tokens) tiles of rows (one of up to 16 or 32 rows where its
+// new tokens fit) for each pack of heads, and every tile's keys are taken in runs of about
 // L keys, L = what two blocks a CU would have each if all keys of the call were dealt
 // evenly, kMinRun at the least. Each block finds its tile and run by a scan over the
-// sequences, 64 at a time. The rows behind the last sequence are one sequence more,
-// without keys.
+// sequences, 64 at a time; the rows behind the last sequence come after all. A
+// tile in runs is noted for the join.
 //
 // Blocks: tiles <= packs (rows / tokens + sequences + 1), and runs beyond one a tile <=
 // kFill, since L kFill >= all keys. A tile in runs has more than L keys, so there are up to
@@ -348,27 +384,27 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
 struct PagedTile {
   RowRange q;
   int sequence, lk, tiles, runs;
-  bool few;
+  int units;  // of kFewRows rows that a tile has: 1, 2 or those of kAttnRows
 };
+constexpr int kManyUnits = kAttnRows / kFewRows;
 
 __device__ inline PagedTile paged_tiles(const PagedArgs& a, int s) {
   PagedTile t{};
   t.sequence = s;
-  if (s > a.sq.count) return t;
+  if (s >= a.sq.count) return t;
   t.q = sequence_rows(a.sq, s);
   const int lq = static_cast<int>(t.q.end - t.q.begin);
   if (lq == 0) return t;
-  t.lk = s < a.sq.count ? static_cast<int>(cached_length(a.table, s)) : 0;
-  t.few = lq * a.pack <= kFewRows && s < a.sq.count;
-  t.tiles = t.few ? 1 : (lq + a.tokens - 1) / a.tokens;
+  t.lk = static_cast<int>(cached_length(a.table, s));
+  const int64_t rows = static_cast<int64_t>(lq) * a.pack;
+  t.units = rows <= kFewRows ? 1 : (rows <= 2 * kFewRows ? 2 : kManyUnits);
+  t.tiles = t.units < kManyUnits ? 1 : (lq + a.tokens - 1) / a.tokens;
   t.runs = 1;
   return t;
 }
 
-// Keys that a row of the sequence sees, in the mean. (Here and in find_item nothing is
-// contracted: the join has to come to the very numbers that the blocks came to.)
+// Keys that a row of the sequence sees, in the mean.
 __device__ inline float keys_seen(const PagedTile& t) {
-#pragma clang fp contract(off)
   const float lk = static_cast<float>(t.lk), lq = static_cast<float>(t.q.end - t.q.begin);
   return fmaxf(lk - 0.5f * lq, 0.5f * lk);
 }
@@ -388,73 +424,89 @@ __device__ inline int from_lane(int v, int lane) { return __builtin_amdgcn_readl
 struct PagedItem {
   AttnBlock b;
   int sequence;  // -1: there is none of this number
-  bool few;
+  int units;     // of kFewRows rows: 1, 2 or kManyUnits
   uint32_t unit;  // where its sums go (its runs' begin), in units of kFewRows rows
+  uint32_t tile;  // its number among the tiles in runs
 };
 
-// Tile and run of block `number`, or (JOIN) the tile in runs of this number.
-template <bool JOIN>
+// Tile and run of block `number`. A number beyond the last gets the count of tiles in
+// runs in `tile`.
 __device__ inline PagedItem find_item(const PagedArgs& a, uint32_t number) {
-#pragma clang fp contract(off)
   const int lane = static_cast<int>(threadIdx.x & (kWave - 1));
   PagedItem item{};
   item.sequence = -1;
-  const int entries = a.sq.count + 1;
+  const int count = a.sq.count;
   PagedTile own = paged_tiles(a, lane);
-  float run = 0.f;
+  float run = 0.f, share = 0.f;
   if (a.partial) {
     float work = keys_seen(own) * static_cast<float>(own.tiles) * static_cast<float>(a.packs);
-    for (int s = kWave; s < entries; s += kWave) {
+    for (int s = kWave; s < count; s += kWave) {
       const PagedTile t = paged_tiles(a, s + lane);
       work += keys_seen(t) * static_cast<float>(t.tiles) * static_cast<float>(a.packs);
     }
     work = over_wave(work, [](float x, float y) { return x + y; });
     // (a 1024th more than the mean, for what rounding can lose)
-    run = fmaxf(static_cast<float>(kMinRun), ceilf(work * (1.0009765625f / kFill)));
+    share = work * (1.0009765625f / kFill);
+    run = fmaxf(static_cast<float>(kMinRun), ceilf(share));
   }
-  uint32_t before = 0, units_before = 0;
-  for (int s0 = 0; s0 < entries; s0 += kWave) {
+  const float many = fmaxf(static_cast<float>(kMinRun), ceilf(2.f * share));
+  const uint32_t packs = a.packs;
+  uint32_t before = 0, units_before = 0, split_before = 0;
+  for (int s0 = 0; s0 < count; s0 += kWave) {
     if (s0 > 0) own = paged_tiles(a, s0 + lane);
     if (a.partial && own.tiles > 0) {
-      const float n = ceilf(keys_seen(own) / run);
+      const float n = ceilf(keys_seen(own) / (own.units < kManyUnits ? run : many));
       own.runs = n < 2.f ? 1 : (n > static_cast<float>(kWave) ? kWave : static_cast<int>(n));
     }
-    const uint32_t rows = static_cast<uint32_t>(own.tiles * a.packs);
-    const uint32_t split = own.runs > 1 ? rows : 0u;
-    const uint32_t units = split * own.runs * (own.few ? 1u : kAttnRows / kFewRows);
-    const uint32_t mine = JOIN ? split : rows * own.runs;
-    const uint32_t upto = scan_wave(mine), units_upto = scan_wave(units);
+    const uint32_t tiles = static_cast<uint32_t>(own.tiles) * packs, mine = tiles * own.runs;
+    const uint32_t split = own.runs > 1 ? tiles : 0u;
+    const uint32_t units = split * own.runs * own.units;
+    const uint32_t upto = scan_wave(mine), units_upto = scan_wave(units), split_upto = scan_wave(split);
     const uint64_t hit = __ballot(number < before + upto);
     if (hit) {
       const int at = __builtin_ctzll(hit);
       const uint32_t local = number - (before + from_lane(upto - mine, at));
-      const int tiles = from_lane(own.tiles, at), runs = from_lane(own.runs, at);
-      item.few = from_lane(own.few, at) != 0;
+      const int of = from_lane(own.tiles, at), runs = from_lane(own.runs, at);
+      item.units = from_lane(own.units, at);
       item.sequence = s0 + at;
-      const uint32_t packs = a.packs;
-      const uint32_t step = JOIN ? local / packs : local / packs / runs;
       item.b.pack = __builtin_amdgcn_readfirstlane(local % packs);
-      item.b.split = JOIN ? 0 : __builtin_amdgcn_readfirstlane(local / packs % runs);
+      item.b.split = __builtin_amdgcn_readfirstlane(local / packs % runs);
       item.b.splits = runs;
       // later tiles see more keys, and are begun first
-      const int tile = tiles - 1 - static_cast<int>(__builtin_amdgcn_readfirstlane(step));
+      const int tile = of - 1 - static_cast<int>(__builtin_amdgcn_readfirstlane(local / packs / runs));
+      const uint32_t index = tile * packs + item.b.pack, step = item.units;
+      const bool few = step < kManyUnits;
       item.unit = units_before + from_lane(units_upto - units, at) +
-                  ((tile * packs + item.b.pack) * runs + item.b.split) *
-                      (item.few ? 1u : kAttnRows / kFewRows);
-      item.b.q = sequence_rows(a.sq, item.sequence);
+                  (index * runs + item.b.split) * step;
+      item.tile = split_before + from_lane(split_upto - split, at) + index;
+      item.b.q.begin = from_lane(static_cast<int>(own.q.begin), at);  // (rows are below 2^31)
+      item.b.q.end = from_lane(static_cast<int>(own.q.end), at);
       item.b.lk = from_lane(own.lk, at);
       const int64_t lq = item.b.q.end - item.b.q.begin;
-      item.b.q0 = item.few ? 0 : static_cast<int64_t>(tile) * a.tokens;
-      item.b.last = item.few || lq - item.b.q0 < a.tokens ? lq : item.b.q0 + a.tokens;
+      item.b.q0 = few ? 0 : static_cast<int64_t>(tile) * a.tokens;
+      item.b.last = few || lq - item.b.q0 < a.tokens ? lq : item.b.q0 + a.tokens;
       // (offsets that are not in order can ask for more than there is)
-      const uint32_t need = (JOIN ? runs : 1) * (item.few ? 1u : kAttnRows / kFewRows);
-      if (tile < 0 || tile >= tiles ||
-          (runs > 1 && (item.unit >= a.units || a.units - item.unit < need)))
+      if (tile < 0 || tile >= of ||
+          (runs > 1 && (item.unit >= a.units || a.units - item.unit < step || item.tile >= kFill)))
         item.sequence = -1;
       return item;
     }
     before += from_lane(upto, kWave - 1);
     units_before += from_lane(units_upto, kWave - 1);
+    split_before += from_lane(split_upto, kWave - 1);
+  }
+  item.tile = split_before;
+  // the rows behind the last sequence
+  const uint32_t local = number - before, tile = local / packs;
+  const RowRange rows = sequence_rows(a.sq, count);
+  const int64_t lq = rows.end - rows.begin, q0 = static_cast<int64_t>(tile) * a.tokens;
+  if (q0 < lq) {
+    item.sequence = count;
+    item.b.pack = __builtin_amdgcn_readfirstlane(local % packs);
+    item.b.splits = 1;
+    item.b.q = rows;
+    item.b.q0 = q0;
+    item.b.last = lq - q0 < a.tokens ? lq : q0 + a.tokens;
   }
   return item;
 }
@@ -468,13 +520,23 @@ template <bool BF16, int DQ, int DV>
 __global__ void __launch_bounds__(kAttnThreads, 2) paged_attend_kernel(PagedArgs a) {
   constexpr int kVTiles = DV / 32;
   __shared__ alignas(16) uint16_t stage[2 * kAttnKeys * (DQ + DV)];
-  const PagedItem item = find_item<false>(a, blockIdx.x);
+  const PagedItem item = find_item(a, blockIdx.x);
+  // (the last number is beyond all tiles)
+  if (a.partial && blockIdx.x == gridDim.x - 1 && threadIdx.x == 0)
+    a.split->count = item.tile < kFill ? static_cast<int>(item.tile) : kFill;
   if (item.sequence < 0) return;
   const AttnBlock& b = item.b;
-  float* const part = b.splits > 1 ? sums_of<DV>(a, item.unit) : nullptr;
-  if (item.few) {
+  float* part = nullptr;
+  if (b.splits > 1) {
+    part = sums_of<DV>(a, item.unit);
+    if (b.split == 0 && threadIdx.x == 0)
+      a.split->tile[item.tile] = SplitTile{b.q.begin + b.q0, static_cast<int>(b.last - b.q0) * a.pack,
+                                           b.pack, b.splits, item.units, item.unit, 0};
+  }
+  if (item.units < kManyUnits && item.sequence < a.sq.count) {
     PagedKeys<DQ, DV> keys(a, b, item.sequence, stage);
-    attend_few<BF16, DQ, DV>(a, b, keys, stage, part);
+    if (item.units == 2) attend_few<BF16, DQ, DV, 2>(a, b, keys, stage, part);
+    else attend_few<BF16, DQ, DV, 1>(a, b, keys, stage, part);
     return;
   }
   f32x16_t o[kVTiles];
@@ -491,91 +553,149 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attend_kernel(PagedArgs
   else store_rows<BF16, DQ, DV>(a, b, stage, o, sum);
 }
 
-// The runs of a tile joined, as in attention.hip: a wave takes two rows, a lane a run's
-// maxima and sums of them, then columns.
+// Output row of a tile from its joined sums: a lane two columns (one of 64).
 template <bool BF16, int DV>
-__global__ void __launch_bounds__(kAttnThreads) paged_join_kernel(PagedArgs a, int parts) {
-  constexpr int kCols = DV / 64, kRuns = 4;
-  const PagedItem item = find_item<true>(a, blockIdx.x / parts);
-  if (item.sequence < 0) return;
-  const AttnBlock& b = item.b;
-  const int lane = threadIdx.x & (kWave - 1), runs = b.splits;
-  const int row0 = (blockIdx.x % parts * kAttnWaves + threadIdx.x / kWave) * kJoinRows;
-  const int most = item.few ? kFewRows : kAttnRows, size = most * (DV + 2);
-  auto exists = [&](int row) {
-    return row < most && b.q0 + (row * a.inv_pack >> 16) < b.last && (row * a.inv_pack >> 16) < a.tokens;
-  };
-  if (!exists(row0)) return;
-  const float* const sums = sums_of<DV>(a, item.unit);
+__device__ inline void store_joined(const PagedArgs& a, const SplitTile& tile, int row,
+                                    const float (&acc)[DV / 64], float total) {
+  const int lane = threadIdx.x & (kWave - 1), token = row * a.inv_pack >> 16;
+  const float inv = total == 0.f ? 0.f : 1.0f / total;
+  uint16_t* const out = a.out + ((tile.row + token) * a.heads + tile.pack * a.pack + row -
+                                 token * a.pack) * static_cast<int64_t>(a.d_v);
+  if constexpr (DV == 128) {
+    if (2 * lane < a.d_v)
+      *reinterpret_cast<uint32_t*>(out + 2 * lane) =
+          pack2<BF16>(within_type<BF16>(acc[0] * inv), within_type<BF16>(acc[1] * inv));
+  } else {
+    if (lane < a.d_v)
+      out[lane] = static_cast<uint16_t>(pack2<BF16>(within_type<BF16>(acc[0] * inv), 0.f));
+  }
+}
+
+// ROWS rows of a tile in runs: weights 2^(top - largest top) of the runs, a lane each,
+// then the runs from `begin` on, RUNS of them, a lane its columns. Rows that do not
+// exist read the first's. Every load is on its way before the first is used.
+template <int DV, int ROWS, int RUNS>
+__device__ inline void join_rows(const float* sums, int size, int most, int runs, int begin,
+                                 const int (&row)[ROWS], float (&acc)[ROWS][DV / 64],
+                                 float (&total)[ROWS]) {
+  constexpr int kCols = DV / 64;
+  const int lane = threadIdx.x & (kWave - 1);
   const float* const tops = sums + (lane < runs ? lane : 0) * size + most * DV;
-  float weight[kJoinRows], total[kJoinRows], acc[kJoinRows][kCols] = {};
-  int from[kJoinRows];  // rows that do not exist read the first
+  float weight[ROWS], x[ROWS][RUNS][kCols];
 #pragma unroll
-  for (int r = 0; r < kJoinRows; ++r) {
-    from[r] = exists(row0 + r) ? row0 + r : row0;
-    weight[r] = lane < runs ? tops[from[r]] : -INFINITY;
-    total[r] = lane < runs ? tops[most + from[r]] : 0.f;
+  for (int r = 0; r < ROWS; ++r) {
+    weight[r] = lane < runs ? tops[row[r]] : -INFINITY;
+    total[r] = lane < runs ? tops[most + row[r]] : 0.f;
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i)
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+        x[r][i][c] = sums[(begin + i < runs ? begin + i : 0) * size + row[r] * DV + kCols * lane + c];
   }
 #pragma unroll
-  for (int r = 0; r < kJoinRows; ++r) {
+  for (int r = 0; r < ROWS; ++r) {
     const float top = over_wave(weight[r], [](float x, float y) { return fmaxf(x, y); });
     weight[r] = weight[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(weight[r] - top);
     total[r] = over_wave(total[r] * weight[r], [](float x, float y) { return x + y; });
-  }
-  for (int i0 = 0; i0 < runs; i0 += kRuns) {
-    float x[kJoinRows][kRuns][kCols];
 #pragma unroll
-    for (int r = 0; r < kJoinRows; ++r)
+    for (int c = 0; c < kCols; ++c) acc[r][c] = 0.f;
 #pragma unroll
-      for (int i = 0; i < kRuns; ++i)
+    for (int i = 0; i < RUNS; ++i) {
+      const float w = __uint_as_float(
+          __builtin_amdgcn_readlane(__float_as_uint(weight[r]), (begin + i) & (kWave - 1)));
 #pragma unroll
-        for (int c = 0; c < kCols; ++c)
-          x[r][i][c] = sums[(i0 + i < runs ? i0 + i : i0) * size + from[r] * DV + kCols * lane + c];
-#pragma unroll
-    for (int r = 0; r < kJoinRows; ++r)
-#pragma unroll
-      for (int i = 0; i < kRuns; ++i) {
-        const float w = __uint_as_float(
-            __builtin_amdgcn_readlane(__float_as_uint(weight[r]), (i0 + i) & (kWave - 1)));
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-          acc[r][c] = i0 + i < runs ? fmaf(w, x[r][i][c], acc[r][c]) : acc[r][c];
-      }
-  }
-#pragma unroll
-  for (int r = 0; r < kJoinRows; ++r) {
-    const int row = row0 + r;
-    if (!exists(row)) return;
-    const int token = row * a.inv_pack >> 16;
-    const float inv = total[r] == 0.f ? 0.f : 1.0f / total[r];
-    uint16_t* const out = a.out + ((b.q.begin + b.q0 + token) * a.heads +
-                                   static_cast<int64_t>(b.pack) * a.pack + row - token * a.pack) * a.d_v;
-    if constexpr (DV == 128) {
-      if (2 * lane < a.d_v)
-        *reinterpret_cast<uint32_t*>(out + 2 * lane) =
-            pack2<BF16>(within_type<BF16>(acc[r][0] * inv), within_type<BF16>(acc[r][1] * inv));
-    } else {
-      if (lane < a.d_v)
-        out[lane] = static_cast<uint16_t>(pack2<BF16>(within_type<BF16>(acc[r][0] * inv), 0.f));
+      for (int c = 0; c < kCols; ++c)
+        acc[r][c] = begin + i < runs ? fmaf(w, x[r][i][c], acc[r][c]) : acc[r][c];
     }
   }
 }
 
-// Whether every sequence of a call of so many rows has few.
-bool all_few(int64_t rows, int pack) { return rows * pack <= kFewRows; }
+// The runs of a tile joined, in their order: a block takes a quarter of a tile of 16 or 32
+// rows, 16 rows of one of 128. Up to kJoinRuns runs a wave joins a row by itself, two at a time; more are dealt
+// over the four waves, whose sums then meet in LDS.
+// Bound by latency: the tile, then one trip to memory for each turn of the loop.
+constexpr int kJoinRuns = 8;
+template <bool BF16, int DV>
+__global__ void __launch_bounds__(kAttnThreads) paged_join_kernel(PagedArgs a, int parts) {
+  constexpr int kCols = DV / 64, kShare = kWave / kAttnWaves;  // runs of a wave
+  __shared__ float shared[kAttnWaves][kAttnWaves][DV];
+  const int index = static_cast<int>(blockIdx.x) / parts;
+  if (index >= a.split->count) return;
+  const SplitTile tile = a.split->tile[index];
+  // (offsets that are not in order can leave tiles unnoted: nothing outside the tensors)
+  if (tile.runs < 2 || tile.runs > kWave || tile.pack < 0 || tile.pack >= a.packs || tile.row < 0 ||
+      tile.units < 1 || tile.units > kManyUnits || tile.rows < 0 ||
+      tile.rows > tile.units * kFewRows || tile.row + tile.rows / a.pack > a.sq.rows ||
+      tile.unit >= a.units || a.units - tile.unit < static_cast<uint32_t>(tile.runs * tile.units))
+    return;
+  const int lane = threadIdx.x & (kWave - 1), runs = tile.runs;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int most = tile.units * kFewRows, size = most * (DV + 2);
+  // the rows that exist are the first ones: tokens of `pack` heads
+  const int step = tile.units < kManyUnits ? kJoinFew * tile.units : kJoinMany;
+  const int begin = static_cast<int>(blockIdx.x) % parts * step;
+  const int end = begin + step < tile.rows ? begin + step : tile.rows;
+  if (begin >= end) return;
+  const float* const sums = sums_of<DV>(a, tile.unit);
+  if (runs <= kJoinRuns) {
+    for (int row0 = begin + wave; row0 < end; row0 += 2 * kAttnWaves) {
+      const bool two = row0 + kAttnWaves < end;
+      const int row[2] = {row0, two ? row0 + kAttnWaves : row0};
+      float acc[2][kCols], total[2];
+      join_rows<DV, 2, kJoinRuns>(sums, size, most, runs, 0, row, acc, total);
+      store_joined<BF16, DV>(a, tile, row[0], acc[0], total[0]);
+      if (two) store_joined<BF16, DV>(a, tile, row[1], acc[1], total[1]);
+    }
+    return;
+  }
+  for (int row0 = begin; row0 < end; row0 += kAttnWaves) {
+    int row[kAttnWaves];
+#pragma unroll
+    for (int r = 0; r < kAttnWaves; ++r) row[r] = row0 + r < end ? row0 + r : row0;
+    float acc[kAttnWaves][kCols], total[kAttnWaves];
+    join_rows<DV, kAttnWaves, kShare>(sums, size, most, runs, wave * kShare, row, acc, total);
+    if (row0 > begin) __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kAttnWaves; ++r)
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) shared[wave][r][kCols * lane + c] = acc[r][c];
+    __syncthreads();
+    if (row0 + wave < end) {
+      float all[kCols] = {}, sum = total[0];
+#pragma unroll
+      for (int r = 1; r < kAttnWaves; ++r) sum = wave == r ? total[r] : sum;
+#pragma unroll
+      for (int w = 0; w < kAttnWaves; ++w)
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) all[c] += shared[w][wave][kCols * lane + c];
+      store_joined<BF16, DV>(a, tile, row0 + wave, all, sum);
+    }
+  }
+}
 
-int64_t paged_units(int64_t rows, int64_t capacity, int pack) {
+constexpr int64_t kSplitBytes = (sizeof(SplitTiles) + 255) / 256 * 256;
+
+// The most units that a tile of the call can have.
+int most_units(int64_t rows, int64_t sequences, bool packed, int pack) {
+  const int64_t most = (packed ? rows : rows / sequences) * pack;
+  return most <= kFewRows ? 1 : (most <= 2 * kFewRows ? 2 : kManyUnits);
+}
+
+int64_t paged_units(int64_t rows, int64_t sequences, bool packed, int64_t capacity, int pack) {
   if (capacity <= kMinRun) return 0;  // no tile has more keys than one run
-  return int64_t{2} * kFill * (all_few(rows, pack) ? 1 : kAttnRows / kFewRows);
+  return int64_t{2} * kFill * most_units(rows, sequences, packed, pack);
 }
 
 template <bool BF16>
 int launch_paged(const PagedArgs& a, hipStream_t s) {
   constexpr const char* kName = "lk_attention_paged";
-  const int64_t blocks = a.packs * (a.sq.rows / a.tokens + a.sq.count + 1) + (a.partial ? kFill : 0);
+  const int64_t tiles_most = a.packs * (a.sq.rows / a.tokens + a.sq.count + 1);
+  const int64_t blocks = tiles_most + (a.partial ? kFill + 1 : 0);
   LK_REQUIRE(grid_fits(blocks, kAttnThreads), "too many query rows and heads for one call");
-  const int parts = (all_few(a.sq.rows, a.pack) ? kFewRows : kAttnRows) / kJoinBlockRows;
-  const dim3 grid(static_cast<unsigned>(blocks)), join(static_cast<unsigned>(kFill * parts));
+  const bool few = most_units(a.sq.rows, a.sq.count, a.sq.cu != nullptr, a.pack) < kManyUnits;
+  const int parts = few ? kFewRows / kJoinFew : kAttnRows / kJoinMany;
+  const int64_t tiles = std::min<int64_t>(kFill, tiles_most);
+  const dim3 grid(static_cast<unsigned>(blocks)), join(static_cast<unsigned>(tiles * parts));
 #define LK_PAGED(Q, V)                                                   \
   if (a.d_qk <= Q && a.d_v <= V) {                                       \
     paged_attend_kernel<BF16, Q, V><<<grid, kAttnThreads, 0, s>>>(a);    \
@@ -600,12 +720,14 @@ using namespace lk;
 extern "C" {
 
 int64_t lk_attention_paged_workspace(int64_t rows, int64_t sequences, int64_t capacity,
-                                     int64_t heads, int64_t kv_heads, int64_t d_qk, int64_t d_v) {
+                                     int64_t heads, int64_t kv_heads, int64_t d_qk, int64_t d_v,
+                                     int packed) {
   if (rows < 0 || sequences <= 0 || capacity < 0 || heads <= 0 || kv_heads <= 0 ||
       heads % kv_heads || d_qk <= 0 || d_v <= 0 || d_qk > kAttnMaxQk || d_v > kAttnMaxV)
     return -1;
   const int64_t dv = d_qk <= 64 && d_v <= 64 ? 64 : 128;
-  return paged_units(rows, capacity, attention_pack(heads, kv_heads)) * kFewRows * (dv + 2) * 4;
+  const int64_t units = paged_units(rows, sequences, packed != 0, capacity, attention_pack(heads, kv_heads, kPagedPack));
+  return units == 0 ? 0 : kSplitBytes + units * kFewRows * (dv + 2) * 4;
 }
 
 int lk_attention_paged(const void* q, const void* k_pages, const void* v_pages, void* out,
@@ -648,9 +770,9 @@ int lk_attention_paged(const void* q, const void* k_pages, const void* v_pages, 
   for (const void* p : {q, k_pages, v_pages, static_cast<const void*>(out)})
     LK_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0,
                "attention tensors must start on a 16-byte boundary");
-  const int pack = attention_pack(heads, kv_heads);
+  const int pack = attention_pack(heads, kv_heads, kPagedPack);
   const int64_t need = lk_attention_paged_workspace(rows, sequences, table_width * page_rows, heads,
-                                                    kv_heads, d_qk, d_v);
+                                                    kv_heads, d_qk, d_v, cu != nullptr);
   LK_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
              "attention workspace too small: %lld bytes, %lld needed", (long long)workspace_bytes,
              (long long)need);
@@ -669,8 +791,9 @@ int lk_attention_paged(const void* q, const void* k_pages, const void* v_pages, 
   a.d_qk = static_cast<int>(d_qk), a.d_v = static_cast<int>(d_v);
   a.pack = pack, a.inv_pack = 65536 / pack + 1, a.tokens = kAttnRows / pack;
   a.packs = static_cast<int>(heads) / pack;
-  a.units = static_cast<uint32_t>(paged_units(rows, table_width * page_rows, pack));
-  a.partial = need ? static_cast<float*>(workspace) : nullptr;
+  a.units = static_cast<uint32_t>(paged_units(rows, sequences, cu != nullptr, table_width * page_rows, pack));
+  a.split = need ? static_cast<SplitTiles*>(workspace) : nullptr;
+  a.partial = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kSplitBytes) : nullptr;
   a.scale_log2 = scale == 0.f ? 1.f : scale_log2;
   a.q_keep = scale == 0.f ? 0u : 0xFFFFFFFFu, a.q_flip = scale < 0.f ? 0x80008000u : 0u;
   const hipStream_t s = as_stream(stream);

@@ -330,7 +330,7 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         return out
     q, q_row, q_head = _heads_of(q, batch, rows)
     need = _lib.query("lk_attention_paged_workspace", batch * rows, count, layout[1] * layout[2],
-                      heads, kv_heads, d_qk, d_v)
+                      heads, kv_heads, d_qk, d_v, offsets is not None)
     ws = _w.workspace(need, device) if need else None
     with _w._on(device):
         _lib.call("lk_attention_paged", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),

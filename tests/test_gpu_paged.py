@@ -240,7 +240,7 @@ def _attend(rng, new, cached, page_rows, h, hk, dq, dv, dtype, scale=None, heads
     return args, kw, got
 
 
-@pytest.mark.parametrize("h,hk,dq,dv", [(4, 1, 128, 128), (2, 2, 192, 128), (6, 3, 64, 64), (2, 1, 72, 40),
+@pytest.mark.parametrize("h,hk,dq,dv", [(4, 1, 128, 128), (32, 1, 128, 128), (2, 2, 192, 128), (6, 3, 64, 64), (2, 1, 72, 40),
                                         (1, 1, 8, 8), (32, 1, 64, 128), (10, 2, 136, 64), (7, 1, 128, 24)])
 @pytest.mark.parametrize("new,cached", [([1], [0]), ([1, 1, 1, 1], [0, 63, 64, 130]), ([1, 1], [700, 3]),
                                         ([5, 0, 2], [100, 9, 0]), ([37, 1, 150], [0, 300, 45]),

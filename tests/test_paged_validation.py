@@ -182,8 +182,8 @@ def test_c_abi_refusals_come_before_any_launch(lib):
                   width, stride, page, row, d, page, row, dv, scale, dt, ws, size, None)
 
     long = {"width": 100, "stride": 100}
-    need = lib.lk_attention_paged_workspace(8, 1, 1600, 4, 2, 64, 64)
-    assert need > 0 and lib.lk_attention_paged_workspace(8, 1, 64, 4, 2, 64, 64) == 0
+    need = lib.lk_attention_paged_workspace(8, 1, 1600, 4, 2, 64, 64, 0)
+    assert need > 0 and lib.lk_attention_paged_workspace(8, 1, 64, 4, 2, 64, 64, 0) == 0
     for args, match in (*shared, ({**long}, "workspace too small"), ({**long, "ws": 16, "size": need - 1}, "workspace too"),
                         ({**long, "size": need}, "workspace too"), ({**long, "ws": 8, "size": need}, "16-byte aligned"),
                         ({"seqs": 65537, "rows": 65537}, "up to 65536"), ({"hk": 3}, "multiple of the key heads"), ({"d": 200}, "d_qk"), ({"dv": 136}, "d_v"),
@@ -194,7 +194,7 @@ def test_c_abi_refusals_come_before_any_launch(lib):
     attention(rows=0)
     for bad in ((-1, 1, 64, 4, 2, 64, 64), (8, 0, 64, 4, 2, 64, 64), (8, 1, -1, 4, 2, 64, 64),
                 (8, 1, 64, 3, 2, 64, 64), (8, 1, 64, 4, 2, 200, 64), (8, 1, 64, 4, 2, 64, 136)):
-        assert lib.lk_attention_paged_workspace(*bad) == -1
+        assert lib.lk_attention_paged_workspace(*bad, 0) == -1
 
 
 def _copy(src, dst, pages=8, pointer=16, stride=4096, size=4096, count=1, pairs=None):
