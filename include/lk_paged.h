@@ -61,7 +61,9 @@ LK_API int lk_qk_norm_rope(const void* q, const void* k, const void* q_weight,
  * no page) is not written; its q is rotated as position 0. Rows behind the last sequence
  * write nothing to the cache; their q_out is zeros. heads may be 0 (q, q_out, q_weight unused),
  * rotary 0 (no rotation). dtype is LK_DTYPE_F16 or LK_DTYPE_BF16. Two rows must
- * not go to one place: pages that take new rows belong to one sequence. */
+ * not go to one place: pages that take new rows belong to one sequence. The places
+ * of k_pages and of v_pages do not overlap (refused where the strides show it, or the
+ * two are one), nor what is read. */
 LK_API int lk_paged_append(const void* q, const void* k, const void* v, const void* q_weight,
                            const void* k_weight, const float* cos_sin, const int32_t* page_table,
                            const int32_t* lengths, const int32_t* cu, void* q_out, void* k_pages,

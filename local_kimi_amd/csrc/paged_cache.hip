@@ -348,6 +348,23 @@ int check_heads(int64_t rows, int64_t heads, int64_t kv_heads, int64_t d, int64_
   return LK_OK;
 }
 
+// Whether no two places of a cache share memory, as far as steps that go up tell: each dimension's
+// step takes it past all that the smaller ones reach.
+bool places_apart(int64_t d, int64_t pages, int64_t page, int64_t rows, int64_t row, int64_t heads,
+                  int64_t head) {
+  struct Dim {
+    int64_t step, count;
+  } dims[3] = {{page, pages}, {row, rows}, {head, heads}};
+  std::sort(dims, dims + 3, [](const Dim& x, const Dim& y) { return x.step < y.step; });
+  int64_t reach = d;
+  for (const Dim& x : dims) {
+    if (x.count <= 1) continue;
+    if (x.step < reach) return false;
+    reach += x.step * (x.count - 1);
+  }
+  return true;
+}
+
 // ---------------------------------------------------------------------------
 // Copies of pages
 
@@ -462,6 +479,10 @@ int lk_paged_append(const void* q, const void* k, const void* v, const void* q_w
                                  table_stride, {k_page, k_page_row, k_page_head, v_page, v_page_row,
                                                 v_page_head}))
     return st;
+  LK_REQUIRE(places_apart(d_qk, pages, k_page, page_rows, k_page_row, kv_heads, k_page_head) &&
+                 places_apart(d_v, pages, v_page, page_rows, v_page_row, kv_heads, v_page_head),
+             "the places of a cache that is written must not overlap");
+  LK_REQUIRE(k_pages != v_pages || !k_pages, "keys and values must have pages of their own");
   if (rows == 0) return LK_OK;
   LK_REQUIRE(k && v && lengths && (table_width == 0 || page_table) && (pages == 0 || (k_pages && v_pages)) &&
                  (heads == 0 || (q && q_out)),

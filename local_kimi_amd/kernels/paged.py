@@ -261,7 +261,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pag
     (a position below 0, no page) is not written, and rotated as position 0 where that is
     below 0; rows behind the last sequence write nothing and return zeros. Two sequences'
     new tokens must not share a page: copy a forked sequence's last page first
-    (``PagedCache.extend`` does)."""
+    (``PagedCache.extend`` does). The cache's places must not overlap."""
     batch, rows, heads, kv_heads, d, dtype, device = _check_heads(q, k)
     return _append(q, heads, k, v, batch, rows, kv_heads, d, dtype, device, k_pages, v_pages,
                    page_table, lengths, cos_sin, q_weight, k_weight, eps, cu_seqlens, rotary_offset,

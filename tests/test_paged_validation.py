@@ -159,10 +159,10 @@ def test_c_abi_refusals_come_before_any_launch(lib):
             rope(**args)
 
     def append(seqs=1, rows=8, h=4, hk=2, d=64, dv=64, pages=5, page_rows=16, width=3, stride=3, page=4096,
-               row=128, rotary=64, dt=2, p=16, q=16):
-        _lib.call("lk_paged_append", q, p, p, p, p, 16, p, p, None, q, p, p, seqs, rows, h, hk, d, dv, 256, d,
-                  128, d, 128, dv, pages, page_rows, width, stride, page, row, d, page, row, dv, rotary, 0, 0, 9,
-                  1e-6, dt, 0, None)
+               row=128, rotary=64, dt=2, p=16, q=16, vp=32, head=64):
+        _lib.call("lk_paged_append", q, p, p, p, p, 16, p, p, None, q, p, vp if p else p, seqs, rows, h, hk, d, dv, 256, d,
+                  128, d, 128, dv, pages, page_rows, width, stride, page, row, head, page, row, head, rotary, 0, 0,
+                  9, 1e-6, dt, 0, None)
 
     shared = (({"seqs": 0}, "sequences"), ({"seqs": 1 << 24, "rows": 0}, "sequences"), ({"seqs": 3}, "divide"),
               ({"pages": -1}, "pages"), ({"pages": 1 << 31}, "pages"), ({"page_rows": 24}, "multiple of 16"),
@@ -170,11 +170,14 @@ def test_c_abi_refusals_come_before_any_launch(lib):
               ({"width": 1 << 27, "stride": 1 << 27}, "fewer than 2\\^31"), ({"stride": 2}, "page table"),
               ({"width": 1 << 62, "stride": 1 << 62}, "fewer than 2\\^31"), ({"page": 4}, "multiples of 8"),
               ({"row": -8}, "not negative"), ({"p": None}, "null"), ({"p": 8}, "16-byte"), ({"dt": 0}, "fp16"))
-    for args, match in (*shared, ({"q": None}, "null"), ({"dv": 264}, "value dimension"), ({"dv": 12}, "value dimension"),
+    for args, match in (*shared, ({"q": None}, "null"), ({"page": 0}, "overlap"), ({"row": 64}, "overlap"),
+                        ({"page": 2000}, "overlap"), ({"head": 56}, "overlap"), ({"vp": 16}, "pages of their own"), ({"dv": 264}, "value dimension"), ({"dv": 12}, "value dimension"),
                         ({"rotary": 72}, "rotated slice")):
         with pytest.raises(RuntimeError, match=match):
             append(**args)
     append(rows=0)
+    append(rows=0, head=16 * 64, row=64, page=32 * 64)  # heads first
+    append(rows=0, page=128, row=5 * 128)                # rows of all pages side by side
 
     def attention(seqs=1, rows=8, h=4, hk=2, d=64, dv=64, pages=5, page_rows=16, width=3, stride=3, page=4096,
                   row=128, scale=1.0, dt=2, p=16, qs=256, ws=None, size=0):
