@@ -17,7 +17,7 @@
  * the call's new ones included, which are its last. Lengths are clamped to 0 ..
  * table_width * page_rows. Table entries that name no page (below 0, pages and
  * above) lead nowhere: such positions read as zeros and are not written.
- * page_rows is a multiple of 16.
+ * page_rows is a multiple of 16 up to 65536, table_width * page_rows at most 2^30.
  *
  * cu [sequences + 1] (int32): sequence s has new rows cu[s] to cu[s + 1] - 1; null
  * means equal sequences of rows / sequences. Offsets start with 0 and do not

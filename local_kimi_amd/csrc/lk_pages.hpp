@@ -69,8 +69,8 @@ inline int check_pages(int64_t sequences, int64_t rows, bool offsets, int64_t pa
              "page rows must be a multiple of %d up to 65536, got %lld", kPageStep,
              (long long)page_rows);
   LK_REQUIRE(table_width >= 0 && table_width < (int64_t{1} << 31) &&
-                 table_width * page_rows < (int64_t{1} << 31) && table_stride >= table_width,
-             "the page table must name fewer than 2^31 positions a sequence");
+                 table_width * page_rows <= (int64_t{1} << 30) && table_stride >= table_width,
+             "the page table must name up to 2^30 positions a sequence");
   for (const int64_t s : strides)
     LK_REQUIRE(s >= 0 && s % 8 == 0, "page strides must be multiples of 8 elements, not negative");
   return LK_OK;

@@ -8,12 +8,21 @@
 namespace lk {
 namespace {
 
-constexpr int kFewRows = 16;  // queries x heads of a block for single tokens, or twice that
+// Queries x heads of a block for single tokens: a tile of the 16 x 16 products, or two. Up to
+// 32 heads of one key head share a block, so that its keys are read once: 32 heads on
+// one, 64 tokens on 2.1 million keys 220 us, 361 as two blocks of 16.
+constexpr int kFewRows = 16;
 constexpr int kPagedPack = 32;
-constexpr int kFill = 1024;   // runs that a call's keys are dealt in: four a CU
-constexpr int kMinRun = 256;  // keys of a run, at the least
+// Runs that a call's keys are dealt in: four a CU, so that lengths of all kinds even out.
+// With 512 / 1024 / 2048, 64 tokens on up to 8192 keys x 8 heads took 225 / 216 / 215 us, 1071
+// rows of a mixed step 169 / 165 / 205. Rows of long pieces, bound by their products, take
+// runs of twice the length (2048 rows on 16048 keys 539 us in 1024 runs, 523 so). At least
+// kMinRun keys: 19 rows on 1119 keys take 18 us, in runs of 128 28 (more to join), one token on 16384
+// 23 either way.
+constexpr int kFill = 1024;
+constexpr int kMinRun = 256;
 constexpr int kJoinFew = 4, kJoinMany = 16;  // rows of a block of the join
-constexpr int64_t kMaxSequences = 65536;
+constexpr int64_t kMaxSequences = 65536;  // (each block counts through them)
 
 struct PagedArgs : AttnShape {
   const uint16_t *k, *v;
@@ -31,7 +40,6 @@ struct SplitTile {
   int64_t row;  // its first
   int rows, pack, runs, units;
   uint32_t unit;
-  int unused;
 };
 struct SplitTiles {
   int count;
@@ -155,6 +163,10 @@ __device__ inline f32x4_t mfma16_half(uint2 a, uint2 b, f32x4_t c) {
 // are joined. S^T = K Q^T and O^T += V^T P^T as in attend_rows, on 16 x 16 tiles: a
 // lane holds four scores of a row, which rounded are its part of the next
 // product's operand.
+//
+// Bound by HBM: two tiles of 64 keys a block, two blocks a CU, keep up to 128 KB a CU on their
+// way. 64 tokens on up to 8192 keys x 8 heads of 128 (1.1 GB) take 198 us in all, 5.5 TB/s (7.0 is
+// what a kernel that only reads reaches here); 218 with loads that go through the caches.
 template <bool BF16, int DQ, int DV, int GROUPS>
 __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& b,
                                            PagedKeys<DQ, DV>& keys_of, uint16_t* stage,
@@ -372,8 +384,8 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
 // Who does what. A call's work is found on the device, from the lengths as they are:
 // sequence s has ceil(n / tokens) tiles of rows (one of up to 16 or 32 rows where its
 // new tokens fit) for each pack of heads, and every tile's keys are taken in runs of about
-// L keys, L = what two blocks a CU would have each if all keys of the call were dealt
-// evenly, kMinRun at the least. Each block finds its tile and run by a scan over the
+// L keys, L = a kFill-th of all keys that the call's tiles see (twice that for tiles of
+// kAttnRows), kMinRun at the least. Each block finds its tile and run by a scan over the
 // sequences, 64 at a time; the rows behind the last sequence come after all. A
 // tile in runs is noted for the join.
 //
@@ -383,14 +395,13 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
 
 struct PagedTile {
   RowRange q;
-  int sequence, lk, tiles, runs;
+  int lk, tiles, runs;
   int units;  // of kFewRows rows that a tile has: 1, 2 or those of kAttnRows
 };
 constexpr int kManyUnits = kAttnRows / kFewRows;
 
 __device__ inline PagedTile paged_tiles(const PagedArgs& a, int s) {
   PagedTile t{};
-  t.sequence = s;
   if (s >= a.sq.count) return t;
   t.q = sequence_rows(a.sq, s);
   const int lq = static_cast<int>(t.q.end - t.q.begin);
@@ -531,7 +542,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attend_kernel(PagedArgs
     part = sums_of<DV>(a, item.unit);
     if (b.split == 0 && threadIdx.x == 0)
       a.split->tile[item.tile] = SplitTile{b.q.begin + b.q0, static_cast<int>(b.last - b.q0) * a.pack,
-                                           b.pack, b.splits, item.units, item.unit, 0};
+                                           b.pack, b.splits, item.units, item.unit};
   }
   if (item.units < kManyUnits && item.sequence < a.sq.count) {
     PagedKeys<DQ, DV> keys(a, b, item.sequence, stage);

@@ -167,8 +167,8 @@ def test_c_abi_refusals_come_before_any_launch(lib):
     shared = (({"seqs": 0}, "sequences"), ({"seqs": 1 << 24, "rows": 0}, "sequences"), ({"seqs": 3}, "divide"),
               ({"pages": -1}, "pages"), ({"pages": 1 << 31}, "pages"), ({"page_rows": 24}, "multiple of 16"),
               ({"page_rows": 0}, "multiple of 16"), ({"page_rows": 65552}, "multiple of 16"),
-              ({"width": 1 << 27, "stride": 1 << 27}, "fewer than 2\\^31"), ({"stride": 2}, "page table"),
-              ({"width": 1 << 62, "stride": 1 << 62}, "fewer than 2\\^31"), ({"page": 4}, "multiples of 8"),
+              ({"width": (1 << 26) + 1, "stride": 1 << 27}, "up to 2\\^30"), ({"stride": 2}, "page table"),
+              ({"width": 1 << 62, "stride": 1 << 62}, "up to 2\\^30"), ({"page": 4}, "multiples of 8"),
               ({"row": -8}, "not negative"), ({"p": None}, "null"), ({"p": 8}, "16-byte"), ({"dt": 0}, "fp16"))
     for args, match in (*shared, ({"q": None}, "null"), ({"page": 0}, "overlap"), ({"row": 64}, "overlap"),
                         ({"page": 2000}, "overlap"), ({"head": 56}, "overlap"), ({"vp": 16}, "pages of their own"), ({"dv": 264}, "value dimension"), ({"dv": 12}, "value dimension"),
