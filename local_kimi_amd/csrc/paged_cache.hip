@@ -337,8 +337,9 @@ int check_heads(int64_t rows, int64_t heads, int64_t kv_heads, int64_t d, int64_
   LK_REQUIRE(rotary >= 0 && rotary % 8 == 0 && offset >= 0 && offset % 8 == 0 && rotary <= d &&
                  offset <= d - rotary,
              "the rotated slice must lie within the head, in multiples of 8");
-  LK_REQUIRE(rotary == 0 || (cos_sin && on_16(cos_sin) && table_rows > 0),
-             "a rotation needs a table of angles on a 16-byte boundary");
+  LK_REQUIRE(rotary == 0 || (cos_sin && on_16(cos_sin) && table_rows > 0 &&
+                             table_rows < (int64_t{1} << 31)),
+             "a rotation needs a table of angles of 1 .. 2^31 - 1 rows on a 16-byte boundary");
   LK_REQUIRE(!with_q || (q_weight == nullptr) == (k_weight == nullptr),
              "both norm weights must be given, or neither");
   LK_REQUIRE(on_16(q_weight) && on_16(k_weight), "norm weights must start on a 16-byte boundary");

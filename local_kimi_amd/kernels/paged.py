@@ -28,7 +28,7 @@ import torch
 
 from .. import _lib
 from . import w4a16 as _w
-from .attention import ATTENTION_MAX_QK_DIM, ATTENTION_MAX_V_DIM, _rows
+from .attention import ATTENTION_MAX_QK_DIM, ATTENTION_MAX_V_DIM
 from .kda import _aligned, _offsets
 
 HEAD_MAX_DIM = 256
@@ -151,10 +151,11 @@ def _heads_of(t: torch.Tensor, batch: int, rows: int) -> tuple[torch.Tensor, int
     """``t`` [batch, rows, heads, d] as the kernels address it, copied where its layout is
     another, and the strides of its rows and heads."""
     a, b, c, one = t.stride()
-    if one == 1 and (batch == 1 or a == rows * b) and (b | c) % 8 == 0 and b < 1 << 24 \
-            and t.data_ptr() % 16 == 0:
+    if rows == 1:  # (a token of each sequence: any step between them)
+        b = a
+    if one == 1 and (batch == 1 or a == rows * b) and (b | c) % 8 == 0 and t.data_ptr() % 16 == 0:
         return t, b, c
-    t = _rows(t)
+    t = t.clone(memory_format=torch.contiguous_format)
     return t, t.stride(1), t.stride(2)
 
 

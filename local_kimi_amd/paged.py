@@ -34,6 +34,7 @@ class PageBook:
         self.users = [0] * pages                                       # of each page
         self.pages: list[list[int] | None] = [None] * sequences        # of each sequence
         self.lengths = [0] * sequences
+        self.changed: set[int] = set()  # sequences whose pages changed; its reader clears it
         self._free = list(range(pages))  # a heap: the lowest goes first
 
     @property
@@ -55,6 +56,7 @@ class PageBook:
         """A new, empty sequence."""
         i = self._vacant()
         self.pages[i], self.lengths[i] = [], 0
+        self.changed.add(i)
         return i
 
     def fork(self, sequence: int) -> int:
@@ -64,12 +66,14 @@ class PageBook:
         for p in held:
             self.users[p] += 1
         self.pages[i], self.lengths[i] = list(held), self.lengths[sequence]
+        self.changed.add(i)
         return i
 
     def free(self, sequence: int) -> None:
         for p in self._check(sequence):
             self._release(p)
         self.pages[sequence], self.lengths[sequence] = None, 0
+        self.changed.add(sequence)
 
     def _release(self, page: int) -> None:
         self.users[page] -= 1
@@ -110,9 +114,11 @@ class PageBook:
                 self._release(held[-1])
                 held[-1] = self._take()
                 dst.append(held[-1])
+                self.changed.add(s)
             self.lengths[s] += n
             while len(held) * self.page_rows < self.lengths[s]:
                 held.append(self._take())
+                self.changed.add(s)
         return src, dst
 
     def compact(self) -> Copies:
@@ -125,6 +131,8 @@ class PageBook:
             self.users[a], self.users[b] = 0, self.users[a]
         self.pages = [held if held is None else [to.get(p, p) for p in held] for held in self.pages]
         self._free = list(range(used, len(self.users)))
+        if to:
+            self.changed.update(i for i, held in enumerate(self.pages) if held)
         return src, dst
 
 
@@ -138,7 +146,7 @@ class PagedCache:
     ``extend`` by one token each, then per layer ``qk_norm_rope_append`` and
     ``attention_paged`` on these tensors: a sequence that is not in use has length 0, is
     not written and attends to nothing. ``rows_of`` picks the rows of some sequences.
-    Work is issued on the current stream; the table's upload waits for the host's copy."""
+    Copies and uploads are issued on the current stream, and nothing waits for them."""
 
     def __init__(self, pages: int, sequences: int, capacity: int, *, layers: int, kv_heads: int,
                  d_qk: int, d_v: int, page_rows: int = 64, dtype: torch.dtype = torch.bfloat16,
@@ -151,17 +159,25 @@ class PagedCache:
             return torch.zeros((layers, pages, page_rows, kv_heads, d), dtype=dtype, device=device)
 
         self.k_pages, self.v_pages = list(made(d_qk)), list(made(d_v))
-        self.page_table = torch.full((sequences, self.book.width), -1, dtype=torch.int32,
-                                     device=device)
+        self._table = torch.full((sequences, self.book.width), -1, dtype=torch.int32)
+        self.page_table = self._table.to(device, copy=True)
         self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
+
+    def _upload(self, target: torch.Tensor, values: torch.Tensor) -> None:
+        # from pinned memory of its own, so that the copy takes its turn on the stream
+        target.copy_(values.pin_memory() if target.is_cuda else values, non_blocking=True)
 
     def _carry_out(self, copies: Copies) -> None:
         if copies[0]:
             copy_pages([*self.k_pages, *self.v_pages], *copies)
-        width = self.book.width
-        rows = [(held or []) + [-1] * (width - len(held or [])) for held in self.book.pages]
-        self.page_table.copy_(torch.tensor(rows, dtype=torch.int32))
-        self.lengths.copy_(torch.tensor(self.book.lengths, dtype=torch.int32))
+        if self.book.changed:
+            for i in self.book.changed:
+                held = self.book.pages[i] or []
+                self._table[i].fill_(-1)
+                self._table[i, :len(held)] = torch.tensor(held, dtype=torch.int32)
+            self.book.changed.clear()
+            self._upload(self.page_table, self._table)
+        self._upload(self.lengths, torch.tensor(self.book.lengths, dtype=torch.int32))
 
     def add(self) -> int:
         """A new, empty sequence."""
@@ -190,5 +206,6 @@ class PagedCache:
 
     def rows_of(self, sequences: Sequence[int]) -> tuple[torch.Tensor, torch.Tensor]:
         """``page_table`` and ``lengths`` of these sequences, in this order (copies)."""
-        at = torch.tensor(list(sequences), dtype=torch.int64).to(self.lengths.device)
+        at = torch.empty(len(sequences), dtype=torch.int64, device=self.lengths.device)
+        self._upload(at, torch.tensor(list(sequences), dtype=torch.int64))
         return self.page_table[at], self.lengths[at]

@@ -113,6 +113,10 @@ def test_layouts_of_queries_tables_and_lengths():
     for t in (wide[:, 5:5 + table.shape[1]], table.t().contiguous().t()):
         assert torch.equal(attention_paged(q, k, v, t, lengths.long()), want)
     assert torch.equal(attention_paged(q, k, v, table, torch.stack((lengths, lengths), 1)[:, 0]), want)
+    last = torch.zeros((3, 5, 8, 128), device=DEV).bfloat16()
+    last[:, -1:] = q[:, 1:]
+    one = attention_paged(q[:, 1:].contiguous(), k, v, table, lengths)
+    assert torch.equal(attention_paged(last[:, -1:], k, v, table, lengths), one)
     # one row of the table for all
     same = attention_paged(q, k, v, table[:1].expand(3, -1), lengths[:1].expand(3))
     assert torch.equal(same, attention_paged(q, k, v, table[:1].repeat(3, 1), lengths[:1].repeat(3)))
@@ -219,6 +223,34 @@ def test_a_captured_decode_step_follows_its_lengths():
         _ = (out.float() + 1).sum().item()  # unrelated work between replays
     for a, b in zip(state[0], eager[0]):
         assert torch.equal(a, b)
+
+
+def test_a_cache_that_is_extended_while_its_steps_run():
+    """Uploads take their turn on the stream: 30 steps issued without a wait equal the
+    same steps one by one."""
+    from local_kimi_amd.kernels import attention_paged, paged_append
+    from local_kimi_amd.paged import PagedCache
+
+    g = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.randn((30, 4, 1, 2, 128), generator=g, device=DEV).bfloat16()
+    outs = []
+    for wait in (True, False):
+        cache = PagedCache(64, 6, 200, layers=1, kv_heads=2, d_qk=128, d_v=128, page_rows=16)
+        seqs = [cache.add() for _ in range(3)]
+        cache.extend(seqs, [100, 14, 31])
+        got = []
+        for i in range(30):
+            if i == 10:
+                seqs.append(cache.fork(seqs[2]))
+            cache.extend(seqs, [1] * len(seqs))
+            if wait:
+                torch.cuda.synchronize()
+            n = len(seqs)
+            table, lengths = cache.rows_of(seqs)
+            paged_append(x[i, :n], x[i, :n], cache.k_pages[0], cache.v_pages[0], table, lengths)
+            got.append(attention_paged(x[i, :n], cache.k_pages[0], cache.v_pages[0], table, lengths))
+        outs.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
 
 
 @pytest.mark.parametrize("cu", [[0, 90, 30, 60, 100], [40, 20, 0, 300, 100], [-7, 5, 2 ** 31 - 1, 3, 9], [100, 100, 0, 0, 0],

@@ -125,6 +125,13 @@ def test_a_cache_mirrors_its_book():
     assert cache.lengths.tolist() == [20, 3, 0]
     table, lengths = cache.rows_of([b, a])
     assert table.tolist() == [[2, -1, -1], [0, 1, -1]] and lengths.tolist() == [3, 20]
+    c = cache.fork(a)
+    assert c == 2 and cache.page_table[2].tolist() == [0, 1, -1] and cache.lengths.tolist() == [20, 3, 20]
+    cache.extend([b], [13])  # to the end of its page: the table stays
+    assert cache.page_table[1].tolist() == [2, -1, -1] and cache.lengths.tolist() == [20, 16, 20]
+    cache.extend([b], [1])
+    assert cache.page_table[1].tolist() == [2, 3, -1]
+    cache.free(c)
     cache.free(b)
     assert cache.lengths.tolist() == [20, 0, 0] and cache.page_table[1].tolist() == [-1, -1, -1]
     assert cache.compact() == 0
