@@ -22,7 +22,9 @@ constexpr int kPagedPack = 32;
 constexpr int kFill = 1024;
 constexpr int kMinRun = 256;
 constexpr int kJoinFew = 4, kJoinMany = 16;  // rows of a block of the join
-constexpr int64_t kMaxSequences = 65536;  // (each block counts through them)
+constexpr int64_t kMaxSequences = 65536;
+// From here on a launch of its own counts through the sequences.
+constexpr int64_t kPlanSequences = 256;
 
 struct PagedArgs : AttnShape {
   const uint16_t *k, *v;
@@ -33,6 +35,7 @@ struct PagedArgs : AttnShape {
   struct SplitTiles* split;
   float* partial;
   uint32_t units;  // of kFewRows rows that `partial` holds
+  struct PlanEntry* plan;  // of each sequence, and behind the last; null: every block counts
 };
 
 // A tile whose keys are in runs, for the join.
@@ -440,6 +443,61 @@ struct PagedItem {
   uint32_t tile;  // its number among the tiles in runs
 };
 
+// Keys of a run, about: tiles of few rows, and of kAttnRows.
+struct RunLengths {
+  float few, many;
+};
+
+__device__ inline RunLengths run_lengths(float work) {
+  // (a 1024th more than the mean, for what rounding can lose)
+  const float share = work * (1.0009765625f / kFill);
+  return {fmaxf(static_cast<float>(kMinRun), ceilf(share)),
+          fmaxf(static_cast<float>(kMinRun), ceilf(2.f * share))};
+}
+
+__device__ inline float tile_work(const PagedArgs& a, const PagedTile& t) {
+  return keys_seen(t) * static_cast<float>(t.tiles) * static_cast<float>(a.packs);
+}
+
+__device__ inline int runs_of(const PagedArgs& a, const PagedTile& t, const RunLengths& length) {
+  if (!a.partial || t.tiles == 0) return 1;
+  const float n = ceilf(keys_seen(t) / (t.units < kManyUnits ? length.few : length.many));
+  return n < 2.f ? 1 : (n > static_cast<float>(kWave) ? kWave : static_cast<int>(n));
+}
+
+// What comes before a sequence: blocks, units of sums, tiles in runs; and its own runs.
+struct PlanEntry {
+  uint32_t first, unit, split;
+  int runs;
+};
+
+// Block `local` of sequence `s`, with what comes before it.
+__device__ inline void place_item(const PagedArgs& a, int s, const PagedTile& own, uint32_t local,
+                                  const PlanEntry& before, PagedItem& item) {
+  const uint32_t packs = a.packs;
+  item.units = own.units;
+  item.sequence = s;
+  item.b.pack = __builtin_amdgcn_readfirstlane(local % packs);
+  item.b.split = __builtin_amdgcn_readfirstlane(local / packs % before.runs);
+  item.b.splits = before.runs;
+  // later tiles see more keys, and are begun first
+  const int tile =
+      own.tiles - 1 - static_cast<int>(__builtin_amdgcn_readfirstlane(local / packs / before.runs));
+  const uint32_t index = tile * packs + item.b.pack, step = own.units;
+  const bool few = step < kManyUnits;
+  item.unit = before.unit + (index * before.runs + item.b.split) * step;
+  item.tile = before.split + index;
+  item.b.q = own.q;
+  item.b.lk = own.lk;
+  const int64_t lq = own.q.end - own.q.begin;
+  item.b.q0 = few ? 0 : static_cast<int64_t>(tile) * a.tokens;
+  item.b.last = few || lq - item.b.q0 < a.tokens ? lq : item.b.q0 + a.tokens;
+  // (offsets that are not in order can ask for more than there is)
+  if (tile < 0 || tile >= own.tiles ||
+      (before.runs > 1 && (item.unit >= a.units || a.units - item.unit < step || item.tile >= kFill)))
+    item.sequence = -1;
+}
+
 // Tile and run of block `number`. A number beyond the last gets the count of tiles in
 // runs in `tile`.
 __device__ inline PagedItem find_item(const PagedArgs& a, uint32_t number) {
@@ -447,68 +505,64 @@ __device__ inline PagedItem find_item(const PagedArgs& a, uint32_t number) {
   PagedItem item{};
   item.sequence = -1;
   const int count = a.sq.count;
-  PagedTile own = paged_tiles(a, lane);
-  float run = 0.f, share = 0.f;
-  if (a.partial) {
-    float work = keys_seen(own) * static_cast<float>(own.tiles) * static_cast<float>(a.packs);
-    for (int s = kWave; s < count; s += kWave) {
-      const PagedTile t = paged_tiles(a, s + lane);
-      work += keys_seen(t) * static_cast<float>(t.tiles) * static_cast<float>(a.packs);
-    }
-    work = over_wave(work, [](float x, float y) { return x + y; });
-    // (a 1024th more than the mean, for what rounding can lose)
-    share = work * (1.0009765625f / kFill);
-    run = fmaxf(static_cast<float>(kMinRun), ceilf(share));
-  }
-  const float many = fmaxf(static_cast<float>(kMinRun), ceilf(2.f * share));
-  const uint32_t packs = a.packs;
   uint32_t before = 0, units_before = 0, split_before = 0;
-  for (int s0 = 0; s0 < count; s0 += kWave) {
-    if (s0 > 0) own = paged_tiles(a, s0 + lane);
-    if (a.partial && own.tiles > 0) {
-      const float n = ceilf(keys_seen(own) / (own.units < kManyUnits ? run : many));
-      own.runs = n < 2.f ? 1 : (n > static_cast<float>(kWave) ? kWave : static_cast<int>(n));
+  if (a.plan) {
+    // the last sequence that begins at or before this number, 64 candidates at a time
+    int lo = 0, span = count + 1;
+    while (span > 1) {
+      const int step = (span + kWave - 1) / kWave, off = lane * step, at = lo + (off < span ? off : 0);
+      const int n = __popcll(__ballot(off < span && a.plan[at].first <= number));
+      const int skip = n > 0 ? (n - 1) * step : 0;
+      lo += skip;
+      span = span - skip < step ? span - skip : step;
     }
-    const uint32_t tiles = static_cast<uint32_t>(own.tiles) * packs, mine = tiles * own.runs;
-    const uint32_t split = own.runs > 1 ? tiles : 0u;
-    const uint32_t units = split * own.runs * own.units;
-    const uint32_t upto = scan_wave(mine), units_upto = scan_wave(units), split_upto = scan_wave(split);
-    const uint64_t hit = __ballot(number < before + upto);
-    if (hit) {
-      const int at = __builtin_ctzll(hit);
-      const uint32_t local = number - (before + from_lane(upto - mine, at));
-      const int of = from_lane(own.tiles, at), runs = from_lane(own.runs, at);
-      item.units = from_lane(own.units, at);
-      item.sequence = s0 + at;
-      item.b.pack = __builtin_amdgcn_readfirstlane(local % packs);
-      item.b.split = __builtin_amdgcn_readfirstlane(local / packs % runs);
-      item.b.splits = runs;
-      // later tiles see more keys, and are begun first
-      const int tile = of - 1 - static_cast<int>(__builtin_amdgcn_readfirstlane(local / packs / runs));
-      const uint32_t index = tile * packs + item.b.pack, step = item.units;
-      const bool few = step < kManyUnits;
-      item.unit = units_before + from_lane(units_upto - units, at) +
-                  (index * runs + item.b.split) * step;
-      item.tile = split_before + from_lane(split_upto - split, at) + index;
-      item.b.q.begin = from_lane(static_cast<int>(own.q.begin), at);  // (rows are below 2^31)
-      item.b.q.end = from_lane(static_cast<int>(own.q.end), at);
-      item.b.lk = from_lane(own.lk, at);
-      const int64_t lq = item.b.q.end - item.b.q.begin;
-      item.b.q0 = few ? 0 : static_cast<int64_t>(tile) * a.tokens;
-      item.b.last = few || lq - item.b.q0 < a.tokens ? lq : item.b.q0 + a.tokens;
-      // (offsets that are not in order can ask for more than there is)
-      if (tile < 0 || tile >= of ||
-          (runs > 1 && (item.unit >= a.units || a.units - item.unit < step || item.tile >= kFill)))
-        item.sequence = -1;
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const PlanEntry entry = a.plan[lo];
+    if (lo < count) {
+      const PagedTile own = paged_tiles(a, lo);
+      if (number >= entry.first) place_item(a, lo, own, number - entry.first, entry, item);
       return item;
     }
-    before += from_lane(upto, kWave - 1);
-    units_before += from_lane(units_upto, kWave - 1);
-    split_before += from_lane(split_upto, kWave - 1);
+    before = entry.first;
+  } else {
+    PagedTile own = paged_tiles(a, lane);
+    RunLengths length{};
+    if (a.partial) {
+      float work = tile_work(a, own);
+      for (int s = kWave; s < count; s += kWave) work += tile_work(a, paged_tiles(a, s + lane));
+      length = run_lengths(over_wave(work, [](float x, float y) { return x + y; }));
+    }
+    for (int s0 = 0; s0 < count; s0 += kWave) {
+      if (s0 > 0) own = paged_tiles(a, s0 + lane);
+      own.runs = runs_of(a, own, length);
+      const uint32_t tiles = static_cast<uint32_t>(own.tiles) * a.packs, mine = tiles * own.runs;
+      const uint32_t split = own.runs > 1 ? tiles : 0u;
+      const uint32_t units = split * own.runs * own.units;
+      const uint32_t upto = scan_wave(mine), units_upto = scan_wave(units), split_upto = scan_wave(split);
+      const uint64_t hit = __ballot(number < before + upto);
+      if (hit) {
+        const int at = __builtin_ctzll(hit);
+        PagedTile t{};
+        t.q.begin = from_lane(static_cast<int>(own.q.begin), at);  // (rows are below 2^31)
+        t.q.end = from_lane(static_cast<int>(own.q.end), at);
+        t.lk = from_lane(own.lk, at);
+        t.tiles = from_lane(own.tiles, at);
+        t.units = from_lane(own.units, at);
+        const PlanEntry entry{before + from_lane(upto - mine, at),
+                              units_before + from_lane(units_upto - units, at),
+                              split_before + from_lane(split_upto - split, at),
+                              from_lane(own.runs, at)};
+        place_item(a, s0 + at, t, number - entry.first, entry, item);
+        return item;
+      }
+      before += from_lane(upto, kWave - 1);
+      units_before += from_lane(units_upto, kWave - 1);
+      split_before += from_lane(split_upto, kWave - 1);
+    }
+    item.tile = split_before;
   }
-  item.tile = split_before;
   // the rows behind the last sequence
-  const uint32_t local = number - before, tile = local / packs;
+  const uint32_t packs = a.packs, local = number - before, tile = local / packs;
   const RowRange rows = sequence_rows(a.sq, count);
   const int64_t lq = rows.end - rows.begin, q0 = static_cast<int64_t>(tile) * a.tokens;
   if (q0 < lq) {
@@ -522,6 +576,54 @@ __device__ inline PagedItem find_item(const PagedArgs& a, uint32_t number) {
   return item;
 }
 
+// The same scan once for all blocks, by one of them, where there are many sequences.
+// 1024 tokens on up to 1024 keys x 8 heads: see kPlanSequences.
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / kWave;
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedArgs a) {
+  __shared__ float works[kPlanWaves];
+  __shared__ uint32_t sums[3][kPlanWaves];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, count = a.sq.count;
+  RunLengths length{};
+  if (a.partial) {
+    float work = 0.f;
+    for (int s = tid; s < count; s += kPlanThreads) work += tile_work(a, paged_tiles(a, s));
+    work = over_wave(work, [](float x, float y) { return x + y; });
+    if (lane == 0) works[wave] = work;
+    __syncthreads();
+    work = 0.f;
+    for (int w = 0; w < kPlanWaves; ++w) work += works[w];
+    length = run_lengths(work);
+  }
+  uint32_t before[3] = {0, 0, 0};
+  for (int s0 = 0; s0 <= count; s0 += kPlanThreads) {
+    const int s = s0 + tid;
+    const PagedTile own = paged_tiles(a, s);
+    const int runs = runs_of(a, own, length);
+    const uint32_t tiles = static_cast<uint32_t>(own.tiles) * a.packs;
+    const uint32_t split = runs > 1 ? tiles : 0u;
+    const uint32_t mine[3] = {tiles * runs, split * runs * own.units, split};
+    uint32_t upto[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      upto[i] = scan_wave(mine[i]);
+      if (lane == kWave - 1) sums[i][wave] = upto[i];
+    }
+    __syncthreads();
+    uint32_t at[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      at[i] = before[i] + upto[i] - mine[i];
+      for (int w = 0; w < kPlanWaves; ++w) {
+        if (w < wave) at[i] += sums[i][w];
+        before[i] += sums[i][w];
+      }
+    }
+    if (s <= count) a.plan[s] = PlanEntry{at[0], at[1], at[2], runs};
+    if (s == count && a.partial) a.split->count = at[2] < kFill ? static_cast<int>(at[2]) : kFill;
+    __syncthreads();
+  }
+}
+
 template <int DV>
 __device__ inline float* sums_of(const PagedArgs& a, uint32_t unit) {
   return a.partial + static_cast<int64_t>(unit) * (kFewRows * (DV + 2));
@@ -533,7 +635,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) paged_attend_kernel(PagedArgs
   __shared__ alignas(16) uint16_t stage[2 * kAttnKeys * (DQ + DV)];
   const PagedItem item = find_item(a, blockIdx.x);
   // (the last number is beyond all tiles)
-  if (a.partial && blockIdx.x == gridDim.x - 1 && threadIdx.x == 0)
+  if (a.partial && !a.plan && blockIdx.x == gridDim.x - 1 && threadIdx.x == 0)
     a.split->count = item.tile < kFill ? static_cast<int>(item.tile) : kFill;
   if (item.sequence < 0) return;
   const AttnBlock& b = item.b;
@@ -697,6 +799,11 @@ int64_t paged_units(int64_t rows, int64_t sequences, bool packed, int64_t capaci
   return int64_t{2} * kFill * most_units(rows, sequences, packed, pack);
 }
 
+int64_t plan_bytes(int64_t sequences) {
+  if (sequences < kPlanSequences) return 0;
+  return ((sequences + 1) * static_cast<int64_t>(sizeof(PlanEntry)) + 255) / 256 * 256;
+}
+
 template <bool BF16>
 int launch_paged(const PagedArgs& a, hipStream_t s) {
   constexpr const char* kName = "lk_attention_paged";
@@ -706,6 +813,10 @@ int launch_paged(const PagedArgs& a, hipStream_t s) {
   const bool few = most_units(a.sq.rows, a.sq.count, a.sq.cu != nullptr, a.pack) < kManyUnits;
   const int parts = few ? kFewRows / kJoinFew : kAttnRows / kJoinMany;
   const int64_t tiles = std::min<int64_t>(kFill, tiles_most);
+  if (a.plan) {
+    paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
+    if (const int st = check_launch(kName)) return st;
+  }
   const dim3 grid(static_cast<unsigned>(blocks)), join(static_cast<unsigned>(tiles * parts));
 #define LK_PAGED(Q, V)                                                   \
   if (a.d_qk <= Q && a.d_v <= V) {                                       \
@@ -738,7 +849,7 @@ int64_t lk_attention_paged_workspace(int64_t rows, int64_t sequences, int64_t ca
     return -1;
   const int64_t dv = d_qk <= 64 && d_v <= 64 ? 64 : 128;
   const int64_t units = paged_units(rows, sequences, packed != 0, capacity, attention_pack(heads, kv_heads, kPagedPack));
-  return units == 0 ? 0 : kSplitBytes + units * kFewRows * (dv + 2) * 4;
+  return plan_bytes(sequences) + (units == 0 ? 0 : kSplitBytes + units * kFewRows * (dv + 2) * 4);
 }
 
 int lk_attention_paged(const void* q, const void* k_pages, const void* v_pages, void* out,
@@ -803,8 +914,14 @@ int lk_attention_paged(const void* q, const void* k_pages, const void* v_pages, 
   a.pack = pack, a.inv_pack = 65536 / pack + 1, a.tokens = kAttnRows / pack;
   a.packs = static_cast<int>(heads) / pack;
   a.units = static_cast<uint32_t>(paged_units(rows, sequences, cu != nullptr, table_width * page_rows, pack));
-  a.split = need ? static_cast<SplitTiles*>(workspace) : nullptr;
-  a.partial = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kSplitBytes) : nullptr;
+  // the plan, the tiles in runs, their sums
+  char* at = static_cast<char*>(workspace);
+  if (plan_bytes(sequences)) a.plan = reinterpret_cast<PlanEntry*>(at);
+  at += plan_bytes(sequences);
+  if (a.units) {
+    a.split = reinterpret_cast<SplitTiles*>(at);
+    a.partial = reinterpret_cast<float*>(at + kSplitBytes);
+  }
   a.scale_log2 = scale == 0.f ? 1.f : scale_log2;
   a.q_keep = scale == 0.f ? 0u : 0xFFFFFFFFu, a.q_flip = scale < 0.f ? 0x80008000u : 0u;
   const hipStream_t s = as_stream(stream);

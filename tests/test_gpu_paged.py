@@ -147,7 +147,8 @@ def _cache(rng, lengths, page_rows, hk, d_qk, d_v, dtype, spare=3, heads_first=F
 
 
 @pytest.mark.parametrize("h,hk,d,dv,rotary,offset,page_rows", [
-    (4, 2, 128, 128, 128, 0, 16), (2, 2, 192, 128, 64, 128, 64), (3, 1, 64, 40, 16, 8, 48)])
+    (4, 2, 128, 128, 128, 0, 16), (2, 2, 192, 128, 64, 128, 64), (3, 1, 64, 40, 16, 8, 48),
+    (2, 1, 40, 128, 24, 8, 32), (1, 1, 16, 256, 16, 0, 16)])
 @pytest.mark.parametrize("new,cached", [([1], [0]), ([1, 1, 1], [15, 0, 100]), ([40, 0, 1, 17], [3, 9, 64, 0]),
                                         ([5, 5], [-2, 30])])
 @pytest.mark.parametrize("heads_first", [False, True])

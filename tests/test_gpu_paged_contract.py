@@ -308,3 +308,35 @@ def test_scores_of_minus_infinity(rng, keys, rows):
     mean = v[int(table[0, 2]), :, 0].float().mean(0)
     # p of one, sums of sixteen: one rounding of the result
     assert bool(((got - mean).abs() <= 2.0 ** -8 * mean.abs() + 2.0 ** -20).all())
+
+
+@pytest.mark.parametrize("n", [255, 256, 700, 1500])
+def test_many_sequences_in_all_forms(n):
+    """Around and beyond the number from which a launch of its own counts them: each
+    sequence alone gives its results to a rounding of each side's p and sums."""
+    from local_kimi_amd.kernels import attention_paged
+
+    rng = np.random.default_rng(n)
+    new = [int(x) for x in rng.integers(0, 3, n)]
+    cached = [int(x) for x in rng.integers(0, 40, n)]
+    new[7], cached[7] = 40, 30
+    new[n - 3], cached[n - 3] = 1, 5000
+    new[n // 2], cached[n // 2] = 5, 2000
+    q, k, v, table, lengths, cu = _case(n, new, cached, h=4, hk=2, dq=64, dv=64)
+    q = torch.cat((q, torch.ones_like(q[:, :70])), 1)  # rows behind the last sequence
+    got = attention_paged(q, k, v, table, lengths, cu_seqlens=cu)
+    assert torch.equal(got, attention_paged(q, k, v, table, lengths, cu_seqlens=cu))
+    assert not got[0, sum(new):].any()
+    at, largest = np.concatenate(([0], np.cumsum(new))), v.float().abs().amax().item()
+    for s in sorted({*range(0, n, 29), 7, n // 2, n - 3, n - 1}):
+        if new[s]:
+            rows = slice(int(at[s]), int(at[s + 1]))
+            one = attention_paged(q[:, rows], k, v, table[s:s + 1], lengths[s:s + 1])
+            # p and the output rounded on both sides, each by 2^-9 of at most the largest value
+            assert (got[:, rows].float() - one.float()).abs().amax().item() <= 4 * 2.0 ** -9 * largest, s
+    # a batch of single tokens, none in runs
+    q1 = torch.randn((n, 1, 4, 64), device=DEV).bfloat16()
+    few = lengths.clamp(max=100)
+    got = attention_paged(q1, k, v, table[:, :8], few)
+    one = torch.cat([attention_paged(q1[i:i + 1], k, v, table[i:i + 1, :8], few[i:i + 1]) for i in range(0, n, 50)])
+    assert torch.equal(got[::50], one)
