@@ -389,8 +389,8 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
 // new tokens fit) for each pack of heads, and every tile's keys are taken in runs of about
 // L keys, L = a kFill-th of all keys that the call's tiles see (twice that for tiles of
 // kAttnRows), kMinRun at the least. Each block finds its tile and run by a scan over the
-// sequences, 64 at a time; the rows behind the last sequence come after all. A
-// tile in runs is noted for the join.
+// sequences, 64 at a time, or from paged_plan_kernel's; the rows behind the last sequence come
+// after all. A tile in runs is noted for the join.
 //
 // Blocks: tiles <= packs (rows / tokens + sequences + 1), and runs beyond one a tile <=
 // kFill, since L kFill >= all keys. A tile in runs has more than L keys, so there are up to
@@ -576,8 +576,8 @@ __device__ inline PagedItem find_item(const PagedArgs& a, uint32_t number) {
   return item;
 }
 
-// The same scan once for all blocks, by one of them, where there are many sequences.
-// 1024 tokens on up to 1024 keys x 8 heads: see kPlanSequences.
+// The same scan once for all blocks, by a block of its own. (Its runs may differ from those that
+// the blocks would find by a rounding of `work`; a call has the one or the others.)
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / kWave;
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedArgs a) {
   __shared__ float works[kPlanWaves];
