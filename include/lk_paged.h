@@ -14,9 +14,10 @@
  * page_table [sequences, table_width] (int32, rows table_stride apart) gives each
  * sequence's pages in order: its position i is row i % page_rows of page
  * page_table[s][i / page_rows]. lengths [sequences] (int32): a sequence's positions,
- * the call's new ones included, which are its last. Lengths are clamped to 0 ..
- * table_width * page_rows. Table entries that name no page (below 0, pages and
- * above) lead nowhere: such positions read as zeros and are not written.
+ * the call's new ones included, which are its last; below 0 counts as 0. What lies beyond
+ * table_width * page_rows is not written, and lengths are read up to there. Table entries
+ * that name no page (below 0, pages and above) lead nowhere: such positions read as
+ * zeros and are not written.
  * page_rows is a multiple of 16 up to 65536, table_width * page_rows at most 2^30.
  *
  * cu [sequences + 1] (int32): sequence s has new rows cu[s] to cu[s + 1] - 1; null
@@ -58,7 +59,7 @@ LK_API int lk_qk_norm_rope(const void* q, const void* k, const void* q_weight,
  * New row i of the n of sequence s is position p = lengths[s] - n + i: q (as above) goes
  * to q_out [rows, heads, d_qk] (dense), k (as above) and v [rows, kv_heads, d_v]
  * (as it is) to position p of k_pages and v_pages. What has no place there (p < 0,
- * no page) is not written; its q is rotated as position 0. Rows behind the last sequence
+ * beyond the table, no page) is not written; p < 0 is rotated as 0. Rows behind the last sequence
  * write nothing to the cache; their q_out is zeros. heads may be 0 (q, q_out, q_weight unused),
  * rotary 0 (no rotation). dtype is LK_DTYPE_F16 or LK_DTYPE_BF16. Two rows must
  * not go to one place: pages that take new rows belong to one sequence. The places

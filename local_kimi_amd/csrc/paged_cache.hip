@@ -174,9 +174,10 @@ __global__ void __launch_bounds__(kHeadThreads) head_rope_kernel(HeadArgs a) {
       int pos = -1;
       int64_t kp = -1, vp = -1;
       if (s < a.sq.count && t >= rows.begin && t < rows.end) {
-        const int64_t at = cached_length(a.table, s) - (rows.end - t);
+        const int64_t length = a.table.lengths[s];
+        const int64_t at = (length < 0 ? 0 : length) - (rows.end - t);
         pos = at < 0 ? 0 : static_cast<int>(at);
-        if (at >= 0) {
+        if (at >= 0 && at < static_cast<int64_t>(a.table.width) * a.table.page_rows) {
           const uint32_t block = static_cast<uint32_t>(pos) / static_cast<uint32_t>(a.table.page_rows);
           const int64_t page = a.table.pages_of[s * a.table.stride + block];
           const int64_t row = pos - static_cast<int64_t>(block) * a.table.page_rows;

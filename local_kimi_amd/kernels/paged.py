@@ -259,8 +259,8 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pag
     Token i of the n that the call has of sequence s is position ``lengths[s]`` - n + i.
     B sequences of S new tokens each, or with ``cu_seqlens`` [N + 1] (int32 or int64, on
     the device, from 0, not decreasing) one row of N packed ones. A token without a place
-    (a position below 0, no page) is not written, and rotated as position 0 where that is
-    below 0; rows behind the last sequence write nothing and return zeros. Two sequences'
+    (a position below 0 or beyond the table, no page) is not written; positions below 0 are
+    rotated as 0. Rows behind the last sequence write nothing and return zeros. Two sequences'
     new tokens must not share a page: copy a forked sequence's last page first
     (``PagedCache.extend`` does). The cache's places must not overlap."""
     batch, rows, heads, kv_heads, d, dtype, device = _check_heads(q, k)

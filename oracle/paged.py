@@ -40,11 +40,11 @@ def places(table, lengths, page_rows, pages, rows, cu=None):
     """Sequence (-1: none), position, page (-1: none) and row in it of each new row."""
     out = np.full((rows, 4), -1, dtype=np.int64)
     for s, (at, n) in enumerate(bounds(cu, rows, len(lengths))):
-        length = min(max(int(lengths[s]), 0), table.shape[1] * page_rows)
+        length = max(int(lengths[s]), 0)
         for i in range(n):
             p = length - n + i
             out[at + i] = s, p, -1, -1
-            if p >= 0 and 0 <= table[s, p // page_rows] < pages:
+            if 0 <= p < table.shape[1] * page_rows and 0 <= table[s, p // page_rows] < pages:
                 out[at + i, 2:] = table[s, p // page_rows], p % page_rows
     return out
 

@@ -206,9 +206,13 @@ def test_appends_write_nowhere_without_a_page(rng):
     table = torch.tensor([[-1, -5], [4, 2 ** 31 - 1], [-(2 ** 31), 7], [0, 1], [2, 3]], dtype=torch.int32,
                          device=DEV)
     paged_append(k, 2 * k, *dev, table, torch.tensor([3, 20, 1, 0, 2 ** 31 - 1], dtype=torch.int32, device=DEV))
-    for t, x in zip(dev, (1, 2)):  # the last sequence alone has a place: the table's last
+    assert not dev[0].any() and not dev[1].any()
+    # three tokens of which the first alone is within the table
+    three = k[:1].expand(1, 3, 2, 64) * torch.arange(1, 4, device=DEV)[:, None, None].half()
+    paged_append(three, three, *dev, table[3:4], torch.tensor([34], device=DEV))
+    for t in dev:
         want = torch.zeros_like(t)
-        want[3, 15] = x
+        want[1, 15] = 1
         assert torch.equal(t, want)
 
 

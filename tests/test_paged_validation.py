@@ -228,6 +228,7 @@ def test_the_oracles_forms_agree(rng):
     got = P.places(table, [20, 40], 16, 4, 5, np.array([0, 2, 4]))
     assert got.tolist() == [[0, 18, 0, 2], [0, 19, 0, 3], [1, 38, 2, 6], [1, 39, 2, 7], [-1, -1, -1, -1]]
     assert P.places(table, [1, 20], 16, 4, 4)[:, 1:].tolist() == [[-1, -1, -1], [0, 3, 0], [18, -1, -1], [19, -1, -1]]
+    assert P.places(table, [0, 50], 16, 4, 2)[:, 1:].tolist() == [[-1, -1, -1], [49, -1, -1]]
     x, a = rng.normal(size=(3, 2, 16)), rng.uniform(0, 6, (9, 4))
     cs = np.concatenate((np.cos(a), np.sin(a)), 1)
     for interleaved in (False, True):
