@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kHeadThreads) head_rope_kernel(HeadArgs a) {
             }
           }
           if (turned) {
-// interleaved: pair i lies at values 2 i and 2 i + 1 of the two groups
+            // interleaved: pair i lies at values 2 i and 2 i + 1 of the two groups
             float p[G], q[G];
 #pragma unroll
             for (int i = 0; i < G; ++i) {
