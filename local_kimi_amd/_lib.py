@@ -87,7 +87,7 @@ SIGNATURES: dict[str, list] = {
                         _I64, _I64, _I64, _I, _I64, _I, _F, _I, _I, _P],
     "lk_paged_append": [*[_P] * 12, *[_I64] * 24, _I, _I64, _F, _I, _I, _P],
     "lk_attention_paged": [*[_P] * 7, *[_I64] * 18, _F, _I, _P, _I64, _P],
-    "lk_copy_pages": [_P, _P, _P, _I64, _P, _P, _I64, _I64, _P],
+    "lk_copy_pages": [_P, _P, _P, _I64, _P, _P, _I64, _I64, _P, _P],
     "lk_rms_norm": [_P, _P, _P, _I64, _I64, _F, _I, _I, _P],
     "lk_add_rms_norm": [_P, _P, _P, _P, _P, _I64, _I64, _F, _I, _I, _P],
     "lk_rms_gated_norm": [_P, _P, _P, _P, _I64, _I64, _F, _I, _I, _I, _I, _P],

@@ -371,23 +371,36 @@ bool places_apart(int64_t d, int64_t pages, int64_t page, int64_t rows, int64_t 
 // Copies of pages
 
 constexpr int kCopyThreads = 256;
-constexpr int kCopyPairs = 192;    // of a launch: the lists travel as its arguments
+constexpr int kCopyPairs = 192;    // of a launch whose lists travel as its arguments
 constexpr int kCopyTensors = 64;   // of a launch
 
 struct CopyArgs {
   char* tensor[kCopyTensors];
   int64_t stride[kCopyTensors];
   int32_t chunks[kCopyTensors];  // of 16 bytes a page
+  const int32_t *src_of, *dst_of;  // lists in device memory, else null and here:
   int32_t src[kCopyPairs], dst[kCopyPairs];
+  int32_t pairs;
 };
 static_assert(sizeof(CopyArgs) <= 4096, "kernel arguments");
 
+// 16 bytes a thread. Bound by HBM (1100 pages of 128 KB in 4 tensors, 1.15 GB: 205 us, 5.6 TB/s; in
+// six launches, the lists in their arguments, 217). PACKED: pages smaller than a block's threads
+// follow one another in a block.
+template <bool PACKED>
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(CopyArgs a) {
-  const int z = blockIdx.z, pair = blockIdx.y;
-  const uint4* const from = reinterpret_cast<const uint4*>(a.tensor[z] + a.src[pair] * a.stride[z]);
-  uint4* const to = reinterpret_cast<uint4*>(a.tensor[z] + a.dst[pair] * a.stride[z]);
-  const int i = blockIdx.x * kCopyThreads + threadIdx.x;
-  if (i < a.chunks[z]) to[i] = from[i];
+  const int z = blockIdx.z, chunks = a.chunks[z];
+  uint32_t i = blockIdx.x * kCopyThreads + threadIdx.x, pair = blockIdx.y;
+  if constexpr (PACKED) {
+    if (chunks == 0) return;
+    pair = i / static_cast<uint32_t>(chunks);
+    i -= pair * chunks;
+  }
+  if (pair >= static_cast<uint32_t>(a.pairs) || i >= static_cast<uint32_t>(chunks)) return;
+  const int64_t src = a.src_of ? a.src_of[pair] : a.src[pair];
+  const int64_t dst = a.dst_of ? a.dst_of[pair] : a.dst[pair];
+  reinterpret_cast<uint4*>(a.tensor[z] + dst * a.stride[z])[i] =
+      reinterpret_cast<const uint4*>(a.tensor[z] + src * a.stride[z])[i];
 }
 
 // A page is written once, and is no other pair's source: what a launch reads it
@@ -516,7 +529,7 @@ int lk_paged_append(const void* q, const void* k, const void* v, const void* q_w
 
 int lk_copy_pages(void* const* tensors, const int64_t* page_strides, const int64_t* page_bytes,
                   int64_t count, const int32_t* src, const int32_t* dst, int64_t pairs,
-                  int64_t pages, void* stream) {
+                  int64_t pages, const int32_t* lists, void* stream) {
   LK_REQUIRE(count >= 0 && pairs >= 0 && pages >= 0 && pages < (int64_t{1} << 31) &&
                  pairs < (int64_t{1} << 31),
              "tensors, pairs and pages must be in 0 .. 2^31 - 1");
@@ -535,21 +548,32 @@ int lk_copy_pages(void* const* tensors, const int64_t* page_strides, const int64
   if (const int st = check_pairs(src, dst, pairs, pages)) return st;
   if (most == 0) return LK_OK;
   const hipStream_t s = as_stream(stream);
+  const int64_t chunks = most / 16;
+  const bool packed = chunks < kCopyThreads;
+  // of a launch: what its arguments hold, or a grid takes
+  const int64_t step = lists ? (packed ? (int64_t{1} << 30) / chunks : 65535) : kCopyPairs;
   for (int64_t z0 = 0; z0 < count; z0 += kCopyTensors)
-    for (int64_t p0 = 0; p0 < pairs; p0 += kCopyPairs) {
+    for (int64_t p0 = 0; p0 < pairs; p0 += step) {
       CopyArgs a{};
       const int z = static_cast<int>(std::min<int64_t>(kCopyTensors, count - z0));
-      const int n = static_cast<int>(std::min<int64_t>(kCopyPairs, pairs - p0));
+      const int64_t n = std::min<int64_t>(step, pairs - p0);
       for (int i = 0; i < z; ++i) {
         a.tensor[i] = static_cast<char*>(tensors[z0 + i]);
         a.stride[i] = page_strides[z0 + i];
         a.chunks[i] = static_cast<int32_t>(page_bytes[z0 + i] / 16);
       }
-      std::copy(src + p0, src + p0 + n, a.src);
-      std::copy(dst + p0, dst + p0 + n, a.dst);
-      const dim3 grid(static_cast<unsigned>((most / 16 + kCopyThreads - 1) / kCopyThreads),
-                      static_cast<unsigned>(n), static_cast<unsigned>(z));
-      copy_pages_kernel<<<grid, kCopyThreads, 0, s>>>(a);
+      a.pairs = static_cast<int32_t>(n);
+      if (lists) {
+        a.src_of = lists + p0, a.dst_of = lists + pairs + p0;
+      } else {
+        std::copy(src + p0, src + p0 + n, a.src);
+        std::copy(dst + p0, dst + p0 + n, a.dst);
+      }
+      const int64_t blocks = ((packed ? n : 1) * chunks + kCopyThreads - 1) / kCopyThreads;
+      const dim3 grid(static_cast<unsigned>(blocks), packed ? 1u : static_cast<unsigned>(n),
+                      static_cast<unsigned>(z));
+      if (packed) copy_pages_kernel<true><<<grid, kCopyThreads, 0, s>>>(a);
+      else copy_pages_kernel<false><<<grid, kCopyThreads, 0, s>>>(a);
       if (const int st = check_launch("lk_copy_pages")) return st;
     }
   return LK_OK;

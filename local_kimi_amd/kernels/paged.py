@@ -34,6 +34,9 @@ from .kda import _aligned, _offsets
 HEAD_MAX_DIM = 256
 PAGE_ROWS_STEP = 16
 
+_COPY_PAIRS = 192  # that a launch has room for in its arguments
+_ERR_ARGUMENT = 1
+
 _DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
@@ -376,7 +379,7 @@ def _page_list(pages: Sequence[int] | torch.Tensor, what: str) -> array:
 def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int] | torch.Tensor,
                dst: Sequence[int] | torch.Tensor) -> None:
     """Page ``src[i]`` to page ``dst[i]`` (dimension 0) of every tensor: all layers' caches,
-    in one launch per 192 pairs of 64 tensors.
+    in one launch for 64 tensors (while a graph is captured: and 192 pairs).
 
     ``src`` and ``dst`` are sequences of integers or integer tensors on the host; a page is
     written once at most, and is no other pair's source (ValueError). A captured graph
@@ -409,13 +412,15 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int] | torch.Tenso
         raise ValueError("the HIP copy requires CUDA tensors")
     if not a:
         return
-    if min(a) < 0 or max(a) >= pages or min(b) < 0 or max(b) >= pages:
-        raise ValueError(f"page numbers must be in 0 .. {pages - 1}")
-    moved = [x for x in zip(a, b) if x[0] != x[1]]
-    written = {y for _, y in moved}
-    if len(written) != len(moved) or not written.isdisjoint(x for x, _ in moved):
-        raise ValueError("a page may be written once, and not be another pair's source")
+    count, lists = len(a), None
+    if count > _COPY_PAIRS and not torch.cuda.is_current_stream_capturing():
+        # from pinned memory of its own, so that the upload takes its turn on the stream
+        lists = torch.frombuffer(a + b, dtype=torch.int32).pin_memory().to(device, non_blocking=True)
     tables = [array("q", x) for x in (pointers, steps, sizes)]
     with _w._on(device):
-        _lib.call("lk_copy_pages", *(t.buffer_info()[0] for t in tables), len(pointers),
-                  a.buffer_info()[0], b.buffer_info()[0], len(a), pages, _w._stream(device))
+        status = _lib.load().lk_copy_pages(
+            *(t.buffer_info()[0] for t in tables), len(pointers), a.buffer_info()[0],
+            b.buffer_info()[0], count, pages, _pointer(lists), _w._stream(device))
+    if status:
+        message = _lib.load().lk_last_error().decode(errors="replace")
+        raise (ValueError if status == _ERR_ARGUMENT else RuntimeError)(f"lk_copy_pages: {message}")

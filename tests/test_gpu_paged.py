@@ -377,7 +377,7 @@ def test_graph_replays_with_other_lengths_and_pages(rng):
 # copies, and all of it together
 
 
-@pytest.mark.parametrize("pairs", [1, 3, 200, 700])
+@pytest.mark.parametrize("pairs", [1, 3, 192, 193, 700, 30000])
 def test_copies_of_pages(rng, pairs):
     from local_kimi_amd.kernels import copy_pages
 
@@ -395,6 +395,17 @@ def test_copies_of_pages(rng, pairs):
         w[dst] = w[src]
         assert torch.equal(t, w)
     copy_pages([ts[0]] * 70, [], [])
+    graph, t = torch.cuda.CUDAGraph(), ts[0]  # the lists travel as arguments
+    with torch.cuda.graph(graph):
+        copy_pages(ts, dst, src if pairs == 1 else [int(x) for x in order[:pairs]])
+    t.normal_()
+    first = t.clone()
+    for _ in range(3):
+        t.copy_(first)
+        graph.replay()
+        want = first.clone()
+        want[[int(x) for x in order[:pairs]]] = first[dst]
+        assert torch.equal(t, want)
     many = [torch.full((2, 16), float(i), device=DEV) for i in range(70)]
     for i, t in enumerate(many):
         t[1] = -i
@@ -407,8 +418,9 @@ def test_copies_that_depend_on_each_other_are_refused():
 
     t = torch.randn((8, 16, 2, 8), device=DEV)
     want = t.clone()
-    for src, dst, match in (([0, 1], [2, 2], "written once"), ([0, 2], [2, 3], "source"), ([0, 1], [1, 0], "source"),
-                            ([8], [1], "0 .. 7"), ([0], [-1], "0 .. 7"), (torch.tensor([1]), [9], "0 .. 7")):
+    for src, dst, match in (([0, 1], [2, 2], "written twice"), ([0, 2], [2, 3], "both read"), ([0, 1], [1, 0], "both read"),
+                            ([8], [1], "page 8 to 1 of a cache of 8"), ([0], [-1], "to -1"), (torch.tensor([1]), [9], "to 9"),
+                            ([0] * 300, [1] * 300, "written twice")):
         with pytest.raises(ValueError, match=match):
             copy_pages([t], src, dst)
     copy_pages([t], [3, 4], [3, 4])

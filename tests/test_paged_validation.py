@@ -203,7 +203,7 @@ def test_c_abi_refusals_come_before_any_launch(lib):
 def _copy(src, dst, pages=8, pointer=16, stride=4096, size=4096, count=1, pairs=None):
     ints = [(ctypes.c_int32 * max(1, len(x)))(*x) for x in (src, dst)]
     _lib.call("lk_copy_pages", (ctypes.c_void_p * 1)(pointer), (ctypes.c_int64 * 1)(stride),
-              (ctypes.c_int64 * 1)(size), count, *ints, len(src) if pairs is None else pairs, pages, None)
+              (ctypes.c_int64 * 1)(size), count, *ints, len(src) if pairs is None else pairs, pages, None, None)
 
 
 def test_copies_are_refused_that_depend_on_each_other(lib):
