@@ -14,8 +14,9 @@
  * page_table [sequences, table_width] (int32, rows table_stride apart) gives each
  * sequence's pages in order: its position i is row i % page_rows of page
  * page_table[s][i / page_rows]. lengths [sequences] (int32): a sequence's positions,
- * the call's new ones included, which are its last; below 0 counts as 0. What lies beyond
- * table_width * page_rows is not written, and lengths are read up to there. Table entries
+ * the call's new ones included, which are its last; below 0 counts as 0. Positions beyond
+ * table_width * page_rows are not written and not seen: rows keep the positions that the
+ * length gives them, also where it passes that. Table entries
  * that name no page (below 0, pages and above) lead nowhere: such positions read as
  * zeros and are not written.
  * page_rows is a multiple of 16 up to 65536, table_width * page_rows at most 2^30.
@@ -82,7 +83,7 @@ LK_API int lk_paged_append(const void* q, const void* k, const void* v, const vo
  * q [rows, heads, d_qk] (strided as above), out [rows, heads, d_v] (dense, overlaps
  * nothing), all in dtype (LK_DTYPE_F16 or LK_DTYPE_BF16); query head h reads key head
  * h / (heads / kv_heads). d_qk is a multiple of 8 up to 192, d_v up to 128. Query i of
- * the n of sequence s sees positions 0 .. lengths[s] - n + i. One that sees none
+ * the n of sequence s sees positions 0 .. lengths[s] - n + i, within the table. One that sees none
  * gets zeros, as do the rows behind the last sequence.
  *   o_i = sum_j p_ij v_j,  p_i = softmax over the positions seen of scale * q_i . k_j
  * Scores and sums in fp32; p is rounded to dtype for its product with v. What a query

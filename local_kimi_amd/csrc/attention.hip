@@ -56,7 +56,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attention_kernel(AttnArgs a) 
   const int64_t q0 = at.tile * a.tokens;
   if (q0 >= lq) return;
   const int64_t last = q0 + a.tokens < lq ? q0 + a.tokens : lq;  // the block's, exclusive
-  const AttnBlock b{tile.q, tile.k.end - tile.k.begin, q0, last, pack, split, a.splits};
+  const int64_t lk = tile.k.end - tile.k.begin;
+  const AttnBlock b{tile.q, lk, lk - (tile.q.end - tile.q.begin), q0, last, pack, split, a.splits};
   f32x16_t o[kVTiles];
 #pragma unroll
   for (int t = 0; t < kVTiles; ++t)

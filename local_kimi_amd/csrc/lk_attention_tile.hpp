@@ -33,6 +33,7 @@ struct AttnShape {
 struct AttnBlock {
   RowRange q;  // rows of the sequence
   int64_t lk;  // its keys
+  int64_t ahead;  // query i sees those up to ahead + i (lk - lq, or more: all of them at lk)
   int64_t q0, last;
   int pack, split, splits;
 };
@@ -212,9 +213,13 @@ __device__ __forceinline__ void attend_rows(const AttnShape& a, const AttnBlock&
   const int row = wave * 32 + n, token = row * a.inv_pack >> 16;
   const int64_t qi = q0 + token;  // the lane's, of this head
   const int h = b.pack * a.pack + row - token * a.pack;
-  const int64_t ahead = lk - lq;
+  const int64_t ahead = b.ahead;
+  // the last key that the lane's query sees, and the wave's first
+  const int sees = static_cast<int>(qi + ahead < lk ? qi + ahead : lk - 1);
+  const int first_sees = static_cast<int>(qw + ahead < lk ? qw + ahead : lk - 1);
   // keys seen by the block's last query, and by the wave's
-  const int64_t all = last + ahead < 0 ? 0 : last + ahead;
+  const int64_t most_seen = last + ahead < lk ? last + ahead : lk;
+  const int64_t all = most_seen < 0 ? 0 : most_seen;
   // this block's run of them, and the wave's end of it
   const int64_t per = ((all + b.splits - 1) / b.splits + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
   const int64_t from = b.split * per < all ? b.split * per : all;
@@ -304,11 +309,11 @@ __device__ __forceinline__ void attend_rows(const AttnShape& a, const AttnBlock&
       // an infinity or a NaN in V would turn into one of its own: such values
       // are taken out of the product there and added at the end, for the
       // queries that see them.
-      const bool edge = k0 + kAttnKeys - 1 > qw + ahead;  // a query does not see all of them
+      const bool edge = k0 + kAttnKeys - 1 > first_sees;  // a query does not see all of them
       if (edge) {
         // keys of this tile that the lane's query sees, from its first register on
-        const int seen =
-            static_cast<int>(qi + ahead - k0 < kAttnKeys ? qi + ahead - k0 + 1 : kAttnKeys) - 4 * half;
+        const int left = sees - static_cast<int>(k0);
+        const int seen = (left < kAttnKeys ? left + 1 : kAttnKeys) - 4 * half;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -376,7 +381,7 @@ __device__ __forceinline__ void attend_rows(const AttnShape& a, const AttnBlock&
   sum += __shfl_xor(sum, 32);
   if (__builtin_expect(bad, 0)) {
     // the infinities and NaNs left out above, for the queries that see them
-    int64_t key = qw + ahead + 1 < 0 ? 0 : (qw + ahead + 1) / kAttnKeys * kAttnKeys;
+    int64_t key = first_sees < 0 ? 0 : (first_sees + int64_t{1}) / kAttnKeys * kAttnKeys;
     key = key < from ? from : key;
     int left = a.d_v - 4 * half;
 #pragma unroll 1
@@ -389,7 +394,7 @@ __device__ __forceinline__ void attend_rows(const AttnShape& a, const AttnBlock&
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int d = 32 * t + 8 * (r / 4) + r % 4;
-          const float x = d < left && key <= qi + ahead ? value_of<BF16>(row[4 * half + d]) : 0.f;
+          const float x = d < left && key <= sees ? value_of<BF16>(row[4 * half + d]) : 0.f;
           if (!(fabsf(x) < INFINITY)) o[t][r] += x;
         }
     }

@@ -33,6 +33,13 @@ struct PageTable {
   int width, page_rows;
 };
 
+// The position of the first of sequence s's n new rows (below 0: it has no place), whatever the
+// table can name: the last rows of a length beyond it have no place, the others keep theirs.
+__device__ inline int64_t positions_before(const PageTable& t, int s, int64_t n) {
+  const int64_t length = t.lengths[s];
+  return (length < 0 ? 0 : length) - n;
+}
+
 // Positions of sequence s, its new ones among them: within what its row of the table can name.
 __device__ inline int64_t cached_length(const PageTable& t, int s) {
   const int64_t n = t.lengths[s], most = static_cast<int64_t>(t.width) * t.page_rows;

@@ -185,7 +185,11 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
   int token[GROUPS];
 #pragma unroll
   for (int j = 0; j < GROUPS; ++j) token[j] = (kFewRows * j + n) * a.inv_pack >> 16;
-  const int ahead = lk - lq;  // query i sees the keys up to ahead + i
+  const int ahead = static_cast<int>(b.ahead);
+  const int first_sees = ahead < lk ? ahead : lk - 1;  // the last key that the first query sees
+  int sees[GROUPS];                                    // and the lane's
+#pragma unroll
+  for (int j = 0; j < GROUPS; ++j) sees[j] = token[j] + ahead < lk ? token[j] + ahead : lk - 1;
   const int per = ((lk + b.splits - 1) / b.splits + kAttnKeys - 1) / kAttnKeys * kAttnKeys;
   const int64_t from64 = static_cast<int64_t>(b.split) * per;
   const int from = from64 < lk ? static_cast<int>(from64) : lk;
@@ -246,7 +250,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (k0 + 2 * kAttnKeys < to) keys_of.template fetch<true>(k0 + 2 * kAttnKeys, buf);
     if (p0 < lk) {
-      const bool edge = p0 + kPageStep - 1 > ahead;  // not seen by every query
+      const bool edge = p0 + kPageStep - 1 > first_sees;  // not seen by every query
       if (edge) {
 #pragma unroll
         for (int t = 0; t < kVTiles; ++t) {
@@ -264,7 +268,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
 #pragma unroll
         for (int i = 0; i < kQSteps; ++i) s = mfma16<BF16>(kf[i], qf[j][i], s);
         if (edge) {
-          const int seen = token[j] + ahead + 1 - p0 - 4 * g;
+          const int seen = sees[j] + 1 - p0 - 4 * g;
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[i] = i < seen ? s[i] : -INFINITY;
         }
@@ -312,7 +316,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
 #pragma unroll 1
     for (int key = from; key < to; ++key) {
       const int p0 = key / kPageStep * kPageStep;
-      if ((p0 - from) / kPageStep % kAttnWaves != wave || p0 + kPageStep - 1 <= ahead) continue;
+      if ((p0 - from) / kPageStep % kAttnWaves != wave || p0 + kPageStep - 1 <= first_sees) continue;
       const uint16_t* const row = keys_of.value_row(key);
       if (!row) continue;
       asm volatile("" : "+v"(left));  // (as in attend_rows)
@@ -323,7 +327,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int d = 16 * t + i;
-            const float x = d < left && key <= token[j] + ahead ? value_of<BF16>(row[4 * g + d]) : 0.f;
+            const float x = d < left && key <= sees[j] ? value_of<BF16>(row[4 * g + d]) : 0.f;
             if (!(fabsf(x) < INFINITY)) o[j][t][i] += x;
           }
     }
@@ -399,6 +403,7 @@ __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& 
 struct PagedTile {
   RowRange q;
   int lk, tiles, runs;
+  int ahead;  // positions before its first new one, lk at the most
   int units;  // of kFewRows rows that a tile has: 1, 2 or those of kAttnRows
 };
 constexpr int kManyUnits = kAttnRows / kFewRows;
@@ -410,6 +415,8 @@ __device__ inline PagedTile paged_tiles(const PagedArgs& a, int s) {
   const int lq = static_cast<int>(t.q.end - t.q.begin);
   if (lq == 0) return t;
   t.lk = static_cast<int>(cached_length(a.table, s));
+  t.ahead = static_cast<int>(positions_before(a.table, s, lq));
+  t.ahead = t.ahead < t.lk ? t.ahead : t.lk;
   const int64_t rows = static_cast<int64_t>(lq) * a.pack;
   t.units = rows <= kFewRows ? 1 : (rows <= 2 * kFewRows ? 2 : kManyUnits);
   t.tiles = t.units < kManyUnits ? 1 : (lq + a.tokens - 1) / a.tokens;
@@ -489,6 +496,7 @@ __device__ inline void place_item(const PagedArgs& a, int s, const PagedTile& ow
   item.tile = before.split + index;
   item.b.q = own.q;
   item.b.lk = own.lk;
+  item.b.ahead = own.ahead;
   const int64_t lq = own.q.end - own.q.begin;
   item.b.q0 = few ? 0 : static_cast<int64_t>(tile) * a.tokens;
   item.b.last = few || lq - item.b.q0 < a.tokens ? lq : item.b.q0 + a.tokens;
@@ -546,6 +554,7 @@ __device__ inline PagedItem find_item(const PagedArgs& a, uint32_t number) {
         t.q.begin = from_lane(static_cast<int>(own.q.begin), at);  // (rows are below 2^31)
         t.q.end = from_lane(static_cast<int>(own.q.end), at);
         t.lk = from_lane(own.lk, at);
+        t.ahead = from_lane(own.ahead, at);
         t.tiles = from_lane(own.tiles, at);
         t.units = from_lane(own.units, at);
         const PlanEntry entry{before + from_lane(upto - mine, at),

@@ -174,8 +174,7 @@ __global__ void __launch_bounds__(kHeadThreads) head_rope_kernel(HeadArgs a) {
       int pos = -1;
       int64_t kp = -1, vp = -1;
       if (s < a.sq.count && t >= rows.begin && t < rows.end) {
-        const int64_t length = a.table.lengths[s];
-        const int64_t at = (length < 0 ? 0 : length) - (rows.end - t);
+        const int64_t at = positions_before(a.table, s, rows.end - rows.begin) + (t - rows.begin);
         pos = at < 0 ? 0 : static_cast<int>(at);
         if (at >= 0 && at < static_cast<int64_t>(a.table.width) * a.table.page_rows) {
           const uint32_t block = static_cast<uint32_t>(pos) / static_cast<uint32_t>(a.table.page_rows);

@@ -296,9 +296,9 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``q`` [B, S, H, d_qk], float16 or bfloat16 like the cache; H a multiple of H_kv, d_qk
     a multiple of 8 up to 192, d_v up to 128. B sequences of S new tokens, or with
     ``cu_seqlens`` [N + 1] one row of N packed ones, single tokens and long pieces side by
-    side. New token i of n sees positions 0 .. ``lengths[s]`` - n + i; one that sees none
-    gets zeros, as do the rows behind the last sequence. Lengths are clamped to what the
-    table's row can name; positions without a page read as zeros.
+    side. New token i of n sees positions 0 .. ``lengths[s]`` - n + i, of those that the table's
+    row can name; one that sees none gets zeros, as do the rows behind the last sequence.
+    Positions within the table that have no page read as zeros.
 
     Returns [B, S, H, d_v] in q's dtype. ``scale`` defaults to d_qk ** -0.5. Scores and
     sums are fp32; the probabilities are rounded to the inputs' dtype for their product

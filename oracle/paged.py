@@ -51,12 +51,15 @@ def places(table, lengths, page_rows, pages, rows, cu=None):
 
 def attention_paged(q, k_pages, v_pages, table, lengths, scale, cu=None):
     """q [T, H, dqk], pages [P, R, Hkv, d]: each sequence's positions gathered in order
-    (zeros where there is no page), then the attention of dense keys. Returns its
-    (out, spread, score) and the longest sequence."""
+    (zeros where there is no page, none beyond the table), then for each token the attention of
+    dense keys, of which it sees those up to its own position. Returns its (out, spread, score)
+    and the longest sequence."""
     page_rows = k_pages.shape[1]
-    keys, values, total = [], [], [0]
+    at = places(table, lengths, page_rows, k_pages.shape[0], q.shape[0], cu)[:, :2]
+    most = table.shape[1] * page_rows
+    keys, values = [], []
     for s, length in enumerate(lengths):
-        length = min(max(int(length), 0), table.shape[1] * page_rows)
+        length = min(max(int(length), 0), most)
         for pages, out in ((k_pages, keys), (v_pages, values)):
             rows = np.zeros((length, *pages.shape[2:]))
             for p in range(length):
@@ -64,7 +67,12 @@ def attention_paged(q, k_pages, v_pages, table, lengths, scale, cu=None):
                 if 0 <= page < pages.shape[0]:
                     rows[p] = pages[page, p % page_rows]
             out.append(rows)
-        total.append(total[-1] + length)
-    got = attention_prefill(q, np.concatenate(keys), np.concatenate(values), scale, len(lengths), cu,
-                            np.array(total))
-    return (*got, max(np.diff(total), default=0))
+    got = [np.zeros((*q.shape[:2], v_pages.shape[3])), np.zeros((*q.shape[:2], v_pages.shape[3])),
+           np.zeros(q.shape[:2])]
+    for i, (s, p) in enumerate(at):
+        seen = min(p + 1, most)
+        if s >= 0 and seen > 0:
+            one = attention_prefill(q[i:i + 1], keys[s][:seen], values[s][:seen], scale)
+            for t, x in zip(got, one):
+                t[i] = x[0]
+    return (*got, max((len(k) for k in keys), default=0))
