@@ -113,8 +113,8 @@ LK_API int lk_attention_paged(const void* q, const void* k_pages, const void* v_
  * tensors, page_strides, page_bytes: host arrays of `count` device pointers, bytes from
  * a page to the next and bytes of a page (dense, multiples of 16, pointers on 16
  * bytes). src, dst: host arrays of `pairs` page numbers in 0 .. pages - 1; a page is
- * written once at most and is not a source too (a pair of one page with
- * itself does nothing); others are refused. The host's lists are read before the call
+ * written once at most and is not a source too; others are refused. A pair of one page
+ * with itself does nothing and counts for neither. The host's lists are read before the call
  * returns. lists: null, or device memory of 2 pairs int32 with src, then dst, which saves a launch
  * for every 192 pairs. */
 LK_API int lk_copy_pages(void* const* tensors, const int64_t* page_strides,

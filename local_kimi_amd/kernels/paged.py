@@ -382,8 +382,8 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int] | torch.Tenso
     in one launch for 64 tensors (while a graph is captured: and 192 pairs).
 
     ``src`` and ``dst`` are sequences of integers or integer tensors on the host; a page is
-    written once at most, and is no other pair's source (ValueError). A captured graph
-    keeps the lists it was captured with. Pages must be dense, in any order of their
+    written once at most, and is no other pair's source (ValueError); a pair of a page with
+    itself does nothing. A captured graph keeps the lists it was captured with. Pages must be dense, in any order of their
     dimensions, and multiples of 16 bytes; the tensors must not overlap each other."""
     a, b = _page_list(src, "src"), _page_list(dst, "dst")
     if len(a) != len(b):
