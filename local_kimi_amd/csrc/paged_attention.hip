@@ -744,10 +744,12 @@ __global__ void __launch_bounds__(kAttnThreads) paged_join_kernel(PagedArgs a, i
   const int index = static_cast<int>(blockIdx.x) / parts;
   if (index >= a.split->count) return;
   const SplitTile tile = a.split->tile[index];
-  // (offsets that are not in order can leave tiles unnoted: nothing outside the tensors)
+  // (offsets that are not in order can leave tiles unnoted, so that this is what the workspace held:
+  // whatever that is, nothing outside the tensors)
   if (tile.runs < 2 || tile.runs > kWave || tile.pack < 0 || tile.pack >= a.packs || tile.row < 0 ||
       tile.units < 1 || tile.units > kManyUnits || tile.rows < 0 ||
-      tile.rows > tile.units * kFewRows || tile.row + tile.rows / a.pack > a.sq.rows ||
+      tile.rows > tile.units * kFewRows || tile.row > a.sq.rows ||
+      (a.sq.rows - tile.row) * a.pack < tile.rows ||
       tile.unit >= a.units || a.units - tile.unit < static_cast<uint32_t>(tile.runs * tile.units))
     return;
   const int lane = threadIdx.x & (kWave - 1), runs = tile.runs;
