@@ -205,7 +205,12 @@ class PagedCache:
         return len(copies[0])
 
     def rows_of(self, sequences: Sequence[int]) -> tuple[torch.Tensor, torch.Tensor]:
-        """``page_table`` and ``lengths`` of these sequences, in this order (copies)."""
+        """``page_table`` and ``lengths`` of these sequences, in this order (copies); one that is
+        not in use has length 0 and no pages."""
+        sequences = [int(s) for s in sequences]
+        for s in sequences:
+            if not 0 <= s < len(self.book.pages):  # (an index on the device would fault there)
+                raise ValueError(f"there is no sequence {s} of {len(self.book.pages)}")
         at = torch.empty(len(sequences), dtype=torch.int64, device=self.lengths.device)
-        self._upload(at, torch.tensor(list(sequences), dtype=torch.int64))
+        self._upload(at, torch.tensor(sequences, dtype=torch.int64))
         return self.page_table[at], self.lengths[at]
