@@ -141,12 +141,16 @@ class PagedCache:
     ``pages`` pages that the ``layers`` full attention layers use alike.
 
     ``k_pages[layer]`` and ``v_pages[layer]`` [pages, rows, kv_heads, d], ``page_table``
-    [sequences, pages a sequence] and ``lengths`` [sequences] stay where they are, so that
-    a captured graph finds later contents there. A decode step over all sequences is
-    ``extend`` by one token each, then per layer ``qk_norm_rope_append`` and
-    ``attention_paged`` on these tensors: a sequence that is not in use has length 0, is
-    not written and attends to nothing. ``rows_of`` picks the rows of some sequences.
-    Copies and uploads are issued on the current stream, and nothing waits for them."""
+    [sequences, pages a sequence], ``lengths`` and ``step_lengths`` [sequences] stay where
+    they are, so that a captured graph finds later contents there. ``step_lengths`` are the
+    lengths of the sequences that the last ``extend`` gave tokens, and 0 for the others.
+
+    A decode step over all sequences is ``extend`` by one token for each that takes part, then
+    per layer ``qk_norm_rope_append`` and ``attention_paged`` on ``page_table`` and
+    ``step_lengths``: a sequence that did not grow, or is not in use, is not written and
+    attends to nothing. (By ``lengths`` its row would replace its last token, also in a page that
+    a fork shares.) ``rows_of`` picks the rows of some sequences, by ``lengths``. Copies
+    and uploads are issued on the current stream, and nothing waits for them."""
 
     def __init__(self, pages: int, sequences: int, capacity: int, *, layers: int, kv_heads: int,
                  d_qk: int, d_v: int, page_rows: int = 64, dtype: torch.dtype = torch.bfloat16,
@@ -161,7 +165,9 @@ class PagedCache:
         self.k_pages, self.v_pages = list(made(d_qk)), list(made(d_v))
         self._table = torch.full((sequences, self.book.width), -1, dtype=torch.int32)
         self.page_table = self._table.to(device, copy=True)
-        self.lengths = torch.zeros(sequences, dtype=torch.int32, device=device)
+        self._counts = torch.zeros((2, sequences), dtype=torch.int32, device=device)
+        self.lengths, self.step_lengths = self._counts
+        self._grown: set[int] = set()  # by the last extend
 
     def _upload(self, target: torch.Tensor, values: torch.Tensor) -> None:
         # from pinned memory of its own, so that the copy takes its turn on the stream
@@ -177,7 +183,8 @@ class PagedCache:
                 self._table[i, :len(held)] = torch.tensor(held, dtype=torch.int32)
             self.book.changed.clear()
             self._upload(self.page_table, self._table)
-        self._upload(self.lengths, torch.tensor(self.book.lengths, dtype=torch.int32))
+        step = [n if i in self._grown else 0 for i, n in enumerate(self.book.lengths)]
+        self._upload(self._counts, torch.tensor((self.book.lengths, step), dtype=torch.int32))
 
     def add(self) -> int:
         """A new, empty sequence."""
@@ -186,7 +193,9 @@ class PagedCache:
     def extend(self, sequences: Sequence[int], tokens: Sequence[int]) -> None:
         """Room for more tokens, counted in ``lengths``: the next calls on the cache write
         and read them as the sequences' new ones. Shared last pages are copied first."""
-        self._carry_out(self.book.extend(sequences, tokens))
+        copies = self.book.extend(sequences, tokens)
+        self._grown = {int(s) for s, n in zip(sequences, tokens) if n}
+        self._carry_out(copies)
 
     def fork(self, sequence: int) -> int:
         """A new sequence that starts with the tokens of ``sequence``, on its pages."""
@@ -196,6 +205,7 @@ class PagedCache:
 
     def free(self, sequence: int) -> None:
         self.book.free(sequence)
+        self._grown.discard(sequence)
         self._carry_out(([], []))
 
     def compact(self) -> int:
