@@ -58,6 +58,8 @@ def rope_table(positions: int, rotary_dim: int, theta: float = 10000.0, *,
 
 def _check_angles(cos_sin, d, rotary_offset, device) -> tuple[torch.Tensor, int, int]:
     """The table as the kernels read it, its positions and its width."""
+    if not isinstance(cos_sin, torch.Tensor):
+        raise TypeError(f"cos_sin must be a tensor, got {type(cos_sin).__name__}")
     shape = cos_sin.shape
     if len(shape) != 2 or shape[0] == 0:
         raise ValueError("cos_sin must have shape [positions, rotary_dim]")
@@ -252,12 +254,13 @@ def _append(q, heads, k, v, batch, rows, kv_heads, d, dtype, device, k_pages, v_
 
 def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
                         v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
-                        cos_sin: torch.Tensor, q_weight: torch.Tensor | None = None,
+                        cos_sin: torch.Tensor | None, q_weight: torch.Tensor | None = None,
                         k_weight: torch.Tensor | None = None, eps: float = 1e-6, *,
                         cu_seqlens: torch.Tensor | None = None, rotary_offset: int = 0,
                         interleaved: bool = False) -> torch.Tensor:
     """``qk_norm_rope`` of new tokens at their positions in their sequences, with the
-    keys and ``v`` [B, S, H_kv, d_v] written to the cache; returns the queries.
+    keys and ``v`` [B, S, H_kv, d_v] written to the cache; returns the queries. With
+    ``cos_sin`` None nothing is rotated.
 
     Token i of the n that the call has of sequence s is position ``lengths[s]`` - n + i.
     B sequences of S new tokens each, or with ``cu_seqlens`` [N + 1] (int32 or int64, on
