@@ -17,13 +17,15 @@ constexpr int kPagedPack = 32;
 // With 512 / 1024 / 2048, 64 tokens on up to 8192 keys x 8 heads took 225 / 216 / 215 us, 1071
 // rows of a mixed step 169 / 165 / 205. Rows of long pieces, bound by their products, take
 // runs of twice the length (2048 rows on 16048 keys 539 us in 1024 runs, 523 so). At least
-// kMinRun keys: 19 rows on 1119 keys take 18 us, in runs of 128 28 (more to join), one token on 16384
-// 23 either way.
+// kMinRun keys: 19 rows on 1119 keys take 18 us, in runs of 128 (nine, so that the join takes four waves
+// a row) 28, one token on 16384 23 either way.
 constexpr int kFill = 1024;
 constexpr int kMinRun = 256;
 constexpr int kJoinFew = 4, kJoinMany = 16;  // rows of a block of the join
 constexpr int64_t kMaxSequences = 65536;
-// From here on a launch of its own counts through the sequences.
+// From here on a launch of its own counts through the sequences. With it / without it, single tokens x 8
+// heads of 128 on up to 512 keys: 64 sequences 29 / 26 us, 128 46 / 46, 255 64 / 71, 512 115 / 150, 1024
+// 220 / 367; on up to 128 keys 64 11 / 8, 256 33 / 33, 1024 113 / 168.
 constexpr int64_t kPlanSequences = 256;
 
 struct PagedArgs : AttnShape {
@@ -107,7 +109,7 @@ struct PagedKeys {
   }
 
   // Rows without a page, and those behind the sequence's last, read as zeros.
-  // ONCE: past the caches, for keys that no other block reads.
+  // ONCE: past the caches, for keys that one block reads (attend_few).
   template <bool ONCE = false>
   __device__ __forceinline__ void fetch(int64_t at, int buf) {
     const int k0 = static_cast<int>(at);
@@ -168,8 +170,12 @@ __device__ inline f32x4_t mfma16_half(uint2 a, uint2 b, f32x4_t c) {
 // product's operand.
 //
 // Bound by HBM: two tiles of 64 keys a block, two blocks a CU, keep up to 128 KB a CU on their
-// way. 64 tokens on up to 8192 keys x 8 heads of 128 (1.1 GB) take 198 us in all, 5.5 TB/s (7.0 is
-// what a kernel that only reads reaches here); 218 with loads that go through the caches.
+// way. 64 tokens on up to 8192 keys x 8 heads of 128 (1.1 GB) take 191 us in all, 5.7 TB/s (7.0 is
+// what a kernel that only reads reaches here). Loads go past the caches: 64 tokens on 8192 keys each take
+// 346 us, 382 through the caches. Where several blocks read the same keys the caches would serve, and
+// the kernel does not look for that: several packs on a key head (64 heads on 1, 64 tokens on 16384
+// keys: 195 us, 170 through the caches; 37 on 1, a pack each, on 8192: 1271 and 547) and forks of one
+// prompt (64 of one of 8192: 136 and 124).
 template <bool BF16, int DQ, int DV, int GROUPS>
 __device__ __forceinline__ void attend_few(const PagedArgs& a, const AttnBlock& b,
                                            PagedKeys<DQ, DV>& keys_of, uint16_t* stage,

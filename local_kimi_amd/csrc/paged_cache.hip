@@ -383,7 +383,7 @@ struct CopyArgs {
 };
 static_assert(sizeof(CopyArgs) <= 4096, "kernel arguments");
 
-// 16 bytes a thread. Bound by HBM (1100 pages of 128 KB in 4 tensors, 1.15 GB: 205 us, 5.6 TB/s; in
+// 16 bytes a thread. Bound by HBM (1100 pages of 128 KB in 4 tensors, 1.15 GB: 201 us, 5.7 TB/s; in
 // six launches, the lists in their arguments, 217). PACKED: pages smaller than a block's threads
 // follow one another in a block. IDLE: the lists pair a page with itself, which stores nothing, since
 // another pair may write the page (other lists are spared the comparison, which every block waits
