@@ -88,6 +88,8 @@ class PageBook:
     def extend(self, sequences: Sequence[int], tokens: Sequence[int]) -> Copies:
         """Room for ``tokens[i]`` more tokens of ``sequences[i]``; returns the copies that
         come before they are written."""
+        # (as plain numbers: those of a tensor are equal, and not the same in a set)
+        sequences, tokens = [int(s) for s in sequences], [int(n) for n in tokens]
         if len(sequences) != len(tokens) or len(set(sequences)) != len(sequences):
             raise ValueError("extend takes each sequence once, with a number of tokens")
         need, sharers = 0, {}
@@ -193,8 +195,9 @@ class PagedCache:
     def extend(self, sequences: Sequence[int], tokens: Sequence[int]) -> None:
         """Room for more tokens, counted in ``lengths``: the next calls on the cache write
         and read them as the sequences' new ones. Shared last pages are copied first."""
+        sequences, tokens = [int(s) for s in sequences], [int(n) for n in tokens]
         copies = self.book.extend(sequences, tokens)
-        self._grown = {int(s) for s, n in zip(sequences, tokens) if n}
+        self._grown = {s for s, n in zip(sequences, tokens) if n}
         self._carry_out(copies)
 
     def fork(self, sequence: int) -> int:
@@ -205,7 +208,7 @@ class PagedCache:
 
     def free(self, sequence: int) -> None:
         self.book.free(sequence)
-        self._grown.discard(sequence)
+        self._grown.discard(int(sequence))
         self._carry_out(([], []))
 
     def compact(self) -> int:
