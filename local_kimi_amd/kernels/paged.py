@@ -416,11 +416,12 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int] | torch.Tenso
     if not a:
         return
     count, lists = len(a), None
-    if count > _COPY_PAIRS and not torch.cuda.is_current_stream_capturing():
-        # from pinned memory of its own, so that the upload takes its turn on the stream
-        lists = torch.frombuffer(a + b, dtype=torch.int32).pin_memory().to(device, non_blocking=True)
     tables = [array("q", x) for x in (pointers, steps, sizes)]
     with _w._on(device):
+        # (whether the stream that the launch goes to is captured: that of the tensors' device)
+        if count > _COPY_PAIRS and not torch.cuda.is_current_stream_capturing():
+            # from pinned memory of its own, so that the upload takes its turn on the stream
+            lists = torch.frombuffer(a + b, dtype=torch.int32).pin_memory().to(device, non_blocking=True)
         status = _lib.load().lk_copy_pages(
             *(t.buffer_info()[0] for t in tables), len(pointers), a.buffer_info()[0],
             b.buffer_info()[0], count, pages, _pointer(lists), _w._stream(device))
