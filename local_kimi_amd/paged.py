@@ -10,6 +10,7 @@ a book's copies out with ``kernels.copy_pages``.
 from __future__ import annotations
 
 import heapq
+from array import array
 from collections.abc import Sequence
 
 import torch
@@ -35,6 +36,7 @@ class PageBook:
         self.pages: list[list[int] | None] = [None] * sequences        # of each sequence
         self.lengths = [0] * sequences
         self.changed: set[int] = set()  # sequences whose pages changed; its reader clears it
+        self.grown: list[int] = []      # sequences that the last extend gave tokens
         self._free = list(range(pages))  # a heap: the lowest goes first
 
     @property
@@ -73,6 +75,7 @@ class PageBook:
         for p in self._check(sequence):
             self._release(p)
         self.pages[sequence], self.lengths[sequence] = None, 0
+        self.grown = [s for s in self.grown if s != sequence]
         self.changed.add(sequence)
 
     def _release(self, page: int) -> None:
@@ -89,7 +92,7 @@ class PageBook:
         """Room for ``tokens[i]`` more tokens of ``sequences[i]``; returns the copies that
         come before they are written."""
         # (as plain numbers: those of a tensor are equal, and not the same in a set)
-        sequences, tokens = [int(s) for s in sequences], [int(n) for n in tokens]
+        sequences, tokens = list(map(int, sequences)), list(map(int, tokens))
         if len(sequences) != len(tokens) or len(set(sequences)) != len(sequences):
             raise ValueError("extend takes each sequence once, with a number of tokens")
         need, sharers = 0, {}
@@ -109,6 +112,7 @@ class PageBook:
         if need > len(self._free):
             raise RuntimeError(f"{need} pages are needed, {len(self._free)} are free")
         src, dst = [], []
+        self.grown = [s for s, n in zip(sequences, tokens) if n]
         for s, n in zip(sequences, tokens):
             held = self.pages[s]
             if n and self.lengths[s] % self.page_rows and self.users[held[-1]] > 1:
@@ -169,7 +173,6 @@ class PagedCache:
         self.page_table = self._table.to(device, copy=True)
         self._counts = torch.zeros((2, sequences), dtype=torch.int32, device=device)
         self.lengths, self.step_lengths = self._counts
-        self._grown: set[int] = set()  # by the last extend
 
     def _upload(self, target: torch.Tensor, values: torch.Tensor) -> None:
         # from pinned memory of its own, so that the copy takes its turn on the stream
@@ -185,8 +188,11 @@ class PagedCache:
                 self._table[i, :len(held)] = torch.tensor(held, dtype=torch.int32)
             self.book.changed.clear()
             self._upload(self.page_table, self._table)
-        step = [n if i in self._grown else 0 for i, n in enumerate(self.book.lengths)]
-        self._upload(self._counts, torch.tensor((self.book.lengths, step), dtype=torch.int32))
+        step = [0] * len(self.book.lengths)
+        for i in self.book.grown:
+            step[i] = self.book.lengths[i]
+        counts = torch.frombuffer(array("i", self.book.lengths + step), dtype=torch.int32)
+        self._upload(self._counts, counts.view(2, -1))
 
     def add(self) -> int:
         """A new, empty sequence."""
@@ -195,10 +201,7 @@ class PagedCache:
     def extend(self, sequences: Sequence[int], tokens: Sequence[int]) -> None:
         """Room for more tokens, counted in ``lengths``: the next calls on the cache write
         and read them as the sequences' new ones. Shared last pages are copied first."""
-        sequences, tokens = [int(s) for s in sequences], [int(n) for n in tokens]
-        copies = self.book.extend(sequences, tokens)
-        self._grown = {s for s, n in zip(sequences, tokens) if n}
-        self._carry_out(copies)
+        self._carry_out(self.book.extend(sequences, tokens))
 
     def fork(self, sequence: int) -> int:
         """A new sequence that starts with the tokens of ``sequence``, on its pages."""
@@ -208,7 +211,6 @@ class PagedCache:
 
     def free(self, sequence: int) -> None:
         self.book.free(sequence)
-        self._grown.discard(int(sequence))
         self._carry_out(([], []))
 
     def compact(self) -> int:
