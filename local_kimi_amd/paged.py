@@ -16,6 +16,7 @@ from collections.abc import Sequence
 import torch
 
 from .kernels.paged import PAGE_ROWS_STEP, copy_pages
+from .kernels.w4a16 import _on
 
 Copies = tuple[list[int], list[int]]  # pages read, pages written
 
@@ -156,7 +157,8 @@ class PagedCache:
     ``step_lengths``: a sequence that did not grow, or is not in use, is not written and
     attends to nothing. (By ``lengths`` its row would replace its last token, also in a page that
     a fork shares.) ``rows_of`` picks the rows of some sequences, by ``lengths``. Copies
-    and uploads are issued on the current stream, and nothing waits for them."""
+    and uploads are issued on the current stream, and nothing waits for them; calls that make
+    them are refused while it is captured."""
 
     def __init__(self, pages: int, sequences: int, capacity: int, *, layers: int, kv_heads: int,
                  d_qk: int, d_v: int, page_rows: int = 64, dtype: torch.dtype = torch.bfloat16,
@@ -173,6 +175,15 @@ class PagedCache:
         self.page_table = self._table.to(device, copy=True)
         self._counts = torch.zeros((2, sequences), dtype=torch.int32, device=device)
         self.lengths, self.step_lengths = self._counts
+
+    def _check_stream(self) -> None:
+        """Before anything changes: a replay would upload from memory that is long free."""
+        if not self.lengths.is_cuda:
+            return
+        with _on(self.lengths.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a paged cache is extended, forked, freed from, compacted and asked "
+                                   "for rows outside the captured graph")
 
     def _upload(self, target: torch.Tensor, values: torch.Tensor) -> None:
         # from pinned memory of its own, so that the copy takes its turn on the stream
@@ -201,20 +212,24 @@ class PagedCache:
     def extend(self, sequences: Sequence[int], tokens: Sequence[int]) -> None:
         """Room for more tokens, counted in ``lengths``: the next calls on the cache write
         and read them as the sequences' new ones. Shared last pages are copied first."""
+        self._check_stream()
         self._carry_out(self.book.extend(sequences, tokens))
 
     def fork(self, sequence: int) -> int:
         """A new sequence that starts with the tokens of ``sequence``, on its pages."""
+        self._check_stream()
         i = self.book.fork(sequence)
         self._carry_out(([], []))
         return i
 
     def free(self, sequence: int) -> None:
+        self._check_stream()
         self.book.free(sequence)
         self._carry_out(([], []))
 
     def compact(self) -> int:
         """Moves the pages in use to the front of the tensors; returns how many moved."""
+        self._check_stream()
         copies = self.book.compact()
         self._carry_out(copies)
         return len(copies[0])
@@ -222,6 +237,7 @@ class PagedCache:
     def rows_of(self, sequences: Sequence[int]) -> tuple[torch.Tensor, torch.Tensor]:
         """``page_table`` and ``lengths`` of these sequences, in this order (copies); one that is
         not in use has length 0 and no pages."""
+        self._check_stream()
         sequences = [int(s) for s in sequences]
         for s in sequences:
             if not 0 <= s < len(self.book.pages):  # (an index on the device would fault there)

@@ -105,3 +105,29 @@ def test_a_sequence_that_sits_out_keeps_its_tokens(captured):
             else:
                 assert not out[s].any(), (i, s)
         assert not out[4].any()
+
+
+@pytest.mark.gpu
+def test_a_capture_refuses_what_uploads():
+    """Before anything changes, in the book or on the device; the capture goes on."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    cache = PagedCache(30, 4, 96, layers=1, kv_heads=1, d_qk=8, d_v=8, page_rows=16)
+    a = cache.add()
+    cache.extend([a], [20])
+    b = cache.fork(a)
+    before = [list(x) for x in (cache.book.lengths, cache.book.users, cache.book.pages[a], cache.book.pages[b])]
+    graph, x = torch.cuda.CUDAGraph(), torch.ones(8, device="cuda")
+    with torch.cuda.graph(graph):
+        y = x + 1
+        for call in (lambda: cache.extend([a], [1]), lambda: cache.fork(a), lambda: cache.free(b), cache.compact,
+                     lambda: cache.rows_of([a])):
+            with pytest.raises(RuntimeError, match="outside the captured graph"):
+                call()
+        z = cache.step_lengths + 1
+    assert before == [list(x) for x in (cache.book.lengths, cache.book.users, cache.book.pages[a], cache.book.pages[b])]
+    cache.extend([b], [2])
+    for _ in range(3):
+        x += 1
+        graph.replay()
+        assert torch.equal(y, x + 1) and z.tolist() == [1, 23, 1, 1]
