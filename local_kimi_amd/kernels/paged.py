@@ -386,8 +386,9 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int] | torch.Tenso
 
     ``src`` and ``dst`` are sequences of integers or integer tensors on the host; a page is
     written once at most, and is no other pair's source (ValueError); a pair of a page with
-    itself does nothing. A captured graph keeps the lists it was captured with. Pages must be dense, in any order of their
-    dimensions, and multiples of 16 bytes; the tensors must not overlap each other."""
+    itself does nothing. A captured graph keeps the lists it was captured with. Pages must be
+    dense, in any order of their dimensions, and multiples of 16 bytes; the tensors must not
+    overlap each other."""
     a, b = _page_list(src, "src"), _page_list(dst, "dst")
     if len(a) != len(b):
         raise ValueError("src and dst must be lists of one length")
